@@ -58,9 +58,17 @@ PROTOTYPES = {
     "adkv_rope_qk": (_i, [_vp] * 6 + [_i] * 5 + [C.c_int64] * 8 + [_i, _vp]),
     "adkv_quant_f32": (_i, [_vp] * 12 + [_i] * 3 + [C.c_int64, C.c_int64] + [_i] * 3 + [_f, _f, _vp]),
     "adkv_quant_f32_pair": (_i, [_vp] * 7 + [_i] * 6 + [_f, _f, _vp]),
+    "adkv_extend_workspace_bytes": (C.c_int64, [_i] * 10),
+    "adkv_extend": (_i, [_vp] * 12 + [_f, _vp] + [_i] * 9 + [_vp, _vp, _i, _i, _vp, _vp, C.c_int64, _vp]),
     "adkv_fp16_decode_workspace_bytes": (C.c_int64, [_i] * 3),
     "adkv_fp16_decode": (_i, [_vp] * 5 + [C.c_int64] + [_i] * 4 + [_f, _vp]),
 }
+
+class Prefix(C.Structure):
+    """``adkv_prefix`` of include/adkv_hip.h."""
+    _fields_ = [(n, _vp) for n in ("k_codes", "v_codes", "k_params", "v_params", "k_ckpt", "v_ckpt")] + \
+        [(n, _i) for n in ("tokens", "n_super", "n_ckpt_cap", "ckpt_interval")]
+
 
 _lib = None
 

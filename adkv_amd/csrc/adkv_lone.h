@@ -110,39 +110,6 @@ struct LoneLoads {
     }
 };
 
-// The entries of unit i of the words in flight, two tokens each; with 2-bit codes a byte of a word is four tokens and
-// an LDS read returns two entries.
-template <int BITS>
-__device__ __forceinline__ void lone_lookup(uint2 *e, const uint2 *lut, const uint32_t *buf, int i, uint32_t lane_copy)
-{
-    if constexpr (BITS == 4) {
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-            e[k] = lut_get(lut, buf[i], lane_copy, k);
-    } else {
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const uint4 v = lut2_get(lut, buf[i / 2], lane_copy, i % 2 * 2 + k);
-            e[2 * k] = make_uint2(v.x, v.y);
-            e[2 * k + 1] = make_uint2(v.z, v.w);
-        }
-    }
-}
-// The table for them (see lone_fill for 4 bits): 16 copies of 16-byte entries.
-template <int NT>
-__device__ __forceinline__ void lone_fill2(uint2 *lut, int tid)
-{
-    uint4 *l4 = reinterpret_cast<uint4 *>(lut);
-#pragma unroll
-    for (int i = 0; i < LUT_ENTRIES * LUT2_COPIES; i += NT) {
-        if (LUT_ENTRIES * LUT2_COPIES % NT != 0 && i + tid >= LUT_ENTRIES * LUT2_COPIES)
-            break;
-        const int b = (i + tid) / LUT2_COPIES;
-        const auto entry = [](int code) { return as_u32(splat((h1)(code - 2))) & 0x7FFFFFFFu; };
-        l4[i + tid] = make_uint4(entry(b & 3), entry(b >> 2 & 3), entry(b >> 4 & 3), entry(b >> 6));
-    }
-}
-
 // The last segment's end: hands out the state after token T - 1, records it where token T opens an interval,
 // quantises token T into its word (gemv.cu:744-798, 1105-1157) and returns its value r16(q*sc + zp).
 template <int D, int BITS>

@@ -13,6 +13,7 @@ by hand-written gfx950 kernels behind ``libadkv_hip.so``.  Differences, all on t
 from __future__ import annotations
 
 import functools
+from typing import NamedTuple
 
 import torch
 
@@ -632,3 +633,144 @@ def decode_step_workspace_bytes(B: int, nq: int, nh: int, T: int, DIM: int, n_ck
     """Bytes ``decode_step`` needs for ``nq`` query heads over ``nh`` KV heads."""
     return int(_lib.lib().adkv_decode_step_workspace_bytes(B, nq, nh, T, DIM, n_ckpt_cap,
                                                             ckpt_interval))
+
+
+class SharedPrefix(NamedTuple):
+    """Codes of tokens that every sequence of a batch begins with, held once (extension: ``extend``): caches and checkpoints of one
+    sequence, ``[1, nh, ...]``, of which the first ``tokens`` tokens are meant, and the parameters that they were quantised with.
+    The sequences' own streams go on from the state behind the last of them (``append_kv``'s ``state``, ``forward_qk``'s
+    ``state_out``): their parameters are these with that state's zp and sc in place of the first two."""
+    k_cache: torch.Tensor
+    v_cache: torch.Tensor
+    tokens: int
+    k_params: tuple
+    v_params: tuple
+    k_ckpt: torch.Tensor | None = None
+    v_ckpt: torch.Tensor | None = None
+
+
+def _stride3(t: torch.Tensor):
+    """Element strides of the first three of four axes, 0 along an axis of length one."""
+    return (_lib.C.c_int64 * 3)(*[st if n > 1 else 0 for st, n in zip(t.stride()[:3], t.shape[:3])])
+
+
+def extend(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    k_new: torch.Tensor,
+    v_new: torch.Tensor,
+    k_params,
+    v_params,
+    T: int,
+    scaling: float,
+    mask: torch.Tensor | None = None,
+    *,
+    prefix: SharedPrefix | None = None,
+    k_ckpt: torch.Tensor | None = None,
+    v_ckpt: torch.Tensor | None = None,
+    ckpt_interval: int = 0,
+    bits: int = 4,
+    workspace: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``n >= 1`` new tokens of every sequence at once: quantised into slots ``T .. T+n-1`` of both caches (codes as ``append_kv``
+    writes them) and attended with, each over the prefix, the cached tokens and the new ones up to itself.
+
+    The reference takes tokens one at a time (src/adkv/hf/llama_adkv.py:235-276); ``n`` calls of ``decode_step`` write the same
+    codes and give the same outputs up to rounding (scores stay fp32 here; a new token's value is what every later call reads).
+
+    Args:
+        q: ``[B, Hq, n, 128]`` float16 or bfloat16, 1, 2, 4 or 8 query heads per KV head; any strides with contiguous channels.
+        k_new, v_new: ``[B, nh, n, 128]`` of the same type, strided likewise.
+        k_params, v_params: the five ``[nh, 128]`` fp16 tensors; with a prefix zp and sc are the state behind its last token.
+        mask: additive, ``[B or 1, Hq or 1, n or 1, P+T+n]`` (or three axes, ``[B or 1, Hq or 1, P+T+n]``, for all n alike), columns in the
+            order prefix, own tokens.  fp16, bfloat16 and fp32 are read in place.  Later tokens are hidden without it.
+        prefix: tokens that the whole batch begins with; its checkpoints are every ``ckpt_interval`` tokens too.
+        workspace: uint8, 256-byte aligned, ``extend_workspace_bytes`` long, to avoid the per-call allocation.
+
+    Returns ``[B, n, Hq, 128]`` in ``q``'s type.  Rows that the mask leaves nothing of are NaN.
+    """
+    k_params, v_params = tuple(k_params), tuple(v_params)
+    act = q.dtype
+    _chk(act in (torch.float16, torch.bfloat16), "q must be float16 or bfloat16")
+    _chk(k_new.dtype == act and v_new.dtype == act, "k_new and v_new must have q's type")
+    _chk(q.dim() == 4 and k_new.dim() == 4 and k_new.shape == v_new.shape, "q must be [B, Hq, n, DIM], k_new and v_new [B, nh, n, DIM]")
+    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        _chk(t.dtype == torch.uint8 and t.dim() == 6, f"{name} must be uint8 [B, nh, n_super_cap, DIM/4, 4, 4]")
+        _chk(t.is_contiguous(), f"{name} must be contiguous (appended in place)")
+    _chk(k_cache.shape == v_cache.shape, "k_cache and v_cache shapes differ")
+    B, nq, n, DIM = q.shape
+    nh, n_super_cap = k_cache.shape[1], k_cache.shape[2]
+    _chk(k_new.shape == (B, nh, n, DIM) and k_cache.shape[0] == B and k_cache.shape[3:] == (DIM // _TILE, 4, 4),
+         "q, k_new, v_new and the caches disagree in shape")
+    _chk(DIM == 128, "extend needs DIM == 128")
+    _chk(nh > 0 and nq % nh == 0 and nq // nh in _GROUPS, "query heads must be 1, 2, 4 or 8 times the KV heads")
+    _chk(B > 0 and n > 0, "extend needs at least one sequence and one new token")
+    _chk(T >= 0, "T must be non-negative")
+    _chk(bits in (2, 4), "bits must be 2 or 4")
+    tps = 32 // bits
+    _chk(-(-(T + n) // tps) <= n_super_cap, f"k_cache has no room for {T + n} tokens")
+    kp = _params(k_params, ("k_zp", "k_sc", "k_alpha", "k_beta", "k_t"), nh, DIM)
+    vp = _params(v_params, ("v_zp", "v_sc", "v_alpha", "v_beta", "v_t"), nh, DIM)
+    _chk((k_ckpt is None) == (v_ckpt is None), "give both checkpoint tensors or neither")
+    kcp, ccap, civ = _ckpt_args(k_ckpt, ckpt_interval, B, nh, DIM, bits)
+    vcp, vcap, _ = _ckpt_args(v_ckpt, ckpt_interval, B, nh, DIM, bits)
+    _chk(ccap == vcap, "K and V checkpoint tensors must have the same capacity")
+    tensors = [q, k_cache, v_cache, k_new, v_new, *kp, *vp] + ([k_ckpt, v_ckpt] if k_ckpt is not None else [])
+    arr = _lib.C.c_void_p * 5
+    P = pcap = piv = 0
+    pre = None
+    if prefix is not None:
+        P = int(prefix.tokens)
+        _chk(P >= 0, "a prefix cannot have a negative number of tokens")
+        for t in (prefix.k_cache, prefix.v_cache):
+            _chk(t.dtype == torch.uint8 and t.is_contiguous() and t.dim() == 6 and t.shape[:2] == (1, nh) and t.shape[3:] == (DIM // _TILE, 4, 4),
+                 "a prefix's caches must be contiguous uint8 [1, nh, n_super, DIM/4, 4, 4]")
+        _chk(prefix.k_cache.shape == prefix.v_cache.shape and -(-P // tps) <= prefix.k_cache.shape[2], "the prefix's caches do not hold its tokens")
+        pkp = _params(tuple(prefix.k_params), ("k_zp", "k_sc", "k_alpha", "k_beta", "k_t"), nh, DIM)
+        pvp = _params(tuple(prefix.v_params), ("v_zp", "v_sc", "v_alpha", "v_beta", "v_t"), nh, DIM)
+        _chk((prefix.k_ckpt is None) == (prefix.v_ckpt is None), "give both of the prefix's checkpoint tensors or neither")
+        pkc, pcap, piv = _ckpt_args(prefix.k_ckpt, ckpt_interval, 1, nh, DIM, bits)
+        pvc, pvcap, _ = _ckpt_args(prefix.v_ckpt, ckpt_interval, 1, nh, DIM, bits)
+        _chk(pcap == pvcap, "the prefix's checkpoint tensors must have the same capacity")
+        tensors += [prefix.k_cache, prefix.v_cache, *pkp, *pvp] + ([prefix.k_ckpt, prefix.v_ckpt] if prefix.k_ckpt is not None else [])
+        pk, pv = arr(*[t.data_ptr() for t in pkp]), arr(*[t.data_ptr() for t in pvp])
+        if P > 0 and prefix.k_cache.shape[2] > 0:
+            pre = _lib.Prefix(prefix.k_cache.data_ptr(), prefix.v_cache.data_ptr(), _lib.C.cast(pk, _lib.C.c_void_p),
+                              _lib.C.cast(pv, _lib.C.c_void_p), pkc, pvc, P, prefix.k_cache.shape[2], pcap, piv)
+    if mask is not None:
+        mask = mask[:, :, None] if mask.dim() == 3 else mask
+        _chk(mask.dim() == 4 and mask.shape[3] == P + T + n and mask.shape[0] in (1, B) and mask.shape[1] in (1, nq) and mask.shape[2] in (1, n),
+             "mask must broadcast to [B, nh, n, P + T + n]")
+    dev = _need_device(*tensors)
+    mst, mdt = None, 0
+    if mask is not None:
+        mdt = _MASK_DT.get(mask.dtype, 0)
+        mask = mask.to(device=dev, dtype=mask.dtype if mdt else torch.float32)
+        if mask.stride(3) != 1 and mask.shape[3] > 1:
+            mask = mask.contiguous()
+        mst = _stride3(mask)
+    if q.stride(3) != 1 or any(st % 2 for st, k in zip(q.stride()[:3], q.shape[:3]) if k > 1) or q.data_ptr() % 4:
+        q = q.contiguous()
+    xk, ks = _row_strides(k_new)
+    xv, vs = _row_strides(v_new)
+    if workspace is None:
+        workspace = torch.empty(extend_workspace_bytes(B, nq, nh, T, n, ccap, civ, P, pcap), dtype=torch.uint8, device=dev)
+    _chk(workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.device == dev, "workspace must be a uint8 tensor on the same device")
+    out = torch.empty((B, n, nq, DIM), dtype=act, device=dev)
+    with _lib.device_guard(dev):
+        rc = _lib.lib().adkv_extend(
+            q.data_ptr(), _stride3(q), k_cache.data_ptr(), v_cache.data_ptr(), xk.data_ptr(), xv.data_ptr(), ks, vs,
+            arr(*[t.data_ptr() for t in kp]), arr(*[t.data_ptr() for t in vp]), _ptr(mask), mst, float(scaling), out.data_ptr(),
+            B, nq, nh, T, n, DIM, n_super_cap, bits, (_DT_BF16 if act == torch.bfloat16 else _DT_F16) | mdt << 8,
+            kcp, vcp, ccap, civ, None if pre is None else _lib.C.addressof(pre), workspace.data_ptr(), workspace.numel(),
+            _lib.current_stream_ptr(dev))
+    _lib.check(rc, "extend")
+    return out
+
+
+def extend_workspace_bytes(B: int, nq: int, nh: int, T: int, n: int, n_ckpt_cap: int = 0, ckpt_interval: int = 0, P: int = 0,
+                           prefix_n_ckpt_cap: int = 0) -> int:
+    """Bytes ``extend`` needs for ``n`` new tokens behind ``T`` cached ones and a prefix of ``P``."""
+    return int(_lib.lib().adkv_extend_workspace_bytes(B, nq, nh, T, n, n_ckpt_cap, ckpt_interval, P, prefix_n_ckpt_cap,
+                                                      ckpt_interval if prefix_n_ckpt_cap else 0))

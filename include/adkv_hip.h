@@ -418,6 +418,42 @@ int adkv_rope_qk(const void *q, const void *k, const void *cos, const void *sin,
                  int64_t q_sb, int64_t q_sh, int64_t q_st, int64_t k_sb, int64_t k_sh, int64_t k_st,
                  int64_t cs_sb, int64_t cs_st, int bf16, void *stream);
 
+/*
+ * n new tokens of every sequence at once, over codes: quantised as tokens T..T+n-1 of the caches (as adkv_append_kv_pair does it)
+ * and attended with.  Query i of a sequence looks at the prefix, if there is one, and at its own tokens 0..T+i:
+ *   out = softmax(scaling * q.K^T + mask) V
+ * with K and V the values of the codes, as every later call reads them: r16(r16(q*sc) + zp), the new tokens' too.  The reference takes
+ * new tokens one at a time (llama_adkv.py:235-276) and has no prefix.
+ * The prefix is a cache of one sequence that the whole batch shares: each sequence's tokens go on from the state behind its
+ * last one, which has to be given as zp and sc in k_params / v_params ([H, D] like any parameters).  It is replayed once per KV head, whatever
+ * the batch.  Nothing of it is written.
+ *   q        fp16 or bfloat16 (act_dtype, as in adkv_decode_step: rounded to fp16 as it is read) [B, Hq, n, D], 1, 2, 4 or 8 query heads per
+ *            KV head, head dim 128, channels contiguous; q_strides: element strides {batch, head, token}, even, rows 4-byte aligned
+ *   k_new, v_new, k_strides, v_strides   [B, H, n, D] of the same type, as in adkv_append_kv_pair
+ *   mask     optional, added to the scores: element strides {batch, head, query}, 0 where it is the same for all; its columns are the
+ *            prefix's tokens, then the own ones (P + T + n); fp32, or fp16 / bfloat16 by act_dtype | ADKV_MASK_DT(dt).  A row that it
+ *            leaves nothing of (-inf throughout) is NaN.
+ *   out      [B, n, Hq, D] in q's type, 8-byte aligned
+ * The state in front of token T is replayed from the checkpoint before it; where T opens an interval its checkpoint is recorded, and
+ * those that the new tokens cross.  Sums and scores are fp32; weights are rounded to fp16 relative to the largest so far.  A value that is
+ * infinite or NaN in a channel reaches that channel of all n queries of the call, also of those in front of its token.
+ * workspace: >= adkv_extend_workspace_bytes(...) bytes, 256-byte aligned (the prefix's arguments 0 without one).
+ */
+typedef struct {
+    const void *k_codes, *v_codes;                /* uint8 [H, n_super, D/4, 4, 4] */
+    const void *const *k_params, *const *v_params; /* host arrays of five device pointers, as in adkv_decode_step */
+    const void *k_ckpt, *v_ckpt;                  /* fp16 [H, n_ckpt_cap, D, 2], or both NULL */
+    int tokens, n_super, n_ckpt_cap, ckpt_interval;
+} adkv_prefix;
+int64_t adkv_extend_workspace_bytes(int B, int Hq, int H, int T, int n, int n_ckpt_cap, int ckpt_interval, int prefix_tokens,
+                                    int prefix_n_ckpt_cap, int prefix_ckpt_interval);
+int adkv_extend(const void *q, const int64_t *q_strides, void *k_cache, void *v_cache, const void *k_new, const void *v_new,
+                const int64_t *k_strides, const int64_t *v_strides, const void *const *k_params, const void *const *v_params,
+                const void *mask, const int64_t *mask_strides, float scaling, void *out,
+                int B, int Hq, int H, int T, int n, int D, int n_super_cap, int bits, int act_dtype,
+                void *k_ckpt, void *v_ckpt, int n_ckpt_cap, int ckpt_interval, const adkv_prefix *prefix,
+                void *workspace, int64_t workspace_bytes, void *stream);
+
 /* ---- comparator, not part of the drop-in boundary ----
  * fp16-KV single-query attention (split-K flash decoding), standing in for the uncompressed fp16
  * cache that ADKV's memory and latency claims are made against (tools/memory_comparison_fig.py:46-56
