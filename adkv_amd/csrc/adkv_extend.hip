@@ -7,6 +7,8 @@
 // grow with the batch but by matrix instructions.  The context of a KV head is cut at checkpoints into pieces, each of which leaves
 // (m, l, o) = (max x, sum e^(x-m), sum e^(x-m) V) per query row; pieces are joined by M = max m, out = sum e^(m-M) o / sum e^(m-M) l.
 // Scores, m, l, o are fp32; the weights e^(x-m) are rounded to fp16 for the matrix cores, relative to the largest so far.
+#include <math.h>
+
 #include <algorithm>
 
 #include "adkv_device.h"
@@ -19,12 +21,19 @@ namespace adkv_ext {
 using namespace adkv;
 
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
-typedef float f8v __attribute__((ext_vector_type(8)));
+typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+typedef float f2v __attribute__((ext_vector_type(2)));
 
 constexpr int D = 128;
-constexpr int TILE = 64;                 // tokens
-constexpr int TILE_BYTES = D * TILE * 2; // a channel's tokens are 128 consecutive bytes
-constexpr int PRODUCERS = 4, CONSUMERS = 4, THREADS = 64 * (PRODUCERS + CONSUMERS);
+constexpr int PRODUCERS = 4;
+// Two shapes of workgroup.  Many rows: tiles of 64 tokens, eight waves that multiply, one workgroup per CU.  Few rows (at most 16 per unit):
+// tiles of 32, four such waves, two workgroups per CU: a wave that replays alone on its SIMD uses half of the issue slots.
+template <bool FEW> struct Shape {
+    static constexpr int TILE = FEW ? 32 : 64, MULTIPLIERS = FEW ? 4 : 8, THREADS = 64 * (PRODUCERS + MULTIPLIERS);
+    // Many: the code table of 64 KB, two buffers of a K and a V tile of 16 KB each.  Few: half as many copies of the table's entries, in the first
+    // half of every 256 bytes of 64 KB, and the buffers, of 8 KB a tile, in the second halves.
+    static constexpr int BUFFER = 32768, VALUES = 16384, FIRST = FEW ? 128 : 65536, LDS = FEW ? 65536 : 131072;
+};
 constexpr int MAX_TOKENS = 1 << 24; // 64 bytes each: a piece's codes are addressed in 32 bits
 constexpr float LOG2E = 1.44269504088896340736f;
 
@@ -34,37 +43,150 @@ struct Tensor { // K or V of a source
     const h1 *zp, *sc, *al, *be, *tg;
 };
 
-// Codes and the query rows that look at them.  The prefix has a unit per KV head and the rows (sequence, token, query head of
-// the group); an own source has a unit per sequence and KV head and the rows (token, query head).
+// Codes: the prefix's, a unit per KV head, or the sequences' own ones, a unit per sequence and KV head.
+struct Extent {
+    int tokens, n_super, n_ckpt;
+    int interval, intervals; // checkpoint intervals; the last goes on to the last token
+    int seen;                // tokens that the first of the new tokens looks at; each later one at one more if causal
+    int causal;
+    int col;                 // where its tokens are in the mask
+};
 struct Source {
     Tensor t[2];
-    int tokens, n_super, n_ckpt;
-    int interval, intervals, nseg; // a piece is a run of whole checkpoint intervals
-    int units, blocks, rows;       // query blocks per unit, query rows per unit
-    int items;                     // units * blocks * nseg
-    int seen;                      // tokens that the first of the new tokens looks at; each later one at one more if causal
-    int causal;
-    int col;                       // where its tokens are in the mask
-    int piece;                     // number of its first piece among all partial results
+    Extent x;
+};
+
+// x / d for x * d < 2^32: see divide()
+struct Div {
+    uint32_t d, mul;
+};
+
+// Query rows and the sources that they look at.  Group 0 has the rows (sequence, token, query head of the group) of a KV head and
+// looks at the prefix; group 1 has the rows (token, query head) of a sequence and KV head and looks at its own codes, behind the prefix
+// if `joint`.  Its items: a block of rows with one piece of the checkpoint intervals.
+struct Group {
+    int units, blocks, nseg, rows, items;
+    int from, to;          // sources
+    int per_piece, longer; // intervals of a piece; the first `longer` ones have one more
+    int piece, split;      // number of its first partial result; partial results per piece
+    Div by_unit, by_block;
 };
 
 struct Args {
     Source s[2]; // prefix, own
+    Group g[2];
     const h1 *q;
     long q_sb, q_sh, q_st;
     const void *mask;
     long m_sb, m_sh, m_st;
     int mask_dt;
-    float *partial; // [pieces, rows, D]
-    float2 *ml;     // [pieces, rows]: m, l
+    float *partial; // [partial results, rows, D]
+    float2 *ml;     // [partial results, rows]: m, l
+    h1 *out;        // not null: a row has one partial result, and goes here
     long rows;      // B * n * Hq, in the order of the output [B, n, Hq]
-    int B, H, G, n;
+    int H, log_g;
+    Div by_head, by_token;
+    int n;
     int act_bf16;
-    float scaling;
+    float scaling; // not negative: the queries' signs are changed instead
+    int negate;
+    // one new token: quantised by the waves that replay the own tokens in front of it, its row here
+    int append;
+    const uint16_t *x[2];
+    long x_sb[2], x_sh[2];
 };
 
-// where a channel's 16-byte pieces of a tile are: eight lanes' writes and a matrix operand's reads spread over the banks
-__device__ __forceinline__ int piece_of(int c, int unit) { return c * (TILE * 2) + ((unit ^ (c >> 1 & 7)) << 4); }
+// The arguments are read where the launch has put them: indexed by what a wave is at, a copy would live in scratch memory.
+#define ADKV_KERNARG const __attribute__((address_space(4)))
+typedef ADKV_KERNARG Args KArgs;
+__device__ __forceinline__ int divide(int x, const Div &by) { return by.d == 1 ? x : (int)__umulhi((uint32_t)x, by.mul); }
+__device__ __forceinline__ int divide(int x, ADKV_KERNARG Div &by) { return by.d == 1 ? x : (int)__umulhi((uint32_t)x, by.mul); }
+// all of a structure at once: field by field, between branches, every read is a wait
+template <typename T>
+__device__ __forceinline__ T all_of(ADKV_KERNARG T &from)
+{
+    struct Words {
+        uint32_t w[sizeof(T) / 4];
+    } x;
+    const auto p = (ADKV_KERNARG uint32_t *)&from;
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(T) / 4; i++)
+        x.w[i] = p[i];
+    return __builtin_bit_cast(T, x);
+}
+// a pointer from there is one to global memory, which the compiler cannot know
+template <typename T>
+__device__ __forceinline__ __attribute__((address_space(1))) T *global(T *p) { return (__attribute__((address_space(1))) T *)p; }
+
+// The tiles of a workgroup, one after the other: those of an item's piece in one source, then in the other, then the next item's.  What
+// the arguments have of an item or a span is read when it is opened: a read per tile is a wait per tile.
+template <int TILE>
+struct Walk {
+    int i, group, b, h, block, seg, end; // item; end: interval behind its piece, counted over its sources
+    int rows, prefix;                    // of the group; intervals of the prefix if the piece may begin there
+    int src, first, t0, t1, k, n;        // span: a run of tokens of a source, in tiles; the tile
+    int items;
+    bool ends;                           // the span is its item's last
+    __device__ __forceinline__ Walk(KArgs &a, int items_, int item) : i(item), items(items_) { open(a); }
+    __device__ __forceinline__ void open(KArgs &a)
+    {
+        group = i < a.g[0].items ? 0 : 1;
+        const Group g = all_of(a.g[group]);
+        int at = i - (group ? a.g[0].items : 0);
+        const int unit = divide(at, g.by_unit);
+        at -= unit * (g.blocks * g.nseg);
+        seg = divide(at, g.by_block);
+        block = at - seg * g.blocks;
+        b = group ? divide(unit, a.by_head) : 0;
+        h = unit - b * a.H;
+        rows = g.rows;
+        prefix = g.from == 0 ? a.s[0].x.intervals : 0;
+        const int begin = seg * g.per_piece + min(seg, g.longer);
+        end = begin + g.per_piece + (seg < g.longer ? 1 : 0);
+        span(a, begin < prefix ? begin : begin - prefix, begin < prefix ? 0 : 1);
+    }
+    __device__ __forceinline__ void span(KArgs &a, int first_, int src_)
+    {
+        src = src_;
+        first = first_;
+        const Extent s = all_of(a.s[src].x);
+        const int e = src ? end - prefix : end;
+        t0 = first * s.interval;
+        t1 = e >= s.intervals ? s.tokens : e * s.interval;
+        k = 0;
+        n = (t1 - t0 + TILE - 1) / TILE;
+        ends = src == 1 || end <= prefix;
+    }
+    __device__ __forceinline__ bool last_of_item() const { return k + 1 == n && ends; }
+    __device__ __forceinline__ bool more() const { return i + (int)gridDim.x < items; }
+    __device__ __forceinline__ bool last() const { return last_of_item() && !more(); }
+    // to the next tile, which is there
+    __device__ __forceinline__ void go(KArgs &a)
+    {
+        if (++k < n)
+            return;
+        if (!ends) {
+            span(a, 0, 1);
+        } else {
+            i += gridDim.x;
+            open(a);
+        }
+    }
+    __device__ __forceinline__ int code_unit(KArgs &a) const { return src ? b * a.H + h : h; }
+};
+
+// Where a tile's values are, in pieces of 16 bytes whose order changes with the channel so that what is accessed in one clock lies in different
+// banks.  32 channels are 4096 bytes, 16 are 2048, in either shape.
+// Many rows: a channel's 64 tokens are a row of 128 bytes.  Keys: piece u is tokens 8u..; the transposing reads of 16 lanes take 32 bytes of four
+// consecutive channels, writes 16 of eight.  Values: piece 4 * kk + r is tokens 32 * kk + 4 * r.. and 32 * kk + 16 + 4 * r.., the ones whose
+// weights a lane of quarter r has; reads take 16 bytes of sixteen channels.
+// Few rows: two channels' 32 tokens are 128 bytes, piece u of either is tokens 8u..
+__device__ __forceinline__ int few_piece(int c, int u) { return (c >> 1) * 256 + ((((c & 1) << 2 | u) ^ (c & 2) ^ (c >> 2 & 1)) << 4); }
+template <bool FEW> __device__ __forceinline__ int key_piece(int c, int u)
+{
+    return FEW ? few_piece(c, u) : c * 128 + ((u ^ (c & 3) << 1 ^ (c >> 2 & 1)) << 4);
+}
+template <bool FEW> __device__ __forceinline__ int value_piece(int c, int u) { return FEW ? few_piece(c, u) : c * 128 + ((u ^ (c >> 1 & 7)) << 4); }
 
 template <bool MAX>
 __device__ __forceinline__ float fold_quarters(float v) // over the lanes l % 16
@@ -85,356 +207,8 @@ __device__ __forceinline__ float fold_quarters(float v) // over the lanes l % 16
     return MAX ? fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y)) : __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y);
 }
 
-// ---------------------------------------------------------------------------------------------------------------- producers
-// A wave replays 64 channels of K or V, one per lane, a tile at a time.
-template <int BITS>
-struct Producer {
-    static constexpr int WPT = TILE * BITS / 32; // words of a channel per tile
-    static constexpr int UPW = 32 / BITS / 8;    // units of eight tokens per word
-    Lone st;
-    __amdgpu_buffer_rsrc_t codes; // reads behind the last word of the piece are dropped
-    int next, c, left;            // tokens that are left of the piece
-    uint32_t buf[2][WPT];
-
-    __device__ __forceinline__ void start(const Tensor &t, const Source &s, int unit, int h, int channel, int first, int t1)
-    {
-        c = channel;
-        const int t0 = first * s.interval, pi = h * D + c;
-        left = t1 - t0;
-        const int words = (left + 32 / BITS - 1) / (32 / BITS);
-        codes = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint32_t *>(t.codes) + ((size_t)unit * s.n_super + t0 / (32 / BITS)) * D, 0,
-                                                  words * D * 4, 0x00027000);
-        next = c * 4;
-        h1 zp = t.zp[pi], sc = t.sc[pi];
-        if (first > 0) {
-            const h2 r = as_h2(*reinterpret_cast<const uint32_t *>(t.ckpt + (((size_t)unit * s.n_ckpt + first - 1) * D + c) * 2));
-            zp = r.x;
-            sc = r.y;
-        }
-        const h1 one = (h1)1.0f, be = t.be[pi], bt = be * t.tg[pi]; // omt = 1 - beta*target, both steps rounded
-        st.z = as_u32((h2){zp, (h1)0.0f});
-        st.r = as_u32((h2){(h1)0.0f, sc});
-        st.ca = as_u32((h2){t.al[pi], one});
-        st.cf = as_u32((h2){one, be});
-        st.c0 = as_u32((h2){(h1)0.0f, one - bt});
-        load(buf[0]);
-        load(buf[1]);
-    }
-    __device__ __forceinline__ void load(uint32_t *b)
-    {
-#pragma unroll
-        for (int i = 0; i < WPT; i++)
-            b[i] = __builtin_amdgcn_raw_buffer_load_b32(codes, next + i * D * 4, 0, 0);
-        next += WPT * D * 4;
-    }
-    // the next tile from the words of buffer I, which then take those of the tile after the next
-    template <int I>
-    __device__ __forceinline__ void tile(const uint2 *lut, uint32_t lane_copy, char *to)
-    {
-        uint2 e[2][4];
-        lone_lookup<BITS>(e[0], lut, buf[I], 0, lane_copy);
-#pragma unroll
-        for (int u = 0; u < TILE / 8; u++) {
-            if (u + 1 < TILE / 8)
-                lone_lookup<BITS>(e[(u & 1) ^ 1], lut, buf[I], u + 1, lane_copy);
-            __builtin_amdgcn_sched_barrier(0);
-            uint32_t x[4];
-            lone_eight(st, e[u & 1], x);
-            if (left < (u + 1) * 8) { // values behind the last token are zero: their weights are, and the rest may be anything
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int n = left - u * 8 - 2 * k;
-                    x[k] = n >= 2 ? x[k] : n == 1 ? x[k] & 0xFFFFu : 0u;
-                }
-            }
-            *reinterpret_cast<uint4 *>(to + piece_of(c, u)) = make_uint4(x[0], x[1], x[2], x[3]);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        left -= TILE;
-        load(buf[I]);
-    }
-};
-
-// ---------------------------------------------------------------------------------------------------------------- consumers
-template <int DT>
-__device__ __forceinline__ float widen(uint32_t v)
+__device__ __forceinline__ void store_four(h1 *to, f4v v, int act_bf16)
 {
-    return DT == ADKV_DT_F32 ? __uint_as_float(v) : DT == ADKV_DT_F16 ? (float)__builtin_bit_cast(h1, (uint16_t)v) : __uint_as_float(v << 16);
-}
-// a mask row at the 8 tokens from t on, of which `there` are in the source
-template <int DT>
-__device__ __forceinline__ f8v mask_eight(const char *row, int t, int there)
-{
-    constexpr int SIZE = DT == ADKV_DT_F32 ? 4 : 2;
-    const char *p = row + (long)t * SIZE;
-    f8v m = {};
-    if (there >= 8) {
-        if constexpr (SIZE == 4) {
-            __builtin_memcpy(&m, p, 32);
-        } else {
-            uint4 u;
-            __builtin_memcpy(&u, p, 16);
-            m = (f8v){widen<DT>(u.x & 0xFFFFu), widen<DT>(u.x >> 16), widen<DT>(u.y & 0xFFFFu), widen<DT>(u.y >> 16),
-                      widen<DT>(u.z & 0xFFFFu), widen<DT>(u.z >> 16), widen<DT>(u.w & 0xFFFFu), widen<DT>(u.w >> 16)};
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-            if (e < there)
-                m[e] = widen<DT>(SIZE == 4 ? reinterpret_cast<const uint32_t *>(p)[e] : reinterpret_cast<const uint16_t *>(p)[e]);
-    }
-    return m;
-}
-
-// NB blocks of 16 query rows.  Scores come as columns (lane l: row l % 16, tokens 8 * (l / 16) + 0..7 of every 32), which is as the
-// weights are taken by the product with V; the outputs are columns too, so that a row's maximum and sum are its lanes' own.
-template <int NB>
-struct Consumer {
-    h8v q[NB][4];
-    f4v o[NB][8];
-    float m[NB], l[NB];
-    long out[NB];         // the row among all rows, -1: none
-    int limit[NB];        // tokens of the source that it looks at
-    const char *mask[NB]; // its mask at the source's first token
-
-    __device__ __forceinline__ void start(const Args &a, const Source &s, bool prefix, int unit, int first_block, int step, int lane)
-    {
-        const int r16 = lane & 15, quarter = lane >> 4;
-#pragma unroll
-        for (int k = 0; k < NB; k++) {
-            const int row = (first_block + k * step) * 16 + r16, r = min(row, s.rows - 1);
-            const int g = r % a.G, token = r / a.G;
-            const int b = prefix ? token / a.n : unit / a.H, i = prefix ? token % a.n : token, h = prefix ? unit : unit % a.H;
-            const int hq = h * a.G + g;
-            out[k] = row < s.rows ? ((long)b * a.n + i) * (a.H * a.G) + hq : -1;
-            limit[k] = s.causal ? s.seen + i : s.seen;
-            const h1 *src = a.q + b * a.q_sb + hq * a.q_sh + i * a.q_st + quarter * 8;
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                uint4 u;
-                __builtin_memcpy(&u, src + c * 32, 16);
-                if (a.act_bf16)
-                    u = make_uint4(as_u32(act2(u.x, 1)), as_u32(act2(u.y, 1)), as_u32(act2(u.z, 1)), as_u32(act2(u.w, 1)));
-                q[k][c] = __builtin_bit_cast(h8v, u);
-            }
-            mask[k] = nullptr;
-            if (a.mask != nullptr)
-                mask[k] = (const char *)a.mask + (b * a.m_sb + hq * a.m_sh + i * a.m_st + s.col) * (a.mask_dt == ADKV_DT_F32 ? 4 : 2);
-            m[k] = -INFINITY;
-            l[k] = 0.0f;
-#pragma unroll
-            for (int c = 0; c < 8; c++)
-                o[k][c] = (f4v){0.0f, 0.0f, 0.0f, 0.0f};
-        }
-    }
-
-    // the tile of the tokens from t on
-    __device__ __forceinline__ void tile(const char *keys, const char *values, int t, const Args &a, const Source &s, int lane)
-    {
-        typedef short s4v __attribute__((ext_vector_type(4)));
-        typedef __attribute__((address_space(3))) s4v *Lds;
-        const int r16 = lane & 15, quarter = lane >> 4;
-        f4v sc[NB][2][2];
-        // Block j of 16 keys out of 32: row m is token 8 * (m / 4) + 4 * j + m % 4, so that a lane gets eight consecutive ones of both
-        // blocks.  A transposing read hands 16 lanes 4 channels of their tokens: lane i reads channel i / 4, the tokens of chunk i % 4.
-        const auto kbase = (__attribute__((address_space(3))) const char *)keys;
-#pragma unroll
-        for (int kk = 0; kk < 2; kk++) {
-            int at[2];
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-                at[i] = piece_of(quarter * 8 + i * 4 + (r16 >> 2), kk * 4 + (r16 & 3));
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-#pragma unroll
-                for (int k = 0; k < NB; k++)
-                    sc[k][kk][j] = (f4v){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const s4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(kbase + at[0] + c * 32 * TILE * 2 + j * 8));
-                    const s4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(kbase + at[1] + c * 32 * TILE * 2 + j * 8));
-                    const uint2 u = __builtin_bit_cast(uint2, x), v = __builtin_bit_cast(uint2, y);
-                    const h8v key = __builtin_bit_cast(h8v, make_uint4(u.x, u.y, v.x, v.y));
-#pragma unroll
-                    for (int k = 0; k < NB; k++)
-                        sc[k][kk][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, q[k][c], sc[k][kk][j], 0, 0, 0);
-                }
-            }
-        }
-        h8v w[NB][2];
-#pragma unroll
-        for (int k = 0; k < NB; k++) {
-            float x[16];
-#pragma unroll
-            for (int e = 0; e < 16; e++)
-                x[e] = sc[k][e >> 3][e >> 2 & 1][e & 3] * a.scaling;
-            if (a.mask != nullptr) {
-#pragma unroll
-                for (int kk = 0; kk < 2; kk++) {
-                    const int at = t + kk * 32 + quarter * 8;
-                    const f8v add = a.mask_dt == ADKV_DT_F32   ? mask_eight<ADKV_DT_F32>(mask[k], at, s.tokens - at)
-                                    : a.mask_dt == ADKV_DT_F16 ? mask_eight<ADKV_DT_F16>(mask[k], at, s.tokens - at)
-                                                               : mask_eight<ADKV_DT_BF16>(mask[k], at, s.tokens - at);
-#pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        x[kk * 8 + e] += add[e];
-                }
-            }
-            if (t + TILE > s.seen) {
-#pragma unroll
-                for (int e = 0; e < 16; e++)
-                    x[e] = t + (e >> 3) * 32 + quarter * 8 + (e & 7) < limit[k] ? x[e] : -INFINITY;
-            }
-            float mx = x[0];
-#pragma unroll
-            for (int e = 1; e < 16; e++)
-                mx = fmaxf(mx, x[e]);
-            mx = fmaxf(m[k], fold_quarters<true>(mx));
-            if (__any(mx > m[k])) {
-                const float shrink = m[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[k] - mx) * LOG2E);
-                m[k] = mx;
-                l[k] *= shrink;
-#pragma unroll
-                for (int c = 0; c < 8; c++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        o[k][c][e] *= shrink;
-            }
-            const float ref = mx == -INFINITY ? 0.0f : mx; // nothing but -inf so far: all weights are zero
-            float sum = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                x[e] = __builtin_amdgcn_exp2f((x[e] - ref) * LOG2E);
-                sum += x[e];
-            }
-            l[k] += sum;
-#pragma unroll
-            for (int kk = 0; kk < 2; kk++) {
-                uint32_t p[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    p[e] = as_u32((h2){(h1)x[kk * 8 + 2 * e], (h1)x[kk * 8 + 2 * e + 1]});
-                w[k][kk] = __builtin_bit_cast(h8v, make_uint4(p[0], p[1], p[2], p[3]));
-            }
-        }
-#pragma unroll
-        for (int kk = 0; kk < 2; kk++)
-#pragma unroll
-            for (int c = 0; c < 8; c++) {
-                const h8v v = *reinterpret_cast<const h8v *>(values + c * 16 * TILE * 2 + piece_of(r16, kk * 4 + quarter));
-#pragma unroll
-                for (int k = 0; k < NB; k++)
-                    o[k][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, w[k][kk], o[k][c], 0, 0, 0);
-            }
-    }
-
-    __device__ __forceinline__ void finish(const Args &a, int piece, int lane)
-    {
-#pragma unroll
-        for (int k = 0; k < NB; k++) {
-            const float sum = fold_quarters<false>(l[k]);
-            if (out[k] < 0)
-                continue;
-            const long at = piece * a.rows + out[k];
-            if (lane < 16)
-                a.ml[at] = make_float2(m[k], sum);
-#pragma unroll
-            for (int c = 0; c < 8; c++)
-                *reinterpret_cast<f4v *>(a.partial + at * D + c * 16 + (lane >> 4) * 4) = o[k][c];
-        }
-    }
-};
-
-// Four waves replay the tile after the one that the other four multiply with: a wave of either kind per SIMD, two buffers, a
-// barrier per tile.
-template <int BITS, int NB>
-__global__ __launch_bounds__(THREADS) void attend_kernel(Args a)
-{
-    // the table at LDS offset 0; two buffers of a K and a V tile
-    __shared__ uint4 smem[(LUT_WORDS64 * 8 + 4 * TILE_BYTES) / 16];
-    uint2 *lut = reinterpret_cast<uint2 *>(smem);
-    char *tiles = reinterpret_cast<char *>(smem) + LUT_WORDS64 * 8;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const bool prefix = (int)blockIdx.x < a.s[0].items;
-    const Source &s = a.s[prefix ? 0 : 1];
-    int item = (int)blockIdx.x - (prefix ? 0 : a.s[0].items);
-    const int block = item % s.blocks;
-    item /= s.blocks;
-    const int seg = item % s.nseg, unit = item / s.nseg;
-    const int first = (int)((long)s.intervals * seg / s.nseg), end = (int)((long)s.intervals * (seg + 1) / s.nseg);
-    const int t0 = first * s.interval, t1 = seg == s.nseg - 1 ? s.tokens : end * s.interval;
-    const int ntiles = (t1 - t0 + TILE - 1) / TILE;
-
-    if (wave < PRODUCERS) {
-        Producer<BITS> p;
-        p.start(s.t[wave >> 1], s, unit, prefix ? unit : unit % a.H, (wave & 1) * 64 + lane, first, t1);
-        if constexpr (BITS == 4)
-            lone_fill<THREADS>(lut, threadIdx.x);
-        else
-            lone_fill2<THREADS>(lut, threadIdx.x);
-        __syncthreads();
-        const uint32_t lane_copy = BITS == 4 ? (uint32_t)(lane & (LUT_COPIES - 1)) * 8u : (uint32_t)(lane & (LUT2_COPIES - 1)) * 16u;
-        char *to = tiles + (wave >> 1) * TILE_BYTES;
-        for (int i = 0; i <= ntiles; i += 2) { // one more than there are: the last pair of buffers is multiplied meanwhile
-            if (i < ntiles)
-                p.template tile<0>(lut, lane_copy, to);
-            __syncthreads();
-            if (i == ntiles)
-                break;
-            if (i + 1 < ntiles)
-                p.template tile<1>(lut, lane_copy, to + 2 * TILE_BYTES);
-            __syncthreads();
-        }
-    } else {
-        const int mine = block * (NB * CONSUMERS) + wave - PRODUCERS;      // blocks of 16 rows: this one, and CONSUMERS further
-        const int there = (s.rows + 15) / 16 - mine;
-        const bool any = there > 0;
-        Consumer<NB> c;
-        if (any)
-            c.start(a, s, prefix, unit, mine, CONSUMERS, lane);
-        if constexpr (BITS == 4)
-            lone_fill<THREADS>(lut, threadIdx.x);
-        else
-            lone_fill2<THREADS>(lut, threadIdx.x);
-        __syncthreads();
-        for (int i = 0; i < ntiles; i++) {
-            __syncthreads();
-            const char *from = tiles + (i & 1) * 2 * TILE_BYTES;
-            if (any)
-                c.tile(from, from + TILE_BYTES, t0 + i * TILE, a, s, lane);
-        }
-        __syncthreads();
-        if (any)
-            c.finish(a, s.piece + seg, lane);
-    }
-}
-
-// out = sum e^(m-M) o / sum e^(m-M) l over the pieces, in their order.  Four channels per lane; bound by reading the partial outputs.
-__global__ __launch_bounds__(256) void join_kernel(const float *__restrict__ partial, const float2 *__restrict__ ml, h1 *__restrict__ out,
-                                                   long rows, int pieces, int act_bf16)
-{
-    const long row = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int c = (threadIdx.x & 31) * 4;
-    if (row >= rows)
-        return;
-    float M = -INFINITY;
-    for (int k = 0; k < pieces; k++)
-        M = fmaxf(M, ml[k * rows + row].x);
-    const float ref = M == -INFINITY ? 0.0f : M; // a row whose mask leaves nothing: 0 / 0
-    float L = 0.0f;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int k = 0; k < pieces; k++) {
-        const float2 p = ml[k * rows + row];
-        const float e = __builtin_amdgcn_exp2f((p.x - ref) * LOG2E);
-        const float4 v = *reinterpret_cast<const float4 *>(partial + (k * rows + row) * D + c);
-        L = __builtin_fmaf(p.y, e, L);
-        o.x = __builtin_fmaf(v.x, e, o.x);
-        o.y = __builtin_fmaf(v.y, e, o.y);
-        o.z = __builtin_fmaf(v.z, e, o.z);
-        o.w = __builtin_fmaf(v.w, e, o.w);
-    }
-    const float inv = 1.0f / L;
-    const float r[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
     uint32_t w[2];
 #pragma unroll
     for (int i = 0; i < 2; i++) {
@@ -442,15 +216,678 @@ __global__ __launch_bounds__(256) void join_kernel(const float *__restrict__ par
             uint32_t b[2];
 #pragma unroll
             for (int k = 0; k < 2; k++) { // to nearest even, from fp32
-                const uint32_t u = __float_as_uint(r[2 * i + k]);
+                const uint32_t u = __float_as_uint(v[2 * i + k]);
                 b[k] = (u & 0x7FFFFFFFu) > 0x7F800000u ? 0x7FC0u : (u + 0x7FFFu + (u >> 16 & 1u)) >> 16;
             }
             w[i] = b[0] | b[1] << 16;
         } else {
-            w[i] = as_u32((h2){(h1)r[2 * i], (h1)r[2 * i + 1]});
+            w[i] = as_u32((h2){(h1)v[2 * i], (h1)v[2 * i + 1]});
         }
     }
-    *reinterpret_cast<uint2 *>(out + row * D + c) = make_uint2(w[0], w[1]);
+    typedef uint32_t u2v __attribute__((ext_vector_type(2)));
+    *(__attribute__((address_space(1))) u2v *)to = (u2v){w[0], w[1]};
+}
+
+// ---------------------------------------------------------------------------------------------------------------- producers
+// A wave replays 64 channels of K or V, one per lane, a tile at a time.
+
+// Where a span's loads are
+struct Feed {
+    const uint32_t *codes, *ck;
+    const h1 *zp, *sc, *al, *be, *tg;
+    const uint16_t *x;
+    int bytes;
+    template <int BITS, int TILE> __device__ __forceinline__ void open(KArgs &a, const Walk<TILE> &at, int kind)
+    {
+        const Extent s = all_of(a.s[at.src].x);
+        const Tensor t = all_of(a.s[at.src].t[kind]);
+        const int unit = at.code_unit(a);
+        constexpr int TPW = 32 / BITS;
+        codes = t.codes + ((size_t)unit * s.n_super + at.t0 / TPW) * D;
+        bytes = (at.t1 - at.t0 + TPW - 1) / TPW * (D * 4);
+        // the first span has no checkpoint: any word will do
+        ck = at.first > 0 ? reinterpret_cast<const uint32_t *>(t.ckpt) + ((size_t)unit * s.n_ckpt + at.first - 1) * D : codes;
+        zp = t.zp + at.h * D;
+        sc = t.sc + at.h * D;
+        al = t.al + at.h * D;
+        be = t.be + at.h * D;
+        tg = t.tg + at.h * D;
+        x = a.x[kind] + at.b * a.x_sb[kind] + at.h * a.x_sh[kind];
+    }
+};
+
+// What a tile needs from memory, loaded two tiles ahead.  There is no condition around the loads of the words: the compiler would wait for every load
+// in flight behind one.  (With words loaded behind each whole tile, and none behind the last one of an item, a tile of 64 tokens took 2.4 us, the
+// memory's latency.)
+template <int BITS, int TILE>
+struct Loads {
+    static constexpr int WPT = TILE * BITS / 32; // words of a channel per tile
+    uint32_t w[WPT], ck;
+    h1 zp, sc, al, be, tg;
+    uint16_t fresh;
+
+    __device__ __forceinline__ void start(const Feed &f, int k, int c)
+    {
+        // reads behind the last word of the span are dropped
+        const auto codes = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint32_t *>(f.codes), 0, f.bytes, 0x00027000);
+        const int next = (k * WPT * D + c) * 4;
+#pragma unroll
+        for (int i = 0; i < WPT; i++)
+            w[i] = __builtin_amdgcn_raw_buffer_load_b32(codes, next + i * D * 4, 0, 0);
+        if (k > 0)
+            return;
+        ck = global(f.ck)[c];
+        zp = global(f.zp)[c];
+        sc = global(f.sc)[c];
+        al = global(f.al)[c];
+        be = global(f.be)[c];
+        tg = global(f.tg)[c];
+        fresh = global(f.x)[c];
+    }
+    __device__ __forceinline__ Lone state(bool from_ckpt) const
+    {
+        const h2 f = from_ckpt ? as_h2(ck) : (h2){zp, sc};
+        const h1 one = (h1)1.0f, bt = be * tg; // omt = 1 - beta*target, both steps rounded
+        Lone st;
+        st.z = as_u32((h2){f.x, (h1)0.0f});
+        st.r = as_u32((h2){(h1)0.0f, f.y});
+        st.ca = as_u32((h2){al, one});
+        st.cf = as_u32((h2){one, be});
+        st.c0 = as_u32((h2){(h1)0.0f, one - bt});
+        return st;
+    }
+};
+
+template <bool KEYS, bool FEW>
+__device__ __forceinline__ void put_unit(char *to, int c, int u, const uint32_t *x)
+{
+    if constexpr (KEYS || FEW) {
+        *reinterpret_cast<uint4 *>(to + key_piece<FEW>(c, u)) = make_uint4(x[0], x[1], x[2], x[3]);
+    } else {
+        const int piece = u / 4 * 4 + u % 2 * 2, half = u / 2 % 2 * 8;
+        *reinterpret_cast<uint2 *>(to + value_piece<false>(c, piece) + half) = make_uint2(x[0], x[1]);
+        *reinterpret_cast<uint2 *>(to + value_piece<false>(c, piece + 1) + half) = make_uint2(x[2], x[3]);
+    }
+}
+
+// a whole tile from the words w
+template <int BITS, bool KEYS, bool FEW>
+__device__ __forceinline__ void whole_tile(Lone &st, const uint32_t *w, const uint2 *lut, uint32_t lane_copy, char *to, int c)
+{
+    constexpr int TILE = Shape<FEW>::TILE;
+    uint2 e[2][4];
+    lone_lookup<BITS>(e[0], lut, w, 0, lane_copy);
+#pragma unroll
+    for (int u = 0; u < TILE / 8; u++) {
+        if (u + 1 < TILE / 8)
+            lone_lookup<BITS>(e[(u & 1) ^ 1], lut, w, u + 1, lane_copy);
+        __builtin_amdgcn_sched_barrier(0);
+        uint32_t x[4];
+        lone_eight(st, e[u & 1], x);
+        put_unit<KEYS, FEW>(to, c, u, x);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// The last tile of a span: n < TILE tokens, or n == TILE with the appended one among them.  What is behind them is zero: its weights
+// are, and the rest of a buffer may be anything.  append: the n-th token is new, the last of its stream.
+template <int BITS, bool KEYS, bool FEW>
+__device__ __forceinline__ void part_tile(Lone &st, const uint32_t *w, char *to, int c, int n, bool append, uint16_t fresh, KArgs &a,
+                                          const Walk<Shape<FEW>::TILE> &at)
+{
+    constexpr int TPW = 32 / BITS, TILE = Shape<FEW>::TILE;
+    for (int u = 0; u < TILE / 8; u++) {
+        uint32_t x[4] = {};
+        if (u * 8 < n) {
+            uint32_t word = 0;
+#pragma unroll
+            for (int k = 0; k < TILE / TPW; k++)
+                word = u * 8 / TPW == k ? w[k] : word;
+            word >>= u * 8 % TPW * BITS;
+            const int there = min(n - u * 8 - (append ? 1 : 0), 8); // old ones
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (i < there)
+                    x[i >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, lone_token(st, (int)(word >> BITS * i & Code<BITS>::FIELD) + Code<BITS>::QLO))
+                                 << (i & 1) * 16;
+            if (append && there >= 0 && there < 8 && u * 8 + there == n - 1) {
+                const Extent s = all_of(a.s[1].x);
+                const Tensor t = all_of(a.s[1].t[KEYS ? 0 : 1]);
+                const int unit = at.code_unit(a), T = at.t1 - 1;
+                const auto ck = global(reinterpret_cast<uint32_t *>(const_cast<h1 *>(t.ckpt))) + (size_t)unit * s.n_ckpt * D + c;
+                // the state in front of token T, and behind it, where an interval ends there
+                const int j = s.interval > 0 ? T / s.interval : 0, rest = s.interval > 0 ? T - j * s.interval : 1;
+                if (rest == 0 && j > 0 && j <= s.n_ckpt)
+                    ck[(size_t)(j - 1) * D] = as_u32((h2){lone_zp(st), lone_sc(st)});
+                const int q = quantize<BITS>(act2(fresh, a.act_bf16).x, lone_zp(st), lone_sc(st));
+                const auto home = global(const_cast<uint32_t *>(t.codes)) + ((size_t)unit * s.n_super + T / TPW) * D + c;
+                const int sh = T % TPW * BITS;
+                uint32_t whole = 0;
+#pragma unroll
+                for (int k = 0; k < TILE / TPW; k++)
+                    whole = u * 8 / TPW == k ? w[k] : whole;
+                *home = (whole & ~(Code<BITS>::FIELD << sh)) | (uint32_t)(q - Code<BITS>::QLO) << sh;
+                const uint32_t v = (uint32_t)__builtin_bit_cast(uint16_t, lone_token(st, q)) << (there & 1) * 16;
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    x[k] |= there >> 1 == k ? v : 0u;
+                if (rest + 1 == s.interval && j < s.n_ckpt)
+                    ck[(size_t)j * D] = as_u32((h2){lone_zp(st), lone_sc(st)});
+            }
+        }
+        put_unit<KEYS, FEW>(to, c, u, x);
+    }
+}
+
+template <int BITS, bool KEYS, bool FEW>
+__device__ __forceinline__ void produce(KArgs &a, int items, const uint2 *lut, char *tiles, int c, int lane)
+{
+    using S = Shape<FEW>;
+    constexpr int KIND = KEYS ? 0 : 1, TILE = S::TILE, COPIES = (BITS == 4 ? LUT_COPIES : LUT2_COPIES) / (FEW ? 2 : 1);
+    const uint32_t lane_copy = (uint32_t)(lane & (COPIES - 1)) * (BITS == 4 ? 8u : 16u);
+    const int append_end = a.append ? a.s[1].x.tokens : -1;
+    Loads<BITS, TILE> ahead[2];
+    uint16_t fresh = 0;
+    Walk<TILE> at(a, items, blockIdx.x), then = at, next = at; // the tile, the one after it, the one whose loads go out next
+    Feed feed;
+    feed.open<BITS>(a, next, KIND);
+    auto step = [&]() __attribute__((always_inline)) {
+        if (next.last())
+            return; // the same again, never used
+        next.go(a);
+        if (next.k == 0)
+            feed.open<BITS>(a, next, KIND);
+    };
+    ahead[0].start(feed, next.k, c);
+    step();
+    then = next;
+    ahead[1].start(feed, next.k, c);
+    __syncthreads(); // the table
+    Lone st = {};
+    // returns whether that was the last
+    auto tile = [&](auto ic) __attribute__((always_inline)) {
+        constexpr int I = decltype(ic)::value;
+        const Loads<BITS, TILE> cur = ahead[I];
+        step();
+        ahead[I].start(feed, next.k, c);
+        if (at.k == 0) {
+            st = cur.state(at.first > 0);
+            fresh = cur.fresh;
+        }
+        char *to = tiles + I * S::BUFFER + (KEYS ? 0 : S::VALUES);
+        const int left = at.t1 - at.t0 - at.k * TILE;
+        const bool append = at.src && at.t1 == append_end;
+        if (left > TILE || (left == TILE && !append))
+            whole_tile<BITS, KEYS, FEW>(st, cur.w, lut, lane_copy, to, c);
+        else
+            part_tile<BITS, KEYS, FEW>(st, cur.w, to, c, left, append, fresh, a, at);
+        __syncthreads();
+        if (at.last())
+            return true;
+        at = then;
+        then = next;
+        return false;
+    };
+    while (!tile(std::integral_constant<int, 0>{}) && !tile(std::integral_constant<int, 1>{}))
+        ;
+}
+
+// ---------------------------------------------------------------------------------------------------------------- consumers
+// The mask of a lane's 4 * J tokens of a step, as it is in memory; rows are as aligned as their elements.
+template <int J, int MASK>
+struct MaskRaw {
+    static constexpr int WORDS = 2 * J * MASK; // MASK: 1 of 16 bits, 2 fp32
+    typedef uint32_t u2a __attribute__((ext_vector_type(2), aligned(2)));
+    typedef uint32_t u4a __attribute__((ext_vector_type(4), aligned(4)));
+    uint32_t w[WORDS];
+    // tokens t + 16 * i.. for i < J, of which `there` are in the source
+    __device__ __forceinline__ void load(const char *row, int t, int there)
+    {
+        const auto p = global(row + (long)t * (2 * MASK));
+        if (__all(there >= 16 * (J - 1) + 4)) {
+#pragma unroll
+            for (int i = 0; i < J; i++) {
+                if constexpr (MASK == 1) {
+                    const u2a u = *(const __attribute__((address_space(1))) u2a *)(p + i * 32);
+                    w[2 * i] = u.x;
+                    w[2 * i + 1] = u.y;
+                } else {
+                    const u4a u = *(const __attribute__((address_space(1))) u4a *)(p + i * 64);
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        w[4 * i + e] = u[e];
+                }
+            }
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < WORDS; e++)
+            w[e] = 0;
+#pragma unroll
+        for (int e = 0; e < 4 * J; e++) {
+            const int at = (e >> 2) * 16 + (e & 3);
+            if (at < there) {
+                if constexpr (MASK == 1)
+                    w[e >> 1] |= (uint32_t)((const __attribute__((address_space(1))) uint16_t *)p)[at] << (e & 1) * 16;
+                else
+                    w[e] = ((const __attribute__((address_space(1))) uint32_t *)p)[at];
+            }
+        }
+    }
+    // x = x * scaling + mask
+    __device__ __forceinline__ void add(float *x, float scaling, int dt) const
+    {
+        if constexpr (MASK == 2) {
+#pragma unroll
+            for (int e = 0; e < 4 * J; e++)
+                x[e] = __builtin_fmaf(x[e], scaling, __uint_as_float(w[e]));
+        } else if (dt == ADKV_DT_F16) {
+#pragma unroll
+            for (int e = 0; e < 2 * J; e++) {
+                x[2 * e] = __builtin_fmaf(x[2 * e], scaling, (float)as_h2(w[e]).x);
+                x[2 * e + 1] = __builtin_fmaf(x[2 * e + 1], scaling, (float)as_h2(w[e]).y);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 2 * J; e++) {
+                x[2 * e] = __builtin_fmaf(x[2 * e], scaling, __uint_as_float(w[e] << 16));
+                x[2 * e + 1] = __builtin_fmaf(x[2 * e + 1], scaling, __uint_as_float(w[e] & 0xFFFF0000u));
+            }
+        }
+    }
+};
+template <int J> struct MaskRaw<J, 0> {
+};
+
+// NB blocks of 16 query rows, J times 16 tokens a step.  Scores come as columns (lane l: row l % 16, of every 16 tokens 4 * (l / 16) + 0..3),
+// which is as the weights are taken by the product with V; the outputs are columns too, so that a row's maximum and sum are its lanes' own.
+// Without a mask scores are kept as q.K and the scaling is the exponent's: e^(scaling * (s - m)) is one multiply-add and an exp2.
+// MASK: 0 none, 1 of 16 bits, 2 fp32; m is then the largest of scaling * s + mask.
+template <int NB, int J, int MASK>
+struct Consumer {
+    static constexpr bool FEW = J == 1;
+    using W = Walk<Shape<FEW>::TILE>;
+    static constexpr int NC = FEW ? 4 : 8; // blocks of 16 channels of the outputs
+    h8v q[NB][4];
+    f4v o[NB][NC];
+    float m[NB], l[NB];
+    int row[NB];          // of the unit
+    int limit[NB];        // tokens of the source that it looks at
+    const char *mask[NB]; // its mask at the source's first token
+    int seen, tokens;     // of the source: what every row looks at, all
+    MaskRaw<J, MASK> masks[NB];
+
+    // of row r of a unit: sequence, token, query head
+    __device__ __forceinline__ static void place(KArgs &a, const W &at, int r, int &b, int &i, int &hq)
+    {
+        const int token = r >> a.log_g;
+        b = at.group ? at.b : divide(token, a.by_token);
+        i = at.group ? token : token - b * a.n;
+        hq = (at.h << a.log_g) + (r & ((1 << a.log_g) - 1));
+    }
+    // the queries' loads, of blocks `block`, block + stride..; ready() makes them what is multiplied
+    __device__ __forceinline__ static void load(KArgs &a, const W &at, int block, int stride, int lane, h8v (*to)[4])
+    {
+        const int rows = at.rows;
+#pragma unroll
+        for (int k = 0; k < NB; k++) {
+            int b, i, hq;
+            place(a, at, min((block + k * stride) * 16 + (lane & 15), rows - 1), b, i, hq);
+            const h1 *src = a.q + b * a.q_sb + hq * a.q_sh + i * a.q_st + (lane >> 4) * 8;
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                // rows are 4-byte aligned
+                typedef uint32_t u4a __attribute__((ext_vector_type(4), aligned(4)));
+                to[k][c] = __builtin_bit_cast(h8v, (u4v)*global(reinterpret_cast<const u4a *>(src + c * 32)));
+            }
+        }
+    }
+    __device__ __forceinline__ void ready(KArgs &a, const h8v (*from)[4])
+    {
+        const uint32_t sign = a.negate ? 0x80008000u : 0u;
+#pragma unroll
+        for (int k = 0; k < NB; k++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                uint4 u = __builtin_bit_cast(uint4, from[k][c]);
+                if (a.act_bf16)
+                    u = make_uint4(as_u32(act2(u.x, 1)), as_u32(act2(u.y, 1)), as_u32(act2(u.z, 1)), as_u32(act2(u.w, 1)));
+                q[k][c] = __builtin_bit_cast(h8v, make_uint4(u.x ^ sign, u.y ^ sign, u.z ^ sign, u.w ^ sign));
+            }
+    }
+    __device__ __forceinline__ void clear(KArgs &a, const W &at, int block, int stride, int lane)
+    {
+#pragma unroll
+        for (int k = 0; k < NB; k++) {
+            row[k] = (block + k * stride) * 16 + (lane & 15);
+            m[k] = -INFINITY;
+            l[k] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+                o[k][c] = (f4v){0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+    // what a row looks at of a span's source
+    __device__ __forceinline__ void look(KArgs &a, const W &at)
+    {
+        const Extent s = all_of(a.s[at.src].x);
+        seen = s.seen;
+        tokens = s.tokens;
+#pragma unroll
+        for (int k = 0; k < NB; k++) {
+            int b, i, hq;
+            place(a, at, min(row[k], at.rows - 1), b, i, hq);
+            limit[k] = s.causal ? s.seen + i : s.seen;
+            if constexpr (MASK != 0)
+                mask[k] = (const char *)a.mask + (b * a.m_sb + hq * a.m_sh + i * a.m_st + s.col) * (MASK == 2 ? 4 : 2);
+        }
+    }
+
+    // the mask of the tokens from t on
+    __device__ __forceinline__ void look_at(int t, int lane)
+    {
+        if constexpr (MASK != 0) {
+            t += (lane >> 4) * 4;
+#pragma unroll
+            for (int k = 0; k < NB; k++)
+                masks[k].load(mask[k], t, tokens - t);
+        }
+    }
+    // the scores of the step-th step of a tile, as q.K
+    __device__ __forceinline__ void scores(const char *keys, int step, int lane, f4v (*sc)[J])
+    {
+        typedef short s4v __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s4v *Lds;
+        const int r16 = lane & 15, quarter = lane >> 4;
+        // A transposing read hands 16 lanes four channels of 16 tokens: lane i reads channel i / 4, tokens 4 * (i % 4)..
+        const auto kbase = (__attribute__((address_space(3))) const char *)keys;
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            int at[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                at[i] = key_piece<FEW>(quarter * 8 + i * 4 + (r16 >> 2), (step * J + j) * 2 + (r16 >> 1 & 1)) + (r16 & 1) * 8;
+#pragma unroll
+            for (int k = 0; k < NB; k++)
+                sc[k][j] = (f4v){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const s4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(kbase + at[0] + c * 4096));
+                const s4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(kbase + at[1] + c * 4096));
+                const uint2 u = __builtin_bit_cast(uint2, x), v = __builtin_bit_cast(uint2, y);
+                const h8v key = __builtin_bit_cast(h8v, make_uint4(u.x, u.y, v.x, v.y));
+#pragma unroll
+                for (int k = 0; k < NB; k++)
+                    sc[k][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, q[k][c], sc[k][j], 0, 0, 0);
+            }
+        }
+    }
+
+    // scores of the tokens from t on to weights of fp16; the row's maximum, sum and outputs go along
+    __device__ __forceinline__ void weights(KArgs &a, int t, int lane, const f4v (*sc)[J], uint32_t (*w)[2 * J])
+    {
+        const int quarter = lane >> 4;
+#pragma unroll
+        for (int k = 0; k < NB; k++) {
+            float x[4 * J];
+#pragma unroll
+            for (int e = 0; e < 4 * J; e++)
+                x[e] = sc[k][e >> 2][e & 3];
+            if constexpr (MASK != 0)
+                masks[k].add(x, a.scaling, a.mask_dt);
+            if (t + 16 * J > seen) {
+#pragma unroll
+                for (int e = 0; e < 4 * J; e++)
+                    x[e] = t + (e >> 2) * 16 + quarter * 4 + (e & 3) < limit[k] ? x[e] : -INFINITY;
+            }
+            float mx = x[0];
+#pragma unroll
+            for (int e = 1; e < 4 * J; e++)
+                mx = fmaxf(mx, x[e]);
+            mx = fmaxf(m[k], fold_quarters<true>(mx));
+            const float c = MASK != 0 ? LOG2E : a.scaling * LOG2E;
+            if (__any(mx > m[k])) {
+                const float shrink = m[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[k] - mx) * c);
+                m[k] = mx;
+                l[k] *= shrink;
+#pragma unroll
+                for (int cc = 0; cc < NC; cc++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        o[k][cc][e] *= shrink;
+            }
+            const float ref = mx == -INFINITY ? 0.0f : mx; // nothing but -inf so far: all weights are zero
+            float sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4 * J; e++) {
+                // beside a mask the difference first: the largest may be as large as its type's lowest value
+                x[e] = __builtin_amdgcn_exp2f(MASK != 0 ? (x[e] - ref) * c : __builtin_fmaf(x[e], c, -ref * c));
+                sum += x[e];
+            }
+            l[k] += sum;
+#pragma unroll
+            for (int e = 0; e < 2 * J; e++)
+                w[k][e] = as_u32((h2){(h1)x[2 * e], (h1)x[2 * e + 1]});
+        }
+    }
+    // Half of a product's 32 tokens where a step has 16: the other half is zero on both sides.
+    __device__ __forceinline__ void outputs(const char *values, int step, int lane, const uint32_t (*w)[2 * J])
+    {
+#pragma unroll
+        for (int kk = 0; kk < (J + 1) / 2; kk++)
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                const int quarter = lane >> 4, piece = FEW ? step * 2 + (quarter >> 1) : (step * (J / 2) + kk) * 4 + quarter;
+                const char *p = values + c * 2048 + value_piece<FEW>(lane & 15, piece);
+                uint4 v;
+                if constexpr (FEW) {
+                    const uint2 half = *reinterpret_cast<const uint2 *>(p + (quarter & 1) * 8);
+                    v = make_uint4(half.x, half.y, 0, 0);
+                } else {
+                    v = *reinterpret_cast<const uint4 *>(p);
+                }
+#pragma unroll
+                for (int k = 0; k < NB; k++) {
+                    const uint4 p4 = FEW ? make_uint4(w[k][0], w[k][1], 0, 0) : make_uint4(w[k][kk * 4], w[k][kk * 4 + 1], w[k][kk * 4 + 2], w[k][kk * 4 + 3]);
+                    o[k][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8v, v), __builtin_bit_cast(h8v, p4), o[k][c], 0, 0, 0);
+                }
+            }
+    }
+
+    // part: of a piece's partial results; c0: the first block of channels
+    __device__ __forceinline__ void finish(KArgs &a, const W &at, int part, int c0, int lane)
+    {
+        const Group g = all_of(a.g[at.group]);
+#pragma unroll
+        for (int k = 0; k < NB; k++) {
+            const float sum = fold_quarters<false>(l[k]);
+            if (row[k] >= at.rows)
+                continue;
+            int b, i, hq;
+            place(a, at, row[k], b, i, hq);
+            const long r = ((long)b * a.n + i) * (a.H << a.log_g) + hq;
+            if (a.out != nullptr) {
+                const float inv = 1.0f / sum;
+#pragma unroll
+                for (int c = 0; c < NC; c++)
+                    store_four(a.out + r * D + (c0 + c) * 16 + (lane >> 4) * 4, o[k][c] * inv, a.act_bf16);
+                continue;
+            }
+            const long to = (g.piece + at.seg * g.split + part) * a.rows + r;
+            if (lane < 16 && c0 == 0)
+                *(__attribute__((address_space(1))) f2v *)global(a.ml + to) = (f2v){MASK != 0 || m[k] == -INFINITY ? m[k] : m[k] * a.scaling, sum};
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+                *(__attribute__((address_space(1))) f4v *)global(a.partial + to * D + (c0 + c) * 16 + (lane >> 4) * 4) = o[k][c];
+        }
+    }
+};
+
+// Few rows (at most 16): two pairs of waves multiply half of a tile's tokens each, with partial results of their own, a wave for half of the channels
+// of the outputs; both make the weights.  Else a wave has up to two
+// blocks of 16 rows out of a workgroup's sixteen, and all tokens.
+template <bool FEW, int MASK>
+__device__ __forceinline__ void consume(KArgs &a, int items, const char *tiles, int wave, int lane)
+{
+    using S = Shape<FEW>;
+    constexpr int NB = FEW ? 1 : 2, J = FEW ? 1 : 2, TILE = S::TILE, STEPS = FEW ? 1 : TILE / 32, WAVES = S::MULTIPLIERS;
+    using C = Consumer<NB, J, MASK>;
+    C c;
+    h8v spare[NB][4]; // few rows: the next item's queries, from this one's start on; else they take the present ones' registers
+    h8v(*const ahead)[4] = FEW ? spare : c.q;
+    typename C::W at(a, items, blockIdx.x), next = at; // next: the next item's first tile, once its queries are asked for
+    auto block = [&](const typename C::W &w) __attribute__((always_inline)) { return FEW ? 0 : w.block * (NB * WAVES) + wave; };
+    C::load(a, at, block(at), WAVES, lane, ahead);
+    c.ready(a, ahead);
+    __syncthreads(); // the table
+    bool opened = true; // at the item's first tile
+    auto tile = [&](auto ic) __attribute__((always_inline)) {
+        const char *from = tiles + decltype(ic)::value * S::BUFFER;
+        const bool ends = at.last_of_item(), more = at.more(), mine = block(at) * 16 < at.rows;
+        const int t = at.t0 + at.k * TILE;
+        if (opened) {
+            c.clear(a, at, block(at), WAVES, lane);
+            if (FEW && more) {
+                next = typename C::W(a, items, at.i + gridDim.x);
+                C::load(a, next, block(next), WAVES, lane, ahead);
+            }
+        }
+        if (at.k == 0)
+            c.look(a, at);
+        opened = ends;
+        if (mine)
+            c.look_at(t + (FEW ? (wave & 1) * 16 : 0), lane);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < STEPS; i++) {
+            const int step = FEW ? wave & 1 : i;
+            f4v sc[NB][J];
+            uint32_t w[NB][2 * J];
+            if (mine)
+                c.scores(from, step, lane, sc);
+            if (!FEW && i == STEPS - 1 && ends && more) { // the queries are done with: the next item's take their registers
+                next = typename C::W(a, items, at.i + gridDim.x);
+                C::load(a, next, block(next), WAVES, lane, ahead);
+            }
+            if (mine) {
+                c.weights(a, t + step * 16 * J, lane, sc, w);
+                if (i + 1 < STEPS)
+                    c.look_at(t + (step + 1) * 16 * J, lane);
+                c.outputs(from + S::VALUES + (FEW ? (wave >> 1) * 4 * 2048 : 0), step, lane, w);
+            }
+        }
+        if (ends) {
+            if (more)
+                c.ready(a, ahead); // in front of the stores, which it would wait for
+            if (mine)
+                c.finish(a, at, FEW ? wave & 1 : 0, FEW ? (wave >> 1) * 4 : 0, lane);
+            if (!more)
+                return true;
+            at = next;
+        } else {
+            at.go(a);
+        }
+        return false;
+    };
+    while (!tile(std::integral_constant<int, 0>{}) && !tile(std::integral_constant<int, 1>{}))
+        ;
+}
+
+// The code table with its copies in the first half of every 256 bytes (see Shape, lone_fill, lone_fill2)
+template <int BITS, int NT>
+__device__ __forceinline__ void fill_half(char *lds, int tid)
+{
+    for (int i = tid; i < LUT_ENTRIES * 8; i += NT) {
+        const int b = i >> 3;
+        const auto entry = [](int code) { return as_u32(splat((h1)(code - (BITS == 4 ? 8 : 2)))) & 0x7FFFFFFFu; };
+        uint4 v;
+        if constexpr (BITS == 4) {
+            const uint32_t x = entry(b & 15), y = entry(b >> 4);
+            v = make_uint4(x, y, x, y);
+        } else {
+            v = make_uint4(entry(b & 3), entry(b >> 2 & 3), entry(b >> 4 & 3), entry(b >> 6));
+        }
+        *reinterpret_cast<uint4 *>(lds + b * 256 + (i & 7) * 16) = v;
+    }
+}
+
+// Four waves replay the tile after the one that the others multiply with, one per SIMD, through two buffers and a barrier per tile.
+// A workgroup goes on to its next item without a gap.
+template <int BITS, bool FEW, int MASK>
+__global__ __launch_bounds__(Shape<FEW>::THREADS) void attend_kernel(Args)
+{
+    using S = Shape<FEW>;
+    KArgs &a = *(KArgs *)__builtin_amdgcn_kernarg_segment_ptr();
+    __shared__ uint4 smem[S::LDS / 16]; // the table at LDS offset 0
+    uint2 *lut = reinterpret_cast<uint2 *>(smem);
+    char *tiles = reinterpret_cast<char *>(smem) + S::FIRST;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int items = a.g[0].items + a.g[1].items;
+    if constexpr (FEW)
+        fill_half<BITS, S::THREADS>(reinterpret_cast<char *>(smem), threadIdx.x);
+    else if constexpr (BITS == 4)
+        lone_fill<S::THREADS>(lut, threadIdx.x);
+    else
+        lone_fill2<S::THREADS>(lut, threadIdx.x);
+    if (wave < 2)
+        produce<BITS, true, FEW>(a, items, lut, tiles, wave * 64 + lane, lane);
+    else if (wave < PRODUCERS)
+        produce<BITS, false, FEW>(a, items, lut, tiles, (wave - 2) * 64 + lane, lane);
+    else
+        consume<FEW, MASK>(a, items, tiles, wave - PRODUCERS, lane);
+}
+
+// out = sum e^(m-M) o / sum e^(m-M) l over the pieces.  Four channels per lane, 32 lanes per row, WAYS of them for a share of the
+// pieces each, in a fixed order: where rows are few the pieces are many and a lane that walks through all of them waits for each
+// (128 rows of 100 pieces 25 us, with WAYS = 8 %s).
+template <int WAYS>
+__global__ __launch_bounds__(256) void join_kernel(const float *__restrict__ partial, const float2 *__restrict__ ml, h1 *__restrict__ out,
+                                                   long rows, int pieces, int act_bf16)
+{
+    constexpr int ROWS = 8 / WAYS;
+    __shared__ f4v part[WAYS > 1 ? 256 : 1];
+    __shared__ f2v stat[WAYS > 1 ? 8 : 1];
+    const int group = threadIdx.x >> 5, way = group % WAYS, c = (threadIdx.x & 31) * 4;
+    const long row = min((long)blockIdx.x * ROWS + group / WAYS, rows - 1);
+    float M = -INFINITY;
+    for (int k = way; k < pieces; k += WAYS)
+        M = fmaxf(M, ml[k * rows + row].x);
+    if constexpr (WAYS > 1) {
+        if (c == 0)
+            stat[group].x = M;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < WAYS; i++)
+            M = fmaxf(M, stat[group / WAYS * WAYS + i].x);
+    }
+    const float ref = M == -INFINITY ? 0.0f : M; // a row whose mask leaves nothing: 0 / 0
+    float L = 0.0f;
+    f4v o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int k = way; k < pieces; k += WAYS) {
+        const float2 p = ml[k * rows + row];
+        const float e = __builtin_amdgcn_exp2f((p.x - ref) * LOG2E);
+        const f4v v = *reinterpret_cast<const f4v *>(partial + (k * rows + row) * D + c);
+        L = __builtin_fmaf(p.y, e, L);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            o[i] = __builtin_fmaf(v[i], e, o[i]);
+    }
+    if constexpr (WAYS > 1) {
+        part[threadIdx.x] = o;
+        if (c == 0)
+            stat[group].y = L;
+        __syncthreads();
+        if (way > 0)
+            return;
+#pragma unroll
+        for (int i = 1; i < WAYS; i++) {
+            L += stat[group + i].y;
+            o += part[threadIdx.x + i * 32];
+        }
+    }
+    if ((long)blockIdx.x * ROWS + group / WAYS < rows)
+        store_four(out + row * D + c, o * (1.0f / L), act_bf16);
 }
 
 // The state behind token T - 1 of every channel, from the last checkpoint in front of it: at most an interval, a token at a time.
@@ -459,10 +896,10 @@ template <int BITS>
 __global__ __launch_bounds__(128) void state_kernel(Source s, int H, int n_ckpt, h1 *k_state, h1 *v_state)
 {
     constexpr int TPW = 32 / BITS;
-    const int unit = blockIdx.x, c = threadIdx.x, pi = unit % H * D + c, T = s.tokens;
+    const int unit = blockIdx.x, c = threadIdx.x, pi = unit % H * D + c, T = s.x.tokens;
     const Tensor t = s.t[blockIdx.y];
     const h1 one = (h1)1.0f, be = t.be[pi], bt = be * t.tg[pi];
-    const int first = s.interval > 0 ? min((T - 1) / s.interval, n_ckpt) : 0;
+    const int first = s.x.interval > 0 ? min((T - 1) / s.x.interval, n_ckpt) : 0;
     h2 from = {t.zp[pi], t.sc[pi]};
     if (first > 0)
         from = as_h2(*reinterpret_cast<const uint32_t *>(t.ckpt + (((size_t)unit * n_ckpt + first - 1) * D + c) * 2));
@@ -472,70 +909,100 @@ __global__ __launch_bounds__(128) void state_kernel(Source s, int H, int n_ckpt,
     st.ca = as_u32((h2){t.al[pi], one});
     st.cf = as_u32((h2){one, be});
     st.c0 = as_u32((h2){(h1)0.0f, one - bt});
-    const uint32_t *w = t.codes + (size_t)unit * s.n_super * D + c;
-    for (int at = first * s.interval; at < T; at += TPW) {
-        const uint32_t word = w[(size_t)(at / TPW) * D];
+    const uint32_t *w = t.codes + (size_t)unit * s.x.n_super * D + c;
+    constexpr int AHEAD = 8;
+    uint32_t buf[2][AHEAD];
+    const int at0 = first * s.x.interval / TPW, words = (T + TPW - 1) / TPW;
+    auto load = [&](int at, uint32_t *b) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < TPW; i++)
-            if (at + i < T)
-                lone_token(st, (int)(word >> (BITS * i) & Code<BITS>::FIELD) + Code<BITS>::QLO);
+        for (int i = 0; i < AHEAD; i++)
+            b[i] = w[(size_t)min(at + i, words - 1) * D];
+    };
+    load(at0, buf[0]);
+    for (int at = at0; at < words; at += AHEAD) {
+        load(at + AHEAD, buf[1]);
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++)
+#pragma unroll
+            for (int k = 0; k < TPW; k++)
+                if ((at + i) * TPW + k < T)
+                    lone_token(st, (int)(buf[0][i] >> (BITS * k) & Code<BITS>::FIELD) + Code<BITS>::QLO);
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++)
+            buf[0][i] = buf[1][i];
     }
     const uint32_t zs = as_u32((h2){lone_zp(st), lone_sc(st)});
     *reinterpret_cast<uint32_t *>((blockIdx.y ? v_state : k_state) + ((size_t)unit * D + c) * 2) = zs;
-    if (s.interval > 0 && T % s.interval == 0 && T / s.interval - 1 < n_ckpt)
-        *reinterpret_cast<uint32_t *>(const_cast<h1 *>(t.ckpt) + (((size_t)unit * n_ckpt + T / s.interval - 1) * D + c) * 2) = zs;
+    if (s.x.interval > 0 && T % s.x.interval == 0 && T / s.x.interval - 1 < n_ckpt)
+        *reinterpret_cast<uint32_t *>(const_cast<h1 *>(t.ckpt) + (((size_t)unit * n_ckpt + T / s.x.interval - 1) * D + c) * 2) = zs;
 }
 
 struct Plan {
-    int nb;          // blocks of 16 rows per consumer wave
-    int nseg[2];     // pieces of the prefix (0: there is none) and of an own context
-    int intervals[2], blocks[2];
-    long pieces() const { return nseg[0] + nseg[1]; }
+    bool joint;      // the prefix is walked with the rows of each sequence by themselves
+    int launches;
+    bool few[2];     // of a launch
+    int groups[2];   // of a launch, a bit each
+    int nseg[2], blocks[2], split[2], intervals[2]; // of a group; intervals: of a source
+    long pieces() const { return (long)nseg[0] * split[0] + (long)nseg[1] * split[1]; }
 };
 
 static int usable_intervals(int tokens, int interval, int n_ckpt)
 {
-    return interval > 0 ? std::min((tokens + interval - 1) / interval, n_ckpt + 1) : 1;
+    return interval > 0 ? std::max(std::min((tokens + interval - 1) / interval, n_ckpt + 1), 1) : 1;
 }
 
-// A workgroup takes a CU.  The length of a piece is chosen for the shortest launch by the model rounds of workgroups x (tiles of a
-// piece + what a workgroup starts with).
+// Workgroups walk through items, one per CU, two for few rows.  Rows of a sequence that half fill a workgroup's 256 or more walk through the prefix
+// by themselves: it is replayed as often as with blocks of the whole batch's rows, and their outputs need no joining.  The length of a piece is
+// chosen for the shortest call by the model (us): a workgroup's items x (64 tokens of a piece x 1.6 or 2.5 + 1), and 4 TB/s for the partial results,
+// written and read.  T: the own tokens in front of the new ones.
 static Plan plan(int B, int H, int G, int n, int P, int p_interval, int p_ckpt, int T, int interval, int n_ckpt)
 {
-    Plan p;
+    Plan p = {};
     const long rows[2] = {(long)B * n * G, (long)n * G};
-    const int units[2] = {H, B * H}, tokens[2] = {P, T};
-    p.nb = std::max(P > 0 ? rows[0] : 0, rows[1]) > 16 * CONSUMERS ? 2 : 1;
+    p.joint = P > 0 && rows[1] >= 128;
+    const bool both = P > 0 && !p.joint, few[2] = {rows[0] <= 16, rows[1] <= 16};
     p.intervals[0] = P > 0 ? usable_intervals(P, p_interval, p_ckpt) : 0;
-    p.intervals[1] = usable_intervals(T, interval, n_ckpt);
-    for (int i = 0; i < 2; i++)
-        p.blocks[i] = (int)((rows[i] + 16 * CONSUMERS * p.nb - 1) / (16 * CONSUMERS * p.nb));
-    const long cus = cu_count();
-    double best = -1.0;
-    p.nseg[0] = p.nseg[1] = 1;
-    int chosen[2] = {p.intervals[0] ? 1 : 0, 1};
-    for (int len = 4; len < (1 << 20); len += std::max(len / 4, 1)) { // tiles
-        int ns[2];
-        long items = 0, longest = 0;
-        for (int i = 0; i < 2; i++) {
-            const long tiles = (tokens[i] + TILE - 1) / TILE;
-            ns[i] = (int)std::min<long>(p.intervals[i], (tiles + len - 1) / len);
-            ns[i] = p.intervals[i] ? std::max(ns[i], 1) : 0;
-            items += (long)units[i] * p.blocks[i] * ns[i];
-            if (ns[i])
-                longest = std::max(longest, (tiles + ns[i] - 1) / ns[i]);
+    // the state in front of a single new token may not be recorded yet
+    p.intervals[1] = usable_intervals(n == 1 ? T : T + n, interval, n_ckpt);
+    p.launches = both && few[0] != few[1] ? 2 : 1;
+    p.groups[0] = p.launches == 2 ? 1 : both ? 3 : 2;
+    p.groups[1] = 2;
+    p.few[0] = both ? few[0] : few[1];
+    p.few[1] = few[1];
+    const long units[2] = {H, (long)B * H}, total = (long)B * n * G * H;
+    const long tiles[2] = {(P + 63) / 64, (T + n + 63) / 64 + (p.joint ? (P + 63) / 64 : 0)};
+    const int intervals[2] = {p.intervals[0], p.intervals[1] + (p.joint ? p.intervals[0] : 0)};
+    for (int i = 0; i < p.launches; i++) {
+        const bool f = p.few[i];
+        const long slots = cu_count() * (f ? 2L : 1L);
+        double best = -1.0;
+        for (int len = 1; len < (1 << 20); len += std::max(len / 4, 1)) { // of 64 tokens
+            int ns[2] = {0, 0};
+            long items = 0, longest = 0, pieces = 0;
+            bool shortest = true;
+            for (int k = 0; k < 2; k++) {
+                if (!(p.groups[i] >> k & 1))
+                    continue;
+                p.blocks[k] = f ? 1 : (int)((rows[k] + 255) / 256);
+                p.split[k] = f ? 2 : 1;
+                ns[k] = (int)std::max<long>(std::min<long>(intervals[k], (tiles[k] + len - 1) / len), 1);
+                items += units[k] * p.blocks[k] * ns[k];
+                longest = std::max(longest, (tiles[k] + ns[k] - 1) / ns[k]);
+                pieces += (long)ns[k] * p.split[k];
+                shortest = shortest && ns[k] == 1;
+            }
+            const bool direct = pieces == 1 && p.launches == 1;
+            const double cost = (double)((items + slots - 1) / slots) * (longest * (f ? 1.6 : 2.5) + 1.0) + (direct ? 0.0 : 4.0 + pieces * total * 1024 / 4e6);
+            if (best < 0 || cost < best) {
+                best = cost;
+                for (int k = 0; k < 2; k++)
+                    if (p.groups[i] >> k & 1)
+                        p.nseg[k] = ns[k];
+            }
+            if (shortest)
+                break;
         }
-        const double cost = (double)((items + cus - 1) / cus) * (longest + 4) + 0.02 * (ns[0] + ns[1]);
-        if (best < 0 || cost < best) {
-            best = cost;
-            chosen[0] = ns[0];
-            chosen[1] = ns[1];
-        }
-        if (ns[0] <= 1 && ns[1] <= 1)
-            break;
     }
-    p.nseg[0] = chosen[0];
-    p.nseg[1] = chosen[1];
     return p;
 }
 
@@ -552,7 +1019,7 @@ int64_t adkv_extend_workspace_bytes(int B, int Hq, int H, int T, int n, int n_ck
 {
     if (B <= 0 || H <= 0 || Hq <= 0 || Hq % H || T < 0 || n <= 0 || P < 0 || T > MAX_TOKENS || n > MAX_TOKENS - T || P > MAX_TOKENS)
         return 0;
-    const Plan p = plan(B, H, Hq / H, n, P, prefix_n_ckpt_cap > 0 ? prefix_ckpt_interval : 0, prefix_n_ckpt_cap, T + n,
+    const Plan p = plan(B, H, Hq / H, n, P, prefix_n_ckpt_cap > 0 ? prefix_ckpt_interval : 0, prefix_n_ckpt_cap, T,
                         n_ckpt_cap > 0 ? ckpt_interval : 0, n_ckpt_cap);
     const int64_t rows = (int64_t)B * n * Hq;
     return 2 * pad256((int64_t)B * H * D * 4) + pad256(p.pieces() * rows * 8) + p.pieces() * rows * D * 4;
@@ -623,7 +1090,7 @@ int adkv_extend(const void *q, const int64_t *q_strides, void *k_cache, void *v_
     if (!workspace || workspace_bytes < need)
         return ADKV_E_WORKSPACE;
 
-    const Plan pl = plan(B, H, G, n, P, p_interval, p_cap, T + n, ckpt_interval, n_ckpt_cap);
+    const Plan pl = plan(B, H, G, n, P, p_interval, p_cap, T, ckpt_interval, n_ckpt_cap);
     char *ws = (char *)workspace;
     const int64_t state_bytes = pad256((int64_t)B * H * D * 4);
     h1 *k_state = (h1 *)ws, *v_state = (h1 *)(ws + state_bytes);
@@ -633,46 +1100,56 @@ int adkv_extend(const void *q, const int64_t *q_strides, void *k_cache, void *v_
     auto tensor = [](const void *codes, const void *ckpt, const void *const *p) {
         return Tensor{(const uint32_t *)codes, (const h1 *)ckpt, (const h1 *)p[0], (const h1 *)p[1], (const h1 *)p[2], (const h1 *)p[3], (const h1 *)p[4]};
     };
+    auto div = [](int64_t d) { return Div{(uint32_t)d, (uint32_t)(((1ull << 32) + d - 1) / d)}; };
     Source &pre = a.s[0], &own = a.s[1];
     pre = Source{};
     if (P > 0) {
         pre.t[0] = tensor(prefix->k_codes, prefix->k_ckpt, prefix->k_params);
         pre.t[1] = tensor(prefix->v_codes, prefix->v_ckpt, prefix->v_params);
-        pre.tokens = pre.seen = P;
-        pre.n_super = prefix->n_super;
-        pre.n_ckpt = p_cap;
-        pre.interval = p_interval;
-        pre.units = H;
-        pre.rows = (int)((int64_t)B * n * G);
+        pre.x.tokens = pre.x.seen = P;
+        pre.x.n_super = prefix->n_super;
+        pre.x.n_ckpt = p_cap;
+        pre.x.interval = p_interval;
+        pre.x.intervals = pl.intervals[0];
     }
+    own = Source{};
     own.t[0] = tensor(k_cache, k_ckpt, k_params);
     own.t[1] = tensor(v_cache, v_ckpt, v_params);
-    own.tokens = T + n;
-    own.seen = T + 1;
-    own.causal = 1;
-    own.n_super = n_super_cap;
-    own.n_ckpt = n_ckpt_cap;
-    own.interval = ckpt_interval;
-    own.units = B * H;
-    own.rows = n * G;
-    own.col = P;
-    own.piece = pl.nseg[0];
-    pre.causal = 0;
-    pre.col = pre.piece = 0;
-    int64_t items = 0;
+    own.x.tokens = T + n;
+    own.x.seen = T + 1;
+    own.x.causal = 1;
+    own.x.n_super = n_super_cap;
+    own.x.n_ckpt = n_ckpt_cap;
+    own.x.interval = ckpt_interval;
+    own.x.intervals = pl.intervals[1];
+    own.x.col = P;
+    Group groups[2] = {};
     for (int i = 0; i < 2; i++) {
-        Source &s = a.s[i];
-        s.intervals = pl.intervals[i];
-        s.nseg = pl.nseg[i];
-        s.blocks = pl.blocks[i];
-        const int64_t k = (int64_t)s.units * s.blocks * s.nseg;
-        if (k > INT32_MAX)
+        Group &g = groups[i];
+        if (pl.nseg[i] == 0)
+            continue;
+        g.units = i ? B * H : H;
+        g.blocks = pl.blocks[i];
+        g.nseg = pl.nseg[i];
+        g.rows = (int)(i ? (int64_t)n * G : (int64_t)B * n * G);
+        const int64_t items = (int64_t)g.units * g.blocks * g.nseg;
+        if (items * ((int64_t)g.blocks * g.nseg) >= 1ll << 32)
             return ADKV_E_SHAPE;
-        s.items = (int)k;
-        items += k;
+        g.items = (int)items;
+        g.from = i == 0 || pl.joint ? 0 : 1;
+        g.to = i;
+        const int intervals = (i == 0 || pl.joint ? pl.intervals[0] : 0) + (i ? pl.intervals[1] : 0);
+        g.per_piece = intervals / g.nseg;
+        g.longer = intervals % g.nseg;
+        g.piece = i ? pl.nseg[0] * pl.split[0] : 0;
+        g.split = pl.split[i];
+        g.by_unit = div((int64_t)g.blocks * g.nseg);
+        g.by_block = div(g.blocks);
     }
-    if (items > INT32_MAX)
+    if ((int64_t)B * H * H >= 1ll << 32 || (int64_t)B * n * n >= 1ll << 32)
         return ADKV_E_SHAPE;
+    a.by_head = div(H);
+    a.by_token = div(n);
     a.q = (const h1 *)q;
     a.q_sb = q_strides[0];
     a.q_sh = q_strides[1];
@@ -686,30 +1163,60 @@ int adkv_extend(const void *q, const int64_t *q_strides, void *k_cache, void *v_
     }
     a.mask_dt = mask_dt;
     a.rows = rows;
-    a.B = B;
     a.H = H;
-    a.G = G;
+    a.log_g = G == 1 ? 0 : G == 2 ? 1 : G == 4 ? 2 : 3;
     a.n = n;
     a.act_bf16 = act_dtype == ADKV_DT_BF16;
-    a.scaling = scaling;
+    // hidden tokens are -inf times it, which has to stay -inf: a scaling of zero is a small one
+    a.scaling = scaling == 0.0f ? 1e-30f : fabsf(scaling);
+    a.negate = scaling < 0.0f;
+    a.append = n == 1;
 
-    // the new tokens' codes
-    if (T > 0) {
-        Source before = own;
-        before.tokens = T;
-        const auto kernel = bits == 4 ? state_kernel<4> : state_kernel<2>;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(B * H), 2), dim3(D), 0, (hipStream_t)stream, before, H, n_ckpt_cap, k_state, v_state);
+    const int64_t *strides[2] = {k_strides, v_strides}; // as adkv_append_kv_pair has them
+    for (int i = 0; i < 2; i++) {
+        a.x[i] = (const uint16_t *)(i ? v_new : k_new);
+        a.x_sb[i] = strides[i] ? strides[i][0] : (int64_t)H * n * D;
+        a.x_sh[i] = strides[i] ? strides[i][1] : (int64_t)n * D;
+    }
+    if (n > 1) {
+        if (T > 0) {
+            Source before = own;
+            before.x.tokens = T;
+            const auto kernel = bits == 4 ? state_kernel<4> : state_kernel<2>;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)(B * H), 2), dim3(D), 0, (hipStream_t)stream, before, H, n_ckpt_cap, k_state, v_state);
+            if ((rc = check_launch()))
+                return rc;
+        }
+        if ((rc = adkv_append_kv_pair(k_cache, v_cache, k_new, v_new, act_dtype, k_strides, v_strides, k_params, v_params, B, H, T, n, D,
+                                      n_super_cap, bits, k_state, v_state, k_ckpt, v_ckpt, n_ckpt_cap, ckpt_interval, stream)))
+            return rc;
+    }
+    const bool direct = pl.pieces() == 1;
+    a.out = direct ? (h1 *)out : nullptr;
+    const int kind = !mask ? 0 : mask_dt == ADKV_DT_F32 ? 2 : 1;
+    typedef void (*Kernel)(Args);
+    static const Kernel kernels[2][2][3] = {
+        {{attend_kernel<4, false, 0>, attend_kernel<4, false, 1>, attend_kernel<4, false, 2>},
+         {attend_kernel<4, true, 0>, attend_kernel<4, true, 1>, attend_kernel<4, true, 2>}},
+        {{attend_kernel<2, false, 0>, attend_kernel<2, false, 1>, attend_kernel<2, false, 2>},
+         {attend_kernel<2, true, 0>, attend_kernel<2, true, 1>, attend_kernel<2, true, 2>}}};
+    for (int i = 0; i < pl.launches; i++) {
+        for (int k = 0; k < 2; k++) {
+            a.g[k] = groups[k];
+            if (!(pl.groups[i] >> k & 1))
+                a.g[k].items = 0;
+        }
+        const int64_t items = (int64_t)a.g[0].items + a.g[1].items;
+        hipLaunchKernelGGL(kernels[bits == 2][pl.few[i]][kind], dim3((unsigned)std::min<int64_t>(items, cu_count() * (pl.few[i] ? 2 : 1))),
+                           dim3(pl.few[i] ? Shape<true>::THREADS : Shape<false>::THREADS), 0, (hipStream_t)stream, a);
         if ((rc = check_launch()))
             return rc;
     }
-    if ((rc = adkv_append_kv_pair(k_cache, v_cache, k_new, v_new, act_dtype, k_strides, v_strides, k_params, v_params, B, H, T, n, D, n_super_cap,
-                                  bits, k_state, v_state, k_ckpt, v_ckpt, n_ckpt_cap, ckpt_interval, stream)))
-        return rc;
-    const auto kernel = bits == 4 ? (pl.nb == 2 ? attend_kernel<4, 2> : attend_kernel<4, 1>) : (pl.nb == 2 ? attend_kernel<2, 2> : attend_kernel<2, 1>);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)items), dim3(THREADS), 0, (hipStream_t)stream, a);
-    if ((rc = check_launch()))
-        return rc;
-    hipLaunchKernelGGL(join_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, (hipStream_t)stream, a.partial, a.ml, (h1 *)out, rows,
+    if (direct)
+        return ADKV_OK;
+    const auto join = rows <= 8192 && pl.pieces() >= 4 ? join_kernel<8> : join_kernel<1>;
+    const int64_t per = rows <= 8192 && pl.pieces() >= 4 ? 1 : 8;
+    hipLaunchKernelGGL(join, dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, (hipStream_t)stream, a.partial, a.ml, (h1 *)out, rows,
                        (int)pl.pieces(), a.act_bf16);
     return check_launch();
 }
