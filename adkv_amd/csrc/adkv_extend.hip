@@ -4,9 +4,17 @@
 //   x[i, t] = scaling * q_i . K_t + mask[i, t],  t over the P prefix tokens and the own tokens up to the query's;  out_i = sum softmax(x_i)_t V_t
 //
 // The prefix is replayed once for the batch and multiplied with the queries of all sequences as one matrix, so that its cost does not
-// grow with the batch but by matrix instructions.  The context of a KV head is cut at checkpoints into pieces, each of which leaves
+// grow with the batch but by matrix instructions.  The context of a KV head is cut into pieces, each of which leaves
 // (m, l, o) = (max x, sum e^(x-m), sum e^(x-m) V) per query row; pieces are joined by M = max m, out = sum e^(m-M) o / sum e^(m-M) l.
-// Scores, m, l, o are fp32; the weights e^(x-m) are rounded to fp16 for the matrix cores, relative to the largest so far.
+// Scores, m, l, o are fp32; the weights e^(x-m) are rounded to fp16 for the matrix cores, relative to the largest so far (or to one that
+// is at most 2^8 times smaller: see weights()).
+//
+// Two ways through the codes of a source, by the query rows of a unit (a KV head of the prefix with the rows of the whole batch, or of a
+// sequence with its own):
+//   at most 16 (few)   attend_kernel: the waves that replay hand tiles of values to waves that multiply, through the LDS
+//   more (many)        values_kernel writes the values to memory as tiles of fp16, attend_many_kernel reads them.  Replaying in the multiplying
+//                      workgroup takes as many issue slots as the softmax of 256 rows, once per 256 rows, and its LDS; 8 x 512
+//                      new tokens on a prefix of 4096, 32 heads, took 1000 us that way
 #include <math.h>
 
 #include <algorithm>
@@ -23,17 +31,16 @@ using namespace adkv;
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
 typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 typedef float f2v __attribute__((ext_vector_type(2)));
+typedef uint32_t u2v __attribute__((ext_vector_type(2)));
 
 constexpr int D = 128;
 constexpr int PRODUCERS = 4;
-// Two shapes of workgroup.  Many rows: tiles of 64 tokens, eight waves that multiply, one workgroup per CU.  Few rows (at most 16 per unit):
-// tiles of 32, four such waves, two workgroups per CU: a wave that replays alone on its SIMD uses half of the issue slots.
-template <bool FEW> struct Shape {
-    static constexpr int TILE = FEW ? 32 : 64, MULTIPLIERS = FEW ? 4 : 8, THREADS = 64 * (PRODUCERS + MULTIPLIERS);
-    // Many: the code table of 64 KB, two buffers of a K and a V tile of 16 KB each.  Few: half as many copies of the table's entries, in the first
-    // half of every 256 bytes of 64 KB, and the buffers, of 8 KB a tile, in the second halves.
-    static constexpr int BUFFER = 32768, VALUES = 16384, FIRST = FEW ? 128 : 65536, LDS = FEW ? 65536 : 131072;
-};
+// Few rows: tiles of 32 tokens, four waves that replay and four that multiply, two workgroups per CU: a wave that replays alone on its SIMD uses half
+// of the issue slots.  Of 64 KB of LDS the code table (half as many copies of its entries as elsewhere) has the first half of every 256 bytes, and two
+// buffers of a K and a V tile of 8 KB the second halves.
+constexpr int FEW_TILE = 32, FEW_THREADS = 512, FEW_BUFFER = 32768, FEW_VALUES = 16384, FEW_FIRST = 128, FEW_LDS = 65536;
+// Many rows: tiles of 64 tokens, 16 KB of keys and as many of values, three of them in the LDS; eight waves of up to 32 rows.
+constexpr int TILE = 64, TILE_BYTES = 32768, TILE_VALUES = 16384, MANY_THREADS = 512, MANY_ROWS = 256;
 constexpr int MAX_TOKENS = 1 << 24; // 64 bytes each: a piece's codes are addressed in 32 bits
 constexpr float LOG2E = 1.44269504088896340736f;
 
@@ -65,7 +72,7 @@ struct Div {
 // looks at the prefix; group 1 has the rows (token, query head) of a sequence and KV head and looks at its own codes, behind the prefix
 // if `joint`.  Its items: a block of rows with one piece of the checkpoint intervals.
 struct Group {
-    int units, blocks, nseg, rows, items;
+    int first_unit, blocks, nseg, rows, items;
     int from, to;          // sources
     int per_piece, longer; // intervals of a piece; the first `longer` ones have one more
     int piece, split;      // number of its first partial result; partial results per piece
@@ -73,13 +80,15 @@ struct Group {
 };
 
 struct Args {
-    Source s[2]; // prefix, own
+    Source s[2]; // prefix, own; many rows: the codes are tiles of values, of units from the group's first on, and intervals are tiles
     Group g[2];
     const h1 *q;
     long q_sb, q_sh, q_st;
     const void *mask;
     long m_sb, m_sh, m_st;
     int mask_dt;
+    const uint32_t *mask_bits; // see mask_tiles_kernel; may be null
+    int mask_words, mask_own_tile;
     float *partial; // [partial results, rows, D]
     float2 *ml;     // [partial results, rows]: m, l
     h1 *out;        // not null: a row has one partial result, and goes here
@@ -120,7 +129,7 @@ __device__ __forceinline__ __attribute__((address_space(1))) T *global(T *p) { r
 
 // The tiles of a workgroup, one after the other: those of an item's piece in one source, then in the other, then the next item's.  What
 // the arguments have of an item or a span is read when it is opened: a read per tile is a wait per tile.
-template <int TILE>
+template <int TOKENS>
 struct Walk {
     int i, group, b, h, block, seg, end; // item; end: interval behind its piece, counted over its sources
     int rows, prefix;                    // of the group; intervals of the prefix if the piece may begin there
@@ -133,8 +142,8 @@ struct Walk {
         group = i < a.g[0].items ? 0 : 1;
         const Group g = all_of(a.g[group]);
         int at = i - (group ? a.g[0].items : 0);
-        const int unit = divide(at, g.by_unit);
-        at -= unit * (g.blocks * g.nseg);
+        const int of_launch = divide(at, g.by_unit), unit = of_launch + g.first_unit;
+        at -= of_launch * (g.blocks * g.nseg);
         seg = divide(at, g.by_block);
         block = at - seg * g.blocks;
         b = group ? divide(unit, a.by_head) : 0;
@@ -154,7 +163,7 @@ struct Walk {
         t0 = first * s.interval;
         t1 = e >= s.intervals ? s.tokens : e * s.interval;
         k = 0;
-        n = (t1 - t0 + TILE - 1) / TILE;
+        n = (t1 - t0 + TOKENS - 1) / TOKENS;
         ends = src == 1 || end <= prefix;
     }
     __device__ __forceinline__ bool last_of_item() const { return k + 1 == n && ends; }
@@ -176,24 +185,22 @@ struct Walk {
 };
 
 // Where a tile's values are, in pieces of 16 bytes whose order changes with the channel so that what is accessed in one clock lies in different
-// banks.  32 channels are 4096 bytes, 16 are 2048, in either shape.
+// banks.  32 channels are 4096 bytes, 16 are 2048, in either kind of tile.
 // Many rows: a channel's 64 tokens are a row of 128 bytes.  Keys: piece u is tokens 8u..; the transposing reads of 16 lanes take 32 bytes of four
-// consecutive channels, writes 16 of eight.  Values: piece 4 * kk + r is tokens 32 * kk + 4 * r.. and 32 * kk + 16 + 4 * r.., the ones whose
-// weights a lane of quarter r has; reads take 16 bytes of sixteen channels.
+// consecutive channels.  Values: piece 4 * kk + r is tokens 32 * kk + 4 * r.. and 32 * kk + 16 + 4 * r.., the ones whose weights a lane of
+// quarter r has; reads take 16 bytes of sixteen channels.
 // Few rows: two channels' 32 tokens are 128 bytes, piece u of either is tokens 8u..
 __device__ __forceinline__ int few_piece(int c, int u) { return (c >> 1) * 256 + ((((c & 1) << 2 | u) ^ (c & 2) ^ (c >> 2 & 1)) << 4); }
-template <bool FEW> __device__ __forceinline__ int key_piece(int c, int u)
-{
-    return FEW ? few_piece(c, u) : c * 128 + ((u ^ (c & 3) << 1 ^ (c >> 2 & 1)) << 4);
-}
-template <bool FEW> __device__ __forceinline__ int value_piece(int c, int u) { return FEW ? few_piece(c, u) : c * 128 + ((u ^ (c >> 1 & 7)) << 4); }
+__device__ __forceinline__ int many_key_piece(int c, int u) { return c * 128 + ((u ^ (c & 3) << 1 ^ (c >> 2 & 1)) << 4); }
+__device__ __forceinline__ int many_value_piece(int c, int u) { return c * 128 + ((u ^ (c >> 1 & 7)) << 4); }
+template <bool FEW> __device__ __forceinline__ int key_piece(int c, int u) { return FEW ? few_piece(c, u) : many_key_piece(c, u); }
+template <bool FEW> __device__ __forceinline__ int value_piece(int c, int u) { return FEW ? few_piece(c, u) : many_value_piece(c, u); }
 
 template <bool MAX>
 __device__ __forceinline__ float fold_quarters(float v) // over the lanes l % 16
 {
     unsigned a = __builtin_bit_cast(unsigned, v), b;
     asm volatile("v_mov_b32 %0, %1" : "=v"(b) : "v"(a)); // two copies: the compiler folds a swap of a register with itself
-    typedef unsigned u2v __attribute__((ext_vector_type(2)));
     u2v r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
     unsigned x = r.x, y = r.y;
     asm volatile("" : "+v"(x), "+v"(y));
@@ -224,12 +231,23 @@ __device__ __forceinline__ void store_four(h1 *to, f4v v, int act_bf16)
             w[i] = as_u32((h2){(h1)v[2 * i], (h1)v[2 * i + 1]});
         }
     }
-    typedef uint32_t u2v __attribute__((ext_vector_type(2)));
     *(__attribute__((address_space(1))) u2v *)to = (u2v){w[0], w[1]};
 }
 
 // ---------------------------------------------------------------------------------------------------------------- producers
 // A wave replays 64 channels of K or V, one per lane, a tile at a time.
+
+__device__ __forceinline__ Lone state_of(h2 zp_sc, h1 al, h1 be, h1 tg)
+{
+    const h1 one = (h1)1.0f, bt = be * tg; // omt = 1 - beta*target, both steps rounded
+    Lone st;
+    st.z = as_u32((h2){zp_sc.x, (h1)0.0f});
+    st.r = as_u32((h2){(h1)0.0f, zp_sc.y});
+    st.ca = as_u32((h2){al, one});
+    st.cf = as_u32((h2){one, be});
+    st.c0 = as_u32((h2){(h1)0.0f, one - bt});
+    return st;
+}
 
 // Where a span's loads are
 struct Feed {
@@ -237,7 +255,7 @@ struct Feed {
     const h1 *zp, *sc, *al, *be, *tg;
     const uint16_t *x;
     int bytes;
-    template <int BITS, int TILE> __device__ __forceinline__ void open(KArgs &a, const Walk<TILE> &at, int kind)
+    template <int BITS> __device__ __forceinline__ void open(KArgs &a, const Walk<FEW_TILE> &at, int kind)
     {
         const Extent s = all_of(a.s[at.src].x);
         const Tensor t = all_of(a.s[at.src].t[kind]);
@@ -259,9 +277,9 @@ struct Feed {
 // What a tile needs from memory, loaded two tiles ahead.  There is no condition around the loads of the words: the compiler would wait for every load
 // in flight behind one.  (With words loaded behind each whole tile, and none behind the last one of an item, a tile of 64 tokens took 2.4 us, the
 // memory's latency.)
-template <int BITS, int TILE>
+template <int BITS>
 struct Loads {
-    static constexpr int WPT = TILE * BITS / 32; // words of a channel per tile
+    static constexpr int WPT = FEW_TILE * BITS / 32; // words of a channel per tile
     uint32_t w[WPT], ck;
     h1 zp, sc, al, be, tg;
     uint16_t fresh;
@@ -284,64 +302,45 @@ struct Loads {
         tg = global(f.tg)[c];
         fresh = global(f.x)[c];
     }
-    __device__ __forceinline__ Lone state(bool from_ckpt) const
-    {
-        const h2 f = from_ckpt ? as_h2(ck) : (h2){zp, sc};
-        const h1 one = (h1)1.0f, bt = be * tg; // omt = 1 - beta*target, both steps rounded
-        Lone st;
-        st.z = as_u32((h2){f.x, (h1)0.0f});
-        st.r = as_u32((h2){(h1)0.0f, f.y});
-        st.ca = as_u32((h2){al, one});
-        st.cf = as_u32((h2){one, be});
-        st.c0 = as_u32((h2){(h1)0.0f, one - bt});
-        return st;
-    }
+    __device__ __forceinline__ Lone state(bool from_ckpt) const { return state_of(from_ckpt ? as_h2(ck) : (h2){zp, sc}, al, be, tg); }
 };
 
-template <bool KEYS, bool FEW>
 __device__ __forceinline__ void put_unit(char *to, int c, int u, const uint32_t *x)
 {
-    if constexpr (KEYS || FEW) {
-        *reinterpret_cast<uint4 *>(to + key_piece<FEW>(c, u)) = make_uint4(x[0], x[1], x[2], x[3]);
-    } else {
-        const int piece = u / 4 * 4 + u % 2 * 2, half = u / 2 % 2 * 8;
-        *reinterpret_cast<uint2 *>(to + value_piece<false>(c, piece) + half) = make_uint2(x[0], x[1]);
-        *reinterpret_cast<uint2 *>(to + value_piece<false>(c, piece + 1) + half) = make_uint2(x[2], x[3]);
-    }
+    *reinterpret_cast<uint4 *>(to + few_piece(c, u)) = make_uint4(x[0], x[1], x[2], x[3]);
 }
 
 // a whole tile from the words w
-template <int BITS, bool KEYS, bool FEW>
+template <int BITS>
 __device__ __forceinline__ void whole_tile(Lone &st, const uint32_t *w, const uint2 *lut, uint32_t lane_copy, char *to, int c)
 {
-    constexpr int TILE = Shape<FEW>::TILE;
     uint2 e[2][4];
     lone_lookup<BITS>(e[0], lut, w, 0, lane_copy);
 #pragma unroll
-    for (int u = 0; u < TILE / 8; u++) {
-        if (u + 1 < TILE / 8)
+    for (int u = 0; u < FEW_TILE / 8; u++) {
+        if (u + 1 < FEW_TILE / 8)
             lone_lookup<BITS>(e[(u & 1) ^ 1], lut, w, u + 1, lane_copy);
         __builtin_amdgcn_sched_barrier(0);
         uint32_t x[4];
         lone_eight(st, e[u & 1], x);
-        put_unit<KEYS, FEW>(to, c, u, x);
+        put_unit(to, c, u, x);
         __builtin_amdgcn_sched_barrier(0);
     }
 }
 
-// The last tile of a span: n < TILE tokens, or n == TILE with the appended one among them.  What is behind them is zero: its weights
+// The last tile of a span: fewer tokens than a tile has, or as many with the appended one among them.  What is behind them is zero: its weights
 // are, and the rest of a buffer may be anything.  append: the n-th token is new, the last of its stream.
-template <int BITS, bool KEYS, bool FEW>
+template <int BITS, bool KEYS>
 __device__ __forceinline__ void part_tile(Lone &st, const uint32_t *w, char *to, int c, int n, bool append, uint16_t fresh, KArgs &a,
-                                          const Walk<Shape<FEW>::TILE> &at)
+                                          const Walk<FEW_TILE> &at)
 {
-    constexpr int TPW = 32 / BITS, TILE = Shape<FEW>::TILE;
-    for (int u = 0; u < TILE / 8; u++) {
+    constexpr int TPW = 32 / BITS;
+    for (int u = 0; u < FEW_TILE / 8; u++) {
         uint32_t x[4] = {};
         if (u * 8 < n) {
             uint32_t word = 0;
 #pragma unroll
-            for (int k = 0; k < TILE / TPW; k++)
+            for (int k = 0; k < FEW_TILE / TPW; k++)
                 word = u * 8 / TPW == k ? w[k] : word;
             word >>= u * 8 % TPW * BITS;
             const int there = min(n - u * 8 - (append ? 1 : 0), 8); // old ones
@@ -364,7 +363,7 @@ __device__ __forceinline__ void part_tile(Lone &st, const uint32_t *w, char *to,
                 const int sh = T % TPW * BITS;
                 uint32_t whole = 0;
 #pragma unroll
-                for (int k = 0; k < TILE / TPW; k++)
+                for (int k = 0; k < FEW_TILE / TPW; k++)
                     whole = u * 8 / TPW == k ? w[k] : whole;
                 *home = (whole & ~(Code<BITS>::FIELD << sh)) | (uint32_t)(q - Code<BITS>::QLO) << sh;
                 const uint32_t v = (uint32_t)__builtin_bit_cast(uint16_t, lone_token(st, q)) << (there & 1) * 16;
@@ -375,20 +374,19 @@ __device__ __forceinline__ void part_tile(Lone &st, const uint32_t *w, char *to,
                     ck[(size_t)j * D] = as_u32((h2){lone_zp(st), lone_sc(st)});
             }
         }
-        put_unit<KEYS, FEW>(to, c, u, x);
+        put_unit(to, c, u, x);
     }
 }
 
-template <int BITS, bool KEYS, bool FEW>
+template <int BITS, bool KEYS>
 __device__ __forceinline__ void produce(KArgs &a, int items, const uint2 *lut, char *tiles, int c, int lane)
 {
-    using S = Shape<FEW>;
-    constexpr int KIND = KEYS ? 0 : 1, TILE = S::TILE, COPIES = (BITS == 4 ? LUT_COPIES : LUT2_COPIES) / (FEW ? 2 : 1);
+    constexpr int KIND = KEYS ? 0 : 1, COPIES = (BITS == 4 ? LUT_COPIES : LUT2_COPIES) / 2;
     const uint32_t lane_copy = (uint32_t)(lane & (COPIES - 1)) * (BITS == 4 ? 8u : 16u);
     const int append_end = a.append ? a.s[1].x.tokens : -1;
-    Loads<BITS, TILE> ahead[2];
+    Loads<BITS> ahead[2];
     uint16_t fresh = 0;
-    Walk<TILE> at(a, items, blockIdx.x), then = at, next = at; // the tile, the one after it, the one whose loads go out next
+    Walk<FEW_TILE> at(a, items, blockIdx.x), then = at, next = at; // the tile, the one after it, the one whose loads go out next
     Feed feed;
     feed.open<BITS>(a, next, KIND);
     auto step = [&]() __attribute__((always_inline)) {
@@ -407,20 +405,20 @@ __device__ __forceinline__ void produce(KArgs &a, int items, const uint2 *lut, c
     // returns whether that was the last
     auto tile = [&](auto ic) __attribute__((always_inline)) {
         constexpr int I = decltype(ic)::value;
-        const Loads<BITS, TILE> cur = ahead[I];
+        const Loads<BITS> cur = ahead[I];
         step();
         ahead[I].start(feed, next.k, c);
         if (at.k == 0) {
             st = cur.state(at.first > 0);
             fresh = cur.fresh;
         }
-        char *to = tiles + I * S::BUFFER + (KEYS ? 0 : S::VALUES);
-        const int left = at.t1 - at.t0 - at.k * TILE;
+        char *to = tiles + I * FEW_BUFFER + (KEYS ? 0 : FEW_VALUES);
+        const int left = at.t1 - at.t0 - at.k * FEW_TILE;
         const bool append = at.src && at.t1 == append_end;
-        if (left > TILE || (left == TILE && !append))
-            whole_tile<BITS, KEYS, FEW>(st, cur.w, lut, lane_copy, to, c);
+        if (left > FEW_TILE || (left == FEW_TILE && !append))
+            whole_tile<BITS>(st, cur.w, lut, lane_copy, to, c);
         else
-            part_tile<BITS, KEYS, FEW>(st, cur.w, to, c, left, append, fresh, a, at);
+            part_tile<BITS, KEYS>(st, cur.w, to, c, left, append, fresh, a, at);
         __syncthreads();
         if (at.last())
             return true;
@@ -506,7 +504,7 @@ template <int J> struct MaskRaw<J, 0> {
 template <int NB, int J, int MASK>
 struct Consumer {
     static constexpr bool FEW = J == 1;
-    using W = Walk<Shape<FEW>::TILE>;
+    using W = Walk<FEW ? FEW_TILE : TILE>;
     static constexpr int NC = FEW ? 4 : 8; // blocks of 16 channels of the outputs
     h8v q[NB][4];
     f4v o[NB][NC];
@@ -515,6 +513,10 @@ struct Consumer {
     int limit[NB];        // tokens of the source that it looks at
     const char *mask[NB]; // its mask at the source's first token
     int seen, tokens;     // of the source: what every row looks at, all
+    const uint32_t *bits[NB]; // many rows: which of the mask's tiles have anything in them, from the source's first tile on; may be null
+    int bit0, from;           // the source's first tile among all; the span's first token
+    uint32_t word[NB];        // of the tiles around the present one
+    bool masked[NB];          // this tile's mask was loaded
     MaskRaw<J, MASK> masks[NB];
 
     // of row r of a unit: sequence, token, query head
@@ -580,21 +582,37 @@ struct Consumer {
             limit[k] = s.causal ? s.seen + i : s.seen;
             if constexpr (MASK != 0)
                 mask[k] = (const char *)a.mask + (b * a.m_sb + hq * a.m_sh + i * a.m_st + s.col) * (MASK == 2 ? 4 : 2);
+            if constexpr (MASK != 0 && !FEW) {
+                bits[k] = a.mask_bits != nullptr ? a.mask_bits + ((long)b * a.n + i) * a.mask_words : nullptr;
+                bit0 = at.src ? a.mask_own_tile : 0;
+                from = at.t0;
+                word[k] = ~0u;
+            }
         }
     }
 
     // the mask of the tokens from t on
-    __device__ __forceinline__ void look_at(int t, int lane)
+    template <int NA> __device__ __forceinline__ void look_at(int t, int lane)
     {
         if constexpr (MASK != 0) {
+            const int tile = FEW ? 0 : bit0 + t / TILE, first = t;
             t += (lane >> 4) * 4;
 #pragma unroll
-            for (int k = 0; k < NB; k++)
-                masks[k].load(mask[k], t, tokens - t);
+            for (int k = 0; k < NA; k++) {
+                if constexpr (FEW) {
+                    masked[k] = true;
+                } else {
+                    if (bits[k] != nullptr && (first == from || (tile & 31) == 0))
+                        word[k] = global(bits[k])[tile >> 5];
+                    masked[k] = __any(word[k] >> (tile & 31) & 1);
+                }
+                if (masked[k])
+                    masks[k].load(mask[k], t, tokens - t);
+            }
         }
     }
     // the scores of the step-th step of a tile, as q.K
-    __device__ __forceinline__ void scores(const char *keys, int step, int lane, f4v (*sc)[J])
+    template <int NA> __device__ __forceinline__ void scores(const char *keys, int step, int lane, f4v (*sc)[J])
     {
         typedef short s4v __attribute__((ext_vector_type(4)));
         typedef __attribute__((address_space(3))) s4v *Lds;
@@ -608,7 +626,7 @@ struct Consumer {
             for (int i = 0; i < 2; i++)
                 at[i] = key_piece<FEW>(quarter * 8 + i * 4 + (r16 >> 2), (step * J + j) * 2 + (r16 >> 1 & 1)) + (r16 & 1) * 8;
 #pragma unroll
-            for (int k = 0; k < NB; k++)
+            for (int k = 0; k < NA; k++)
                 sc[k][j] = (f4v){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int c = 0; c < 4; c++) {
@@ -617,24 +635,31 @@ struct Consumer {
                 const uint2 u = __builtin_bit_cast(uint2, x), v = __builtin_bit_cast(uint2, y);
                 const h8v key = __builtin_bit_cast(h8v, make_uint4(u.x, u.y, v.x, v.y));
 #pragma unroll
-                for (int k = 0; k < NB; k++)
+                for (int k = 0; k < NA; k++)
                     sc[k][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, q[k][c], sc[k][j], 0, 0, 0);
             }
         }
     }
 
     // scores of the tokens from t on to weights of fp16; the row's maximum, sum and outputs go along
-    __device__ __forceinline__ void weights(KArgs &a, int t, int lane, const f4v (*sc)[J], uint32_t (*w)[2 * J])
+    template <int NA> __device__ __forceinline__ void weights(KArgs &a, int t, int lane, const f4v (*sc)[J], uint32_t (*w)[2 * J])
     {
         const int quarter = lane >> 4;
 #pragma unroll
-        for (int k = 0; k < NB; k++) {
+        for (int k = 0; k < NA; k++) {
             float x[4 * J];
 #pragma unroll
             for (int e = 0; e < 4 * J; e++)
                 x[e] = sc[k][e >> 2][e & 3];
-            if constexpr (MASK != 0)
-                masks[k].add(x, a.scaling, a.mask_dt);
+            if constexpr (MASK != 0) {
+                if (masked[k]) {
+                    masks[k].add(x, a.scaling, a.mask_dt);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4 * J; e++)
+                        x[e] *= a.scaling;
+                }
+            }
             if (t + 16 * J > seen) {
 #pragma unroll
                 for (int e = 0; e < 4 * J; e++)
@@ -644,9 +669,11 @@ struct Consumer {
 #pragma unroll
             for (int e = 1; e < 4 * J; e++)
                 mx = fmaxf(mx, x[e]);
-            mx = fmaxf(m[k], fold_quarters<true>(mx));
+            // The largest so far is looked for again only where a weight would be more than 2^8: weights relative to one that is smaller than the
+            // largest by up to that are as exact.
             const float c = MASK != 0 ? LOG2E : a.scaling * LOG2E;
-            if (__any(mx > m[k])) {
+            if (__any((mx - m[k]) * c > 8.0f || m[k] == -INFINITY)) {
+                mx = fmaxf(m[k], fold_quarters<true>(mx));
                 const float shrink = m[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[k] - mx) * c);
                 m[k] = mx;
                 l[k] *= shrink;
@@ -656,7 +683,7 @@ struct Consumer {
                     for (int e = 0; e < 4; e++)
                         o[k][cc][e] *= shrink;
             }
-            const float ref = mx == -INFINITY ? 0.0f : mx; // nothing but -inf so far: all weights are zero
+            const float ref = m[k] == -INFINITY ? 0.0f : m[k]; // nothing but -inf so far: all weights are zero
             float sum = 0.0f;
 #pragma unroll
             for (int e = 0; e < 4 * J; e++) {
@@ -671,7 +698,7 @@ struct Consumer {
         }
     }
     // Half of a product's 32 tokens where a step has 16: the other half is zero on both sides.
-    __device__ __forceinline__ void outputs(const char *values, int step, int lane, const uint32_t (*w)[2 * J])
+    template <int NA> __device__ __forceinline__ void outputs(const char *values, int step, int lane, const uint32_t (*w)[2 * J])
     {
 #pragma unroll
         for (int kk = 0; kk < (J + 1) / 2; kk++)
@@ -687,7 +714,7 @@ struct Consumer {
                     v = *reinterpret_cast<const uint4 *>(p);
                 }
 #pragma unroll
-                for (int k = 0; k < NB; k++) {
+                for (int k = 0; k < NA; k++) {
                     const uint4 p4 = FEW ? make_uint4(w[k][0], w[k][1], 0, 0) : make_uint4(w[k][kk * 4], w[k][kk * 4 + 1], w[k][kk * 4 + 2], w[k][kk * 4 + 3]);
                     o[k][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8v, v), __builtin_bit_cast(h8v, p4), o[k][c], 0, 0, 0);
                 }
@@ -723,71 +750,50 @@ struct Consumer {
     }
 };
 
-// Few rows (at most 16): two pairs of waves multiply half of a tile's tokens each, with partial results of their own, a wave for half of the channels
-// of the outputs; both make the weights.  Else a wave has up to two
-// blocks of 16 rows out of a workgroup's sixteen, and all tokens.
-template <bool FEW, int MASK>
+// Few rows: two pairs of waves multiply half of a tile's tokens each, with partial results of their own, a wave for half of the channels of the
+// outputs; both make the weights.
+template <int MASK>
 __device__ __forceinline__ void consume(KArgs &a, int items, const char *tiles, int wave, int lane)
 {
-    using S = Shape<FEW>;
-    constexpr int NB = FEW ? 1 : 2, J = FEW ? 1 : 2, TILE = S::TILE, STEPS = FEW ? 1 : TILE / 32, WAVES = S::MULTIPLIERS;
-    using C = Consumer<NB, J, MASK>;
+    using C = Consumer<1, 1, MASK>;
+    const int step = wave & 1, c0 = (wave >> 1) * 4;
     C c;
-    h8v spare[NB][4]; // few rows: the next item's queries, from this one's start on; else they take the present ones' registers
-    h8v(*const ahead)[4] = FEW ? spare : c.q;
-    typename C::W at(a, items, blockIdx.x), next = at; // next: the next item's first tile, once its queries are asked for
-    auto block = [&](const typename C::W &w) __attribute__((always_inline)) { return FEW ? 0 : w.block * (NB * WAVES) + wave; };
-    C::load(a, at, block(at), WAVES, lane, ahead);
+    h8v ahead[1][4]; // the next item's queries, from this one's start on
+    typename C::W at(a, items, blockIdx.x), next = at; // next: the next item's first tile
+    C::load(a, at, 0, 0, lane, ahead);
     c.ready(a, ahead);
     __syncthreads(); // the table
     bool opened = true; // at the item's first tile
     auto tile = [&](auto ic) __attribute__((always_inline)) {
-        const char *from = tiles + decltype(ic)::value * S::BUFFER;
-        const bool ends = at.last_of_item(), more = at.more(), mine = block(at) * 16 < at.rows;
-        const int t = at.t0 + at.k * TILE;
+        const char *from = tiles + decltype(ic)::value * FEW_BUFFER;
+        const bool ends = at.last_of_item(), more = at.more();
+        const int t = at.t0 + at.k * FEW_TILE + step * 16;
         if (opened) {
-            c.clear(a, at, block(at), WAVES, lane);
-            if (FEW && more) {
+            c.clear(a, at, 0, 0, lane);
+            if (more) {
                 next = typename C::W(a, items, at.i + gridDim.x);
-                C::load(a, next, block(next), WAVES, lane, ahead);
+                C::load(a, next, 0, 0, lane, ahead);
             }
         }
         if (at.k == 0)
             c.look(a, at);
         opened = ends;
-        if (mine)
-            c.look_at(t + (FEW ? (wave & 1) * 16 : 0), lane);
+        c.template look_at<1>(t, lane);
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < STEPS; i++) {
-            const int step = FEW ? wave & 1 : i;
-            f4v sc[NB][J];
-            uint32_t w[NB][2 * J];
-            if (mine)
-                c.scores(from, step, lane, sc);
-            if (!FEW && i == STEPS - 1 && ends && more) { // the queries are done with: the next item's take their registers
-                next = typename C::W(a, items, at.i + gridDim.x);
-                C::load(a, next, block(next), WAVES, lane, ahead);
-            }
-            if (mine) {
-                c.weights(a, t + step * 16 * J, lane, sc, w);
-                if (i + 1 < STEPS)
-                    c.look_at(t + (step + 1) * 16 * J, lane);
-                c.outputs(from + S::VALUES + (FEW ? (wave >> 1) * 4 * 2048 : 0), step, lane, w);
-            }
-        }
-        if (ends) {
-            if (more)
-                c.ready(a, ahead); // in front of the stores, which it would wait for
-            if (mine)
-                c.finish(a, at, FEW ? wave & 1 : 0, FEW ? (wave >> 1) * 4 : 0, lane);
-            if (!more)
-                return true;
-            at = next;
-        } else {
+        f4v sc[1][1];
+        uint32_t w[1][2];
+        c.template scores<1>(from, step, lane, sc);
+        c.template weights<1>(a, t, lane, sc, w);
+        c.template outputs<1>(from + FEW_VALUES + c0 * 2048, step, lane, w);
+        if (!ends) {
             at.go(a);
+            return false;
         }
-        return false;
+        if (more)
+            c.ready(a, ahead); // in front of the stores, which it would wait for
+        c.finish(a, at, step, c0, lane);
+        at = next;
+        return !more;
     };
     while (!tile(std::integral_constant<int, 0>{}) && !tile(std::integral_constant<int, 1>{}))
         ;
@@ -813,33 +819,307 @@ __device__ __forceinline__ void fill_half(char *lds, int tid)
 
 // Four waves replay the tile after the one that the others multiply with, one per SIMD, through two buffers and a barrier per tile.
 // A workgroup goes on to its next item without a gap.
-template <int BITS, bool FEW, int MASK>
-__global__ __launch_bounds__(Shape<FEW>::THREADS) void attend_kernel(Args)
+template <int BITS, int MASK>
+__global__ __launch_bounds__(FEW_THREADS) void attend_kernel(Args)
 {
-    using S = Shape<FEW>;
     KArgs &a = *(KArgs *)__builtin_amdgcn_kernarg_segment_ptr();
-    __shared__ uint4 smem[S::LDS / 16]; // the table at LDS offset 0
-    uint2 *lut = reinterpret_cast<uint2 *>(smem);
-    char *tiles = reinterpret_cast<char *>(smem) + S::FIRST;
+    __shared__ uint4 smem[FEW_LDS / 16]; // the table at LDS offset 0
+    const uint2 *lut = reinterpret_cast<const uint2 *>(smem);
+    char *tiles = reinterpret_cast<char *>(smem) + FEW_FIRST;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int items = a.g[0].items + a.g[1].items;
-    if constexpr (FEW)
-        fill_half<BITS, S::THREADS>(reinterpret_cast<char *>(smem), threadIdx.x);
-    else if constexpr (BITS == 4)
-        lone_fill<S::THREADS>(lut, threadIdx.x);
-    else
-        lone_fill2<S::THREADS>(lut, threadIdx.x);
+    fill_half<BITS, FEW_THREADS>(reinterpret_cast<char *>(smem), threadIdx.x);
     if (wave < 2)
-        produce<BITS, true, FEW>(a, items, lut, tiles, wave * 64 + lane, lane);
+        produce<BITS, true>(a, items, lut, tiles, wave * 64 + lane, lane);
     else if (wave < PRODUCERS)
-        produce<BITS, false, FEW>(a, items, lut, tiles, (wave - 2) * 64 + lane, lane);
+        produce<BITS, false>(a, items, lut, tiles, (wave - 2) * 64 + lane, lane);
     else
-        consume<FEW, MASK>(a, items, tiles, wave - PRODUCERS, lane);
+        consume<MASK>(a, items, tiles, wave - PRODUCERS, lane);
+}
+
+// ---------------------------------------------------------------------------------------------------------------- many rows
+struct Images {
+    Source s[2]; // the sources' codes
+    char *to[2]; // their tiles, of the units from `first` on
+    int first[2], runs[2], items[2]; // runs of checkpoint intervals per unit
+    int H;
+    Div by_run[2];
+};
+
+// The values of a run of tokens of 64 channels of K or V as tiles in memory, as the LDS has them: 8 tokens of a channel are 16 bytes.  Four waves an
+// item, two items a workgroup, four waves to a SIMD, which then is bound by the replay's instructions.
+template <int BITS>
+__global__ __launch_bounds__(512) void values_kernel(Images im)
+{
+    constexpr int TPW = 32 / BITS, WPC = TILE / TPW; // words of a channel per chunk of 64 tokens
+    __shared__ uint4 smem[LUT_WORDS64 / 2];
+    uint2 *lut = reinterpret_cast<uint2 *>(smem);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    int item = (int)blockIdx.x * 2 + (wave >> 2);
+    const bool there = item < im.items[0] + im.items[1], own = there && item >= im.items[0];
+    const int kind = wave >> 1 & 1, c = (wave & 1) * 64 + lane;
+    item -= own ? im.items[0] : 0;
+    const Extent &x = own ? im.s[1].x : im.s[0].x;
+    const Tensor &t = own ? (kind ? im.s[1].t[1] : im.s[1].t[0]) : (kind ? im.s[0].t[1] : im.s[0].t[0]);
+    const int runs = own ? im.runs[1] : im.runs[0], of_launch = divide(there ? item : 0, own ? im.by_run[1] : im.by_run[0]);
+    const int unit = of_launch + (own ? im.first[1] : im.first[0]), run = item - of_launch * runs;
+    const int per = x.intervals / runs, longer = x.intervals % runs, first = run * per + min(run, longer), end = first + per + (run < longer ? 1 : 0);
+    const int t0 = first * x.interval, t1 = end >= x.intervals ? x.tokens : end * x.interval;
+    const int h = own ? unit % im.H : unit, pi = h * D + c;
+
+    const int words = there ? (t1 - t0 + TPW - 1) / TPW : 0;
+    // reads behind the last word are dropped
+    const auto codes = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint32_t *>(t.codes) + ((size_t)unit * x.n_super + t0 / TPW) * D, 0, words * D * 4,
+                                                         0x00027000);
+    int next = c * 4;
+    uint32_t w[2][WPC];
+    auto load = [&](uint32_t *to) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < WPC; i++)
+            to[i] = __builtin_amdgcn_raw_buffer_load_b32(codes, next + i * D * 4, 0, 0);
+        next += WPC * D * 4;
+    };
+    Lone st = {};
+    if (there) {
+        load(w[0]);
+        load(w[1]);
+        h2 from = {t.zp[pi], t.sc[pi]};
+        if (first > 0)
+            from = as_h2(*reinterpret_cast<const uint32_t *>(t.ckpt + (((size_t)unit * x.n_ckpt + first - 1) * D + c) * 2));
+        st = state_of(from, t.al[pi], t.be[pi], t.tg[pi]);
+    }
+    if constexpr (BITS == 4)
+        lone_fill<512>(lut, threadIdx.x);
+    else
+        lone_fill2<512>(lut, threadIdx.x);
+    __syncthreads();
+    if (!there)
+        return;
+    const uint32_t lane_copy = BITS == 4 ? (uint32_t)(lane & (LUT_COPIES - 1)) * 8u : (uint32_t)(lane & (LUT2_COPIES - 1)) * 16u;
+    const int tiles = (x.tokens + TILE - 1) / TILE;
+    const auto image = global((own ? im.to[1] : im.to[0]) + (size_t)of_launch * tiles * TILE_BYTES + kind * TILE_VALUES);
+    // unit n of eight tokens of the source
+    auto put = [&](int n, const uint32_t *v) __attribute__((always_inline)) {
+        const auto to = image + (size_t)(n >> 3) * TILE_BYTES + c * 16;
+        const int u = n & 7;
+        if (kind == 0) {
+            *(__attribute__((address_space(1))) u4v *)(to + u * 2048) = (u4v){v[0], v[1], v[2], v[3]};
+        } else {
+            const int piece = (u & 4) + (u & 1) * 2, half = (u & 2) * 4;
+            *(__attribute__((address_space(1))) u2v *)(to + piece * 2048 + half) = (u2v){v[0], v[1]};
+            *(__attribute__((address_space(1))) u2v *)(to + (piece + 1) * 2048 + half) = (u2v){v[2], v[3]};
+        }
+    };
+    // units n..n + 3 where n is a multiple of four: pieces of values whole
+    auto put_four = [&](int n, const uint32_t (*v)[4]) __attribute__((always_inline)) {
+        const auto to = image + (size_t)(n >> 3) * TILE_BYTES + (n & 7) * 2048 + c * 16;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int k = i / 2, j = i % 2 * 2;
+            const u4v x = kind == 0 ? (u4v){v[i][0], v[i][1], v[i][2], v[i][3]} : (u4v){v[k][j], v[k][j + 1], v[k + 2][j], v[k + 2][j + 1]};
+            *(__attribute__((address_space(1))) u4v *)(to + i * 2048) = x;
+        }
+    };
+    int n = t0 >> 3, left = t1 - t0;
+    const bool fours = (n & 3) == 0;
+    auto chunk = [&](uint32_t *from) __attribute__((always_inline)) {
+        uint32_t cur[WPC], v[4][4];
+#pragma unroll
+        for (int i = 0; i < WPC; i++)
+            cur[i] = from[i];
+        load(from);
+        uint2 e[2][4];
+        lone_lookup<BITS>(e[0], lut, cur, 0, lane_copy);
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            if (u < 7)
+                lone_lookup<BITS>(e[(u & 1) ^ 1], lut, cur, u + 1, lane_copy);
+            __builtin_amdgcn_sched_barrier(0);
+            lone_eight(st, e[u & 1], v[u & 3]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (u % 4 == 3) {
+                if (fours) {
+                    put_four(n + u - 3, v);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        put(n + u - 3 + i, v[i]);
+                }
+            }
+        }
+        n += 8;
+        left -= TILE;
+    };
+    for (;;) {
+        if (left < TILE)
+            break;
+        chunk(w[0]);
+        if (left < TILE) {
+#pragma unroll
+            for (int i = 0; i < WPC; i++)
+                w[0][i] = w[1][i];
+            break;
+        }
+        chunk(w[1]);
+    }
+    // the rest, and zeros up to the end of the source's last tile: their weights are zero, and what is there may be anything
+    const int stop = t1 == x.tokens ? tiles * 8 : n + (left + 7) / 8;
+    for (int u = 0; n < stop; u++, n++) {
+        uint32_t v[4] = {};
+        if (u * 8 < left) {
+            uint32_t word = 0;
+#pragma unroll
+            for (int k = 0; k < WPC; k++)
+                word = u * 8 / TPW == k ? w[0][k] : word;
+            word >>= u * 8 % TPW * BITS;
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (u * 8 + i < left)
+                    v[i >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, lone_token(st, (int)(word >> BITS * i & Code<BITS>::FIELD) + Code<BITS>::QLO))
+                                 << (i & 1) * 16;
+        }
+        put(n, v);
+    }
+}
+
+// Which tiles of a mask's rows have anything in them: a bit per tile of 64 tokens, the prefix's tiles, then the own ones.  A mask that is the same for
+// all heads is read by each of them, tile by tile as long as the tile itself, and is mostly zero: a batch's padding and the tokens behind a query.
+template <typename E>
+__global__ __launch_bounds__(256) void mask_tiles_kernel(const E *mask, long m_sb, long m_st, int n, long jobs, int P, int own, uint32_t *bits, int words)
+{
+    const long job = (long)blockIdx.x * 4 + (threadIdx.x >> 6); // a word of a row
+    if (job >= jobs)
+        return;
+    const long row = job / words;
+    const int w = (int)(job - row * words), lane = threadIdx.x & 63, tiles_p = (P + TILE - 1) / TILE, tiles = tiles_p + (own + TILE - 1) / TILE;
+    const E *p = mask + row / n * m_sb + row % n * m_st;
+    uint32_t mine = 0;
+#pragma unroll 16
+    for (int i = 0; i < 32; i++) {
+        const int k = w * 32 + i, t = (k < tiles_p ? k : k - tiles_p) * TILE + lane;
+        const bool there = k < tiles && t < (k < tiles_p ? P : own);
+        // behind the end the row's first element, for nothing
+        const E v = p[there ? (k < tiles_p ? 0 : P) + t : 0];
+        mine |= __any(there && v != 0) ? 1u << i : 0u;
+    }
+    if (lane == 0)
+        bits[job] = mine;
+}
+
+// A tile in 32 loads of 1 KB straight to the LDS, four by each of eight waves: 0..3 the keys, 4..7 the values.  In memory a tile is pieces of 16 bytes by
+// piece, then by channel; where a lane's piece of the LDS comes from is the same for every tile.
+struct Fetch {
+    uint32_t from[4], to;
+    __device__ __forceinline__ Fetch(int wave, int lane)
+    {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int c = (wave & 3) * 32 + i * 8 + (lane >> 3), at = lane & 7;
+            const int piece = wave < 4 ? at ^ (c & 3) << 1 ^ (c >> 2 & 1) : at ^ (c >> 1 & 7);
+            from[i] = (uint32_t)(piece * 128 + c) * 16 + (wave < 4 ? 0 : TILE_VALUES);
+        }
+        to = (uint32_t)wave * 4096u;
+    }
+    __device__ __forceinline__ void tile(const char *image, uint32_t lds) const
+    {
+        const uint64_t base = (uint64_t)image;
+        const rsrc4 buffer = {(uint32_t)base, (uint32_t)(base >> 32) & 0xFFFFu, (uint32_t)TILE_BYTES, 0x00027000u};
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            load_to_lds(lds + to + i * 1024u, from[i], buffer);
+    }
+};
+
+// Three tiles in the LDS: one being multiplied with, two on their way, a barrier per tile.  Workgroups of one XCD take neighbouring items, which
+// read the same tiles.  Bound by the LDS: eight waves read a tile of 32 KB each, 2048 of about 4700 cycles; matrix instructions are as many.
+// (The second wave of each SIMD a tile behind with its softmax, so that one makes weights while the other multiplies, took 241 registers instead of 207 and
+// was no faster: 128 rows for each of 8 heads over 8192 tokens 32 us instead of 26, long walks the same.)
+template <int MASK>
+__global__ __launch_bounds__(MANY_THREADS) void attend_many_kernel(Args)
+{
+    using C = Consumer<2, 4, MASK>;
+    KArgs &a = *(KArgs *)__builtin_amdgcn_kernarg_segment_ptr();
+    __shared__ uint4 smem[3 * TILE_BYTES / 16];
+    char *tiles = reinterpret_cast<char *>(smem);
+    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)tiles;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int items = a.g[0].items + a.g[1].items;
+    const int here = gridDim.x % 8 == 0 ? blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
+    const Fetch fetch(wave, lane);
+    C c;
+    Walk<TILE> at(a, items, here), next = at; // the tile, the one that is fetched next
+    const char *image = nullptr;              // of the latter
+    auto open = [&]() __attribute__((always_inline)) {
+        const size_t unit = next.code_unit(a) - (next.src ? a.g[1].first_unit : 0);
+        image = (const char *)a.s[next.src].t[0].codes + (unit * a.s[next.src].x.intervals + next.first) * TILE_BYTES;
+    };
+    auto step = [&]() __attribute__((always_inline)) {
+        if (next.last())
+            return; // the same again, never used
+        image += TILE_BYTES;
+        next.go(a);
+        if (next.k == 0)
+            open();
+    };
+    auto block = [&](const Walk<TILE> &w) __attribute__((always_inline)) { return w.block * 16 + wave; };
+    open();
+    fetch.tile(image, lds);
+    step();
+    fetch.tile(image, lds + TILE_BYTES);
+    C::load(a, at, block(at), 8, lane, c.q);
+    bool opened = true;
+    int buffer = 0;
+    for (;;) {
+        if (opened) {
+            c.ready(a, c.q);
+            c.clear(a, at, block(at), 8, lane);
+        }
+        if (at.k == 0)
+            c.look(a, at);
+        const int t = at.t0 + at.k * TILE, mine = (at.rows + 15) / 16 - block(at); // blocks from this wave's first on
+        const bool ends = at.last_of_item(), done = at.last();
+        opened = ends;
+        step();
+        asm volatile("s_waitcnt vmcnt(4)" ::: "memory"); // this wave's part of the tile is there, all but what it fetched last
+        __builtin_amdgcn_s_barrier();                     // and everyone's; and nobody reads the tile before it any more
+        asm volatile("" ::: "memory");
+        fetch.tile(image, lds + (buffer == 0 ? 2 : buffer - 1) * TILE_BYTES);
+        const char *from = tiles + buffer * TILE_BYTES;
+        Walk<TILE> then = at;
+        auto multiply = [&](auto na) __attribute__((always_inline)) {
+            constexpr int NA = decltype(na)::value;
+            f4v sc[2][4];
+            uint32_t w[2][8];
+            c.template look_at<NA>(t, lane);
+            c.template scores<NA>(from, 0, lane, sc);
+            c.template weights<NA>(a, t, lane, sc, w);
+            c.template outputs<NA>(from + TILE_VALUES, 0, lane, w);
+        };
+        if (mine > 8)
+            multiply(std::integral_constant<int, 2>{});
+        else if (mine > 0)
+            multiply(std::integral_constant<int, 1>{});
+        if (!done) {
+            if (ends) {
+                then = Walk<TILE>(a, items, at.i + gridDim.x);
+                C::load(a, then, block(then), 8, lane, c.q);
+            } else {
+                then.go(a);
+            }
+        }
+        if (ends && mine > 0)
+            c.finish(a, at, 0, 0, lane);
+        if (done)
+            break;
+        at = then;
+        buffer = buffer == 2 ? 0 : buffer + 1;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // nothing is written to the LDS any more
 }
 
 // out = sum e^(m-M) o / sum e^(m-M) l over the pieces.  Four channels per lane, 32 lanes per row, WAYS of them for a share of the
 // pieces each, in a fixed order: where rows are few the pieces are many and a lane that walks through all of them waits for each
-// (128 rows of 100 pieces 25 us, with WAYS = 8 %s).
+// (128 rows of 100 pieces 25 us, with WAYS = 8 five).
 template <int WAYS>
 __global__ __launch_bounds__(256) void join_kernel(const float *__restrict__ partial, const float2 *__restrict__ ml, h1 *__restrict__ out,
                                                    long rows, int pieces, int act_bf16)
@@ -938,12 +1218,14 @@ __global__ __launch_bounds__(128) void state_kernel(Source s, int H, int n_ckpt,
 }
 
 struct Plan {
-    bool joint;      // the prefix is walked with the rows of each sequence by themselves
-    int launches;
-    bool few[2];     // of a launch
-    int groups[2];   // of a launch, a bit each
-    int nseg[2], blocks[2], split[2], intervals[2]; // of a group; intervals: of a source
+    bool joint;                     // the prefix is walked with the rows of each sequence by themselves
+    bool there[2], few[2];          // of a group
+    int nseg[2], blocks[2], split[2];
+    int intervals[2], tiles[2];     // of a source
+    bool image[2];                  // whether the source is written out as tiles of values
+    int batch;                      // units of the own source whose tiles are there at a time
     long pieces() const { return (long)nseg[0] * split[0] + (long)nseg[1] * split[1]; }
+    int64_t image_bytes(int i, int H) const { return image[i] ? (int64_t)(i ? batch : H) * tiles[i] * TILE_BYTES : 0; }
 };
 
 static int usable_intervals(int tokens, int interval, int n_ckpt)
@@ -951,53 +1233,60 @@ static int usable_intervals(int tokens, int interval, int n_ckpt)
     return interval > 0 ? std::max(std::min((tokens + interval - 1) / interval, n_ckpt + 1), 1) : 1;
 }
 
-// Workgroups walk through items, one per CU, two for few rows.  Rows of a sequence that half fill a workgroup's 256 or more walk through the prefix
-// by themselves: it is replayed as often as with blocks of the whole batch's rows, and their outputs need no joining.  The length of a piece is
-// chosen for the shortest call by the model (us): a workgroup's items x (64 tokens of a piece x 1.6 or 2.5 + 1), and 4 TB/s for the partial results,
-// written and read.  T: the own tokens in front of the new ones.
+constexpr int64_t IMAGE_MAX = 1ll << 30; // bytes of own tiles at a time, unless one unit's are more
+
+// Rows of a sequence that half fill a workgroup's 256 or more walk through the prefix by themselves: their outputs need no joining.  Workgroups
+// walk through items, two per CU (few rows) or one.  The length of a piece is chosen for the shortest call by the model (us): a workgroup's items x
+// (64 tokens of a piece x 1.3 + 1), and 4 TB/s for the partial results, written and read.
+// T: the own tokens in front of the new ones.
 static Plan plan(int B, int H, int G, int n, int P, int p_interval, int p_ckpt, int T, int interval, int n_ckpt)
 {
     Plan p = {};
-    const long rows[2] = {(long)B * n * G, (long)n * G};
-    p.joint = P > 0 && rows[1] >= 128;
-    const bool both = P > 0 && !p.joint, few[2] = {rows[0] <= 16, rows[1] <= 16};
+    const long rows[2] = {(long)B * n * G, (long)n * G}, units[2] = {H, (long)B * H}, total = (long)B * n * G * H;
+    p.joint = P > 0 && rows[1] >= MANY_ROWS / 2;
+    p.there[0] = P > 0 && !p.joint;
+    p.there[1] = true;
     p.intervals[0] = P > 0 ? usable_intervals(P, p_interval, p_ckpt) : 0;
     // the state in front of a single new token may not be recorded yet
     p.intervals[1] = usable_intervals(n == 1 ? T : T + n, interval, n_ckpt);
-    p.launches = both && few[0] != few[1] ? 2 : 1;
-    p.groups[0] = p.launches == 2 ? 1 : both ? 3 : 2;
-    p.groups[1] = 2;
-    p.few[0] = both ? few[0] : few[1];
-    p.few[1] = few[1];
-    const long units[2] = {H, (long)B * H}, total = (long)B * n * G * H;
-    const long tiles[2] = {(P + 63) / 64, (T + n + 63) / 64 + (p.joint ? (P + 63) / 64 : 0)};
-    const int intervals[2] = {p.intervals[0], p.intervals[1] + (p.joint ? p.intervals[0] : 0)};
-    for (int i = 0; i < p.launches; i++) {
-        const bool f = p.few[i];
+    p.tiles[0] = (P + TILE - 1) / TILE;
+    p.tiles[1] = (T + n + TILE - 1) / TILE;
+    for (int i = 0; i < 2; i++)
+        p.few[i] = rows[i] <= 16;
+    p.image[0] = p.joint || (p.there[0] && !p.few[0]);
+    p.image[1] = !p.few[1];
+    p.batch = (int)std::max<int64_t>(1, std::min<int64_t>((long)B * H, IMAGE_MAX / ((int64_t)p.tiles[1] * TILE_BYTES)));
+    // groups of one kind share a launch
+    for (int k = 0; k < 2; k++) {
+        const bool f = k == 0;
         const long slots = cu_count() * (f ? 2L : 1L);
+        const bool in[2] = {p.there[0] && p.few[0] == f, p.few[1] == f};
+        if (!in[0] && !in[1])
+            continue;
         double best = -1.0;
         for (int len = 1; len < (1 << 20); len += std::max(len / 4, 1)) { // of 64 tokens
             int ns[2] = {0, 0};
             long items = 0, longest = 0, pieces = 0;
             bool shortest = true;
-            for (int k = 0; k < 2; k++) {
-                if (!(p.groups[i] >> k & 1))
+            for (int i = 0; i < 2; i++) {
+                if (!in[i])
                     continue;
-                p.blocks[k] = f ? 1 : (int)((rows[k] + 255) / 256);
-                p.split[k] = f ? 2 : 1;
-                ns[k] = (int)std::max<long>(std::min<long>(intervals[k], (tiles[k] + len - 1) / len), 1);
-                items += units[k] * p.blocks[k] * ns[k];
-                longest = std::max(longest, (tiles[k] + ns[k] - 1) / ns[k]);
-                pieces += (long)ns[k] * p.split[k];
-                shortest = shortest && ns[k] == 1;
+                const long tiles = p.tiles[i] + (i && p.joint ? p.tiles[0] : 0), most = f ? p.intervals[i] : tiles;
+                p.blocks[i] = f ? 1 : (int)((rows[i] + MANY_ROWS - 1) / MANY_ROWS);
+                p.split[i] = f ? 2 : 1;
+                ns[i] = (int)std::max<long>(std::min<long>(most, (tiles + len - 1) / len), 1);
+                items += units[i] * p.blocks[i] * ns[i];
+                longest = std::max(longest, (tiles + ns[i] - 1) / ns[i]);
+                pieces += (long)ns[i] * p.split[i];
+                shortest = shortest && ns[i] == 1;
             }
-            const bool direct = pieces == 1 && p.launches == 1;
-            const double cost = (double)((items + slots - 1) / slots) * (longest * (f ? 1.6 : 2.5) + 1.0) + (direct ? 0.0 : 4.0 + pieces * total * 1024 / 4e6);
+            const bool direct = pieces == 1 && !(p.there[0] && !in[0]);
+            const double cost = (double)((items + slots - 1) / slots) * (longest * 1.3 + 1.0) + (direct ? 0.0 : 4.0 + pieces * total * 1024 / 4e6);
             if (best < 0 || cost < best) {
                 best = cost;
-                for (int k = 0; k < 2; k++)
-                    if (p.groups[i] >> k & 1)
-                        p.nseg[k] = ns[k];
+                for (int i = 0; i < 2; i++)
+                    if (in[i])
+                        p.nseg[i] = ns[i];
             }
             if (shortest)
                 break;
@@ -1007,6 +1296,9 @@ static Plan plan(int B, int H, int G, int n, int P, int p_interval, int p_ckpt, 
 }
 
 static int64_t pad256(int64_t n) { return (n + 255) & ~(int64_t)255; }
+// of which tiles a mask has something in
+static int mask_words(const Plan &p) { return (p.tiles[0] + p.tiles[1] + 31) / 32; }
+static int64_t bits_bytes(const Plan &p, int B, int n) { return p.image[0] || p.image[1] ? pad256((int64_t)B * n * mask_words(p) * 4) : 0; }
 
 } // namespace adkv_ext
 
@@ -1022,7 +1314,7 @@ int64_t adkv_extend_workspace_bytes(int B, int Hq, int H, int T, int n, int n_ck
     const Plan p = plan(B, H, Hq / H, n, P, prefix_n_ckpt_cap > 0 ? prefix_ckpt_interval : 0, prefix_n_ckpt_cap, T,
                         n_ckpt_cap > 0 ? ckpt_interval : 0, n_ckpt_cap);
     const int64_t rows = (int64_t)B * n * Hq;
-    return 2 * pad256((int64_t)B * H * D * 4) + pad256(p.pieces() * rows * 8) + p.pieces() * rows * D * 4;
+    return 2 * pad256((int64_t)B * H * D * 4) + pad256(p.pieces() * rows * 8) + pad256(p.pieces() * rows * D * 4) + p.image_bytes(0, H) + p.image_bytes(1, H) + bits_bytes(p, B, n);
 }
 
 int adkv_extend(const void *q, const int64_t *q_strides, void *k_cache, void *v_cache, const void *k_new, const void *v_new,
@@ -1097,6 +1389,9 @@ int adkv_extend(const void *q, const int64_t *q_strides, void *k_cache, void *v_
     Args a;
     a.ml = (float2 *)(ws + 2 * state_bytes);
     a.partial = (float *)(ws + 2 * state_bytes + pad256(pl.pieces() * rows * 8));
+    char *images[2];
+    images[0] = (char *)a.partial + pad256(pl.pieces() * rows * D * 4);
+    images[1] = images[0] + pl.image_bytes(0, H);
     auto tensor = [](const void *codes, const void *ckpt, const void *const *p) {
         return Tensor{(const uint32_t *)codes, (const h1 *)ckpt, (const h1 *)p[0], (const h1 *)p[1], (const h1 *)p[2], (const h1 *)p[3], (const h1 *)p[4]};
     };
@@ -1123,29 +1418,6 @@ int adkv_extend(const void *q, const int64_t *q_strides, void *k_cache, void *v_
     own.x.interval = ckpt_interval;
     own.x.intervals = pl.intervals[1];
     own.x.col = P;
-    Group groups[2] = {};
-    for (int i = 0; i < 2; i++) {
-        Group &g = groups[i];
-        if (pl.nseg[i] == 0)
-            continue;
-        g.units = i ? B * H : H;
-        g.blocks = pl.blocks[i];
-        g.nseg = pl.nseg[i];
-        g.rows = (int)(i ? (int64_t)n * G : (int64_t)B * n * G);
-        const int64_t items = (int64_t)g.units * g.blocks * g.nseg;
-        if (items * ((int64_t)g.blocks * g.nseg) >= 1ll << 32)
-            return ADKV_E_SHAPE;
-        g.items = (int)items;
-        g.from = i == 0 || pl.joint ? 0 : 1;
-        g.to = i;
-        const int intervals = (i == 0 || pl.joint ? pl.intervals[0] : 0) + (i ? pl.intervals[1] : 0);
-        g.per_piece = intervals / g.nseg;
-        g.longer = intervals % g.nseg;
-        g.piece = i ? pl.nseg[0] * pl.split[0] : 0;
-        g.split = pl.split[i];
-        g.by_unit = div((int64_t)g.blocks * g.nseg);
-        g.by_block = div(g.blocks);
-    }
     if ((int64_t)B * H * H >= 1ll << 32 || (int64_t)B * n * n >= 1ll << 32)
         return ADKV_E_SHAPE;
     a.by_head = div(H);
@@ -1194,23 +1466,99 @@ int adkv_extend(const void *q, const int64_t *q_strides, void *k_cache, void *v_
     const bool direct = pl.pieces() == 1;
     a.out = direct ? (h1 *)out : nullptr;
     const int kind = !mask ? 0 : mask_dt == ADKV_DT_F32 ? 2 : 1;
-    typedef void (*Kernel)(Args);
-    static const Kernel kernels[2][2][3] = {
-        {{attend_kernel<4, false, 0>, attend_kernel<4, false, 1>, attend_kernel<4, false, 2>},
-         {attend_kernel<4, true, 0>, attend_kernel<4, true, 1>, attend_kernel<4, true, 2>}},
-        {{attend_kernel<2, false, 0>, attend_kernel<2, false, 1>, attend_kernel<2, false, 2>},
-         {attend_kernel<2, true, 0>, attend_kernel<2, true, 1>, attend_kernel<2, true, 2>}}};
-    for (int i = 0; i < pl.launches; i++) {
-        for (int k = 0; k < 2; k++) {
-            a.g[k] = groups[k];
-            if (!(pl.groups[i] >> k & 1))
-                a.g[k].items = 0;
-        }
-        const int64_t items = (int64_t)a.g[0].items + a.g[1].items;
-        hipLaunchKernelGGL(kernels[bits == 2][pl.few[i]][kind], dim3((unsigned)std::min<int64_t>(items, cu_count() * (pl.few[i] ? 2 : 1))),
-                           dim3(pl.few[i] ? Shape<true>::THREADS : Shape<false>::THREADS), 0, (hipStream_t)stream, a);
+    const Source sources[2] = {pre, own};
+    a.mask_bits = nullptr;
+    a.mask_words = mask_words(pl);
+    a.mask_own_tile = pl.tiles[0];
+    if (mask && a.m_sh == 0 && H > 1 && (pl.image[0] || pl.image[1])) {
+        uint32_t *bits = (uint32_t *)(images[1] + pl.image_bytes(1, H));
+        const int64_t r = (int64_t)B * n * a.mask_words;
+        const dim3 grid((unsigned)((r + 3) / 4));
+        if (mask_dt == ADKV_DT_F32)
+            hipLaunchKernelGGL(mask_tiles_kernel<uint32_t>, grid, dim3(256), 0, (hipStream_t)stream, (const uint32_t *)mask, a.m_sb, a.m_st, n, (long)r, P,
+                               T + n, bits, a.mask_words);
+        else
+            hipLaunchKernelGGL(mask_tiles_kernel<uint16_t>, grid, dim3(256), 0, (hipStream_t)stream, (const uint16_t *)mask, a.m_sb, a.m_st, n, (long)r, P,
+                               T + n, bits, a.mask_words);
         if ((rc = check_launch()))
             return rc;
+        a.mask_bits = bits;
+    }
+    // units [u0, u1) of a group
+    auto group = [&](int i, int u0, int u1) {
+        Group g = {};
+        g.first_unit = u0;
+        g.blocks = pl.blocks[i];
+        g.nseg = pl.nseg[i];
+        g.rows = (int)(i ? (int64_t)n * G : (int64_t)B * n * G);
+        g.from = i == 0 || pl.joint ? 0 : 1;
+        g.to = i;
+        const int intervals = pl.few[i] ? pl.intervals[i] : pl.tiles[i] + (i && pl.joint ? pl.tiles[0] : 0);
+        g.per_piece = intervals / g.nseg;
+        g.longer = intervals % g.nseg;
+        g.piece = i ? pl.nseg[0] * pl.split[0] : 0;
+        g.split = pl.split[i];
+        g.by_unit = div((int64_t)g.blocks * g.nseg);
+        g.by_block = div(g.blocks);
+        g.items = (int)((int64_t)(u1 - u0) * g.blocks * g.nseg);
+        return g;
+    };
+    for (int i = 0; i < 2; i++) {
+        const int64_t per = (int64_t)pl.blocks[i] * pl.nseg[i], items = per * (i ? (int64_t)B * H : H);
+        if (pl.there[i] && items * per >= 1ll << 32)
+            return ADKV_E_SHAPE;
+    }
+    typedef void (*Kernel)(Args);
+    if ((pl.there[0] && pl.few[0]) || pl.few[1]) {
+        static const Kernel kernels[2][3] = {{attend_kernel<4, 0>, attend_kernel<4, 1>, attend_kernel<4, 2>},
+                                             {attend_kernel<2, 0>, attend_kernel<2, 1>, attend_kernel<2, 2>}};
+        a.g[0] = pl.there[0] && pl.few[0] ? group(0, 0, H) : Group{};
+        a.g[1] = pl.few[1] ? group(1, 0, B * H) : Group{};
+        const int64_t items = (int64_t)a.g[0].items + a.g[1].items;
+        hipLaunchKernelGGL(kernels[bits == 2][kind], dim3((unsigned)std::min<int64_t>(items, 2 * cu_count())), dim3(FEW_THREADS), 0,
+                           (hipStream_t)stream, a);
+        if ((rc = check_launch()))
+            return rc;
+    }
+    if (pl.image[0] || pl.image[1]) {
+        static const Kernel kernels[3] = {attend_many_kernel<0>, attend_many_kernel<1>, attend_many_kernel<2>};
+        for (int i = 0; i < 2; i++)
+            if (pl.image[i]) {
+                a.s[i].t[0].codes = (const uint32_t *)images[i];
+                a.s[i].x.interval = TILE;
+                a.s[i].x.intervals = pl.tiles[i];
+            }
+        for (int u0 = 0; u0 < B * H; u0 += pl.batch) {
+            const int u1 = std::min(B * H, u0 + pl.batch);
+            Images im = {};
+            im.H = H;
+            for (int i = 0; i < 2; i++) {
+                im.s[i] = sources[i];
+                im.to[i] = images[i];
+                im.first[i] = i ? u0 : 0;
+                const int units = !pl.image[i] || (i == 0 && u0 > 0) ? 0 : i ? u1 - u0 : H;
+                // a run per wave slot: four waves a run, sixteen a CU
+                im.runs[i] = std::max(1, std::min(pl.intervals[i], 4 * cu_count() / std::max(units, 1)));
+                im.items[i] = units * im.runs[i];
+                im.by_run[i] = div(im.runs[i]);
+            }
+            const int items = im.items[0] + im.items[1];
+            if (items > 0) {
+                hipLaunchKernelGGL(bits == 4 ? values_kernel<4> : values_kernel<2>, dim3((unsigned)((items + 1) / 2)), dim3(512), 0, (hipStream_t)stream, im);
+                if ((rc = check_launch()))
+                    return rc;
+            }
+            a.g[0] = pl.there[0] && !pl.few[0] && u0 == 0 ? group(0, 0, H) : Group{};
+            a.g[1] = pl.image[1] ? group(1, u0, u1) : Group{};
+            const int64_t work = (int64_t)a.g[0].items + a.g[1].items;
+            if (work > 0) {
+                hipLaunchKernelGGL(kernels[kind], dim3((unsigned)std::min<int64_t>(work, cu_count())), dim3(MANY_THREADS), 0, (hipStream_t)stream, a);
+                if ((rc = check_launch()))
+                    return rc;
+            }
+            if (!pl.image[1])
+                break;
+        }
     }
     if (direct)
         return ADKV_OK;
