@@ -846,16 +846,16 @@ struct Images {
     Div by_run[2];
 };
 
-// The values of a run of tokens of 64 channels of K or V as tiles in memory, as the LDS has them: 8 tokens of a channel are 16 bytes.  Four waves an
-// item, two items a workgroup, four waves to a SIMD, which then is bound by the replay's instructions.
-template <int BITS>
-__global__ __launch_bounds__(512) void values_kernel(Images im)
+// The values of a run of tokens of 64 channels of K or V as tiles in memory, as the LDS has them.  Four waves an item; up
+// to four items a workgroup, where there are as many for every CU: four waves to a SIMD, which then is bound by the replay's instructions.
+template <int BITS, int ITEMS>
+__global__ __launch_bounds__(ITEMS * 256) void values_kernel(Images im)
 {
     constexpr int TPW = 32 / BITS, WPC = TILE / TPW; // words of a channel per chunk of 64 tokens
-    __shared__ uint4 smem[LUT_WORDS64 / 2];
+    __shared__ uint4 smem[LUT_WORDS64 / 2 + ITEMS * 4 * 256];
     uint2 *lut = reinterpret_cast<uint2 *>(smem);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    int item = (int)blockIdx.x * 2 + (wave >> 2);
+    int item = (int)blockIdx.x * ITEMS + (wave >> 2);
     const bool there = item < im.items[0] + im.items[1], own = there && item >= im.items[0];
     const int kind = wave >> 1 & 1, c = (wave & 1) * 64 + lane;
     item -= own ? im.items[0] : 0;
@@ -889,9 +889,9 @@ __global__ __launch_bounds__(512) void values_kernel(Images im)
         st = state_of(from, t.al[pi], t.be[pi], t.tg[pi]);
     }
     if constexpr (BITS == 4)
-        lone_fill<512>(lut, threadIdx.x);
+        lone_fill<ITEMS * 256>(lut, threadIdx.x);
     else
-        lone_fill2<512>(lut, threadIdx.x);
+        lone_fill2<ITEMS * 256>(lut, threadIdx.x);
     __syncthreads();
     if (!there)
         return;
@@ -900,30 +900,43 @@ __global__ __launch_bounds__(512) void values_kernel(Images im)
     const auto image = global((own ? im.to[1] : im.to[0]) + (size_t)of_launch * tiles * TILE_BYTES + kind * TILE_VALUES);
     // unit n of eight tokens of the source
     auto put = [&](int n, const uint32_t *v) __attribute__((always_inline)) {
-        const auto to = image + (size_t)(n >> 3) * TILE_BYTES + c * 16;
+        const auto to = image + (size_t)(n >> 3) * TILE_BYTES;
         const int u = n & 7;
         if (kind == 0) {
-            *(__attribute__((address_space(1))) u4v *)(to + u * 2048) = (u4v){v[0], v[1], v[2], v[3]};
+            *(__attribute__((address_space(1))) u4v *)(to + many_key_piece(c, u)) = (u4v){v[0], v[1], v[2], v[3]};
         } else {
             const int piece = (u & 4) + (u & 1) * 2, half = (u & 2) * 4;
-            *(__attribute__((address_space(1))) u2v *)(to + piece * 2048 + half) = (u2v){v[0], v[1]};
-            *(__attribute__((address_space(1))) u2v *)(to + (piece + 1) * 2048 + half) = (u2v){v[2], v[3]};
+            *(__attribute__((address_space(1))) u2v *)(to + many_value_piece(c, piece) + half) = (u2v){v[0], v[1]};
+            *(__attribute__((address_space(1))) u2v *)(to + many_value_piece(c, piece + 1) + half) = (u2v){v[2], v[3]};
         }
     };
-    // units n..n + 3 where n is a multiple of four: pieces of values whole
-    auto put_four = [&](int n, const uint32_t (*v)[4]) __attribute__((always_inline)) {
-        const auto to = image + (size_t)(n >> 3) * TILE_BYTES + (n & 7) * 2048 + c * 16;
+    // A whole tile by way of the LDS, 32 channels at a time, which makes a store of the wave 1 KB in a row instead of 16 bytes of 64 rows.
+    u4v *stage = reinterpret_cast<u4v *>(smem + LUT_WORDS64 / 2) + wave * 256;
+    auto put_tile = [&](int n, const uint32_t (*v)[4]) __attribute__((always_inline)) {
+        const auto to = image + (size_t)(n >> 3) * TILE_BYTES + (wave & 1) * 8192 + lane * 16;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int k = i / 2, j = i % 2 * 2;
-            const u4v x = kind == 0 ? (u4v){v[i][0], v[i][1], v[i][2], v[i][3]} : (u4v){v[k][j], v[k][j + 1], v[k + 2][j], v[k + 2][j + 1]};
-            *(__attribute__((address_space(1))) u4v *)(to + i * 2048) = x;
+        for (int part = 0; part < 2; part++) {
+            if (lane >> 5 == part) {
+#pragma unroll
+                for (int u = 0; u < 8; u++) {
+                    const int k = (u & 4) + u % 4 / 2, j = u % 2 * 2;
+                    if (kind == 0)
+                        stage[many_key_piece(lane & 31, u) >> 4] = (u4v){v[u][0], v[u][1], v[u][2], v[u][3]};
+                    else
+                        stage[many_value_piece(lane & 31, u) >> 4] = (u4v){v[k][j], v[k][j + 1], v[k + 2][j], v[k + 2][j + 1]};
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                *(__attribute__((address_space(1))) u4v *)(to + part * 4096 + i * 1024) = stage[i * 64 + lane];
+            __builtin_amdgcn_wave_barrier();
         }
     };
     int n = t0 >> 3, left = t1 - t0;
-    const bool fours = (n & 3) == 0;
+    const bool whole = (n & 7) == 0;
     auto chunk = [&](uint32_t *from) __attribute__((always_inline)) {
-        uint32_t cur[WPC], v[4][4];
+        uint32_t cur[WPC], v[8][4];
 #pragma unroll
         for (int i = 0; i < WPC; i++)
             cur[i] = from[i];
@@ -935,17 +948,15 @@ __global__ __launch_bounds__(512) void values_kernel(Images im)
             if (u < 7)
                 lone_lookup<BITS>(e[(u & 1) ^ 1], lut, cur, u + 1, lane_copy);
             __builtin_amdgcn_sched_barrier(0);
-            lone_eight(st, e[u & 1], v[u & 3]);
+            lone_eight(st, e[u & 1], v[u]);
             __builtin_amdgcn_sched_barrier(0);
-            if (u % 4 == 3) {
-                if (fours) {
-                    put_four(n + u - 3, v);
-                } else {
+        }
+        if (whole) {
+            put_tile(n, v);
+        } else {
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        put(n + u - 3 + i, v[i]);
-                }
-            }
+            for (int u = 0; u < 8; u++)
+                put(n + u, v[u]);
         }
         n += 8;
         left -= TILE;
@@ -1006,32 +1017,24 @@ __global__ __launch_bounds__(256) void mask_tiles_kernel(const E *mask, long m_s
         bits[job] = mine;
 }
 
-// A tile in 32 loads of 1 KB straight to the LDS, four by each of eight waves: 0..3 the keys, 4..7 the values.  In memory a tile is pieces of 16 bytes by
-// piece, then by channel; where a lane's piece of the LDS comes from is the same for every tile.
+// A tile in 32 loads of 1 KB straight to the LDS, four by each of eight waves.
 struct Fetch {
-    uint32_t from[4], to;
-    __device__ __forceinline__ Fetch(int wave, int lane)
-    {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int c = (wave & 3) * 32 + i * 8 + (lane >> 3), at = lane & 7;
-            const int piece = wave < 4 ? at ^ (c & 3) << 1 ^ (c >> 2 & 1) : at ^ (c >> 1 & 7);
-            from[i] = (uint32_t)(piece * 128 + c) * 16 + (wave < 4 ? 0 : TILE_VALUES);
-        }
-        to = (uint32_t)wave * 4096u;
-    }
+    uint32_t from, to;
+    __device__ __forceinline__ Fetch(int wave, int lane) : from((uint32_t)wave * 4096u + (uint32_t)lane * 16u), to((uint32_t)wave * 4096u) {}
     __device__ __forceinline__ void tile(const char *image, uint32_t lds) const
     {
         const uint64_t base = (uint64_t)image;
         const rsrc4 buffer = {(uint32_t)base, (uint32_t)(base >> 32) & 0xFFFFu, (uint32_t)TILE_BYTES, 0x00027000u};
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            load_to_lds(lds + to + i * 1024u, from[i], buffer);
+            load_to_lds(lds + to + i * 1024u, from + i * 1024u, buffer);
     }
 };
 
 // Three tiles in the LDS: one being multiplied with, two on their way, a barrier per tile.  Workgroups of one XCD take neighbouring items, which
-// read the same tiles.  Bound by the LDS: eight waves read a tile of 32 KB each, 2048 of about 4700 cycles; matrix instructions are as many.
+// read the same tiles.  A tile with 256 rows takes about 5500 cycles: its matrix instructions 2048 of a SIMD, reads of the LDS 1300, and in between
+// both waves of a SIMD wait for their reads or make weights at the same time.  512 tokens of 8 sequences of 32 heads over 4096 tokens, masked:
+// 492 us, 590 TFLOP/s.
 // (The second wave of each SIMD a tile behind with its softmax, so that one makes weights while the other multiplies, took 241 registers instead of 207 and
 // was no faster: 128 rows for each of 8 heads over 8192 tokens 32 us instead of 26, long walks the same.)
 template <int MASK>
@@ -1237,7 +1240,7 @@ constexpr int64_t IMAGE_MAX = 1ll << 30; // bytes of own tiles at a time, unless
 
 // Rows of a sequence that half fill a workgroup's 256 or more walk through the prefix by themselves: their outputs need no joining.  Workgroups
 // walk through items, two per CU (few rows) or one.  The length of a piece is chosen for the shortest call by the model (us): a workgroup's items x
-// (64 tokens of a piece x 1.3 + 1), and 4 TB/s for the partial results, written and read.
+// (64 tokens of a piece x 1.3 or, of many rows, 2.3, + 1), and 4 TB/s for the partial results, written and read.
 // T: the own tokens in front of the new ones.
 static Plan plan(int B, int H, int G, int n, int P, int p_interval, int p_ckpt, int T, int interval, int n_ckpt)
 {
@@ -1263,6 +1266,7 @@ static Plan plan(int B, int H, int G, int n, int P, int p_interval, int p_ckpt, 
         const bool in[2] = {p.there[0] && p.few[0] == f, p.few[1] == f};
         if (!in[0] && !in[1])
             continue;
+        const double tile = f ? 1.3 : 2.3;
         double best = -1.0;
         for (int len = 1; len < (1 << 20); len += std::max(len / 4, 1)) { // of 64 tokens
             int ns[2] = {0, 0};
@@ -1281,7 +1285,7 @@ static Plan plan(int B, int H, int G, int n, int P, int p_interval, int p_ckpt, 
                 shortest = shortest && ns[i] == 1;
             }
             const bool direct = pieces == 1 && !(p.there[0] && !in[0]);
-            const double cost = (double)((items + slots - 1) / slots) * (longest * 1.3 + 1.0) + (direct ? 0.0 : 4.0 + pieces * total * 1024 / 4e6);
+            const double cost = (double)((items + slots - 1) / slots) * (longest * tile + 1.0) + (direct ? 0.0 : 4.0 + pieces * total * 1024 / 4e6);
             if (best < 0 || cost < best) {
                 best = cost;
                 for (int i = 0; i < 2; i++)
@@ -1544,7 +1548,10 @@ int adkv_extend(const void *q, const int64_t *q_strides, void *k_cache, void *v_
             }
             const int items = im.items[0] + im.items[1];
             if (items > 0) {
-                hipLaunchKernelGGL(bits == 4 ? values_kernel<4> : values_kernel<2>, dim3((unsigned)((items + 1) / 2)), dim3(512), 0, (hipStream_t)stream, im);
+                const int each = items <= cu_count() ? 1 : items <= 2 * cu_count() ? 2 : 4;
+                const auto kernel = bits == 4 ? (each == 1 ? values_kernel<4, 1> : each == 2 ? values_kernel<4, 2> : values_kernel<4, 4>)
+                                              : (each == 1 ? values_kernel<2, 1> : each == 2 ? values_kernel<2, 2> : values_kernel<2, 4>);
+                hipLaunchKernelGGL(kernel, dim3((unsigned)((items + each - 1) / each)), dim3(each * 256), 0, (hipStream_t)stream, im);
                 if ((rc = check_launch()))
                     return rc;
             }
