@@ -56,6 +56,9 @@ PROTOTYPES = {
     "adkv_decode_ov_kernel_name": (C.c_char_p, [_i] * 8),
     "adkv_decode_segments": (_i, [_i] * 8 + [_vp, _i, _vp]),
     "adkv_rope_qk": (_i, [_vp] * 6 + [_i] * 5 + [C.c_int64] * 8 + [_i, _vp]),
+    "adkv_rope_norm_qk": (_i, [_vp] * 8 + [_i] * 6 + [_f] + [_vp] * 3 + [_i, _vp]),
+    "adkv_rope_norm_qk_backward_workspace_bytes": (C.c_int64, [_i]),
+    "adkv_rope_norm_qk_backward": (_i, [_vp] * 12 + [_i] * 6 + [_f] + [_vp] * 7 + [_i, _vp, C.c_int64, _vp]),
     "adkv_quant_f32": (_i, [_vp] * 12 + [_i] * 3 + [C.c_int64, C.c_int64] + [_i] * 3 + [_f, _f, _vp]),
     "adkv_quant_f32_pair": (_i, [_vp] * 7 + [_i] * 6 + [_f, _f, _vp]),
     "adkv_extend_workspace_bytes": (C.c_int64, [_i] * 10),

@@ -540,7 +540,7 @@ struct Consumer {
             for (int c = 0; c < 4; c++) {
                 // rows are 4-byte aligned
                 typedef uint32_t u4a __attribute__((ext_vector_type(4), aligned(4)));
-                to[k][c] = __builtin_bit_cast(h8v, (u4v)*global(reinterpret_cast<const u4a *>(src + c * 32)));
+                to[k][c] = __builtin_bit_cast(h8v, (u4v)*(const __attribute__((address_space(1))) u4a *)(src + c * 32));
             }
         }
     }

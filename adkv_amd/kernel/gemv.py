@@ -500,6 +500,118 @@ def rope_qk(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tens
     return q_out, k_out
 
 
+_NORM_DT = {torch.float32: 0, torch.float16: _DT_F16, torch.bfloat16: _DT_BF16}     # ADKV_DT_*
+
+
+def _norm_rows(t: torch.Tensor):
+    """``t`` if ``adkv_rope_norm_qk`` can read it in place, else a copy: rows contiguous, each at a multiple of 4 elements."""
+    ok = t.stride(-1) == 1 and all(st % 4 == 0 for n, st in zip(t.shape[:-1], t.stride()) if n > 1) \
+        and t.data_ptr() % (4 * t.element_size()) == 0
+    # a copy in memory of its own: contiguous() gives back what is contiguous already, however aligned
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _norm_strides(t: torch.Tensor):
+    # of an axis of one element any stride may be given
+    return (_lib.C.c_int64 * (t.dim() - 1))(*[st if n > 1 else 0 for n, st in zip(t.shape[:-1], t.stride())])
+
+
+def _norm_like(t: torch.Tensor):
+    """Laid out as ``t`` where the kernels can write that."""
+    to = torch.empty_like(t)
+    return to if to.stride(-1) == 1 and all(st % 4 == 0 for st in to.stride()[:-1]) else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def _rope_norm_forward(q, k, cos, sin, q_weight, k_weight, eps):
+    B, Hq, T, D = q.shape
+    H, dev = k.shape[1], q.device
+    q_out = torch.empty((B, Hq, T, D), dtype=q.dtype, device=dev)
+    k_out = torch.empty((B, H, T, D), dtype=q.dtype, device=dev)
+    if B * T:
+        with _lib.device_guard(dev):
+            rc = _lib.lib().adkv_rope_norm_qk(
+                q.data_ptr(), k.data_ptr(), cos.data_ptr(), sin.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(),
+                q_out.data_ptr(), k_out.data_ptr(), B, Hq, H, T, D, cos.shape[-1], eps, _norm_strides(q), _norm_strides(k),
+                _norm_strides(cos), _NORM_DT[q.dtype], _lib.current_stream_ptr(dev))
+        _lib.check(rc, "rope_norm_qk")
+    return q_out, k_out
+
+
+class _RopeNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, *args):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(*args[:6])
+        ctx.eps = args[6]
+        return _rope_norm_forward(*args)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        q, k, cos, sin, q_weight, k_weight = ctx.saved_tensors
+        B, Hq, T, D = q.shape
+        H, dev = k.shape[1], q.device
+        want = ctx.needs_input_grad
+        # a side whose result nobody used has no gradient
+        made = []
+        for i, (x, w) in enumerate(((q, q_weight), (k, k_weight))):
+            used = grads[i] is not None
+            made.append((_norm_like(x) if used and want[i] else None,
+                         (torch.empty_like(w) if B * T else torch.zeros_like(w)) if used and want[4 + i] else None))
+        (dq, dwq), (dk, dwk) = made
+        if B * T and any(t is not None for t in (dq, dwq, dk, dwk)):
+            gq, gk = (None if g is None else _norm_rows(g) for g in grads)
+            need = _lib.lib().adkv_rope_norm_qk_backward_workspace_bytes
+            at = lambda t: None if t is None else t.data_ptr()
+            by = lambda t: None if t is None else _norm_strides(t)
+            with _lib.device_guard(dev):
+                size = 0
+                if dwq is not None or dwk is not None:
+                    size = need(D)
+                    _lib.check(min(size, 0), "rope_norm_qk")
+                workspace = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+                rc = _lib.lib().adkv_rope_norm_qk_backward(
+                    at(gq), at(gk), q.data_ptr(), k.data_ptr(), cos.data_ptr(), sin.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(),
+                    at(dq), at(dk), at(dwq), at(dwk), B, Hq, H, T, D, cos.shape[-1], ctx.eps, by(gq), by(gk), _norm_strides(q),
+                    _norm_strides(k), by(dq), by(dk), _norm_strides(cos), _NORM_DT[q.dtype], at(workspace), size,
+                    _lib.current_stream_ptr(dev))
+            _lib.check(rc, "rope_norm_qk")
+        return dq, dk, None, None, dwq, dwk, None
+
+
+def rope_norm_qk(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, q_weight: torch.Tensor,
+                 k_weight: torch.Tensor, eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMS norm of every head of ``q [B, Hq, T, D]`` and ``k [B, H, T, D]`` with its weight, then the rotary position
+    embedding, in one launch; differentiable.
+
+    ``y = x / sqrt(mean(x*x) + eps) * weight`` of every row, and ``y*cos + rotate_half(y)*sin`` of its first ``R`` channels, the
+    others as they are: :func:`rope_qk` for models that norm the heads first.  Computed in fp32 and rounded once.  fp16,
+    bf16 or fp32, all six tensors of one type; ``cos`` / ``sin``: ``[B, T, R]`` or ``[1, T, R]``, the weights ``[D]``; ``D`` and ``R`` multiples
+    of 8, ``R <= D <= 512``.  Any batch / head / token strides with contiguous channels are read in place; the results are contiguous.
+    Gradients reach ``q``, ``k`` and the weights (the latter's summed in fp32, in the same order every time), not the tables; those
+    of ``q`` and ``k`` are laid out as ``q`` and ``k`` are.
+    """
+    _chk(q.dim() == 4 and k.dim() == 4 and cos.dim() == 3 and sin.dim() == 3, "q, k must be [B, H, T, D] and cos, sin [B, T, R]")
+    B, Hq, T, D = q.shape
+    H, R = k.shape[1], cos.shape[-1]
+    _chk(k.shape[0] == B and k.shape[2] == T and k.shape[3] == D, "q and k disagree in shape")
+    _chk(q.dtype in _NORM_DT, "q must be float16, bfloat16 or float32")
+    _chk(all(t.dtype == q.dtype for t in (k, cos, sin, q_weight, k_weight)), "q, k, cos, sin and the weights must share one dtype")
+    _chk(cos.shape == sin.shape and cos.shape[1] == T and cos.shape[0] in (1, B), "cos, sin must be [B, T, R] or [1, T, R]")
+    _chk(0 < D <= 512 and D % 8 == 0, "head dim must be a multiple of 8 up to 512")
+    _chk(0 < R <= D and R % 8 == 0, "cos, sin must have a multiple of 8 channels, head dim at most")
+    _chk(q_weight.shape == (D,) and k_weight.shape == (D,), "the weights must be [head dim]")
+    _chk(Hq > 0 and H > 0, "q and k must have heads")
+    _chk(not (torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad)), "cos and sin have no gradient")
+    _need_device(q, k, cos, sin, q_weight, k_weight)
+    # copies where there have to be any are made here, where autograd sees them
+    q, k, cos, sin, q_weight, k_weight = (_norm_rows(t) for t in (q, k, cos, sin, q_weight, k_weight))
+    if sin.shape[0] * T and _norm_strides(sin)[:] != _norm_strides(cos)[:]:
+        cos, sin = (t.clone(memory_format=torch.contiguous_format) for t in (cos, sin))
+    wanted = torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, q_weight, k_weight))
+    return (_RopeNorm.apply if wanted else _rope_norm_forward)(q, k, cos, sin, q_weight, k_weight, float(eps))
+
+
 def softmax_scale_mask(logits: torch.Tensor, scaling: float,
                        mask: torch.Tensor | None = None) -> torch.Tensor:
     """``softmax(logits.float()*scaling + mask) -> fp16`` in one launch.

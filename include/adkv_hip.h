@@ -419,6 +419,38 @@ int adkv_rope_qk(const void *q, const void *k, const void *cos, const void *sin,
                  int64_t cs_sb, int64_t cs_st, int bf16, void *stream);
 
 /*
+ * RMS norm of every head of the query and key rows, its weight and the rotary position embedding in one launch (models whose attention
+ * norms its heads; the reference's has no such norm):
+ *   y = x / sqrt(mean(x^2) + eps) * weight          of each row x of D values
+ *   out = y * cos + rotate_half(y) * sin            of its first R values, the others as they are
+ * in fp32, each result rounded once.
+ *   q [B, Hq, T, D], k [B, H, T, D], cos, sin [B, T, R], q_weight, k_weight [D] of one type, dtype (ADKV_DT_*), channels contiguous;
+ *   q_strides, k_strides: element strides {batch, head, token};  table_strides: {batch, token} of cos and sin (0 over the batch for a shared table)
+ *   q_out, k_out   contiguous, of the same type
+ *   D, R           multiples of 8, R <= D <= 512; every row of everything at a multiple of four elements.  Rows of 16-bit types at multiples of 16 bytes
+ *                  whose R and D are multiples of 16 are faster.
+ */
+int adkv_rope_norm_qk(const void *q, const void *k, const void *cos, const void *sin, const void *q_weight, const void *k_weight,
+                      void *q_out, void *k_out, int B, int Hq, int H, int T, int D, int R, float eps, const int64_t *q_strides,
+                      const int64_t *k_strides, const int64_t *table_strides, int dtype, void *stream);
+
+/*
+ * Its gradients: from q_grad and k_grad, those of q_out and k_out, those of q, k and the weights.  The tables have none.
+ *   dq, dk, dq_weight, dk_weight   each may be NULL and is then not made; a side of which neither is made is not read at all
+ *   dq_strides, dk_strides         element strides {batch, head, token} of dq and dk, whose channels are contiguous
+ * The weights' gradients are sums over all rows in fp32, in an order that the sizes and the device alone decide: the same on every call.
+ * workspace: >= adkv_rope_norm_qk_backward_workspace_bytes(D) bytes, 4-byte aligned, read and written by this call only; not needed (NULL)
+ * without gradients of weights.
+ */
+int64_t adkv_rope_norm_qk_backward_workspace_bytes(int D);
+int adkv_rope_norm_qk_backward(const void *q_grad, const void *k_grad, const void *q, const void *k, const void *cos, const void *sin,
+                               const void *q_weight, const void *k_weight, void *dq, void *dk, void *dq_weight, void *dk_weight,
+                               int B, int Hq, int H, int T, int D, int R, float eps, const int64_t *q_grad_strides,
+                               const int64_t *k_grad_strides, const int64_t *q_strides, const int64_t *k_strides,
+                               const int64_t *dq_strides, const int64_t *dk_strides, const int64_t *table_strides, int dtype,
+                               void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
  * n new tokens of every sequence at once, over codes: quantised as tokens T..T+n-1 of the caches (as adkv_append_kv_pair does it)
  * and attended with.  Query i of a sequence looks at the prefix, if there is one, and at its own tokens 0..T+i:
  *   out = softmax(scaling * q.K^T + mask) V
