@@ -13,7 +13,9 @@ reference's cache object works unchanged.  What differs is underneath:
   every ``CKPT_INTERVAL`` tokens (4 bytes per channel per checkpoint, ~3 % of the codes at 256).
   The kernels keep it up to date and use it to replay the time axis in independent segments;
 * the filter state after the last prompt token is carried, so a prompt may be prefilled in chunks
-  (the reference refuses: llama_adkv.py:195-197).
+  (the reference refuses: llama_adkv.py:195-197);
+* several new tokens may be attended with at once (``extend``), and a batch may go on from one prefilled sequence whose codes it
+  shares (``share``); the reference has neither.
 """
 from __future__ import annotations
 
@@ -22,7 +24,7 @@ import math
 import torch
 
 from .. import _lib
-from ..kernel.gemv import append_kv_pair, decode_step, decode_step_workspace_bytes
+from ..kernel.gemv import SharedPrefix, append_kv_pair, decode_step, decode_step_workspace_bytes, extend
 
 SCALE_MIN = math.exp(-4.0)  # kept for API parity; the fp16 recurrence never clamps
 SCALE_MAX = math.exp(4.0)
@@ -73,17 +75,23 @@ class KVCacheLayer_ADKV:
         self._ckpt_interval = CKPT_INTERVAL
         self._views: dict = {}    # id(parameter) -> (parameter, its [H, C] view)
         self._shares_storage = False   # a batch_view(): its buffers belong to another layer object
+        # a share(): what every sequence begins with, (codes, codes, tokens, checkpoints, checkpoints, zp and sc behind it), K then V,
+        # [1, H, ..]; everything above is then of the tokens behind it
+        self._prefix: tuple | None = None
 
     # ------------------------------------------------------------------ HF cache protocol
     def get_seq_length(self) -> int:
-        return self._quant_len
+        return self._quant_len + self._prefix_len()
+
+    def _prefix_len(self) -> int:
+        return 0 if self._prefix is None else self._prefix[2]
 
     def get_mask_sizes(self, cache_position) -> tuple[int, int]:
         """(kv_length, kv_offset) for mask construction.  ``cache_position`` is the query's position
         tensor (transformers 5.3, the version the reference pins) or the query length as an int
         (later 5.x releases)."""
         q_len = cache_position if isinstance(cache_position, int) else cache_position.shape[0]
-        return self._quant_len + q_len, 0
+        return self.get_seq_length() + q_len, 0
 
     @property
     def key_states(self) -> torch.Tensor | None:
@@ -156,6 +164,8 @@ class KVCacheLayer_ADKV:
         prompt of a batch too big for one dense prefill can be quantised slice by slice
         through ``batch_view`` (the dense attention of a long prompt, not the cache, is what
         limits the batch of a single prefill call)."""
+        if self._prefix is not None:
+            raise ValueError("a shared cache is given its room by share()")
         self._init_buffers(B, H, C, torch.device(device))
         self._cap_buffers(tokens)
 
@@ -173,12 +183,35 @@ class KVCacheLayer_ADKV:
             v._key_ckpt, v._value_ckpt = self._key_ckpt[b0:b1], self._value_ckpt[b0:b1]
         v._key_state, v._value_state = self._key_state[b0:b1], self._value_state[b0:b1]
         v._state_valid, v._shares_storage = self._state_valid, True
+        v._prefix = self._prefix
+        return v
+
+    # ------------------------------------------------------------------ one prompt for a whole batch
+    def share(self, B: int, tokens: int = INIT_SEQ_LEN) -> "KVCacheLayer_ADKV":
+        """A layer object of ``B`` sequences that all begin with this one's tokens (a system prompt, a document, a prompt that several
+        answers are sampled for), with room for ``tokens`` more each.  This one holds one sequence, prefilled; its codes are held and
+        read once, not copied, and it may go on by itself.  Steps of the batch give no weights."""
+        if self._key_buf is None or self._B != 1 or self._C != 128 or self._quant_len == 0 or self._prefix is not None:
+            raise ValueError("only the cache of one prefilled sequence with head_dim 128 can be shared")
+        if not self._state_valid:
+            # decode steps append inside the attention kernels: the state behind the last token is not carried
+            raise NotImplementedError("a cache is shared before it is decoded with")
+        if B < 1:
+            raise ValueError("share needs at least one sequence")
+        v = KVCacheLayer_ADKV(self._bits)
+        v._ckpt_interval = self._ckpt_interval
+        ends = [tuple(st[0, :, :, i].contiguous() for i in range(2)) for st in (self._key_state, self._value_state)]
+        v._prefix = (self._key_buf, self._value_buf, self._quant_len, self._key_ckpt, self._value_ckpt, *ends)
+        v._init_buffers(B, self._H, self._C, self._device, v._capacity(INIT_SEQ_LEN, tokens))
         return v
 
     def commit(self, tokens: int) -> None:
         """Declare that every sequence now holds ``tokens`` quantised tokens (all slices prefilled)."""
+        tokens -= self._prefix_len()
         if tokens > self._cap_len:
             raise ValueError("more tokens than the cache holds")
+        if tokens < 0:
+            raise ValueError("fewer tokens than the shared prefix has")
         self._quant_len, self._state_valid = tokens, True
 
     def _check_geometry(self, B: int, H: int, C: int, device: torch.device):
@@ -204,6 +237,10 @@ class KVCacheLayer_ADKV:
         self._views[id(p)] = (p, v)
         return v
 
+    def _own(self, params: tuple, which: int) -> tuple:
+        """The parameters of this cache's own streams: behind a prefix they begin with its last state."""
+        return params if self._prefix is None else (*self._prefix[5 + which], *params[2:])
+
     # ------------------------------------------------------------------ quantise
     def _append_tokens(self, key_states, value_states,
                        key_zp_init, key_scale_init, key_alpha, key_beta, key_quant_target,
@@ -213,8 +250,8 @@ class KVCacheLayer_ADKV:
         append_kv_pair(
             self._key_buf, self._value_buf,
             self._rows(key_states), self._rows(value_states),
-            (key_zp_init, key_scale_init, key_alpha, key_beta, key_quant_target),
-            (value_zp_init, value_scale_init, value_alpha, value_beta, value_quant_target),
+            self._own((key_zp_init, key_scale_init, key_alpha, key_beta, key_quant_target), 0),
+            self._own((value_zp_init, value_scale_init, value_alpha, value_beta, value_quant_target), 1),
             self._quant_len, self._key_state, self._value_state,
             k_ckpt=self._key_ckpt, v_ckpt=self._value_ckpt, ckpt_interval=self._ckpt_interval, bits=self._bits, fresh=fresh)
         self._quant_len += key_states.shape[2]
@@ -263,8 +300,17 @@ class KVCacheLayer_ADKV:
                attention_mask: torch.Tensor | None = None,
                scaling: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
         """One causal decode step: attend over the cached tokens and the new one, append the new
-        K/V codes, return ``(output [B,H,C] in the query's dtype, weights [B,H,ctx+1] fp16)``."""
+        K/V codes, return ``(output [B,H,C] in the query's dtype, weights [B,H,ctx+1] fp16)``
+        (weights ``None`` behind a shared prefix)."""
         ctx = self._quant_len
+        if self._prefix is not None:
+            if query_states.shape[2] != 1 or key_states.shape[2] != 1:
+                raise ValueError("decode expects exactly one query/key/value token")
+            out = self.extend(query_states, key_states, value_states,
+                              key_zp_init, key_scale_init, key_alpha, key_beta, key_quant_target,
+                              value_zp_init, value_scale_init, value_alpha, value_beta, value_quant_target,
+                              attention_mask, scaling)
+            return out[:, 0], None
         if self._key_buf is not None and ctx < self._cap_len:
             r = _lib.host().decode(
                 query_states, key_states, value_states,
@@ -309,6 +355,47 @@ class KVCacheLayer_ADKV:
         self._state_valid = False
         return (out if out.dtype == query_states.dtype else out.to(query_states.dtype)), weights
 
+    # ------------------------------------------------------------------ several tokens
+    def extends(self, config=None) -> bool:
+        """Whether an attention module hands several new tokens over at once: behind a shared prefix always, else where
+        ``config.adkv_extend`` asks for it (one decode step after the other rounds the weights differently)."""
+        return self._prefix is not None or (self._C == 128 and bool(getattr(config, "adkv_extend", False)))
+
+    def extend(self, query_states, key_states, value_states,
+               key_zp_init, key_scale_init, key_alpha, key_beta, key_quant_target,
+               value_zp_init, value_scale_init, value_alpha, value_beta, value_quant_target,
+               attention_mask: torch.Tensor | None = None, scaling: float = 1.0) -> torch.Tensor:
+        """``n`` new tokens at once (head_dim 128): append their codes and attend, each over everything up to itself: a follow-up turn,
+        drafted tokens to be checked, the questions behind a shared prompt.  Queries ``[B, Hq, n, C]``, keys and values
+        ``[B, H, n, C]``; returns ``[B, n, Hq, C]`` in the query's dtype.  ``n`` calls of ``decode`` append the same codes and
+        give the same outputs up to rounding.  A mask is additive, or boolean (true where a token is looked at)."""
+        B, _, n, C = query_states.shape
+        H = key_states.shape[1]
+        if key_states.shape != value_states.shape or key_states.shape[2] != n:
+            raise ValueError("extend expects as many keys and values as queries")
+        if C != 128:
+            raise ValueError("extend needs head_dim 128")
+        self._check_geometry(B, H, C, query_states.device)
+        self._cap_buffers(self._quant_len + n)
+        key = (key_zp_init, key_scale_init, key_alpha, key_beta, key_quant_target)
+        value = (value_zp_init, value_scale_init, value_alpha, value_beta, value_quant_target)
+        prefix = None
+        if self._prefix is not None:
+            kc, vc, tokens, kck, vck = self._prefix[:5]
+            prefix = SharedPrefix(kc, vc, tokens, key, value, kck, vck)
+        if attention_mask is not None and attention_mask.dtype == torch.bool:
+            dt = query_states.dtype if query_states.dtype in (torch.float16, torch.bfloat16) else torch.float32
+            attention_mask = torch.zeros(attention_mask.shape, dtype=dt, device=attention_mask.device).masked_fill_(
+                ~attention_mask, torch.finfo(dt).min)
+        same = query_states.dtype in (torch.float16, torch.bfloat16) and key_states.dtype == query_states.dtype == value_states.dtype
+        act = (lambda t: t) if same else (lambda t: t.to(torch.float16))
+        out = extend(act(query_states), self._key_buf, self._value_buf, act(key_states), act(value_states),
+                     self._own(key, 0), self._own(value, 1), self._quant_len, scaling, attention_mask, prefix=prefix,
+                     k_ckpt=self._key_ckpt, v_ckpt=self._value_ckpt, ckpt_interval=self._ckpt_interval, bits=self._bits)
+        self._quant_len += n
+        self._state_valid = False
+        return out if out.dtype == query_states.dtype else out.to(query_states.dtype)
+
     # ------------------------------------------------------------------ save / restore
     def state_dict(self) -> dict:
         """Everything needed to continue decoding elsewhere: the used part of the code buffers, the
@@ -327,6 +414,14 @@ class KVCacheLayer_ADKV:
             sd["value_ckpt"] = self._value_ckpt[:, :, :nck].contiguous()
         if self._state_valid:
             sd["key_state"], sd["value_state"] = self._key_state.clone(), self._value_state.clone()
+        if self._prefix is not None:
+            key, value, tokens, kck, vck, ks, vs = self._prefix
+            ns, nck = self._n_super(tokens), tokens // self._ckpt_interval if self._ckpt_interval else 0
+            sd["prefix_len"] = tokens
+            sd["prefix_key_codes"], sd["prefix_value_codes"] = key[:, :, :ns].contiguous(), value[:, :, :ns].contiguous()
+            if self._ckpt_interval:
+                sd["prefix_key_ckpt"], sd["prefix_value_ckpt"] = kck[:, :, :nck].contiguous(), vck[:, :, :nck].contiguous()
+            sd["prefix_key_state"], sd["prefix_value_state"] = torch.stack(ks), torch.stack(vs)
         return sd
 
     def load_state_dict(self, sd: dict, device=None) -> None:
@@ -358,11 +453,23 @@ class KVCacheLayer_ADKV:
         if self._state_valid:
             self._key_state.copy_(sd["key_state"])
             self._value_state.copy_(sd["value_state"])
+        self._prefix = None
+        if "prefix_len" in sd:
+            P = int(sd["prefix_len"])
+            to = lambda name: sd[name].to(dev).contiguous() if name in sd else None
+            if tuple(sd["prefix_key_codes"].shape) != (1, H, self._n_super(P), C // 4, 4, 4):
+                raise ValueError("saved code tensor does not match its geometry")
+            if self._ckpt_interval and sd["prefix_key_ckpt"].shape[2] != P // self._ckpt_interval:
+                raise ValueError("saved checkpoints do not cover the saved tokens")
+            self._prefix = (to("prefix_key_codes"), to("prefix_value_codes"), P, to("prefix_key_ckpt"), to("prefix_value_ckpt"),
+                            tuple(to("prefix_key_state")), tuple(to("prefix_value_state")))
 
     # ------------------------------------------------------------------ accounting
     def nbytes(self) -> int:
-        """Device bytes held by this layer (codes + checkpoints)."""
+        """Device bytes held by this layer (codes + checkpoints), those of a shared prefix among them."""
         ts = (self._key_buf, self._value_buf, self._key_ckpt, self._value_ckpt)
+        if self._prefix is not None:
+            ts += tuple(self._prefix[i] for i in (0, 1, 3, 4))
         return sum(t.numel() * t.element_size() for t in ts if t is not None)
 
 
@@ -387,6 +494,12 @@ class KVCache_ADKV(list):
     def commit(self, tokens: int) -> None:
         for layer in self:
             layer.commit(tokens)
+
+    def share(self, B: int, tokens: int = INIT_SEQ_LEN) -> "KVCache_ADKV":
+        """A cache of ``B`` sequences that all begin with this one's tokens (see the layer's ``share``)."""
+        shared = KVCache_ADKV(0)
+        shared.extend(layer.share(B, tokens) for layer in self)
+        return shared
 
     def get_mask_sizes(self, cache_position, layer_idx: int) -> tuple[int, int]:
         return self[layer_idx].get_mask_sizes(cache_position)

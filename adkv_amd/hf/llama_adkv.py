@@ -18,12 +18,13 @@ from transformers.models.llama.modeling_llama import (
     LlamaDecoderLayer,
     LlamaForCausalLM,
     LlamaModel,
+    LlamaRMSNorm,
     apply_rotary_pos_emb,
     eager_attention_forward,
 )
 from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
 
-from ..kernel.gemv import rope_qk
+from ..kernel.gemv import rope_norm_qk, rope_qk
 from .cache import (CAP_LEN, INIT_SEQ_LEN, SCALE_MAX, SCALE_MIN, KVCache_ADKV,  # noqa: F401
                     KVCacheLayer_ADKV)
 
@@ -52,6 +53,27 @@ class LlamaAttention_ADKV(LlamaAttention):
                 # fp16 because the deployment recurrence is fp16; filled by load_adkv_config()
                 self.register_buffer(f"{side}_{name}", torch.empty(width, dtype=torch.float16),
                                      persistent=False)
+        # config.adkv_qk_norm: every head's queries and keys are normed before the rotation (extension; the reference's model has no such norm)
+        if getattr(config, "adkv_qk_norm", False):
+            self.q_norm = LlamaRMSNorm(self.head_dim, eps=config.rms_norm_eps)
+            self.k_norm = LlamaRMSNorm(self.head_dim, eps=config.rms_norm_eps)
+
+    def _rotate(self, q, k, cos, sin):
+        if hasattr(self, "q_norm"):
+            wq, wk = self.q_norm.weight, self.k_norm.weight
+            if (q.is_cuda and all(t.dtype == q.dtype for t in (cos, sin, wq, wk)) and cos.dim() == 3
+                    and q.dtype in (torch.float16, torch.bfloat16, torch.float32) and self.head_dim % 8 == 0 and self.head_dim <= 512):
+                # one launch for both norms and the rotation, and one for their gradients
+                return rope_norm_qk(q, k, cos, sin, wq, wk, self.q_norm.variance_epsilon)
+            return apply_rotary_pos_emb(self.q_norm(q), self.k_norm(k), cos, sin)
+        wants_grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad)
+        if (q.is_cuda and q.dtype in (torch.float16, torch.bfloat16) and cos.dtype == q.dtype
+                and cos.dim() == 3 and self.head_dim % 4 == 0 and not wants_grad):
+            # one launch instead of apply_rotary_pos_emb's ten, same values bit for bit.  The
+            # kernel has no backward pass: whenever autograd is recording, the differentiable
+            # expression the reference calls (llama_adkv.py:336-337) runs instead.
+            return rope_qk(q, k, cos, sin)
+        return apply_rotary_pos_emb(q, k, cos, sin)
 
     def _adkv_params(self, side: str) -> tuple[torch.Tensor, ...]:
         return tuple(getattr(self, f"{side}_{name}") for name in ADKV_PARAM_FIELDS)
@@ -78,15 +100,7 @@ class LlamaAttention_ADKV(LlamaAttention):
         k = self.k_proj(hidden_states).view(split).transpose(1, 2)
         v = self.v_proj(hidden_states).view(split).transpose(1, 2)
         cos, sin = position_embeddings
-        wants_grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad)
-        if (q.is_cuda and q.dtype in (torch.float16, torch.bfloat16) and cos.dtype == q.dtype
-                and cos.dim() == 3 and self.head_dim % 4 == 0 and not wants_grad):
-            # one launch instead of apply_rotary_pos_emb's ten, same values bit for bit.  The
-            # kernel has no backward pass: whenever autograd is recording, the differentiable
-            # expression the reference calls (llama_adkv.py:336-337) runs instead.
-            q, k = rope_qk(q, k, cos, sin)
-        else:
-            q, k = apply_rotary_pos_emb(q, k, cos, sin)
+        q, k = self._rotate(q, k, cos, sin)
 
         layer_cache = None
         if use_cache and past_key_values is not None:
@@ -100,6 +114,12 @@ class LlamaAttention_ADKV(LlamaAttention):
                 q, k, v, *self._adkv_params("key"), *self._adkv_params("value"),
                 attention_mask=attention_mask, scaling=self.scaling)
             return self.o_proj(ctx.reshape(*lead, -1).contiguous()), weights
+
+        if layer_cache is not None and layer_cache.get_seq_length() > 0 and layer_cache.extends(self.config):
+            # all of them at once, over the codes of the earlier ones
+            ctx = layer_cache.extend(q, k, v, *self._adkv_params("key"), *self._adkv_params("value"),
+                                     attention_mask=attention_mask, scaling=self.scaling)
+            return self.o_proj(ctx.reshape(*lead, -1)), None
 
         if layer_cache is not None and layer_cache.get_seq_length() > 0:
             # Several new tokens on top of a cache that already holds codes (a follow-up turn, a
