@@ -9,12 +9,15 @@
 // conversions and error messages.  A number is the library's return code.
 #include <algorithm>
 
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/record_function.h>
 #include <ATen/ops/empty_cuda_dispatch.h>
+#include <c10/core/GradMode.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/DeviceGuardImplInterface.h>
 
@@ -318,6 +321,278 @@ PyObject *append(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     return PyLong_FromLong(rc);
 }
 
+// extend(q, key codes, value codes, k_new, v_new, key params (five), value params (five), T, scaling, mask or None, prefix or
+//        None: (key codes, value codes, tokens, key params, value params, key checkpoints, value checkpoints),
+//        key checkpoints, value checkpoints, interval, bits)
+PyObject *extend(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    if (nargs != 15 || !unwatched() || !PyFloat_CheckExact(args[8]))
+        Py_RETURN_NONE;
+    const at::Tensor *t[5];
+    for (int i = 0; i < 5; i++)
+        if (!(t[i] = plain(args[i])) || t[i]->device() != t[0]->device())
+            Py_RETURN_NONE;
+    const at::Tensor &q = *t[0], &kc = *t[1], &vc = *t[2];
+    const long T = PyLong_AsLong(args[7]), interval = PyLong_AsLong(args[13]), bits = PyLong_AsLong(args[14]);
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    if (!half_type(q) || t[3]->scalar_type() != q.scalar_type() || t[4]->scalar_type() != q.scalar_type() || q.dim() != 4 ||
+        kc.dim() != 6 || kc.scalar_type() != at::kByte || vc.scalar_type() != at::kByte || kc.sizes() != vc.sizes() ||
+        !kc.is_contiguous() || !vc.is_contiguous() || (bits != 2 && bits != 4) || T < 0 || T >= INT32_MAX)
+        Py_RETURN_NONE;
+    const int64_t B = q.size(0), Hq = q.size(1), n = q.size(2), D = q.size(3), H = kc.size(1), n_super = kc.size(2), tps = 32 / bits;
+    if (B <= 0 || H <= 0 || n <= 0 || D != 128 || kc.size(0) != B || kc.size(3) * 4 != D || kc.size(4) != 4 || kc.size(5) != 4 ||
+        Hq % H || (Hq / H != 1 && Hq / H != 2 && Hq / H != 4 && Hq / H != 8) || B * Hq > INT32_MAX || n > INT32_MAX ||
+        (T + n + tps - 1) / tps > n_super || n_super * tps > INT32_MAX || !rows(q))
+        Py_RETURN_NONE;
+    const int64_t token[4] = {B, H, n, D};
+    int64_t strides[2][3], qs[3];
+    for (int i = 0; i < 2; i++) {
+        const at::Tensor &x = *t[3 + i];
+        if (x.sizes() != at::IntArrayRef(token) ||
+            (!x.is_contiguous() && (!rows(x) || x.stride(2) < D || x.stride(0) < 0 || x.stride(1) < 0)))
+            Py_RETURN_NONE;
+        for (int j = 0; j < 3; j++)
+            strides[i][j] = x.stride(j);
+    }
+    for (int j = 0; j < 3; j++)
+        qs[j] = q.size(j) > 1 ? q.stride(j) : 0;
+    const void *kp[5], *vp[5], *pkp[5], *pvp[5], *codes[2] = {};
+    void *ck[2], *pck[2] = {};
+    int64_t n_ckpt, p_ckpt = 0, P = 0, p_super = 0;
+    if (!pointers(args[5], 5, at::kHalf, H * D, q.device(), kp) || !pointers(args[6], 5, at::kHalf, H * D, q.device(), vp) ||
+        !checkpoints(args + 11, B, H, D, interval, bits, q.device(), ck, n_ckpt))
+        Py_RETURN_NONE;
+    if (args[10] != Py_None) {
+        if (!PyTuple_Check(args[10]) || PyTuple_GET_SIZE(args[10]) != 7)
+            Py_RETURN_NONE;
+        PyObject *const *p = &PyTuple_GET_ITEM(args[10], 0);
+        P = PyLong_AsLong(p[2]);
+        if (PyErr_Occurred()) {
+            PyErr_Clear();
+            Py_RETURN_NONE;
+        }
+        const at::Tensor *c[2] = {plain(p[0]), plain(p[1])};
+        for (int i = 0; i < 2; i++) {
+            if (!c[i] || c[i]->device() != q.device() || c[i]->scalar_type() != at::kByte || c[i]->dim() != 6 || !c[i]->is_contiguous() ||
+                c[i]->size(0) != 1 || c[i]->size(1) != H || c[i]->size(3) * 4 != D || c[i]->size(4) != 4 || c[i]->size(5) != 4 ||
+                c[i]->sizes() != c[0]->sizes())
+                Py_RETURN_NONE;
+            codes[i] = c[i]->const_data_ptr();
+        }
+        p_super = c[0]->size(2);
+        if (P <= 0 || P >= INT32_MAX || (P + tps - 1) / tps > p_super || p_super * tps > INT32_MAX ||
+            !pointers(p[3], 5, at::kHalf, H * D, q.device(), pkp) || !pointers(p[4], 5, at::kHalf, H * D, q.device(), pvp) ||
+            !checkpoints(p + 5, 1, H, D, interval, bits, q.device(), pck, p_ckpt))
+            Py_RETURN_NONE;
+    }
+    const void *mask = nullptr;
+    int64_t ms[3] = {};
+    int mask_type = ADKV_DT_F32;
+    if (args[9] != Py_None) {
+        const at::Tensor *m = plain(args[9]);
+        if (!m || m->device() != q.device() || m->dim() != 4 || m->size(3) != P + T + n || (m->size(0) != 1 && m->size(0) != B) ||
+            (m->size(1) != 1 && m->size(1) != Hq) || (m->size(2) != 1 && m->size(2) != n) || m->stride(3) != 1 ||
+            (!half_type(*m) && m->scalar_type() != at::kFloat))
+            Py_RETURN_NONE;
+        for (int j = 0; j < 3; j++)
+            ms[j] = m->size(j) > 1 ? m->stride(j) : 0;
+        mask_type = m->scalar_type() == at::kFloat ? ADKV_DT_F32 : m->scalar_type() == at::kHalf ? ADKV_DT_F16 : ADKV_DT_BF16;
+        mask = m->const_data_ptr();
+    }
+    void *stream;
+    if (!current(q.device(), stream))
+        Py_RETURN_NONE;
+    const int iv = ck[0] ? (int)interval : 0, piv = pck[0] ? (int)interval : 0;
+    const int64_t bytes = adkv_extend_workspace_bytes((int)B, (int)Hq, (int)H, (int)T, (int)n, (int)n_ckpt, iv, (int)P, (int)p_ckpt, piv);
+    if (bytes < 0)
+        Py_RETURN_NONE;
+    at::Tensor out = fresh({B, n, Hq, D}, q, q.scalar_type()), work = fresh({bytes}, q, at::kByte);
+    if (!out.has_storage() || !work.has_storage())
+        Py_RETURN_NONE;
+    void *op = out.mutable_data_ptr(), *wp = work.mutable_data_ptr(), *kcp = kc.mutable_data_ptr(), *vcp = vc.mutable_data_ptr();
+    const void *in[3] = {q.const_data_ptr(), t[3]->const_data_ptr(), t[4]->const_data_ptr()};
+    const int64_t *ks = t[3]->is_contiguous() ? nullptr : strides[0], *vs = t[4]->is_contiguous() ? nullptr : strides[1];
+    const adkv_prefix prefix = {codes[0], codes[1], pkp, pvp, pck[0], pck[1], (int)P, (int)p_super, (int)p_ckpt, piv};
+    const double scaling = PyFloat_AS_DOUBLE(args[8]);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = adkv_extend(in[0], qs, kcp, vcp, in[1], in[2], ks, vs, kp, vp, mask, mask ? ms : nullptr, (float)scaling, op, (int)B, (int)Hq, (int)H,
+                     (int)T, (int)n, (int)D, (int)n_super, (int)bits,
+                     (q.scalar_type() == at::kBFloat16 ? ADKV_DT_BF16 : ADKV_DT_F16) | ADKV_MASK_DT(mask_type), ck[0], ck[1], (int)n_ckpt, iv,
+                     P > 0 ? &prefix : nullptr, wp, bytes, stream);
+    Py_END_ALLOW_THREADS
+    return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(std::move(out));
+}
+
+// rows of four elements each, 16 bytes of fp32: what rope_norm_qk reads in place
+bool fours(const at::Tensor &t)
+{
+    const auto st = t.strides();
+    if (st.back() != 1 || (uintptr_t)t.const_data_ptr() % (4 * t.element_size()))
+        return false;
+    for (size_t j = 0; j + 1 < st.size(); j++)
+        if (t.size(j) > 1 && st[j] % 4)
+            return false;
+    return true;
+}
+
+struct Strides { // of all axes but the last, 0 along one of a single element
+    int64_t of[3] = {};
+    Strides() = default;
+    explicit Strides(const at::Tensor &t)
+    {
+        for (int64_t j = 0; j + 1 < t.dim() && j < 3; j++)
+            of[j] = t.size(j) > 1 ? t.stride(j) : 0;
+    }
+};
+
+int number(at::ScalarType t) { return t == at::kFloat ? ADKV_DT_F32 : t == at::kHalf ? ADKV_DT_F16 : ADKV_DT_BF16; }
+
+void complain(int rc)
+{
+    TORCH_CHECK(rc == 0, "rope_norm_qk: ", adkv_strerror(rc));
+}
+
+// the thread holds the interpreter's lock; false: on another device than the current one, or an odd allocation
+bool norm_forward(const at::Tensor *const *t, double eps, at::Tensor &qo, at::Tensor &ko, int &rc)
+{
+    const at::Tensor &q = *t[0], &k = *t[1], &c = *t[2];
+    void *stream;
+    if (!current(q.device(), stream))
+        return false;
+    qo = fresh(q.sizes(), q, q.scalar_type());
+    ko = fresh(k.sizes(), q, q.scalar_type());
+    if (!qo.has_storage() || !ko.has_storage())
+        return false;
+    void *qp = qo.mutable_data_ptr(), *kp = ko.mutable_data_ptr();
+    const void *in[6];
+    for (int i = 0; i < 6; i++)
+        in[i] = t[i]->const_data_ptr();
+    const Strides qs(q), ks(k), cs(c);
+    Py_BEGIN_ALLOW_THREADS
+    rc = adkv_rope_norm_qk(in[0], in[1], in[2], in[3], in[4], in[5], qp, kp, (int)q.size(0), (int)q.size(1), (int)k.size(1), (int)q.size(2),
+                           (int)q.size(3), (int)c.size(2), (float)eps, qs.of, ks.of, cs.of, number(q.scalar_type()), stream);
+    Py_END_ALLOW_THREADS
+    return true;
+}
+
+// laid out as t where the kernels can write that
+at::Tensor alike(const at::Tensor &t)
+{
+    at::Tensor to = at::empty_like(t);
+    return to.stride(-1) == 1 && fours(to) ? to : at::empty(t.sizes(), t.options());
+}
+
+struct RopeNorm : torch::autograd::Function<RopeNorm> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const at::Tensor &q, const at::Tensor &k,
+                                                  const at::Tensor &cos, const at::Tensor &sin, const at::Tensor &q_weight,
+                                                  const at::Tensor &k_weight, double eps)
+    {
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({q, k, cos, sin, q_weight, k_weight});
+        ctx->saved_data["eps"] = eps;
+        const at::Tensor *t[6] = {&q, &k, &cos, &sin, &q_weight, &k_weight};
+        at::Tensor qo, ko;
+        int rc = 0;
+        TORCH_CHECK(norm_forward(t, eps, qo, ko, rc), "rope_norm_qk: the tensors left the current device");
+        complain(rc);
+        return {qo, ko};
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads)
+    {
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &q = saved[0], &k = saved[1], &c = saved[2];
+        const c10::DeviceGuard guard(q.device());
+        at::Tensor made[4], g[2]; // dq, dk and the weights' gradients
+        {
+            const at::NoGradGuard off;
+            for (int i = 0; i < 2; i++) {
+                if (!grads[i].defined())
+                    continue; // nobody used that result
+                g[i] = fours(grads[i]) ? grads[i] : grads[i].clone(at::MemoryFormat::Contiguous);
+                if (ctx->needs_input_grad(i))
+                    made[i] = alike(saved[i]);
+                if (ctx->needs_input_grad(4 + i))
+                    made[2 + i] = at::empty_like(saved[4 + i]);
+            }
+            const bool weights = made[2].defined() || made[3].defined();
+            const int64_t bytes = weights ? adkv_rope_norm_qk_backward_workspace_bytes((int)q.size(3)) : 0;
+            complain((int)std::min<int64_t>(bytes, 0));
+            at::Tensor work = weights ? at::empty({bytes}, q.options().dtype(at::kByte)) : at::Tensor();
+            const auto to = [](at::Tensor &t) { return t.defined() ? t.mutable_data_ptr() : nullptr; };
+            const auto from = [](const at::Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; };
+            const auto by = [](const at::Tensor &t) { return t.defined() ? Strides(t) : Strides(); };
+            const Strides gs[2] = {by(g[0]), by(g[1])}, xs[2] = {Strides(q), Strides(k)}, ds[2] = {by(made[0]), by(made[1])}, cs(c);
+            void *stream;
+            const PyGILState_STATE lock = PyGILState_Ensure();
+            const bool there = current(q.device(), stream);
+            PyGILState_Release(lock);
+            TORCH_CHECK(there, "rope_norm_qk: no current stream");
+            complain(adkv_rope_norm_qk_backward(from(g[0]), from(g[1]), from(q), from(k), from(c), from(saved[3]), from(saved[4]), from(saved[5]),
+                                                to(made[0]), to(made[1]), to(made[2]), to(made[3]), (int)q.size(0), (int)q.size(1), (int)k.size(1),
+                                                (int)q.size(2), (int)q.size(3), (int)c.size(2), (float)ctx->saved_data["eps"].toDouble(), gs[0].of,
+                                                gs[1].of, xs[0].of, xs[1].of, ds[0].of, ds[1].of, cs.of, number(q.scalar_type()), to(work), bytes,
+                                                stream));
+        }
+        torch::autograd::variable_list all = {made[0], made[1], {}, {}, made[2], made[3], {}};
+        if (c10::GradMode::is_enabled()) {
+            // a gradient of these gradients is refused when it is asked for, not here
+            torch::autograd::variable_list some;
+            for (at::Tensor &t : made)
+                if (t.defined())
+                    some.push_back(t.detach().set_requires_grad(true));
+            const auto refuse = std::make_shared<torch::autograd::DelayedError>("rope_norm_qk can be differentiated once only", (int64_t)some.size());
+            some = (*refuse)(std::move(some));
+            size_t n = 0;
+            for (const int i : {0, 1, 4, 5})
+                if (all[i].defined())
+                    all[i] = some[n++];
+        }
+        return all;
+    }
+};
+
+// rope_norm_qk(q, k, cos, sin, q weight, k weight, eps)
+PyObject *rope_norm_qk(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    if (nargs != 7 || !unwatched() || !PyFloat_CheckExact(args[6]))
+        Py_RETURN_NONE;
+    const at::Tensor *t[6];
+    bool record = false;
+    for (int i = 0; i < 6; i++) {
+        if (!(t[i] = plain(args[i])) || t[i]->scalar_type() != t[0]->scalar_type() || t[i]->device() != t[0]->device() ||
+            t[i]->dim() != (i < 2 ? 4 : i < 4 ? 3 : 1) || !fours(*t[i]))
+            Py_RETURN_NONE;
+        if (t[i]->requires_grad() && c10::GradMode::is_enabled()) {
+            if (i == 2 || i == 3)
+                Py_RETURN_NONE;
+            record = true;
+        }
+    }
+    const at::Tensor &q = *t[0], &k = *t[1], &c = *t[2], &s = *t[3];
+    const int64_t B = q.size(0), Hq = q.size(1), T = q.size(2), D = q.size(3), H = k.size(1), R = c.size(2);
+    if ((!half_type(q) && q.scalar_type() != at::kFloat) || k.size(0) != B || k.size(2) != T || k.size(3) != D || c.sizes() != s.sizes() ||
+        c.size(1) != T || (c.size(0) != 1 && c.size(0) != B) || t[4]->size(0) != D || t[5]->size(0) != D || D <= 0 || D > 512 || D % 8 ||
+        R <= 0 || R > D || R % 8 || B <= 0 || T <= 0 || H <= 0 || Hq <= 0 || B > INT32_MAX || T > INT32_MAX || Hq > INT32_MAX || H > INT32_MAX)
+        Py_RETURN_NONE;
+    const Strides cs(c), ss(s);
+    if (cs.of[0] != ss.of[0] || cs.of[1] != ss.of[1])
+        Py_RETURN_NONE;
+    const double eps = PyFloat_AS_DOUBLE(args[6]);
+    if (record) {
+        auto z = RopeNorm::apply(q, k, c, s, *t[4], *t[5], eps);
+        return pair(std::move(z[0]), std::move(z[1]));
+    }
+    at::Tensor qo, ko;
+    int rc;
+    if (!norm_forward(t, eps, qo, ko, rc))
+        Py_RETURN_NONE;
+    return rc ? PyLong_FromLong(rc) : pair(std::move(qo), std::move(ko));
+}
+
 // quant_f32(x, (alpha, beta, target, zp_init, sc_init), lower, upper, sc_min, sc_max, output_states, free_params)
 //   -> (xhat, zp sequence or None, sc sequence or None)
 PyObject *quant_f32(PyObject *, PyObject *const *args, Py_ssize_t nargs)
@@ -438,6 +713,8 @@ PyMethodDef methods[] = {
     {"init", init, METH_O, "init(function from device index to raw stream)"},
     {"rope_qk", (PyCFunction)(void (*)(void))guarded<rope_qk>, METH_FASTCALL, nullptr},
     {"decode", (PyCFunction)(void (*)(void))guarded<decode>, METH_FASTCALL, nullptr},
+    {"extend", (PyCFunction)(void (*)(void))guarded<extend>, METH_FASTCALL, nullptr},
+    {"rope_norm_qk", (PyCFunction)(void (*)(void))guarded<rope_norm_qk>, METH_FASTCALL, nullptr},
     {"append", (PyCFunction)(void (*)(void))guarded<append>, METH_FASTCALL, nullptr},
     {"quant_f32", (PyCFunction)(void (*)(void))guarded<quant_f32>, METH_FASTCALL, nullptr},
     {"quant_f32_pair", (PyCFunction)(void (*)(void))guarded<quant_f32_pair>, METH_FASTCALL, nullptr},

@@ -591,6 +591,11 @@ def rope_norm_qk(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
     Gradients reach ``q``, ``k`` and the weights (the latter's summed in fp32, in the same order every time), not the tables; those
     of ``q`` and ``k`` are laid out as ``q`` and ``k`` are.
     """
+    r = _lib.host().rope_norm_qk(q, k, cos, sin, q_weight, k_weight, eps)      # None: something to record, check or convert
+    if r is not None:
+        if isinstance(r, int):
+            _lib.check(r, "rope_norm_qk")
+        return r
     _chk(q.dim() == 4 and k.dim() == 4 and cos.dim() == 3 and sin.dim() == 3, "q, k must be [B, H, T, D] and cos, sin [B, T, R]")
     B, Hq, T, D = q.shape
     H, R = k.shape[1], cos.shape[-1]
@@ -803,6 +808,13 @@ def extend(
     Returns ``[B, n, Hq, 128]`` in ``q``'s type.  Rows that the mask leaves nothing of are NaN.
     """
     k_params, v_params = tuple(k_params), tuple(v_params)
+    if workspace is None:
+        r = _lib.host().extend(q, k_cache, v_cache, k_new, v_new, k_params, v_params, T, scaling, mask, prefix, k_ckpt, v_ckpt,
+                               ckpt_interval, bits)
+        if r is not None:      # None: something to check, convert or complain about below
+            if isinstance(r, int):
+                _lib.check(r, "extend")
+            return r
     act = q.dtype
     _chk(act in (torch.float16, torch.bfloat16), "q must be float16 or bfloat16")
     _chk(k_new.dtype == act and v_new.dtype == act, "k_new and v_new must have q's type")

@@ -317,3 +317,41 @@ def test_the_library_refuses_before_any_launch():
     pre = lambda **k: ctypes.byref(_lib.Prefix(**{**dict(k_codes=256, v_codes=256, k_params=arr, v_params=arr, tokens=8, n_super=1), **k}))
     assert call(prefix=pre(k_codes=None)) == -1 and call(prefix=pre(tokens=9)) == -4 and call(prefix=pre(tokens=-1)) == -3
     assert call(prefix=pre(k_ckpt=256)) == -1 and call(prefix=pre(k_codes=260)) == -5
+
+
+def test_host_calls_that_are_left_to_python():
+    h = _lib.host()
+    x = torch.zeros(1, 1, 1, 128, dtype=torch.float16)
+    for f, n in ((h.extend, 15), (h.rope_norm_qk, 7)):
+        assert f() is None and f(*[None] * n) is None and f(*[x] * n) is None and f(*[1 << 70] * n) is None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(3, 2, 2, 150, 70, 1), (2, 1, 4, 97, 33, 40), (2, 2, 1, 0, 20, 9), (2, 2, 1, 30, 0, 3)])
+@pytest.mark.parametrize("mask_type", [None, torch.bfloat16, torch.float32])
+def test_host_calls_equal_the_python_function(gpu, oracle, monkeypatch, size, mask_type):
+    """The same call through the host calls and without them: the same codes, checkpoints and outputs."""
+    import types
+    B, H, G, P, T, n = size
+    results = []
+    real = _lib.host()
+    for taken in (True, False):
+        c = Case(oracle, gpu, *size, dtype=torch.bfloat16, seed=11)
+        mask = None
+        if mask_type is not None:
+            mask = torch.zeros(B, 1, n, P + T + n, dtype=mask_type)
+            mask[0, :, :, :(P + T) // 2] = torch.finfo(mask_type).min
+            mask = mask.to(gpu)
+        calls = []
+
+        def extend(*a):
+            r = real.extend(*a) if taken else None
+            calls.append(r is not None)
+            return r
+        monkeypatch.setattr(_lib, "host", lambda: types.SimpleNamespace(extend=extend))
+        out = c.run(D ** -0.5, mask)
+        monkeypatch.undo()
+        assert calls == [taken]
+        results.append([out.view(torch.int16), *c.cache, *[t.view(torch.int16) for t in c.ckpt]])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)

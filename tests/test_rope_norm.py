@@ -349,3 +349,54 @@ def test_c_refusals():
     assert back(grad=p + 2) == -5
     assert back(dq=None) == 0
     assert lib.adkv_rope_norm_qk_backward_workspace_bytes(0) == -2 and lib.adkv_rope_norm_qk_backward_workspace_bytes(513) == -2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_host_call_equals_the_python_function(monkeypatch, dtype):
+    import types
+    real = _lib.host()
+    for size, kw in (((2, 4, 2, 37, 128, 64), {}), ((1, 3, 1, 5, 80, 80), {"rows": "heads first"}), ((3, 2, 2, 1, 64, 64), {"shared_table": True})):
+        s = make(*size, dtype, **kw)
+        got = real.rope_norm_qk(s["q"], s["k"], s["cos"], s["sin"], s["wq"], s["wk"], EPS)
+        monkeypatch.setattr(_lib, "host", lambda: types.SimpleNamespace(rope_norm_qk=lambda *a: None))
+        want = call(s)
+        monkeypatch.undo()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        # with gradients
+        leaves = [s[n].detach().requires_grad_() for n in ("q", "k", "wq", "wk")]
+        grads = []
+        for taken in (True, False):
+            if not taken:
+                monkeypatch.setattr(_lib, "host", lambda: types.SimpleNamespace(rope_norm_qk=lambda *a: None))
+            z = gemv.rope_norm_qk(leaves[0], leaves[1], s["cos"], s["sin"], leaves[2], leaves[3], EPS)
+            assert ("_RopeNorm" in type(z[0].grad_fn).__name__) == (not taken)
+            grads.append(torch.autograd.grad(z, leaves, (s["gq"], s["gk"].transpose(0, 2).contiguous().transpose(0, 2))))
+            monkeypatch.undo()
+        assert all(torch.equal(a, b) and a.stride() == b.stride() for a, b in zip(*grads))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("taken", (True, False))
+def test_differentiated_once_only(monkeypatch, taken):
+    import types
+    if not taken:
+        monkeypatch.setattr(_lib, "host", lambda: types.SimpleNamespace(rope_norm_qk=lambda *a: None))
+    s = make(2, 3, 1, 6, 64, 64, torch.float32)
+    s["q"] = s["q"].detach().requires_grad_()
+    z = call(s)
+    first, = torch.autograd.grad(z[0], s["q"], s["gq"].requires_grad_(), create_graph=True)
+    plain, = torch.autograd.grad(call(s)[0], s["q"], s["gq"])
+    assert torch.equal(first, plain)
+    with pytest.raises(RuntimeError, match="once"):
+        first.sum().backward()
+
+
+@pytest.mark.gpu
+def test_a_changed_input_is_noticed():
+    s = make(2, 3, 1, 6, 64, 64, torch.float32)
+    s["wq"].requires_grad_()
+    z = call(s)
+    s["q"] += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(z[0], s["wq"], s["gq"])
