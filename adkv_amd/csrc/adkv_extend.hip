@@ -87,8 +87,6 @@ struct Args {
     const void *mask;
     long m_sb, m_sh, m_st;
     int mask_dt;
-    const uint32_t *mask_bits; // see mask_tiles_kernel; may be null
-    int mask_words, mask_own_tile;
     float *partial; // [partial results, rows, D]
     float2 *ml;     // [partial results, rows]: m, l
     h1 *out;        // not null: a row has one partial result, and goes here
@@ -513,10 +511,6 @@ struct Consumer {
     int limit[NB];        // tokens of the source that it looks at
     const char *mask[NB]; // its mask at the source's first token
     int seen, tokens;     // of the source: what every row looks at, all
-    const uint32_t *bits[NB]; // many rows: which of the mask's tiles have anything in them, from the source's first tile on; may be null
-    int bit0, from;           // the source's first tile among all; the span's first token
-    uint32_t word[NB];        // of the tiles around the present one
-    bool masked[NB];          // this tile's mask was loaded
     MaskRaw<J, MASK> masks[NB];
 
     // of row r of a unit: sequence, token, query head
@@ -582,12 +576,6 @@ struct Consumer {
             limit[k] = s.causal ? s.seen + i : s.seen;
             if constexpr (MASK != 0)
                 mask[k] = (const char *)a.mask + (b * a.m_sb + hq * a.m_sh + i * a.m_st + s.col) * (MASK == 2 ? 4 : 2);
-            if constexpr (MASK != 0 && !FEW) {
-                bits[k] = a.mask_bits != nullptr ? a.mask_bits + ((long)b * a.n + i) * a.mask_words : nullptr;
-                bit0 = at.src ? a.mask_own_tile : 0;
-                from = at.t0;
-                word[k] = ~0u;
-            }
         }
     }
 
@@ -595,20 +583,10 @@ struct Consumer {
     template <int NA> __device__ __forceinline__ void look_at(int t, int lane)
     {
         if constexpr (MASK != 0) {
-            const int tile = FEW ? 0 : bit0 + t / TILE, first = t;
             t += (lane >> 4) * 4;
 #pragma unroll
-            for (int k = 0; k < NA; k++) {
-                if constexpr (FEW) {
-                    masked[k] = true;
-                } else {
-                    if (bits[k] != nullptr && (first == from || (tile & 31) == 0))
-                        word[k] = global(bits[k])[tile >> 5];
-                    masked[k] = __any(word[k] >> (tile & 31) & 1);
-                }
-                if (masked[k])
-                    masks[k].load(mask[k], t, tokens - t);
-            }
+            for (int k = 0; k < NA; k++)
+                masks[k].load(mask[k], t, tokens - t);
         }
     }
     // the scores of the step-th step of a tile, as q.K
@@ -651,15 +629,8 @@ struct Consumer {
 #pragma unroll
             for (int e = 0; e < 4 * J; e++)
                 x[e] = sc[k][e >> 2][e & 3];
-            if constexpr (MASK != 0) {
-                if (masked[k]) {
-                    masks[k].add(x, a.scaling, a.mask_dt);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4 * J; e++)
-                        x[e] *= a.scaling;
-                }
-            }
+            if constexpr (MASK != 0)
+                masks[k].add(x, a.scaling, a.mask_dt);
             if (t + 16 * J > seen) {
 #pragma unroll
                 for (int e = 0; e < 4 * J; e++)
@@ -780,11 +751,13 @@ __device__ __forceinline__ void consume(KArgs &a, int items, const char *tiles, 
         opened = ends;
         c.template look_at<1>(t, lane);
         __syncthreads();
-        f4v sc[1][1];
-        uint32_t w[1][2];
-        c.template scores<1>(from, step, lane, sc);
-        c.template weights<1>(a, t, lane, sc, w);
-        c.template outputs<1>(from + FEW_VALUES + c0 * 2048, step, lane, w);
+        if (t < c.tokens) { // of a span's last tile half may be empty
+            f4v sc[1][1];
+            uint32_t w[1][2];
+            c.template scores<1>(from, step, lane, sc);
+            c.template weights<1>(a, t, lane, sc, w);
+            c.template outputs<1>(from + FEW_VALUES + c0 * 2048, step, lane, w);
+        }
         if (!ends) {
             at.go(a);
             return false;
@@ -993,30 +966,6 @@ __global__ __launch_bounds__(ITEMS * 256) void values_kernel(Images im)
     }
 }
 
-// Which tiles of a mask's rows have anything in them: a bit per tile of 64 tokens, the prefix's tiles, then the own ones.  A mask that is the same for
-// all heads is read by each of them, tile by tile as long as the tile itself, and is mostly zero: a batch's padding and the tokens behind a query.
-template <typename E>
-__global__ __launch_bounds__(256) void mask_tiles_kernel(const E *mask, long m_sb, long m_st, int n, long jobs, int P, int own, uint32_t *bits, int words)
-{
-    const long job = (long)blockIdx.x * 4 + (threadIdx.x >> 6); // a word of a row
-    if (job >= jobs)
-        return;
-    const long row = job / words;
-    const int w = (int)(job - row * words), lane = threadIdx.x & 63, tiles_p = (P + TILE - 1) / TILE, tiles = tiles_p + (own + TILE - 1) / TILE;
-    const E *p = mask + row / n * m_sb + row % n * m_st;
-    uint32_t mine = 0;
-#pragma unroll 16
-    for (int i = 0; i < 32; i++) {
-        const int k = w * 32 + i, t = (k < tiles_p ? k : k - tiles_p) * TILE + lane;
-        const bool there = k < tiles && t < (k < tiles_p ? P : own);
-        // behind the end the row's first element, for nothing
-        const E v = p[there ? (k < tiles_p ? 0 : P) + t : 0];
-        mine |= __any(there && v != 0) ? 1u << i : 0u;
-    }
-    if (lane == 0)
-        bits[job] = mine;
-}
-
 // A tile in 32 loads of 1 KB straight to the LDS, four by each of eight waves.
 struct Fetch {
     uint32_t from, to;
@@ -1186,16 +1135,24 @@ __global__ __launch_bounds__(128) void state_kernel(Source s, int H, int n_ckpt,
     h2 from = {t.zp[pi], t.sc[pi]};
     if (first > 0)
         from = as_h2(*reinterpret_cast<const uint32_t *>(t.ckpt + (((size_t)unit * n_ckpt + first - 1) * D + c) * 2));
-    Lone st;
-    st.z = as_u32((h2){from.x, (h1)0.0f});
-    st.r = as_u32((h2){(h1)0.0f, from.y});
-    st.ca = as_u32((h2){t.al[pi], one});
-    st.cf = as_u32((h2){one, be});
-    st.c0 = as_u32((h2){(h1)0.0f, one - bt});
+    const h1 al = t.al[pi], omt = one - bt;
+    h1 zp = from.x, sc = from.y;
+    // token k of a word, whose code and factor of the scale wait for nothing
+    auto token = [&](h1 q, h1 f) __attribute__((always_inline)) {
+        zp = __builtin_fmaf16(al, q * sc, zp);
+        sc = sc * f;
+    };
+    auto pair = [&](uint32_t w, int k, h2 &q, h2 &f) __attribute__((always_inline)) {
+        constexpr uint32_t FIELD = Code<BITS>::FIELD;
+        const int at = 2 * BITS * k;
+        const uint32_t lo = w >> at & FIELD, hi = w >> (at + BITS) & FIELD;
+        q = as_h2(0x64006400u | hi << 16 | lo) - splat((h1)(1024 - Code<BITS>::QLO)); // 1024 + code, then exact
+        f = __builtin_elementwise_fma(splat(be), as_h2(as_u32(q) & 0x7FFF7FFFu), splat(omt));
+    };
     const uint32_t *w = t.codes + (size_t)unit * s.x.n_super * D + c;
     constexpr int AHEAD = 8;
     uint32_t buf[2][AHEAD];
-    const int at0 = first * s.x.interval / TPW, words = (T + TPW - 1) / TPW;
+    const int at0 = first * s.x.interval / TPW, words = (T + TPW - 1) / TPW, whole = T / TPW;
     auto load = [&](int at, uint32_t *b) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < AHEAD; i++)
@@ -1205,16 +1162,32 @@ __global__ __launch_bounds__(128) void state_kernel(Source s, int H, int n_ckpt,
     for (int at = at0; at < words; at += AHEAD) {
         load(at + AHEAD, buf[1]);
 #pragma unroll
-        for (int i = 0; i < AHEAD; i++)
+        for (int i = 0; i < AHEAD; i++) {
+            if (at + i < whole) {
 #pragma unroll
-            for (int k = 0; k < TPW; k++)
-                if ((at + i) * TPW + k < T)
-                    lone_token(st, (int)(buf[0][i] >> (BITS * k) & Code<BITS>::FIELD) + Code<BITS>::QLO);
+                for (int k = 0; k < TPW / 2; k++) {
+                    h2 q, f;
+                    pair(buf[0][i], k, q, f);
+                    token(q.x, f.x);
+                    token(q.y, f.y);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < TPW / 2; k++) {
+                    h2 q, f;
+                    pair(buf[0][i], k, q, f);
+                    if ((at + i) * TPW + 2 * k < T)
+                        token(q.x, f.x);
+                    if ((at + i) * TPW + 2 * k + 1 < T)
+                        token(q.y, f.y);
+                }
+            }
+        }
 #pragma unroll
         for (int i = 0; i < AHEAD; i++)
             buf[0][i] = buf[1][i];
     }
-    const uint32_t zs = as_u32((h2){lone_zp(st), lone_sc(st)});
+    const uint32_t zs = as_u32((h2){zp, sc});
     *reinterpret_cast<uint32_t *>((blockIdx.y ? v_state : k_state) + ((size_t)unit * D + c) * 2) = zs;
     if (s.x.interval > 0 && T % s.x.interval == 0 && T / s.x.interval - 1 < n_ckpt)
         *reinterpret_cast<uint32_t *>(const_cast<h1 *>(t.ckpt) + (((size_t)unit * n_ckpt + T / s.x.interval - 1) * D + c) * 2) = zs;
@@ -1300,9 +1273,6 @@ static Plan plan(int B, int H, int G, int n, int P, int p_interval, int p_ckpt, 
 }
 
 static int64_t pad256(int64_t n) { return (n + 255) & ~(int64_t)255; }
-// of which tiles a mask has something in
-static int mask_words(const Plan &p) { return (p.tiles[0] + p.tiles[1] + 31) / 32; }
-static int64_t bits_bytes(const Plan &p, int B, int n) { return p.image[0] || p.image[1] ? pad256((int64_t)B * n * mask_words(p) * 4) : 0; }
 
 } // namespace adkv_ext
 
@@ -1318,7 +1288,7 @@ int64_t adkv_extend_workspace_bytes(int B, int Hq, int H, int T, int n, int n_ck
     const Plan p = plan(B, H, Hq / H, n, P, prefix_n_ckpt_cap > 0 ? prefix_ckpt_interval : 0, prefix_n_ckpt_cap, T,
                         n_ckpt_cap > 0 ? ckpt_interval : 0, n_ckpt_cap);
     const int64_t rows = (int64_t)B * n * Hq;
-    return 2 * pad256((int64_t)B * H * D * 4) + pad256(p.pieces() * rows * 8) + pad256(p.pieces() * rows * D * 4) + p.image_bytes(0, H) + p.image_bytes(1, H) + bits_bytes(p, B, n);
+    return 2 * pad256((int64_t)B * H * D * 4) + pad256(p.pieces() * rows * 8) + pad256(p.pieces() * rows * D * 4) + p.image_bytes(0, H) + p.image_bytes(1, H);
 }
 
 int adkv_extend(const void *q, const int64_t *q_strides, void *k_cache, void *v_cache, const void *k_new, const void *v_new,
@@ -1471,23 +1441,6 @@ int adkv_extend(const void *q, const int64_t *q_strides, void *k_cache, void *v_
     a.out = direct ? (h1 *)out : nullptr;
     const int kind = !mask ? 0 : mask_dt == ADKV_DT_F32 ? 2 : 1;
     const Source sources[2] = {pre, own};
-    a.mask_bits = nullptr;
-    a.mask_words = mask_words(pl);
-    a.mask_own_tile = pl.tiles[0];
-    if (mask && a.m_sh == 0 && H > 1 && (pl.image[0] || pl.image[1])) {
-        uint32_t *bits = (uint32_t *)(images[1] + pl.image_bytes(1, H));
-        const int64_t r = (int64_t)B * n * a.mask_words;
-        const dim3 grid((unsigned)((r + 3) / 4));
-        if (mask_dt == ADKV_DT_F32)
-            hipLaunchKernelGGL(mask_tiles_kernel<uint32_t>, grid, dim3(256), 0, (hipStream_t)stream, (const uint32_t *)mask, a.m_sb, a.m_st, n, (long)r, P,
-                               T + n, bits, a.mask_words);
-        else
-            hipLaunchKernelGGL(mask_tiles_kernel<uint16_t>, grid, dim3(256), 0, (hipStream_t)stream, (const uint16_t *)mask, a.m_sb, a.m_st, n, (long)r, P,
-                               T + n, bits, a.mask_words);
-        if ((rc = check_launch()))
-            return rc;
-        a.mask_bits = bits;
-    }
     // units [u0, u1) of a group
     auto group = [&](int i, int u0, int u1) {
         Group g = {};
