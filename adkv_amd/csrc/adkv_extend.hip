@@ -40,7 +40,8 @@ constexpr int PRODUCERS = 4;
 // buffers of a K and a V tile of 8 KB the second halves.
 constexpr int FEW_TILE = 32, FEW_THREADS = 512, FEW_BUFFER = 32768, FEW_VALUES = 16384, FEW_FIRST = 128, FEW_LDS = 65536;
 // Many rows: tiles of 64 tokens, 16 KB of keys and as many of values, three of them in the LDS; eight waves of up to 32 rows.
-constexpr int TILE = 64, TILE_BYTES = 32768, TILE_VALUES = 16384, MANY_THREADS = 512, MANY_ROWS = 256;
+constexpr int VMCNT_0 = 0x0F70; // s_waitcnt's operand: all vector loads
+constexpr int TILE = 64, TILE_BYTES = 32768, TILE_VALUES = 16384, MANY_WAVES = 4, MANY_ROWS = MANY_WAVES * 32, JOINT_ROWS = 128;
 constexpr int MAX_TOKENS = 1 << 24; // 64 bytes each: a piece's codes are addressed in 32 bits
 constexpr float LOG2E = 1.44269504088896340736f;
 
@@ -470,6 +471,14 @@ struct MaskRaw {
             }
         }
     }
+    __device__ __forceinline__ bool anything() const
+    {
+        uint32_t any = 0;
+#pragma unroll
+        for (int e = 0; e < WORDS; e++)
+            any |= w[e];
+        return any != 0;
+    }
     // x = x * scaling + mask
     __device__ __forceinline__ void add(float *x, float scaling, int dt) const
     {
@@ -580,13 +589,13 @@ struct Consumer {
     }
 
     // the mask of the tokens from t on
-    template <int NA> __device__ __forceinline__ void look_at(int t, int lane)
+    template <int NA> __device__ __forceinline__ void look_at(int t, int lane, MaskRaw<J, MASK> *to)
     {
         if constexpr (MASK != 0) {
             t += (lane >> 4) * 4;
 #pragma unroll
             for (int k = 0; k < NA; k++)
-                masks[k].load(mask[k], t, tokens - t);
+                to[k].load(mask[k], t, tokens - t);
         }
     }
     // the scores of the step-th step of a tile, as q.K
@@ -629,8 +638,12 @@ struct Consumer {
 #pragma unroll
             for (int e = 0; e < 4 * J; e++)
                 x[e] = sc[k][e >> 2][e & 3];
-            if constexpr (MASK != 0)
-                masks[k].add(x, a.scaling, a.mask_dt);
+            bool plain = true; // x are products yet, and nothing is added to them
+            if constexpr (MASK != 0) {
+                plain = !__any(masks[k].anything());
+                if (!plain)
+                    masks[k].add(x, a.scaling, a.mask_dt);
+            }
             if (t + 16 * J > seen) {
 #pragma unroll
                 for (int e = 0; e < 4 * J; e++)
@@ -642,7 +655,9 @@ struct Consumer {
                 mx = fmaxf(mx, x[e]);
             // The largest so far is looked for again only where a weight would be more than 2^8: weights relative to one that is smaller than the
             // largest by up to that are as exact.
-            const float c = MASK != 0 ? LOG2E : a.scaling * LOG2E;
+            const float c = MASK != 0 ? LOG2E : a.scaling * LOG2E; // of m; with masks scores, else products
+            if (MASK != 0 && plain)
+                mx *= a.scaling;
             if (__any((mx - m[k]) * c > 8.0f || m[k] == -INFINITY)) {
                 mx = fmaxf(m[k], fold_quarters<true>(mx));
                 const float shrink = m[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[k] - mx) * c);
@@ -656,12 +671,20 @@ struct Consumer {
             }
             const float ref = m[k] == -INFINITY ? 0.0f : m[k]; // nothing but -inf so far: all weights are zero
             float sum = 0.0f;
+            if (MASK != 0 && !plain && __any(fabsf(ref) > 1024.0f)) {
+                // the difference first: beside a mask the largest may be as large as its type's lowest value
 #pragma unroll
-            for (int e = 0; e < 4 * J; e++) {
-                // beside a mask the difference first: the largest may be as large as its type's lowest value
-                x[e] = __builtin_amdgcn_exp2f(MASK != 0 ? (x[e] - ref) * c : __builtin_fmaf(x[e], c, -ref * c));
-                sum += x[e];
+                for (int e = 0; e < 4 * J; e++)
+                    x[e] = __builtin_amdgcn_exp2f((x[e] - ref) * c);
+            } else {
+                const float unit = MASK != 0 && plain ? a.scaling * LOG2E : c;
+#pragma unroll
+                for (int e = 0; e < 4 * J; e++)
+                    x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], unit, -ref * c));
             }
+#pragma unroll
+            for (int e = 0; e < 4 * J; e++)
+                sum += x[e];
             l[k] += sum;
 #pragma unroll
             for (int e = 0; e < 2 * J; e++)
@@ -749,7 +772,7 @@ __device__ __forceinline__ void consume(KArgs &a, int items, const char *tiles, 
         if (at.k == 0)
             c.look(a, at);
         opened = ends;
-        c.template look_at<1>(t, lane);
+        c.template look_at<1>(t, lane, c.masks);
         __syncthreads();
         if (t < c.tokens) { // of a span's last tile half may be empty
             f4v sc[1][1];
@@ -968,15 +991,16 @@ __global__ __launch_bounds__(ITEMS * 256) void values_kernel(Images im)
 
 // A tile in 32 loads of 1 KB straight to the LDS, four by each of eight waves.
 struct Fetch {
+    static constexpr uint32_t PART = TILE_BYTES / MANY_WAVES;
     uint32_t from, to;
-    __device__ __forceinline__ Fetch(int wave, int lane) : from((uint32_t)wave * 4096u + (uint32_t)lane * 16u), to((uint32_t)wave * 4096u) {}
+    __device__ __forceinline__ Fetch(int wave, int lane) : from((uint32_t)wave * PART + (uint32_t)lane * 16u), to((uint32_t)wave * PART) {}
     __device__ __forceinline__ void tile(const char *image, uint32_t lds) const
     {
         const uint64_t base = (uint64_t)image;
         const rsrc4 buffer = {(uint32_t)base, (uint32_t)(base >> 32) & 0xFFFFu, (uint32_t)TILE_BYTES, 0x00027000u};
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            load_to_lds(lds + to + i * 1024u, from + i * 1024u, buffer);
+        for (uint32_t i = 0; i < PART; i += 1024)
+            load_to_lds(lds + to + i, from + i, buffer);
     }
 };
 
@@ -987,11 +1011,11 @@ struct Fetch {
 // (The second wave of each SIMD a tile behind with its softmax, so that one makes weights while the other multiplies, took 241 registers instead of 207 and
 // was no faster: 128 rows for each of 8 heads over 8192 tokens 32 us instead of 26, long walks the same.)
 template <int MASK>
-__global__ __launch_bounds__(MANY_THREADS) void attend_many_kernel(Args)
+__global__ __launch_bounds__(MANY_WAVES * 64, 2) void attend_many_kernel(Args)
 {
     using C = Consumer<2, 4, MASK>;
     KArgs &a = *(KArgs *)__builtin_amdgcn_kernarg_segment_ptr();
-    __shared__ uint4 smem[3 * TILE_BYTES / 16];
+    __shared__ uint4 smem[2 * TILE_BYTES / 16];
     char *tiles = reinterpret_cast<char *>(smem);
     const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)tiles;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -1013,18 +1037,17 @@ __global__ __launch_bounds__(MANY_THREADS) void attend_many_kernel(Args)
         if (next.k == 0)
             open();
     };
-    auto block = [&](const Walk<TILE> &w) __attribute__((always_inline)) { return w.block * 16 + wave; };
+    auto block = [&](const Walk<TILE> &w) __attribute__((always_inline)) { return w.block * (2 * MANY_WAVES) + wave; };
     open();
     fetch.tile(image, lds);
-    step();
-    fetch.tile(image, lds + TILE_BYTES);
-    C::load(a, at, block(at), 8, lane, c.q);
-    bool opened = true;
+    C::load(a, at, block(at), MANY_WAVES, lane, c.q);
+    bool opened = true, looked = false; // the tile's mask is there
+    MaskRaw<4, MASK> coming[2];
     int buffer = 0;
     for (;;) {
         if (opened) {
             c.ready(a, c.q);
-            c.clear(a, at, block(at), 8, lane);
+            c.clear(a, at, block(at), MANY_WAVES, lane);
         }
         if (at.k == 0)
             c.look(a, at);
@@ -1032,29 +1055,45 @@ __global__ __launch_bounds__(MANY_THREADS) void attend_many_kernel(Args)
         const bool ends = at.last_of_item(), done = at.last();
         opened = ends;
         step();
-        asm volatile("s_waitcnt vmcnt(4)" ::: "memory"); // this wave's part of the tile is there, all but what it fetched last
-        __builtin_amdgcn_s_barrier();                     // and everyone's; and nobody reads the tile before it any more
+        __builtin_amdgcn_s_waitcnt(VMCNT_0); // this wave's part of the tile is there, and so are loads that the compiler would wait for later
+        __builtin_amdgcn_s_barrier();        // and everyone's; and nobody reads the tile before it any more
         asm volatile("" ::: "memory");
-        fetch.tile(image, lds + (buffer == 0 ? 2 : buffer - 1) * TILE_BYTES);
+        // Loads end in order, and a wait for a mask would be one for a tile that is fetched in front of it or behind it: the next tile's
+        // mask is loaded with the tile.  (fp32 masks have no registers for that.)
+        if constexpr (MASK == 1) {
+            if (looked) {
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+                    c.masks[k] = coming[k];
+            } else if (mine > 0) {
+                c.template look_at<2>(t, lane, c.masks);
+            }
+            looked = mine > 0 && at.k + 1 < at.n;
+            if (looked)
+                c.template look_at<2>(t + TILE, lane, coming);
+        }
+        if constexpr (MASK == 2)
+            if (mine > 0)
+                c.template look_at<2>(t, lane, c.masks);
+        fetch.tile(image, lds + (buffer ^ 1) * TILE_BYTES);
         const char *from = tiles + buffer * TILE_BYTES;
         Walk<TILE> then = at;
         auto multiply = [&](auto na) __attribute__((always_inline)) {
             constexpr int NA = decltype(na)::value;
             f4v sc[2][4];
             uint32_t w[2][8];
-            c.template look_at<NA>(t, lane);
             c.template scores<NA>(from, 0, lane, sc);
             c.template weights<NA>(a, t, lane, sc, w);
             c.template outputs<NA>(from + TILE_VALUES, 0, lane, w);
         };
-        if (mine > 8)
+        if (mine > MANY_WAVES)
             multiply(std::integral_constant<int, 2>{});
         else if (mine > 0)
             multiply(std::integral_constant<int, 1>{});
         if (!done) {
             if (ends) {
                 then = Walk<TILE>(a, items, at.i + gridDim.x);
-                C::load(a, then, block(then), 8, lane, c.q);
+                C::load(a, then, block(then), MANY_WAVES, lane, c.q);
             } else {
                 then.go(a);
             }
@@ -1064,7 +1103,7 @@ __global__ __launch_bounds__(MANY_THREADS) void attend_many_kernel(Args)
         if (done)
             break;
         at = then;
-        buffer = buffer == 2 ? 0 : buffer + 1;
+        buffer ^= 1;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // nothing is written to the LDS any more
 }
@@ -1219,7 +1258,7 @@ static Plan plan(int B, int H, int G, int n, int P, int p_interval, int p_ckpt, 
 {
     Plan p = {};
     const long rows[2] = {(long)B * n * G, (long)n * G}, units[2] = {H, (long)B * H}, total = (long)B * n * G * H;
-    p.joint = P > 0 && rows[1] >= MANY_ROWS / 2;
+    p.joint = P > 0 && rows[1] >= JOINT_ROWS;
     p.there[0] = P > 0 && !p.joint;
     p.there[1] = true;
     p.intervals[0] = P > 0 ? usable_intervals(P, p_interval, p_ckpt) : 0;
@@ -1235,7 +1274,7 @@ static Plan plan(int B, int H, int G, int n, int P, int p_interval, int p_ckpt, 
     // groups of one kind share a launch
     for (int k = 0; k < 2; k++) {
         const bool f = k == 0;
-        const long slots = cu_count() * (f ? 2L : 1L);
+        const long slots = cu_count() * 2L;
         const bool in[2] = {p.there[0] && p.few[0] == f, p.few[1] == f};
         if (!in[0] && !in[1])
             continue;
@@ -1512,7 +1551,7 @@ int adkv_extend(const void *q, const int64_t *q_strides, void *k_cache, void *v_
             a.g[1] = pl.image[1] ? group(1, u0, u1) : Group{};
             const int64_t work = (int64_t)a.g[0].items + a.g[1].items;
             if (work > 0) {
-                hipLaunchKernelGGL(kernels[kind], dim3((unsigned)std::min<int64_t>(work, cu_count())), dim3(MANY_THREADS), 0, (hipStream_t)stream, a);
+                hipLaunchKernelGGL(kernels[kind], dim3((unsigned)std::min<int64_t>(work, 2 * cu_count())), dim3(MANY_WAVES * 64), 0, (hipStream_t)stream, a);
                 if ((rc = check_launch()))
                     return rc;
             }

@@ -355,3 +355,22 @@ def test_host_calls_equal_the_python_function(gpu, oracle, monkeypatch, size, ma
         results.append([out.view(torch.int16), *c.cache, *[t.view(torch.int16) for t in c.ckpt]])
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("size", [(2, 2, 1, 400, 70, 130), (24, 1, 2, 500, 3, 1), (3, 1, 8, 0, 300, 21), (2, 2, 2, 333, 200, 10)])
+def test_masks_that_are_zero_in_places(gpu, oracle, dtype, size):
+    """Stretches of tokens without anything added, with a little added, and hidden, so that every way from one to the next is taken:
+    also where all that was seen so far was hidden."""
+    B, H, G, P, T, n = size
+    c = Case(oracle, gpu, *size, dtype=torch.bfloat16 if dtype == torch.bfloat16 else torch.float16, seed=8)
+    N, low = P + T + n, torch.finfo(dtype).min
+    g = torch.Generator().manual_seed(4)
+    for first in (low, -math.inf, 0.0, 2000.0):
+        mask = torch.zeros(B, 1, n, N, dtype=dtype)
+        mask[:, :, :, :N // 3] = first
+        mask[0, :, :, N // 2:N // 2 + 70] = torch.randn(n, 70, generator=g).to(dtype)[:, :mask.shape[3] - N // 2]
+        mask[-1, :, n // 2:, N // 2:N - 40] = low
+        mask = mask.to(gpu)
+        c.check(c.run(D ** -0.5, mask), D ** -0.5, mask)
