@@ -14,7 +14,7 @@
 //   at most 16 (few)   attend_kernel: the waves that replay hand tiles of values to waves that multiply, through the LDS
 //   more (many)        values_kernel writes the values to memory as tiles of fp16, attend_many_kernel reads them.  Replaying in the multiplying
 //                      workgroup takes as many issue slots as the softmax of 256 rows, once per 256 rows, and its LDS; 8 x 512
-//                      new tokens on a prefix of 4096, 32 heads, took 1000 us that way
+//                      new tokens on a prefix of 4096, 32 heads, took 1000 us that way, where the two kernels take 530
 #include <math.h>
 
 #include <algorithm>
@@ -39,7 +39,7 @@ constexpr int PRODUCERS = 4;
 // of the issue slots.  Of 64 KB of LDS the code table (half as many copies of its entries as elsewhere) has the first half of every 256 bytes, and two
 // buffers of a K and a V tile of 8 KB the second halves.
 constexpr int FEW_TILE = 32, FEW_THREADS = 512, FEW_BUFFER = 32768, FEW_VALUES = 16384, FEW_FIRST = 128, FEW_LDS = 65536;
-// Many rows: tiles of 64 tokens, 16 KB of keys and as many of values, three of them in the LDS; eight waves of up to 32 rows.
+// Many rows: tiles of 64 tokens, 16 KB of keys and as many of values, two of them in the LDS; four waves of up to 32 rows.
 constexpr int VMCNT_0 = 0x0F70; // s_waitcnt's operand: all vector loads
 constexpr int TILE = 64, TILE_BYTES = 32768, TILE_VALUES = 16384, MANY_WAVES = 4, MANY_ROWS = MANY_WAVES * 32, JOINT_ROWS = 128;
 constexpr int MAX_TOKENS = 1 << 24; // 64 bytes each: a piece's codes are addressed in 32 bits
@@ -814,7 +814,9 @@ __device__ __forceinline__ void fill_half(char *lds, int tid)
 }
 
 // Four waves replay the tile after the one that the others multiply with, one per SIMD, through two buffers and a barrier per tile.
-// A workgroup goes on to its next item without a gap.
+// A workgroup goes on to its next item without a gap.  Bound by instruction issue: replay and products of a tile are some 2000 cycles of every
+// SIMD whether its rows are one or sixteen.  128 sequences of 32 heads with 65 tokens each: 42 us (codes of 34 MB are 7); a
+// prefix of 8192 tokens and 4 sequences of 1001, 32 heads: 36 us.
 template <int BITS, int MASK>
 __global__ __launch_bounds__(FEW_THREADS) void attend_kernel(Args)
 {
@@ -842,28 +844,29 @@ struct Images {
     Div by_run[2];
 };
 
-// The values of a run of tokens of 64 channels of K or V as tiles in memory, as the LDS has them.  Four waves an item; up
-// to four items a workgroup, where there are as many for every CU: four waves to a SIMD, which then is bound by the replay's instructions.
-template <int BITS, int ITEMS>
-__global__ __launch_bounds__(ITEMS * 256) void values_kernel(Images im)
+// The values of a run of tokens of K and V as tiles in memory, as the LDS has them: a wave for 64 channels of either, two workgroups to a CU.  Bound by its
+// stores: 4096 tokens of 32 heads are 67 MB of values, 17 us (3.9 TB/s).  Workgroups of four runs, four waves to a SIMD with one table, are done later
+// (the call with 5 new tokens of 16 sequences behind 2048, 8 heads, 67 us instead of 57).
+template <int BITS>
+__global__ __launch_bounds__(256) void values_kernel(Images im)
 {
     constexpr int TPW = 32 / BITS, WPC = TILE / TPW; // words of a channel per chunk of 64 tokens
-    __shared__ uint4 smem[LUT_WORDS64 / 2 + ITEMS * 4 * 256];
+    __shared__ uint4 smem[LUT_WORDS64 / 2 + 4 * 256];
     uint2 *lut = reinterpret_cast<uint2 *>(smem);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    int item = (int)blockIdx.x * ITEMS + (wave >> 2);
-    const bool there = item < im.items[0] + im.items[1], own = there && item >= im.items[0];
-    const int kind = wave >> 1 & 1, c = (wave & 1) * 64 + lane;
+    int item = (int)blockIdx.x;
+    const bool own = item >= im.items[0];
+    const int kind = wave >> 1, c = (wave & 1) * 64 + lane;
     item -= own ? im.items[0] : 0;
     const Extent &x = own ? im.s[1].x : im.s[0].x;
     const Tensor &t = own ? (kind ? im.s[1].t[1] : im.s[1].t[0]) : (kind ? im.s[0].t[1] : im.s[0].t[0]);
-    const int runs = own ? im.runs[1] : im.runs[0], of_launch = divide(there ? item : 0, own ? im.by_run[1] : im.by_run[0]);
+    const int runs = own ? im.runs[1] : im.runs[0], of_launch = divide(item, own ? im.by_run[1] : im.by_run[0]);
     const int unit = of_launch + (own ? im.first[1] : im.first[0]), run = item - of_launch * runs;
     const int per = x.intervals / runs, longer = x.intervals % runs, first = run * per + min(run, longer), end = first + per + (run < longer ? 1 : 0);
     const int t0 = first * x.interval, t1 = end >= x.intervals ? x.tokens : end * x.interval;
     const int h = own ? unit % im.H : unit, pi = h * D + c;
 
-    const int words = there ? (t1 - t0 + TPW - 1) / TPW : 0;
+    const int words = (t1 - t0 + TPW - 1) / TPW;
     // reads behind the last word are dropped
     const auto codes = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint32_t *>(t.codes) + ((size_t)unit * x.n_super + t0 / TPW) * D, 0, words * D * 4,
                                                          0x00027000);
@@ -875,22 +878,17 @@ __global__ __launch_bounds__(ITEMS * 256) void values_kernel(Images im)
             to[i] = __builtin_amdgcn_raw_buffer_load_b32(codes, next + i * D * 4, 0, 0);
         next += WPC * D * 4;
     };
-    Lone st = {};
-    if (there) {
-        load(w[0]);
-        load(w[1]);
-        h2 from = {t.zp[pi], t.sc[pi]};
-        if (first > 0)
-            from = as_h2(*reinterpret_cast<const uint32_t *>(t.ckpt + (((size_t)unit * x.n_ckpt + first - 1) * D + c) * 2));
-        st = state_of(from, t.al[pi], t.be[pi], t.tg[pi]);
-    }
+    load(w[0]);
+    load(w[1]);
+    h2 from = {t.zp[pi], t.sc[pi]};
+    if (first > 0)
+        from = as_h2(*reinterpret_cast<const uint32_t *>(t.ckpt + (((size_t)unit * x.n_ckpt + first - 1) * D + c) * 2));
+    Lone st = state_of(from, t.al[pi], t.be[pi], t.tg[pi]);
     if constexpr (BITS == 4)
-        lone_fill<ITEMS * 256>(lut, threadIdx.x);
+        lone_fill<256>(lut, threadIdx.x);
     else
-        lone_fill2<ITEMS * 256>(lut, threadIdx.x);
+        lone_fill2<256>(lut, threadIdx.x);
     __syncthreads();
-    if (!there)
-        return;
     const uint32_t lane_copy = BITS == 4 ? (uint32_t)(lane & (LUT_COPIES - 1)) * 8u : (uint32_t)(lane & (LUT2_COPIES - 1)) * 16u;
     const int tiles = (x.tokens + TILE - 1) / TILE;
     const auto image = global((own ? im.to[1] : im.to[0]) + (size_t)of_launch * tiles * TILE_BYTES + kind * TILE_VALUES);
@@ -1004,12 +1002,13 @@ struct Fetch {
     }
 };
 
-// Three tiles in the LDS: one being multiplied with, two on their way, a barrier per tile.  Workgroups of one XCD take neighbouring items, which
-// read the same tiles.  A tile with 256 rows takes about 5500 cycles: its matrix instructions 2048 of a SIMD, reads of the LDS 1300, and in between
-// both waves of a SIMD wait for their reads or make weights at the same time.  512 tokens of 8 sequences of 32 heads over 4096 tokens, masked:
-// 492 us, 590 TFLOP/s.
-// (The second wave of each SIMD a tile behind with its softmax, so that one makes weights while the other multiplies, took 241 registers instead of 207 and
-// was no faster: 128 rows for each of 8 heads over 8192 tokens 32 us instead of 26, long walks the same.)
+// Two tiles in the LDS, one being multiplied with and one on its way, a barrier per tile; two workgroups to a CU, which wait at different times (one
+// of eight waves and three tiles: 512 masked tokens of 8 sequences 690 us instead of 530).  Workgroups of one XCD take neighbouring items,
+// which read the same tiles.  A wave's tile with 32 rows is 1024 cycles of matrix instructions and some 1500 of others, half of them the softmax;
+// with two waves to a SIMD it takes 2900, 3500 with a mask: neither pipe is full (matrix cores 29 to 35 % busy), the wave that waits for its reads or
+// results is not covered by one other.  512 tokens of 8 sequences, 32 heads, over 4096 tokens, masked: 430 to 490 us by the clock that the card
+// holds, 590 to 670 TFLOP/s; without fetching its tiles 11 % less, without exponentials 7 % less.  A wave of the SIMD a tile behind, raised
+// priorities around the products and reads of the LDS issued a group ahead changed nothing.
 template <int MASK>
 __global__ __launch_bounds__(MANY_WAVES * 64, 2) void attend_many_kernel(Args)
 {
@@ -1161,7 +1160,8 @@ __global__ __launch_bounds__(256) void join_kernel(const float *__restrict__ par
         store_four(out + row * D + c, o * (1.0f / L), act_bf16);
 }
 
-// The state behind token T - 1 of every channel, from the last checkpoint in front of it: at most an interval, a token at a time.
+// The state behind token T - 1 of every channel, from the last checkpoint in front of it: at most an interval, a token at a time, three dependent
+// operations each (200 tokens: 7 us, 13 with codes taken apart one by one).
 // Where token T opens an interval the state is that interval's checkpoint, which nobody may have recorded yet.
 template <int BITS>
 __global__ __launch_bounds__(128) void state_kernel(Source s, int H, int n_ckpt, h1 *k_state, h1 *v_state)
@@ -1250,8 +1250,9 @@ static int usable_intervals(int tokens, int interval, int n_ckpt)
 
 constexpr int64_t IMAGE_MAX = 1ll << 30; // bytes of own tiles at a time, unless one unit's are more
 
-// Rows of a sequence that half fill a workgroup's 256 or more walk through the prefix by themselves: their outputs need no joining.  Workgroups
-// walk through items, two per CU (few rows) or one.  The length of a piece is chosen for the shortest call by the model (us): a workgroup's items x
+// Rows of a sequence that fill a workgroup walk through the prefix by themselves, and their outputs need no joining (512 tokens of 8 sequences 520 us,
+// 680 with the prefix apart; at 40 rows 60 us instead of 58).  Workgroups
+// walk through items, two per CU.  The length of a piece is chosen for the shortest call by the model (us): a workgroup's items x
 // (64 tokens of a piece x 1.3 or, of many rows, 2.3, + 1), and 4 TB/s for the partial results, written and read.
 // T: the own tokens in front of the new ones.
 static Plan plan(int B, int H, int G, int n, int P, int p_interval, int p_ckpt, int T, int interval, int n_ckpt)
@@ -1540,10 +1541,7 @@ int adkv_extend(const void *q, const int64_t *q_strides, void *k_cache, void *v_
             }
             const int items = im.items[0] + im.items[1];
             if (items > 0) {
-                const int each = items <= cu_count() ? 1 : items <= 2 * cu_count() ? 2 : 4;
-                const auto kernel = bits == 4 ? (each == 1 ? values_kernel<4, 1> : each == 2 ? values_kernel<4, 2> : values_kernel<4, 4>)
-                                              : (each == 1 ? values_kernel<2, 1> : each == 2 ? values_kernel<2, 2> : values_kernel<2, 4>);
-                hipLaunchKernelGGL(kernel, dim3((unsigned)((items + each - 1) / each)), dim3(each * 256), 0, (hipStream_t)stream, im);
+                hipLaunchKernelGGL(bits == 4 ? values_kernel<4> : values_kernel<2>, dim3((unsigned)items), dim3(256), 0, (hipStream_t)stream, im);
                 if ((rc = check_launch()))
                     return rc;
             }

@@ -10,8 +10,11 @@
 // x, which is read for dw and dx anyway: nothing of the way there is kept.
 //
 // Memory bound: an element is read and written once on the way there, read twice and written once on the way back, some 30 operations each.  A
-// row is D / 2 pairs, a lane takes V neighbouring pairs, 16 bytes of either half, all turned or none; the row's 2^log lanes sum by
+// row is D / 2 pairs, a lane takes V neighbouring pairs, all turned or none (eight of 16 bits, 16 bytes of either half, were slower: 53 us
+// instead of 49 for the first size below); the row's 2^log lanes sum by
 // exchanges.  A lane takes its pairs of HEADS heads of a token: cos, sin and the weights are loaded once for them, and all loads are in flight together.
+// Four sequences of 2048 tokens, 32 + 32 heads of 128 values in fp16: 268 MB in 46 us (5.8 TB/s; a copy of 1 GiB reaches 5.1).  Two of 4096 tokens,
+// 32 + 8 heads in bf16: 168 MB in 29 us there and 251 MB in 48 us back (5.8 and 5.2 TB/s), and 4 us for the workgroups' sums of dw.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -27,6 +30,7 @@ using adkv::h1;
 
 constexpr int F32 = ADKV_DT_F32, F16 = ADKV_DT_F16, BF16 = ADKV_DT_BF16;
 constexpr int NT = 256;
+constexpr int V = 4; // pairs of a lane
 constexpr int DIM_MAX = 512; // a row is one wave's at most
 constexpr int COLUMNS = 32; // of the sums of dw
 
@@ -53,7 +57,7 @@ struct Args {
     float *dw;                   // a row of D sums per workgroup
 };
 
-template <int TYPE, int V>
+template <int TYPE>
 struct Piece {
     static constexpr int WORDS = V * (TYPE == F32 ? 4 : 2) / 4, SIZE = TYPE == F32 ? 4 : 2;
     typedef uint32_t Raw __attribute__((ext_vector_type(WORDS)));
@@ -127,9 +131,9 @@ __device__ __forceinline__ void sum_row(float *v, int log)
 struct Lane {
     int row, lo, hi;
     bool there, turned;
-    __device__ __forceinline__ explicit Lane(const Args &a, int v)
+    __device__ __forceinline__ explicit Lane(const Args &a)
     {
-        const int j = threadIdx.x & ((1 << a.log) - 1), pair = j * v;
+        const int j = threadIdx.x & ((1 << a.log) - 1), pair = j * V;
         row = threadIdx.x >> a.log;
         there = j < a.lanes;
         turned = there && pair < a.turned;
@@ -138,7 +142,6 @@ struct Lane {
     }
 };
 
-template <int V>
 __device__ __forceinline__ void turn(float *lo, float *hi, const float *cl, const float *ch, const float *sl, const float *sh)
 {
 #pragma unroll
@@ -148,7 +151,6 @@ __device__ __forceinline__ void turn(float *lo, float *hi, const float *cl, cons
         hi[e] = __builtin_fmaf(y, ch[e], x * sh[e]);
     }
 }
-template <int V>
 __device__ __forceinline__ void turn_back(float *lo, float *hi, const float *cl, const float *ch, const float *sl, const float *sh)
 {
 #pragma unroll
@@ -159,15 +161,15 @@ __device__ __forceinline__ void turn_back(float *lo, float *hi, const float *cl,
     }
 }
 
-template <int TYPE, int V, int HEADS>
+template <int TYPE, int HEADS>
 __global__ __launch_bounds__(NT) void forward_kernel(Args a)
 {
-    using P = Piece<TYPE, V>;
+    using P = Piece<TYPE>;
     using Raw = typename P::Raw;
     const bool is_k = (int)blockIdx.x >= a.k.first;
     const Side s = is_k ? a.k : a.q;
     const int at = (int)blockIdx.x - s.first, group = at / a.blocks, block = at - group * a.blocks;
-    const Lane l(a, V);
+    const Lane l(a);
     const int token = block * (NT >> a.log) + l.row;
     const bool there = l.there && token < a.tokens, turned = l.turned && token < a.tokens;
     const int b = (uint32_t)token / (uint32_t)a.T, t = token - b * a.T, h0 = group * HEADS;
@@ -221,7 +223,7 @@ __global__ __launch_bounds__(NT) void forward_kernel(Args a)
         for (int e = 0; e < 2 * V; e++)
             x[j][e] = x[j][e] * r * w[e];
         if (turned)
-            turn<V>(x[j], x[j] + V, c, c + V, sn, sn + V);
+            turn(x[j], x[j] + V, c, c + V, sn, sn + V);
         const long row = b * s.os.b + (h0 + j) * s.os.h + t * s.os.t;
         P::store(s.out, row + l.lo, x[j]);
         P::store(s.out, row + l.hi, x[j] + V);
@@ -229,14 +231,14 @@ __global__ __launch_bounds__(NT) void forward_kernel(Args a)
 }
 
 // Workgroups walk through blocks of tokens and heads with their part of dw in registers: a sum in an order that the launch alone decides.
-template <int TYPE, int V, int HEADS>
+template <int TYPE, int HEADS>
 __global__ __launch_bounds__(NT) void backward_kernel(Args a)
 {
-    using P = Piece<TYPE, V>;
+    using P = Piece<TYPE>;
     using Raw = typename P::Raw;
     const bool is_k = (int)blockIdx.x >= a.k.first;
     const Side s = is_k ? a.k : a.q;
-    const Lane l(a, V);
+    const Lane l(a);
     __shared__ float sums[NT / 64][DIM_MAX];
     Raw wl = {}, wh = {};
     if (l.there) {
@@ -291,7 +293,7 @@ __global__ __launch_bounds__(NT) void backward_kernel(Args a)
             P::widen(gl[j], g);
             P::widen(gh[j], g + V);
             if (turned)
-                turn_back<V>(g, g + V, c, c + V, sn, sn + V);
+                turn_back(g, g + V, c, c + V, sn, sn + V);
 #pragma unroll
             for (int e = 0; e < 2 * V; e++) {
                 sum[0] = __builtin_fmaf(x[e], x[e], sum[0]);
@@ -376,13 +378,13 @@ __global__ __launch_bounds__(1024) void weight_kernel(const float *__restrict__ 
 
 static int workers(int64_t items, int64_t of, int64_t all)
 {
-    // sixteen waves per CU for both sides together
+    // sixteen waves per CU for both sides together: with more, more sums of dw
     return (int)std::max<int64_t>(1, std::min<int64_t>(items, 4ll * cu_count() * of / all));
 }
 
-// sizes and the tables; also how many pairs a lane takes, and how many heads
+// sizes and the tables; also how many heads a lane takes
 static int prepare(Args &a, const void *cos, const void *sin, int B, int Hq, int H, int T, int D, int R, float eps, const int64_t *table_strides,
-                   int dtype, const void *const *pointers, const int64_t *const *strides, int n, int &v, int &heads)
+                   int dtype, const void *const *pointers, const int64_t *const *strides, int n, int &heads)
 {
     if (B <= 0 || Hq <= 0 || H <= 0 || T <= 0)
         return ADKV_E_SHAPE;
@@ -401,9 +403,7 @@ static int prepare(Args &a, const void *cos, const void *sin, int B, int Hq, int
             steps |= strides[i][0] | strides[i][1] | strides[i][2];
     const int size = dtype == F32 ? 4 : 2;
     bits |= steps * size;
-    // 16 bytes of either half where every row has them so
-    v = dtype != F32 && (bits & 15) == 0 && R % 16 == 0 && (D - R) % 16 == 0 ? 8 : 4;
-    if (bits & (v * size - 1))
+    if (bits & (V * size - 1))
         return ADKV_E_ALIGN;
     a.cos = cos;
     a.sin = sin;
@@ -413,7 +413,7 @@ static int prepare(Args &a, const void *cos, const void *sin, int B, int Hq, int
     a.T = T;
     a.half = D / 2;
     a.turned = R / 2;
-    a.lanes = a.half / v;
+    a.lanes = a.half / V;
     a.log = 0;
     while (1 << a.log < a.lanes)
         a.log++;
@@ -421,6 +421,8 @@ static int prepare(Args &a, const void *cos, const void *sin, int B, int Hq, int
     a.blocks = (a.tokens + rows - 1) / rows;
     a.eps = eps;
     a.inv_d = 1.0f / (float)D;
+    // four heads to a lane where that leaves work for all CUs; else one, and four times the lanes
+    // (the first size above 49 us with four, 59 with one; a token of 128 sequences 3.3 us with one, half a us more with four)
     heads = 4;
     if ((int64_t)a.blocks * ((Hq + 3) / 4 + (H + 3) / 4) < 4 * cu_count())
         heads = 1;
@@ -442,10 +444,10 @@ static Side side(const void *x, const void *w, void *out, const int64_t *strides
 }
 } // namespace adkv_rope_norm
 
-#define ADKV_EACH(kernel)                                                                                                                            \
-    (dtype == F32    ? (heads == 4 ? kernel<F32, 4, 4> : kernel<F32, 4, 1>)                                                                          \
-     : dtype == F16  ? (v == 8 ? (heads == 4 ? kernel<F16, 8, 4> : kernel<F16, 8, 1>) : (heads == 4 ? kernel<F16, 4, 4> : kernel<F16, 4, 1>))       \
-                     : (v == 8 ? (heads == 4 ? kernel<BF16, 8, 4> : kernel<BF16, 8, 1>) : (heads == 4 ? kernel<BF16, 4, 4> : kernel<BF16, 4, 1>)))
+#define ADKV_EACH(kernel)                                            \
+    (dtype == F32    ? (heads == 4 ? kernel<F32, 4> : kernel<F32, 1>) \
+     : dtype == F16  ? (heads == 4 ? kernel<F16, 4> : kernel<F16, 1>) \
+                     : (heads == 4 ? kernel<BF16, 4> : kernel<BF16, 1>))
 
 extern "C" int adkv_rope_norm_qk(const void *q, const void *k, const void *cos, const void *sin, const void *q_weight, const void *k_weight,
                                  void *q_out, void *k_out, int B, int Hq, int H, int T, int D, int R, float eps, const int64_t *q_strides,
@@ -455,10 +457,10 @@ extern "C" int adkv_rope_norm_qk(const void *q, const void *k, const void *cos, 
     if (!q || !k || !cos || !sin || !q_weight || !k_weight || !q_out || !k_out || !q_strides || !k_strides || !table_strides)
         return ADKV_E_NULL;
     Args a = {};
-    int v, heads;
+    int heads;
     const void *const pointers[] = {q, k, q_weight, k_weight, q_out, k_out};
     const int64_t *const strides[] = {q_strides, k_strides, nullptr, nullptr, nullptr, nullptr};
-    if (int rc = prepare(a, cos, sin, B, Hq, H, T, D, R, eps, table_strides, dtype, pointers, strides, 6, v, heads))
+    if (int rc = prepare(a, cos, sin, B, Hq, H, T, D, R, eps, table_strides, dtype, pointers, strides, 6, heads))
         return rc;
     const int64_t qs[3] = {(int64_t)Hq * T * D, (int64_t)T * D, D}, ks[3] = {(int64_t)H * T * D, (int64_t)T * D, D};
     a.q = side(q, q_weight, q_out, q_strides, qs, Hq, heads);
@@ -495,7 +497,7 @@ extern "C" int adkv_rope_norm_qk_backward(const void *q_grad, const void *k_grad
     if (!with_q && !with_k)
         return ADKV_OK;
     Args a = {};
-    int v, heads;
+    int heads;
     const void *pointers[8];
     const int64_t *strides[8];
     int n = 0;
@@ -515,7 +517,7 @@ extern "C" int adkv_rope_norm_qk_backward(const void *q_grad, const void *k_grad
         put(k_weight, nullptr);
         put(dk, dk ? dk_strides : nullptr);
     }
-    if (int rc = prepare(a, cos, sin, B, Hq, H, T, D, R, eps, table_strides, dtype, pointers, strides, n, v, heads))
+    if (int rc = prepare(a, cos, sin, B, Hq, H, T, D, R, eps, table_strides, dtype, pointers, strides, n, heads))
         return rc;
     const bool weights = dq_weight || dk_weight;
     const int64_t need = weights ? adkv_rope_norm_qk_backward_workspace_bytes(D) : 0;

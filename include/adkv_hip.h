@@ -427,8 +427,7 @@ int adkv_rope_qk(const void *q, const void *k, const void *cos, const void *sin,
  *   q [B, Hq, T, D], k [B, H, T, D], cos, sin [B, T, R], q_weight, k_weight [D] of one type, dtype (ADKV_DT_*), channels contiguous;
  *   q_strides, k_strides: element strides {batch, head, token};  table_strides: {batch, token} of cos and sin (0 over the batch for a shared table)
  *   q_out, k_out   contiguous, of the same type
- *   D, R           multiples of 8, R <= D <= 512; every row of everything at a multiple of four elements.  Rows of 16-bit types at multiples of 16 bytes
- *                  whose R and D are multiples of 16 are faster.
+ *   D, R           multiples of 8, R <= D <= 512; every row of everything at a multiple of four elements
  */
 int adkv_rope_norm_qk(const void *q, const void *k, const void *cos, const void *sin, const void *q_weight, const void *k_weight,
                       void *q_out, void *k_out, int B, int Hq, int H, int T, int D, int R, float eps, const int64_t *q_strides,
