@@ -626,6 +626,11 @@ struct Consumer {
                     sc[k][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, q[k][c], sc[k][j], 0, 0, 0);
             }
         }
+        // Beside a mask a branch may follow, and the compiler then counts one wait state too few between a product and what reads it.
+        if constexpr (MASK != 0)
+#pragma unroll
+            for (int k = 0; k < NA; k++)
+                asm volatile("s_nop 7" : "+v"(sc[k][J - 1]));
     }
 
     // scores of the tokens from t on to weights of fp16; the row's maximum, sum and outputs go along

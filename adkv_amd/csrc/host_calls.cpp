@@ -564,7 +564,7 @@ PyObject *rope_norm_qk(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     bool record = false;
     for (int i = 0; i < 6; i++) {
         if (!(t[i] = plain(args[i])) || t[i]->scalar_type() != t[0]->scalar_type() || t[i]->device() != t[0]->device() ||
-            t[i]->dim() != (i < 2 ? 4 : i < 4 ? 3 : 1) || !fours(*t[i]))
+            t[i]->dim() != (i < 2 ? 4 : i < 4 ? 3 : 1) || !fours(*t[i]) || t[i]->_fw_grad(0).defined())
             Py_RETURN_NONE;
         if (t[i]->requires_grad() && c10::GradMode::is_enabled()) {
             if (i == 2 || i == 3)

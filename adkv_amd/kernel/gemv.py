@@ -16,6 +16,7 @@ import functools
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 
@@ -608,6 +609,7 @@ def rope_norm_qk(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
     _chk(q_weight.shape == (D,) and k_weight.shape == (D,), "the weights must be [head dim]")
     _chk(Hq > 0 and H > 0, "q and k must have heads")
     _chk(not (torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad)), "cos and sin have no gradient")
+    _chk(all(forward_ad.unpack_dual(t).tangent is None for t in (q, k, cos, sin, q_weight, k_weight)), "rope_norm_qk has no forward derivatives")
     _need_device(q, k, cos, sin, q_weight, k_weight)
     # copies where there have to be any are made here, where autograd sees them
     q, k, cos, sin, q_weight, k_weight = (_norm_rows(t) for t in (q, k, cos, sin, q_weight, k_weight))
@@ -879,7 +881,8 @@ def extend(
     xk, ks = _row_strides(k_new)
     xv, vs = _row_strides(v_new)
     if workspace is None:
-        workspace = torch.empty(extend_workspace_bytes(B, nq, nh, T, n, ccap, civ, P, pcap), dtype=torch.uint8, device=dev)
+        with _lib.device_guard(dev):       # the size depends on the device
+            workspace = torch.empty(extend_workspace_bytes(B, nq, nh, T, n, ccap, civ, P, pcap), dtype=torch.uint8, device=dev)
     _chk(workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.device == dev, "workspace must be a uint8 tensor on the same device")
     out = torch.empty((B, n, nq, DIM), dtype=act, device=dev)
     with _lib.device_guard(dev):

@@ -400,3 +400,24 @@ def test_a_changed_input_is_noticed():
     s["q"] += 1
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         torch.autograd.grad(z[0], s["wq"], s["gq"])
+
+
+@pytest.mark.gpu
+def test_gradients_of_sums():
+    """Gradients that are one number expanded to a result's shape, and ones of the other result that nobody asked for."""
+    s = make(2, 4, 2, 9, 64, 64, torch.float32)
+    s["q"], s["wq"] = s["q"].detach().requires_grad_(), s["wq"].detach().requires_grad_()
+    call(s)[0].sum().backward()
+    dx, size, dw, dw_size = gradients(s["q"], s["wq"], s["cos"], s["sin"], torch.ones_like(s["gq"]))
+    close(s["q"].grad, dx, size, 64)
+    close(s["wq"].grad, dw, dw_size, 160 + 2 * 4 * 9 / 4)
+
+
+@pytest.mark.gpu
+def test_forward_derivatives_are_refused():
+    from torch.autograd import forward_ad
+    s = make(1, 2, 1, 3, 32, 32, torch.float32)
+    with forward_ad.dual_level():
+        dual = dict(s, q=forward_ad.make_dual(s["q"], torch.ones_like(s["q"])))
+        with pytest.raises(RuntimeError, match="forward derivatives"):
+            call(dual)
