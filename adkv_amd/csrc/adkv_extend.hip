@@ -40,7 +40,7 @@ constexpr int PRODUCERS = 4;
 // buffers of a K and a V tile of 8 KB the second halves.
 constexpr int FEW_TILE = 32, FEW_THREADS = 512, FEW_BUFFER = 32768, FEW_VALUES = 16384, FEW_FIRST = 128, FEW_LDS = 65536;
 // Many rows: tiles of 64 tokens, 16 KB of keys and as many of values, two of them in the LDS; four waves of up to 32 rows.
-constexpr int VMCNT_0 = 0x0F70; // s_waitcnt's operand: all vector loads
+constexpr int ALL_READS = 0x0070; // s_waitcnt's operand: all vector loads, all reads of the LDS
 constexpr int TILE = 64, TILE_BYTES = 32768, TILE_VALUES = 16384, MANY_WAVES = 4, MANY_ROWS = MANY_WAVES * 32, JOINT_ROWS = 128;
 constexpr int MAX_TOKENS = 1 << 24; // 64 bytes each: a piece's codes are addressed in 32 bits
 constexpr float LOG2E = 1.44269504088896340736f;
@@ -1059,8 +1059,8 @@ __global__ __launch_bounds__(MANY_WAVES * 64, 2) void attend_many_kernel(Args)
         const bool ends = at.last_of_item(), done = at.last();
         opened = ends;
         step();
-        __builtin_amdgcn_s_waitcnt(VMCNT_0); // this wave's part of the tile is there, and so are loads that the compiler would wait for later
-        __builtin_amdgcn_s_barrier();        // and everyone's; and nobody reads the tile before it any more
+        __builtin_amdgcn_s_waitcnt(ALL_READS); // this wave's part of the tile is there, what it read of the last one, and loads that the compiler would wait for later
+        __builtin_amdgcn_s_barrier();          // and everyone's; and nobody reads the tile before it any more
         asm volatile("" ::: "memory");
         // Loads end in order, and a wait for a mask would be one for a tile that is fetched in front of it or behind it: the next tile's
         // mask is loaded with the tile.  (fp32 masks have no registers for that.)
