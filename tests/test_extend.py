@@ -374,3 +374,39 @@ def test_masks_that_are_zero_in_places(gpu, oracle, dtype, size):
         mask[-1, :, n // 2:, N // 2:N - 40] = low
         mask = mask.to(gpu)
         c.check(c.run(D ** -0.5, mask), D ** -0.5, mask)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("G,n,P", [(4, 5, 0), (8, 16, 70)])
+def test_own_tiles_in_several_batches(gpu, G, n, P):
+    """More own tokens than there is room for tiles of at a time (1 GiB, two million tokens of a head): sequences of the first and the last batch
+    against the same sequences by themselves.  Codes are equal; of the outputs either side rounds weights (2^-11, small ones 2^-25 a token), sums (2^-14)
+    and the result (2^-11), of values up to `top`."""
+    B, H, T = 66, 16, 2041
+    gen = torch.Generator(device=gpu).manual_seed(3)
+    rand = lambda *s: torch.randn(*s, generator=gen, device=gpu, dtype=torch.float16)
+    params = [p.to(gpu).astuple() for p in (synth.make_params(H, D, seed=s) for s in (1, 2))]
+    pre, own_params = None, params
+    if P:
+        pc, pst = [synth.alloc_cache(1, H, P, D, gpu) for _ in range(2)], [torch.zeros(1, H, D, 2, dtype=torch.float16, device=gpu) for _ in range(2)]
+        gemv.append_kv_pair(*pc, rand(1, H, P, D), rand(1, H, P, D), *params, 0, *pst)
+        pre = gemv.SharedPrefix(*pc, P, *params)
+        own_params = [(st[0, :, :, 0].contiguous(), st[0, :, :, 1].contiguous(), *p[2:]) for st, p in zip(pst, params)]
+    cache = [synth.alloc_cache(B, H, T + n, D, gpu) for _ in range(2)]
+    ckpt = [torch.zeros(B, H, (T + n) // 256 + 1, D, 2, dtype=torch.float16, device=gpu) for _ in range(2)]
+    state = [torch.zeros(B, H, D, 2, dtype=torch.float16, device=gpu) for _ in range(2)]
+    gemv.append_kv_pair(*cache, rand(B, H, T, D), rand(B, H, T, D), *own_params, 0, *state, k_ckpt=ckpt[0], v_ckpt=ckpt[1], ckpt_interval=256)
+    q, new = rand(B, H * G, n, D), [rand(B, H, n, D) for _ in range(2)]
+    parts = [slice(0, 3), slice(B - 3, B)]
+    few = [[t[p].clone() for t in (q, *cache, *new, *ckpt)] for p in parts]
+
+    def run(q, kc, vc, kn, vn, kk, vk):
+        return gemv.extend(q, kc, vc, kn, vn, *own_params, T, D ** -0.5, prefix=pre, k_ckpt=kk, v_ckpt=vk, ckpt_interval=256)
+    whole = run(q, *cache, *new, *ckpt)
+    assert torch.isfinite(whole).all()
+    for p, f in zip(parts, few):
+        got = run(*f)
+        assert torch.equal(f[1], cache[0][p]) and torch.equal(f[2], cache[1][p])
+        assert torch.equal(f[5].view(torch.int16), ckpt[0][p].view(torch.int16)) and torch.equal(f[6].view(torch.int16), ckpt[1][p].view(torch.int16))
+        top = 16.0        # values follow rows of up to 6, and twice that where the scale has not settled
+        assert (got.float() - whole[p].float()).abs().max().item() <= 2 * top * (2.0 ** -11 + 2.0 ** -14 + (P + T + n) * 2.0 ** -25 + 2.0 ** -11)

@@ -299,3 +299,19 @@ def test_norms_without_a_device():
     for layer in model.model.layers:
         assert layer.self_attn.q_norm.weight.grad.abs().sum() > 0 and layer.self_attn.k_norm.weight.grad.abs().sum() > 0
     assert not hasattr(_model("cpu").model.layers[0].self_attn, "q_norm")
+
+
+@pytest.mark.gpu
+def test_extend_in_other_types(gpu):
+    """Rows of fp32 are rounded to fp16 in front of the kernels, as in decode; the result comes back in the query's type."""
+    H, B, n, T = 2, 2, 5, 33
+    kg, vg = (_flat(synth.make_params(H, D, seed=s).to(gpu)) for s in (3, 4))
+    k, v = (synth.make_k(B, H, T + n, D, seed=s, dtype=torch.float16).to(gpu) for s in (1, 2))
+    q = torch.randn(B, H, n, D, generator=torch.Generator().manual_seed(5)).half().to(gpu)
+    outs = []
+    for to in (torch.float16, torch.float32):
+        c = KVCacheLayer_ADKV()
+        c.prefill(k[:, :, :T], v[:, :, :T], *kg, *vg)
+        outs.append(c.extend(q.to(to), k[:, :, T:].to(to), v[:, :, T:].to(to), *kg, *vg, scaling=D ** -0.5))
+        assert outs[-1].dtype == to and outs[-1].shape == (B, n, H, D)
+    assert torch.equal(outs[0].float(), outs[1])
