@@ -1012,8 +1012,9 @@ struct Fetch {
 // which read the same tiles.  A wave's tile with 32 rows is 1024 cycles of matrix instructions and some 1500 of others, half of them the softmax;
 // with two waves to a SIMD it takes 2900, 3500 with a mask: neither pipe is full (matrix cores 29 to 35 % busy), the wave that waits for its reads or
 // results is not covered by one other.  512 tokens of 8 sequences, 32 heads, over 4096 tokens, masked: 430 to 490 us by the clock that the card
-// holds, 590 to 670 TFLOP/s; without fetching its tiles 11 % less, without exponentials 7 % less.  A wave of the SIMD a tile behind, raised
-// priorities around the products and reads of the LDS issued a group ahead changed nothing.
+// holds, 590 to 670 TFLOP/s; without fetching its tiles 11 % less, without exponentials 7 % less.  A wave of the SIMD a tile behind, a
+// raised priority for the softmax or for one of two workgroups and reads of the LDS issued a group ahead changed nothing; a raised priority for the
+// products made it 810.
 template <int MASK>
 __global__ __launch_bounds__(MANY_WAVES * 64, 2) void attend_many_kernel(Args)
 {
