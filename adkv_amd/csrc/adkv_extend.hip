@@ -198,14 +198,16 @@ template <bool FEW> __device__ __forceinline__ int value_piece(int c, int u) { r
 template <bool MAX>
 __device__ __forceinline__ float fold_quarters(float v) // over the lanes l % 16
 {
-    unsigned a = __builtin_bit_cast(unsigned, v), b;
-    asm volatile("v_mov_b32 %0, %1" : "=v"(b) : "v"(a)); // two copies: the compiler folds a swap of a register with itself
+    unsigned a = __builtin_bit_cast(unsigned, v), b = a;
+    // Two copies: the compiler folds a swap of a register with itself.  The copy is its own: behind one in a block of assembly it would
+    // not keep the two wait states that the swap needs.
+    asm volatile("" : "+v"(b));
     u2v r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
     unsigned x = r.x, y = r.y;
     asm volatile("" : "+v"(x), "+v"(y));
     v = MAX ? fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y)) : __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y);
-    a = __builtin_bit_cast(unsigned, v);
-    asm volatile("v_mov_b32 %0, %1" : "=v"(b) : "v"(a));
+    b = a = __builtin_bit_cast(unsigned, v);
+    asm volatile("" : "+v"(b));
     r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
     x = r.x;
     y = r.y;

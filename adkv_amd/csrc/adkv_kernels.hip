@@ -196,11 +196,13 @@ typedef unsigned u2v __attribute__((ext_vector_type(2)));
 
 // s + s[lane ^ 16] / s + s[lane ^ 32] through the gfx950 row/half swap instructions.  Both the copy
 // and the results go through opaque asm statements: handed two identical values, or asked for the
-// float sum of the two results directly, this compiler folds the pair into one register.
+// float sum of the two results directly, this compiler folds the pair into one register.  The statements
+// are empty: the exchange needs two wait states behind what writes its registers, and the compiler keeps them
+// behind its own copy, not behind one that stands in the statement.
 __device__ __forceinline__ float xor16_add(float s)
 {
-    unsigned a = __builtin_bit_cast(unsigned, s), b;
-    asm volatile("v_mov_b32 %0, %1" : "=v"(b) : "v"(a));
+    unsigned a = __builtin_bit_cast(unsigned, s), b = a;
+    asm volatile("" : "+v"(b));
     const u2v r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
     unsigned x = r.x, y = r.y;
     asm volatile("" : "+v"(x), "+v"(y));
@@ -209,8 +211,8 @@ __device__ __forceinline__ float xor16_add(float s)
 
 __device__ __forceinline__ float xor32_add(float s)
 {
-    unsigned a = __builtin_bit_cast(unsigned, s), b;
-    asm volatile("v_mov_b32 %0, %1" : "=v"(b) : "v"(a));
+    unsigned a = __builtin_bit_cast(unsigned, s), b = a;
+    asm volatile("" : "+v"(b));
     const u2v r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
     unsigned x = r.x, y = r.y;
     asm volatile("" : "+v"(x), "+v"(y));
@@ -233,14 +235,14 @@ __device__ __forceinline__ float wave_reduce(float v)
     v = mirror_fold<0x4E, MAX>(v);  // quad_perm [2, 3, 0, 1]
     v = mirror_fold<0x141, MAX>(v); // row_half_mirror
     v = mirror_fold<0x140, MAX>(v); // row_mirror
-    unsigned a = __builtin_bit_cast(unsigned, v), b; // see xor16_add
-    asm volatile("v_mov_b32 %0, %1" : "=v"(b) : "v"(a));
+    unsigned a = __builtin_bit_cast(unsigned, v), b = a; // see xor16_add
+    asm volatile("" : "+v"(b));
     const u2v r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
     unsigned x = r.x, y = r.y;
     asm volatile("" : "+v"(x), "+v"(y));
     v = MAX ? fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y)) : __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y);
-    a = __builtin_bit_cast(unsigned, v);
-    asm volatile("v_mov_b32 %0, %1" : "=v"(b) : "v"(a));
+    b = a = __builtin_bit_cast(unsigned, v);
+    asm volatile("" : "+v"(b));
     const u2v h = __builtin_amdgcn_permlane32_swap(a, b, false, false);
     x = h.x;
     y = h.y;

@@ -41,15 +41,15 @@ __device__ __forceinline__ float head_reduce(float v)
     v = fold_row<0x124, MAX>(v);
     v = fold_row<0x122, MAX>(v);
     v = fold_row<0x121, MAX>(v);
-    unsigned a = __builtin_bit_cast(unsigned, v), b; // see xor16_add
-    asm volatile("v_mov_b32 %0, %1" : "=v"(b) : "v"(a));
+    unsigned a = __builtin_bit_cast(unsigned, v), b = a; // see xor16_add
+    asm volatile("" : "+v"(b));
     const u2v r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
     unsigned x = r.x, y = r.y;
     asm volatile("" : "+v"(x), "+v"(y));
     v = fold<MAX>(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
     if (LPH == 64) {
-        a = __builtin_bit_cast(unsigned, v);
-        asm volatile("v_mov_b32 %0, %1" : "=v"(b) : "v"(a));
+        b = a = __builtin_bit_cast(unsigned, v);
+        asm volatile("" : "+v"(b));
         const u2v h = __builtin_amdgcn_permlane32_swap(a, b, false, false);
         x = h.x;
         y = h.y;
