@@ -519,9 +519,9 @@ struct Consumer {
     f4v o[NB][NC];
     float m[NB], l[NB];
     int row[NB];          // of the unit
-    int limit[NB];        // tokens of the source that it looks at
+    int limit[NB];        // tokens of the source that it looks at, and that the span has
     const char *mask[NB]; // its mask at the source's first token
-    int seen, tokens;     // of the source: what every row looks at, all
+    int seen, tokens;     // of the source: what every row looks at (of the span), all
     MaskRaw<J, MASK> masks[NB];
 
     // of row r of a unit: sequence, token, query head
@@ -574,17 +574,18 @@ struct Consumer {
                 o[k][c] = (f4v){0.0f, 0.0f, 0.0f, 0.0f};
         }
     }
-    // what a row looks at of a span's source
+    // What a row looks at of a span's source, up to the span's end: of few rows a span may end inside a tile, and the tile's rest, which is
+    // zero there, is the next span's.
     __device__ __forceinline__ void look(KArgs &a, const W &at)
     {
         const Extent s = all_of(a.s[at.src].x);
-        seen = s.seen;
+        seen = min(s.seen, at.t1);
         tokens = s.tokens;
 #pragma unroll
         for (int k = 0; k < NB; k++) {
             int b, i, hq;
             place(a, at, min(row[k], at.rows - 1), b, i, hq);
-            limit[k] = s.causal ? s.seen + i : s.seen;
+            limit[k] = min(s.causal ? s.seen + i : s.seen, at.t1);
             if constexpr (MASK != 0)
                 mask[k] = (const char *)a.mask + (b * a.m_sb + hq * a.m_sh + i * a.m_st + s.col) * (MASK == 2 ? 4 : 2);
         }
@@ -781,7 +782,7 @@ __device__ __forceinline__ void consume(KArgs &a, int items, const char *tiles, 
         opened = ends;
         c.template look_at<1>(t, lane, c.masks);
         __syncthreads();
-        if (t < c.tokens) { // of a span's last tile half may be empty
+        if (t < at.t1) { // of a span's last tile half may be empty
             f4v sc[1][1];
             uint32_t w[1][2];
             c.template scores<1>(from, step, lane, sc);
