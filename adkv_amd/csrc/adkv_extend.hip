@@ -679,11 +679,13 @@ struct Consumer {
             }
             const float ref = m[k] == -INFINITY ? 0.0f : m[k]; // nothing but -inf so far: all weights are zero
             float sum = 0.0f;
-            if (MASK != 0 && !plain && __any(fabsf(ref) > 1024.0f)) {
-                // the difference first: beside a mask the largest may be as large as its type's lowest value
+            if (MASK != 0 && __any(fabsf(ref) > 1024.0f)) {
+                // The difference first: beside a mask the largest may be as large as its type's lowest value, also for rows of a plain tile,
+                // of which later tokens are all that they could look at (-inf, which has to stay that).
+                const float unit = plain ? a.scaling : 1.0f;
 #pragma unroll
                 for (int e = 0; e < 4 * J; e++)
-                    x[e] = __builtin_amdgcn_exp2f((x[e] - ref) * c);
+                    x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], unit, -ref) * c);
             } else {
                 const float unit = MASK != 0 && plain ? a.scaling * LOG2E : c;
 #pragma unroll
