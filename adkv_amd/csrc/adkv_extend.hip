@@ -1325,6 +1325,14 @@ static Plan plan(int B, int H, int G, int n, int P, int p_interval, int p_ckpt, 
 
 static int64_t pad256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 
+static int64_t workspace_bytes_of(const Plan &p, int B, int H, int64_t rows)
+{
+    return 2 * pad256((int64_t)B * H * D * 4) + pad256(p.pieces() * rows * 8) + pad256(p.pieces() * rows * D * 4) + p.image_bytes(0, H) + p.image_bytes(1, H);
+}
+
+// rows of the joining launch: a grid is 2^32 threads at most, 32 for a row
+constexpr int64_t JOIN_MAX = (1ll << 27) - 8;
+
 } // namespace adkv_ext
 
 using namespace adkv_ext;
@@ -1338,8 +1346,7 @@ int64_t adkv_extend_workspace_bytes(int B, int Hq, int H, int T, int n, int n_ck
         return 0;
     const Plan p = plan(B, H, Hq / H, n, P, prefix_n_ckpt_cap > 0 ? prefix_ckpt_interval : 0, prefix_n_ckpt_cap, T,
                         n_ckpt_cap > 0 ? ckpt_interval : 0, n_ckpt_cap);
-    const int64_t rows = (int64_t)B * n * Hq;
-    return 2 * pad256((int64_t)B * H * D * 4) + pad256(p.pieces() * rows * 8) + pad256(p.pieces() * rows * D * 4) + p.image_bytes(0, H) + p.image_bytes(1, H);
+    return workspace_bytes_of(p, B, H, (int64_t)B * n * Hq);
 }
 
 int adkv_extend(const void *q, const int64_t *q_strides, void *k_cache, void *v_cache, const void *k_new, const void *v_new,
@@ -1403,11 +1410,26 @@ int adkv_extend(const void *q, const int64_t *q_strides, void *k_cache, void *v_
             p_interval = prefix->ckpt_interval;
         }
     }
-    const int64_t need = adkv_extend_workspace_bytes(B, Hq, H, T, n, n_ckpt_cap, ckpt_interval, P, p_cap, p_interval);
-    if (!workspace || workspace_bytes < need)
+    // everything is refused here, in front of the launches: a call that fails has changed nothing
+    if (n > 1)
+        for (int i = 0; i < 2; i++) { // rows that the encoder reads, as aligned words
+            const int64_t *st = i ? v_strides : k_strides;
+            if ((uintptr_t)(i ? v_new : k_new) & 3)
+                return ADKV_E_ALIGN;
+            if (st && (st[0] < 0 || st[1] < 0 || st[2] < D || ((st[0] | st[1] | st[2]) & 1)))
+                return ADKV_E_SHAPE;
+        }
+    const Plan pl = plan(B, H, G, n, P, p_interval, p_cap, T, ckpt_interval, n_ckpt_cap);
+    if ((int64_t)B * H * H >= 1ll << 32 || (int64_t)B * n * n >= 1ll << 32 || (pl.pieces() > 1 && rows > JOIN_MAX))
+        return ADKV_E_SHAPE;
+    for (int i = 0; i < 2; i++) {
+        const int64_t per = (int64_t)pl.blocks[i] * pl.nseg[i], items = per * (i ? (int64_t)B * H : H);
+        if (pl.there[i] && items * per >= 1ll << 32)
+            return ADKV_E_SHAPE;
+    }
+    if (!workspace || workspace_bytes < workspace_bytes_of(pl, B, H, rows))
         return ADKV_E_WORKSPACE;
 
-    const Plan pl = plan(B, H, G, n, P, p_interval, p_cap, T, ckpt_interval, n_ckpt_cap);
     char *ws = (char *)workspace;
     const int64_t state_bytes = pad256((int64_t)B * H * D * 4);
     h1 *k_state = (h1 *)ws, *v_state = (h1 *)(ws + state_bytes);
@@ -1443,8 +1465,6 @@ int adkv_extend(const void *q, const int64_t *q_strides, void *k_cache, void *v_
     own.x.interval = ckpt_interval;
     own.x.intervals = pl.intervals[1];
     own.x.col = P;
-    if ((int64_t)B * H * H >= 1ll << 32 || (int64_t)B * n * n >= 1ll << 32)
-        return ADKV_E_SHAPE;
     a.by_head = div(H);
     a.by_token = div(n);
     a.q = (const h1 *)q;
@@ -1511,11 +1531,6 @@ int adkv_extend(const void *q, const int64_t *q_strides, void *k_cache, void *v_
         g.items = (int)((int64_t)(u1 - u0) * g.blocks * g.nseg);
         return g;
     };
-    for (int i = 0; i < 2; i++) {
-        const int64_t per = (int64_t)pl.blocks[i] * pl.nseg[i], items = per * (i ? (int64_t)B * H : H);
-        if (pl.there[i] && items * per >= 1ll << 32)
-            return ADKV_E_SHAPE;
-    }
     typedef void (*Kernel)(Args);
     if ((pl.there[0] && pl.few[0]) || pl.few[1]) {
         static const Kernel kernels[2][3] = {{attend_kernel<4, 0>, attend_kernel<4, 1>, attend_kernel<4, 2>},
