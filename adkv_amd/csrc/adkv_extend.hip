@@ -64,9 +64,10 @@ struct Source {
     Extent x;
 };
 
-// x / d for x * d < 2^32: see divide()
+// x / d by a multiplication with 2^64 / d, rounded up, and a shift: exact for any x and d of 31 bits, as the error is below x * d / 2^64.  (With 32
+// bits x * d has to be below 2^32, which 65536 new tokens of one sequence are not.)
 struct Div {
-    uint32_t d, mul;
+    uint32_t d, lo, hi;
 };
 
 // Query rows and the sources that they look at.  Group 0 has the rows (sequence, token, query head of the group) of a KV head and
@@ -107,8 +108,12 @@ struct Args {
 // The arguments are read where the launch has put them: indexed by what a wave is at, a copy would live in scratch memory.
 #define ADKV_KERNARG const __attribute__((address_space(4)))
 typedef ADKV_KERNARG Args KArgs;
-__device__ __forceinline__ int divide(int x, const Div &by) { return by.d == 1 ? x : (int)__umulhi((uint32_t)x, by.mul); }
-__device__ __forceinline__ int divide(int x, ADKV_KERNARG Div &by) { return by.d == 1 ? x : (int)__umulhi((uint32_t)x, by.mul); }
+__device__ __forceinline__ int quotient(uint32_t x, uint32_t d, uint32_t lo, uint32_t hi)
+{
+    return d == 1 ? (int)x : (int)(((uint64_t)x * hi + __umulhi(x, lo)) >> 32);
+}
+__device__ __forceinline__ int divide(int x, const Div &by) { return quotient(x, by.d, by.lo, by.hi); }
+__device__ __forceinline__ int divide(int x, ADKV_KERNARG Div &by) { return quotient(x, by.d, by.lo, by.hi); }
 // all of a structure at once: field by field, between branches, every read is a wait
 template <typename T>
 __device__ __forceinline__ T all_of(ADKV_KERNARG T &from)
@@ -1420,13 +1425,11 @@ int adkv_extend(const void *q, const int64_t *q_strides, void *k_cache, void *v_
                 return ADKV_E_SHAPE;
         }
     const Plan pl = plan(B, H, G, n, P, p_interval, p_cap, T, ckpt_interval, n_ckpt_cap);
-    if ((int64_t)B * H * H >= 1ll << 32 || (int64_t)B * n * n >= 1ll << 32 || (pl.pieces() > 1 && rows > JOIN_MAX))
+    if (pl.pieces() > 1 && rows > JOIN_MAX)
         return ADKV_E_SHAPE;
-    for (int i = 0; i < 2; i++) {
-        const int64_t per = (int64_t)pl.blocks[i] * pl.nseg[i], items = per * (i ? (int64_t)B * H : H);
-        if (pl.there[i] && items * per >= 1ll << 32)
+    for (int i = 0; i < 2; i++) // items are counted in 32 bits, and beyond the last by a launch's workgroups
+        if (pl.there[i] && (i ? (int64_t)B * H : H) * pl.blocks[i] * pl.nseg[i] > INT32_MAX / 4)
             return ADKV_E_SHAPE;
-    }
     if (!workspace || workspace_bytes < workspace_bytes_of(pl, B, H, rows))
         return ADKV_E_WORKSPACE;
 
@@ -1442,7 +1445,10 @@ int adkv_extend(const void *q, const int64_t *q_strides, void *k_cache, void *v_
     auto tensor = [](const void *codes, const void *ckpt, const void *const *p) {
         return Tensor{(const uint32_t *)codes, (const h1 *)ckpt, (const h1 *)p[0], (const h1 *)p[1], (const h1 *)p[2], (const h1 *)p[3], (const h1 *)p[4]};
     };
-    auto div = [](int64_t d) { return Div{(uint32_t)d, (uint32_t)(((1ull << 32) + d - 1) / d)}; };
+    auto div = [](int64_t d) {
+        const uint64_t mul = ~0ull / (uint64_t)d + 1; // of 1 it is 2^64, and not used
+        return Div{(uint32_t)d, (uint32_t)mul, (uint32_t)(mul >> 32)};
+    };
     Source &pre = a.s[0], &own = a.s[1];
     pre = Source{};
     if (P > 0) {

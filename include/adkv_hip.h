@@ -468,6 +468,8 @@ int adkv_rope_norm_qk_backward(const void *q_grad, const void *k_grad, const voi
  * The state in front of token T is replayed from the checkpoint before it; where T opens an interval its checkpoint is recorded, and
  * those that the new tokens cross.  Sums and scores are fp32; weights are rounded to fp16 relative to the largest so far.  A value that is
  * infinite or NaN in a channel reaches that channel of all n queries of the call, also of those in front of its token.
+ * Up to 2^24 tokens of a prefix and of a sequence, fewer than 2^25 sequences x KV heads and fewer than 2^30 rows B * n * Hq; 2^27 - 8 rows
+ * where a row's outputs are joined from several pieces of its context.  Everything is refused before anything is launched.
  * workspace: >= adkv_extend_workspace_bytes(...) bytes, 256-byte aligned (the prefix's arguments 0 without one).
  */
 typedef struct {
