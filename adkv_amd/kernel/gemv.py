@@ -882,7 +882,7 @@ def extend(
     xv, vs = _row_strides(v_new)
     if workspace is None:
         with _lib.device_guard(dev):       # the size depends on the device
-            workspace = torch.empty(extend_workspace_bytes(B, nq, nh, T, n, ccap, civ, P, pcap), dtype=torch.uint8, device=dev)
+            workspace = torch.empty(extend_workspace_bytes(B, nq, nh, T, n, ccap, ckpt_interval, P, pcap), dtype=torch.uint8, device=dev)
     _chk(workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.device == dev, "workspace must be a uint8 tensor on the same device")
     out = torch.empty((B, n, nq, DIM), dtype=act, device=dev)
     with _lib.device_guard(dev):
@@ -898,6 +898,7 @@ def extend(
 
 def extend_workspace_bytes(B: int, nq: int, nh: int, T: int, n: int, n_ckpt_cap: int = 0, ckpt_interval: int = 0, P: int = 0,
                            prefix_n_ckpt_cap: int = 0) -> int:
-    """Bytes ``extend`` needs for ``n`` new tokens behind ``T`` cached ones and a prefix of ``P``."""
+    """Bytes ``extend`` needs for ``n`` new tokens behind ``T`` cached ones and a prefix of ``P``; ``ckpt_interval`` is that of whichever has
+    checkpoints (a capacity above 0), as in ``extend``."""
     return int(_lib.lib().adkv_extend_workspace_bytes(B, nq, nh, T, n, n_ckpt_cap, ckpt_interval, P, prefix_n_ckpt_cap,
                                                       ckpt_interval if prefix_n_ckpt_cap else 0))
