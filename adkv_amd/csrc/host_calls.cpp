@@ -294,7 +294,8 @@ PyObject *append(PyObject *, PyObject *const *args, Py_ssize_t nargs)
         const at::Tensor &x = *t[2 + i];
         for (int j = 0; j < 3; j++)
             strides[i][j] = x.stride(j);
-        if (!x.is_contiguous() && (!rows(x) || x.stride(2) < D || x.stride(0) < 0 || x.stride(1) < 0))
+        if ((uintptr_t)x.const_data_ptr() % 4 ||
+            (!x.is_contiguous() && (!rows(x) || x.stride(2) < D || x.stride(0) < 0 || x.stride(1) < 0)))
             Py_RETURN_NONE;
         const at::Tensor &st = *t[4 + i];
         if (st.scalar_type() != at::kHalf || !st.is_contiguous() || st.numel() != B * H * D * 2)
@@ -351,7 +352,7 @@ PyObject *extend(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     int64_t strides[2][3], qs[3];
     for (int i = 0; i < 2; i++) {
         const at::Tensor &x = *t[3 + i];
-        if (x.sizes() != at::IntArrayRef(token) ||
+        if (x.sizes() != at::IntArrayRef(token) || (uintptr_t)x.const_data_ptr() % 4 ||
             (!x.is_contiguous() && (!rows(x) || x.stride(2) < D || x.stride(0) < 0 || x.stride(1) < 0)))
             Py_RETURN_NONE;
         for (int j = 0; j < 3; j++)

@@ -366,7 +366,8 @@ def _row_strides(t: torch.Tensor):
     the rows where they lie (contiguous channels, even strides, 4-byte aligned), else the tensor
     is packed first."""
     if t.is_contiguous():
-        return t, None
+        # contiguous() would give back a packed tensor that starts between two words as it is
+        return (t.clone(memory_format=torch.contiguous_format) if t.data_ptr() & 3 else t), None
     sb, sh, st, sc = t.stride()
     if sc == 1 and st >= t.shape[3] and not ((sb | sh | st) & 1) and not (t.data_ptr() & 3) \
             and min(sb, sh) >= 0:
@@ -877,7 +878,7 @@ def extend(
             mask = mask.contiguous()
         mst = _stride3(mask)
     if q.stride(3) != 1 or any(st % 2 for st, k in zip(q.stride()[:3], q.shape[:3]) if k > 1) or q.data_ptr() % 4:
-        q = q.contiguous()
+        q = q.clone(memory_format=torch.contiguous_format)     # also where it is packed, but starts between two words
     xk, ks = _row_strides(k_new)
     xv, vs = _row_strides(v_new)
     if workspace is None:
