@@ -461,7 +461,9 @@ class KVCacheLayer_ADKV:
                 raise ValueError("saved code tensor does not match its geometry")
             if self._ckpt_interval and sd["prefix_key_ckpt"].shape[2] != P // self._ckpt_interval:
                 raise ValueError("saved checkpoints do not cover the saved tokens")
-            self._prefix = (to("prefix_key_codes"), to("prefix_value_codes"), P, to("prefix_key_ckpt"), to("prefix_value_ckpt"),
+            # a prefix shorter than an interval has no checkpoint yet, and the kernels take tensors of one at least
+            ck = [t if t is None or t.shape[2] else t.new_zeros(1, H, 1, C, 2) for t in (to("prefix_key_ckpt"), to("prefix_value_ckpt"))]
+            self._prefix = (to("prefix_key_codes"), to("prefix_value_codes"), P, *ck,
                             tuple(to("prefix_key_state")), tuple(to("prefix_value_state")))
 
     # ------------------------------------------------------------------ accounting
