@@ -67,7 +67,9 @@ class KVCacheLayer_ADKV:
         # A decode step appends inside the attention kernels and leaves these stale.
         self._key_state: torch.Tensor | None = None
         self._value_state: torch.Tensor | None = None
-        self._state_valid = False
+        # whether a sequence's is that behind its last token, a byte per sequence, and the sequences that are this object's: a batch_view()
+        # has its parent's bytes, which is how the parent knows that a slice was stepped
+        self._valid, self._span = bytearray(), slice(0, 0)
         self._quant_len = 0
         self._cap_len = 0
         self._B = self._H = self._C = 0
@@ -78,6 +80,15 @@ class KVCacheLayer_ADKV:
         # a share(): what every sequence begins with, (codes, codes, tokens, checkpoints, checkpoints, zp and sc behind it), K then V,
         # [1, H, ..]; everything above is then of the tokens behind it
         self._prefix: tuple | None = None
+
+    @property
+    def _state_valid(self) -> bool:
+        return self._B > 0 and 0 not in self._valid[self._span]
+
+    @_state_valid.setter
+    def _state_valid(self, valid: bool) -> None:
+        if self._valid:      # there are buffers
+            self._valid[self._span] = b"\1" * self._B if valid else bytes(self._B)
 
     # ------------------------------------------------------------------ HF cache protocol
     def get_seq_length(self) -> int:
@@ -139,7 +150,8 @@ class KVCacheLayer_ADKV:
         (self._cap_len, self._key_buf, self._value_buf,
          self._key_ckpt, self._value_ckpt) = self._new_buffers(tokens, alloc)
         mk = lambda: alloc((B, H, C, 2), dtype=torch.float16, device=device)
-        self._key_state, self._value_state, self._state_valid = mk(), mk(), True
+        self._key_state, self._value_state = mk(), mk()
+        self._valid, self._span = bytearray(b"\1" * B), slice(0, B)
 
     def _cap_buffers(self, T: int):
         """Make room for ``T`` tokens.  New slots are zero, as the append kernels expect."""
@@ -182,7 +194,8 @@ class KVCacheLayer_ADKV:
         if self._key_ckpt is not None:
             v._key_ckpt, v._value_ckpt = self._key_ckpt[b0:b1], self._value_ckpt[b0:b1]
         v._key_state, v._value_state = self._key_state[b0:b1], self._value_state[b0:b1]
-        v._state_valid, v._shares_storage = self._state_valid, True
+        v._valid, v._span = self._valid, slice(self._span.start + b0, self._span.start + b1)
+        v._shares_storage = True
         v._prefix = self._prefix
         return v
 
@@ -206,13 +219,14 @@ class KVCacheLayer_ADKV:
         return v
 
     def commit(self, tokens: int) -> None:
-        """Declare that every sequence now holds ``tokens`` quantised tokens (all slices prefilled)."""
+        """Declare that every sequence now holds ``tokens`` quantised tokens (all slices prefilled).  The carried state goes along
+        unless a slice was decoded or extended with."""
         tokens -= self._prefix_len()
         if tokens > self._cap_len:
             raise ValueError("more tokens than the cache holds")
         if tokens < 0:
             raise ValueError("fewer tokens than the shared prefix has")
-        self._quant_len, self._state_valid = tokens, True
+        self._quant_len = tokens
 
     def _check_geometry(self, B: int, H: int, C: int, device: torch.device):
         if self._key_buf is None:
@@ -255,6 +269,7 @@ class KVCacheLayer_ADKV:
             self._quant_len, self._key_state, self._value_state,
             k_ckpt=self._key_ckpt, v_ckpt=self._value_ckpt, ckpt_interval=self._ckpt_interval, bits=self._bits, fresh=fresh)
         self._quant_len += key_states.shape[2]
+        self._state_valid = True
 
     def prefill(self, key_states, value_states,
                 key_zp_init, key_scale_init, key_alpha, key_beta, key_quant_target,
