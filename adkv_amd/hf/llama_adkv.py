@@ -42,6 +42,23 @@ class ADKVConfig:
     quant_target: torch.Tensor
 
 
+def make_head_norms(attn, config) -> None:
+    """config.adkv_qk_norm: every head's queries and keys are normed before the rotation (extension; the reference's model has no such norm)."""
+    if getattr(config, "adkv_qk_norm", False):
+        attn.q_norm = LlamaRMSNorm(attn.head_dim, eps=config.rms_norm_eps)
+        attn.k_norm = LlamaRMSNorm(attn.head_dim, eps=config.rms_norm_eps)
+
+
+def norm_and_rotate(attn, q, k, cos, sin):
+    """The norms that ``make_head_norms`` gave ``attn`` and the rotary embedding of ``q [B, Hq, T, C]`` and ``k [B, H, T, C]``."""
+    wq, wk = attn.q_norm.weight, attn.k_norm.weight
+    if (q.is_cuda and all(t.dtype == q.dtype for t in (cos, sin, wq, wk)) and cos.dim() == 3
+            and q.dtype in (torch.float16, torch.bfloat16, torch.float32) and attn.head_dim % 8 == 0 and attn.head_dim <= 512):
+        # one launch for both norms and the rotation, and one for their gradients
+        return rope_norm_qk(q, k, cos, sin, wq, wk, attn.q_norm.variance_epsilon)
+    return apply_rotary_pos_emb(attn.q_norm(q), attn.k_norm(k), cos, sin)
+
+
 class LlamaAttention_ADKV(LlamaAttention):
     """Llama attention whose single-token steps read the packed ADKV cache."""
 
@@ -53,19 +70,11 @@ class LlamaAttention_ADKV(LlamaAttention):
                 # fp16 because the deployment recurrence is fp16; filled by load_adkv_config()
                 self.register_buffer(f"{side}_{name}", torch.empty(width, dtype=torch.float16),
                                      persistent=False)
-        # config.adkv_qk_norm: every head's queries and keys are normed before the rotation (extension; the reference's model has no such norm)
-        if getattr(config, "adkv_qk_norm", False):
-            self.q_norm = LlamaRMSNorm(self.head_dim, eps=config.rms_norm_eps)
-            self.k_norm = LlamaRMSNorm(self.head_dim, eps=config.rms_norm_eps)
+        make_head_norms(self, config)
 
     def _rotate(self, q, k, cos, sin):
         if hasattr(self, "q_norm"):
-            wq, wk = self.q_norm.weight, self.k_norm.weight
-            if (q.is_cuda and all(t.dtype == q.dtype for t in (cos, sin, wq, wk)) and cos.dim() == 3
-                    and q.dtype in (torch.float16, torch.bfloat16, torch.float32) and self.head_dim % 8 == 0 and self.head_dim <= 512):
-                # one launch for both norms and the rotation, and one for their gradients
-                return rope_norm_qk(q, k, cos, sin, wq, wk, self.q_norm.variance_epsilon)
-            return apply_rotary_pos_emb(self.q_norm(q), self.k_norm(k), cos, sin)
+            return norm_and_rotate(self, q, k, cos, sin)
         wants_grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad)
         if (q.is_cuda and q.dtype in (torch.float16, torch.bfloat16) and cos.dtype == q.dtype
                 and cos.dim() == 3 and self.head_dim % 4 == 0 and not wants_grad):

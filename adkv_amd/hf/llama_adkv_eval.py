@@ -26,7 +26,7 @@ from transformers.models.llama.modeling_llama import (
 from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
 
 from ..train.train_model import quant_f32_pair
-from .llama_adkv import ADKV_PARAM_FIELDS, ADKVConfig  # noqa: F401
+from .llama_adkv import ADKV_PARAM_FIELDS, ADKVConfig, make_head_norms, norm_and_rotate  # noqa: F401
 
 SCALE_MIN = math.exp(-4.0)
 SCALE_MAX = math.exp(4.0)
@@ -196,6 +196,7 @@ class LlamaAttention_ADKV(LlamaAttention):
         n = config.num_key_value_heads * self.head_dim
         for name in self._FP32_BUFFERS:
             self.register_buffer(name, torch.empty(n, dtype=torch.float32), persistent=False)
+        make_head_norms(self, config)
 
     def _apply(self, fn, recurse=True):
         # the quantiser state is fp32 whatever dtype the model is cast to
@@ -221,7 +222,7 @@ class LlamaAttention_ADKV(LlamaAttention):
         k = self.k_proj(hidden_states).view(shape).transpose(1, 2)
         v = self.v_proj(hidden_states).view(shape).transpose(1, 2)
         cos, sin = position_embeddings
-        q, k = apply_rotary_pos_emb(q, k, cos, sin)
+        q, k = norm_and_rotate(self, q, k, cos, sin) if "q_norm" in self._modules else apply_rotary_pos_emb(q, k, cos, sin)
 
         if past_key_values is not None:
             if not isinstance(past_key_values, KVCache_ADKV):
