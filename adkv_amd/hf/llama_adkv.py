@@ -73,7 +73,7 @@ class LlamaAttention_ADKV(LlamaAttention):
         make_head_norms(self, config)
 
     def _rotate(self, q, k, cos, sin):
-        if hasattr(self, "q_norm"):
+        if "q_norm" in self._modules:      # hasattr() of what is not there costs a microsecond per layer
             return norm_and_rotate(self, q, k, cos, sin)
         wants_grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad)
         if (q.is_cuda and q.dtype in (torch.float16, torch.bfloat16) and cos.dtype == q.dtype
