@@ -9,6 +9,7 @@
 // conversions and error messages.  A number is the library's return code.
 #include <algorithm>
 
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -698,6 +699,10 @@ PyObject *guarded(PyObject *self, PyObject *const *args, Py_ssize_t n)
 {
     try {
         return CALL(self, args, n);
+    } catch (python_error &e) {
+        // raised by Python code that a call has come to (a hook of saved tensors; a checkpointed region ends its recomputation that way): the caller's
+        e.restore();
+        return nullptr;
     } catch (const std::exception &) {
         Py_RETURN_NONE; // out of memory, or a mode that allocates otherwise: the Python function meets it too
     }
