@@ -829,8 +829,9 @@ __device__ __forceinline__ void fill_half(char *lds, int tid)
 }
 
 // Four waves replay the tile after the one that the others multiply with, one per SIMD, through two buffers and a barrier per tile.
-// A workgroup goes on to its next item without a gap.  Bound by instruction issue: replay and products of a tile are some 2000 cycles of every
-// SIMD whether its rows are one or sixteen.  128 sequences of 32 heads with 65 tokens each: 42 us (codes of 34 MB are 7); a
+// A workgroup goes on to its next item without a gap.  Replay, hand-over through the LDS and products of a tile are some 2000 cycles of every
+// SIMD whether its rows are one or sixteen, which bounds it; a limit of the replay it is not (a step's own kernels, without the hand-over,
+// replay 2.7 times as many tokens in a time).  128 sequences of 32 heads with 65 tokens each: 43 us (codes of 34 MB are 7); a
 // prefix of 8192 tokens and 4 sequences of 1001, 32 heads: 36 us.
 template <int BITS, int MASK>
 __global__ __launch_bounds__(FEW_THREADS) void attend_kernel(Args)
@@ -1002,7 +1003,7 @@ __global__ __launch_bounds__(256) void values_kernel(Images im)
     }
 }
 
-// A tile in 32 loads of 1 KB straight to the LDS, four by each of eight waves.
+// A tile in 32 loads of 1 KB straight to the LDS, eight by each of four waves.
 struct Fetch {
     static constexpr uint32_t PART = TILE_BYTES / MANY_WAVES;
     uint32_t from, to;
@@ -1021,10 +1022,11 @@ struct Fetch {
 // of eight waves and three tiles: 512 masked tokens of 8 sequences 690 us instead of 530).  Workgroups of one XCD take neighbouring items,
 // which read the same tiles.  A wave's tile with 32 rows is 1024 cycles of matrix instructions and some 1500 of others, half of them the softmax;
 // with two waves to a SIMD it takes 2900, 3500 with a mask: neither pipe is full (matrix cores 29 to 35 % busy), the wave that waits for its reads or
-// results is not covered by one other.  512 tokens of 8 sequences, 32 heads, over 4096 tokens, masked: 430 to 490 us by the clock that the card
-// holds, 590 to 670 TFLOP/s; without fetching its tiles 11 % less, without exponentials 7 % less.  A wave of the SIMD a tile behind, a
+// results is not covered by one other.  512 tokens of 8 sequences, 32 heads, over 4096 tokens, masked: 430 to 510 us by the clock that the card
+// holds, 570 to 670 TFLOP/s; without fetching its tiles 11 % less, without exponentials 7 % less.  A wave of the SIMD a tile behind, a
 // raised priority for the softmax or for one of two workgroups and reads of the LDS issued a group ahead changed nothing; a raised priority for the
-// products made it 810.
+// products made it 810.  Tiles that hold later tokens only are walked through like others: a call that is mostly its own new tokens takes up to twice what it
+// needs (2048 tokens of 32 heads with nothing in front of them 169 us, 235 behind 2048 others).
 template <int MASK>
 __global__ __launch_bounds__(MANY_WAVES * 64, 2) void attend_many_kernel(Args)
 {
@@ -1125,7 +1127,8 @@ __global__ __launch_bounds__(MANY_WAVES * 64, 2) void attend_many_kernel(Args)
 
 // out = sum e^(m-M) o / sum e^(m-M) l over the pieces.  Four channels per lane, 32 lanes per row, WAYS of them for a share of the
 // pieces each, in a fixed order: where rows are few the pieces are many and a lane that walks through all of them waits for each
-// (128 rows of 100 pieces 25 us, with WAYS = 8 five).
+// (128 rows of 100 pieces 25 us, with WAYS = 8 five).  Whole calls with WAYS = 8 and 1, us: 128 rows 44 and 64, 1024 rows 42 and 43 or 59 and 62, 4096
+// rows 93.5 and 95.0, 8192 rows 103 and 102, 16384 rows 122 and 119, 32768 rows 127 and 118; 5120 rows of few pieces 57 and 56.
 template <int WAYS>
 __global__ __launch_bounds__(256) void join_kernel(const float *__restrict__ partial, const float2 *__restrict__ ml, h1 *__restrict__ out,
                                                    long rows, int pieces, int act_bf16)
@@ -1269,7 +1272,9 @@ constexpr int64_t IMAGE_MAX = 1ll << 30; // bytes of own tiles at a time, unless
 // Rows of a sequence that fill a workgroup walk through the prefix by themselves, and their outputs need no joining (512 tokens of 8 sequences 520 us,
 // 680 with the prefix apart; at 40 rows 60 us instead of 58).  Workgroups
 // walk through items, two per CU.  The length of a piece is chosen for the shortest call by the model (us): a workgroup's items x
-// (64 tokens of a piece x 1.3 or, of many rows, 2.3, + 1), and 4 TB/s for the partial results, written and read.
+// (64 tokens of a piece x 1.3 or, of many rows, 2.3, + 1), and 4 TB/s for the partial results, written and read.  With 0.8 and 1.4, these, 2.2 and 3.8,
+// us: 257 new tokens of 4 sequences behind 3001, 8 heads of 4 queries, 157, 145, 146; 33 of one behind 6000 48.4, 45.5, 46.1; a token of 4 sequences
+// over 8192 + 1000 45.7, 43.7, 43.9; of 128 over 4096 + 64 92.5, 93.5, 95.0; of 48 over 7777 + 301, 4 queries, 62.5, 61.0, 60.5; seven other sizes within 2 %.
 // T: the own tokens in front of the new ones.
 static Plan plan(int B, int H, int G, int n, int P, int p_interval, int p_ckpt, int T, int interval, int n_ckpt)
 {

@@ -14,7 +14,7 @@
 // instead of 49 for the first size below); the row's 2^log lanes sum by
 // exchanges.  A lane takes its pairs of HEADS heads of a token: cos, sin and the weights are loaded once for them, and all loads are in flight together.
 // Four sequences of 2048 tokens, 32 + 32 heads of 128 values in fp16: 268 MB in 46 us (5.8 TB/s; a copy of 1 GiB reaches 5.1).  Two of 4096 tokens,
-// 32 + 8 heads in bf16: 168 MB in 29 us there and 251 MB in 48 us back (5.8 and 5.2 TB/s), and 4 us for the workgroups' sums of dw.
+// 32 + 8 heads in bf16: 168 MB in 29 us there and 251 MB in 48 to 50 us back (5.8 and 5.0 to 5.2 TB/s), and 4 us for the workgroups' sums of dw.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
