@@ -50,6 +50,14 @@ def _workspace(dev: torch.device, need: int) -> torch.Tensor:
     return ws
 
 
+def _additive(mask: torch.Tensor | None, query: torch.Tensor) -> torch.Tensor | None:
+    """A boolean mask (sdpa's: true where a token is looked at) as what is added to scores: the lowest value of the query's type where it is false."""
+    if mask is None or mask.dtype is not torch.bool:
+        return mask
+    dt = query.dtype if query.dtype in (torch.float16, torch.bfloat16) else torch.float32
+    return torch.full(mask.shape, torch.finfo(dt).min, dtype=dt, device=mask.device).masked_fill_(mask, 0.0)
+
+
 class KVCacheLayer_ADKV:
     """Quantised K/V store of one attention layer."""
 
@@ -316,7 +324,7 @@ class KVCacheLayer_ADKV:
                scaling: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
         """One causal decode step: attend over the cached tokens and the new one, append the new
         K/V codes, return ``(output [B,H,C] in the query's dtype, weights [B,H,ctx+1] fp16)``
-        (weights ``None`` behind a shared prefix)."""
+        (weights ``None`` behind a shared prefix).  A mask is additive, or boolean (true where a token is looked at)."""
         ctx = self._quant_len
         if self._prefix is not None:
             if query_states.shape[2] != 1 or key_states.shape[2] != 1:
@@ -326,6 +334,7 @@ class KVCacheLayer_ADKV:
                               value_zp_init, value_scale_init, value_alpha, value_beta, value_quant_target,
                               attention_mask, scaling)
             return out[:, 0], None
+        attention_mask = _additive(attention_mask, query_states)
         if self._key_buf is not None and ctx < self._cap_len:
             r = _lib.host().decode(
                 query_states, key_states, value_states,
@@ -398,10 +407,7 @@ class KVCacheLayer_ADKV:
         if self._prefix is not None:
             kc, vc, tokens, kck, vck = self._prefix[:5]
             prefix = SharedPrefix(kc, vc, tokens, key, value, kck, vck)
-        if attention_mask is not None and attention_mask.dtype == torch.bool:
-            dt = query_states.dtype if query_states.dtype in (torch.float16, torch.bfloat16) else torch.float32
-            attention_mask = torch.zeros(attention_mask.shape, dtype=dt, device=attention_mask.device).masked_fill_(
-                ~attention_mask, torch.finfo(dt).min)
+        attention_mask = _additive(attention_mask, query_states)
         same = query_states.dtype in (torch.float16, torch.bfloat16) and key_states.dtype == query_states.dtype == value_states.dtype
         act = (lambda t: t) if same else (lambda t: t.to(torch.float16))
         out = extend(act(query_states), self._key_buf, self._value_buf, act(key_states), act(value_states),

@@ -866,6 +866,7 @@ def extend(
             pre = _lib.Prefix(prefix.k_cache.data_ptr(), prefix.v_cache.data_ptr(), _lib.C.cast(pk, _lib.C.c_void_p),
                               _lib.C.cast(pv, _lib.C.c_void_p), pkc, pvc, P, prefix.k_cache.shape[2], pcap, piv)
     if mask is not None:
+        _chk(mask.dtype != torch.bool, "mask must be additive, not boolean")
         mask = mask[:, :, None] if mask.dim() == 3 else mask
         _chk(mask.dim() == 4 and mask.shape[3] == P + T + n and mask.shape[0] in (1, B) and mask.shape[1] in (1, nq) and mask.shape[2] in (1, n),
              "mask must broadcast to [B, nh, n, P + T + n]")
