@@ -63,6 +63,8 @@ PROTOTYPES = {
     "adkv_quant_f32_pair": (_i, [_vp] * 7 + [_i] * 6 + [_f, _f, _vp]),
     "adkv_extend_workspace_bytes": (C.c_int64, [_i] * 10),
     "adkv_extend": (_i, [_vp] * 12 + [_f, _vp] + [_i] * 9 + [_vp, _vp, _i, _i, _vp, _vp, C.c_int64, _vp]),
+    "adkv_prompt_attention_workspace_bytes": (C.c_int64, [_i] * 7),
+    "adkv_prompt_attention": (_i, [_vp] * 8 + [_f, _vp, _i, _vp] + [_i] * 7 + [_vp, C.c_int64, _vp]),
     "adkv_fp16_decode_workspace_bytes": (C.c_int64, [_i] * 3),
     "adkv_fp16_decode": (_i, [_vp] * 5 + [C.c_int64] + [_i] * 4 + [_f, _vp]),
 }

@@ -1,0 +1,817 @@
+// Causal attention over the dense rows of a prompt, grouped heads, fp16 or bf16.
+//
+//   x[i, t] = scaling * q_i . k_t + mask[i, t],  t up to i + (Tk - Tq);  out_i = sum_t softmax(x_i)_t v_t;  0 where a row looks at nothing
+//
+// One pass over the keys with the running maximum and sum of every row.  The rows of a KV head are those of all its query heads, row r being token
+// r / g of head r % g, so that a block of rows spans few tokens and its keys serve g heads.
+// Products are 32x32x16 matrix instructions, turned so that nothing has to change lanes between them: S^T = K Q^T leaves lane l with 16 of
+// 32 scores of row l % 32, which rounded to the operands' type are as O^T = V^T P^T takes them, if V's tokens are taken in the same order (4h..4h+3,
+// 4h+8.. for half h of the lanes).  V^T comes out of row-major tiles by the LDS's transposing reads.
+// Weights are e^(x - m) for an m that is at most 2^8 smaller than the largest so far, so that outputs are rescaled seldom.  They are rounded to the
+// operands' type for the matrix cores (fp16: after a factor of 2^7, which keeps 2^7 more of the small ones out of the subnormals); the sum that
+// divides them is that of the rounded ones.  Scores, m, sums and outputs are fp32.
+//
+// Two forms:
+//   many  a workgroup is four waves of 32 rows each over shared tiles of 64 keys and values, two tiles in the LDS, a barrier per tile
+//   few   a workgroup is 32 rows, its four waves walk through a quarter of the keys each in tiles of their own and are joined in the LDS; where
+//         that leaves CUs without work the keys are cut into pieces for several workgroups, joined by a second kernel
+#include <math.h>
+
+#include <algorithm>
+
+#include "adkv_device.h"
+
+#include "../../include/adkv_hip.h"
+
+#pragma clang fp contract(off)
+
+namespace adkv_prompt {
+using adkv::check_launch;
+using adkv::cu_count;
+using adkv::load_to_lds;
+using adkv::rsrc4;
+
+typedef uint32_t u2v __attribute__((ext_vector_type(2)));
+typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+typedef float f4v __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+typedef __bf16 b2v __attribute__((ext_vector_type(2)));
+typedef __bf16 b8v __attribute__((ext_vector_type(8)));
+typedef short s4v __attribute__((ext_vector_type(4)));
+typedef float f2v __attribute__((ext_vector_type(2)));
+
+#define LDS __attribute__((address_space(3)))
+#define GLOBAL __attribute__((address_space(1)))
+
+template <typename T> __device__ __forceinline__ LDS T *shared(uint32_t at) { return (LDS T *)(uintptr_t)at; }
+
+constexpr int WAVES = 4, NT = WAVES * 64, ROWS = 32; // rows of a wave
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float SLACK = 8.0f; // how much smaller than the largest (2^) a row's reference may be
+enum { F16 = ADKV_DT_F16, BF16 = ADKV_DT_BF16 };
+
+struct Rows { // of q, k or v
+    const char *p;
+    long sb, sh; // bytes
+    int st;
+};
+struct Args {
+    Rows q, k, v;
+    char *out;                // [B, Tq, H * g, D]
+    const char *mask;
+    long m_sb, m_sh, m_st;    // elements
+    const int *bounds;        // of packed sequences, n_seq + 1, or null
+    float *partial;           // [pieces][rows of all][D], few rows in pieces
+    f2v *ml;                  // [pieces][rows of all]
+    long all;                 // rows of all
+    int B, H, g, Tq, Tk, D, n_seq, mask_dt, pieces;
+    int blocks, units, together; // of a unit (packed: of all sequences); units; units whose blocks are in flight together
+    float scaling;
+    uint32_t by_g;            // 2^32 / g rounded up
+};
+
+template <int TYPE> struct Half;
+template <> struct Half<F16> {
+    typedef h8v v8;
+    static constexpr float BIAS = 7.0f;
+    static __device__ __forceinline__ f16v mfma(u4v a, u4v b, f16v c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float a, float b)
+    {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2v){a, b}, h2v));
+    }
+    static __device__ __forceinline__ float add(uint32_t w, float sum)
+    {
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2v, w), (h2v){(_Float16)1.0f, (_Float16)1.0f}, sum, false);
+    }
+    static __device__ __forceinline__ float number(uint16_t w) { return (float)__builtin_bit_cast(_Float16, w); }
+};
+template <> struct Half<BF16> {
+    typedef b8v v8;
+    static constexpr float BIAS = 0.0f;
+    static __device__ __forceinline__ f16v mfma(u4v a, u4v b, f16v c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float a, float b)
+    {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2v){a, b}, b2v));
+    }
+    static __device__ __forceinline__ float add(uint32_t w, float sum)
+    {
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2v, w), (b2v){(__bf16)1.0f, (__bf16)1.0f}, sum, false);
+    }
+    static __device__ __forceinline__ float number(uint16_t w) { return __uint_as_float((uint32_t)w << 16); }
+};
+
+__device__ __forceinline__ float other_half(float v, bool max)
+{
+    unsigned a = __float_as_uint(v), b = a;
+    asm volatile("" : "+v"(b)); // two copies: the compiler folds a swap of a register with itself
+    const u2v r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    unsigned x = r.x, y = r.y;
+    asm volatile("" : "+v"(x), "+v"(y));
+    return max ? fmaxf(__uint_as_float(x), __uint_as_float(y)) : __uint_as_float(x) + __uint_as_float(y);
+}
+
+// Rows of a tile are DP * 2 bytes in pieces of 16, piece c of row r at place c ^ turn(r), so that neither sixteen rows' reads of one piece
+// nor a transposing read (four consecutive rows, 64 bytes of each) meet in a bank.
+template <int DP> __device__ __forceinline__ constexpr int turn(int r)
+{
+    return DP == 64 ? (r >> 1 & 1) << 2 | (r >> 2 & 3) : (r & 3) << 2 | (r >> 2 & 3);
+}
+
+// The memory of a row axis from row `first` on, of which `there` rows may be read; what is behind them reads as zeros.
+__device__ __forceinline__ rsrc4 rows_from(const char *p, int st, int first, int there, int D)
+{
+    const uint64_t base = (uint64_t)p + (int64_t)first * st;
+    const int64_t bytes = there > 0 ? (int64_t)(there - 1) * st + D * 2 : 0;
+    return (rsrc4){(uint32_t)base, (uint32_t)(base >> 32) & 0xFFFFu, (uint32_t)(bytes < 0x40000000 ? bytes : 0x40000000), 0x00027000u};
+}
+
+// `n` rows straight to the LDS, 1 KB an instruction: rows first, first + 1.. of a tile, whose row 0 the buffer begins with
+template <int DP>
+__device__ __forceinline__ void fetch(uint32_t lds, rsrc4 buffer, int st, int first, int n, int lane, int D)
+{
+    constexpr int PIECES = DP / 8, EACH = 64 / PIECES;
+    const int r = lane / PIECES, c = lane % PIECES;
+#pragma unroll
+    for (int i = 0; i < n; i += EACH) {
+        const int row = first + i + r, piece = c ^ turn<DP>(row);
+        const uint32_t at = piece * 8 < D ? (uint32_t)(row * st + piece * 16) : 0x7FFFFFF0u;
+        load_to_lds(lds + (uint32_t)(first + i) * (DP * 2), at, buffer);
+    }
+}
+
+// Where a workgroup's rows are
+struct Job {
+    int b, h;
+    int q0, k0, n, m;  // first token of its queries and keys, how many; tokens of a sequence
+    int first, rows;   // its first row and how many the sequence has
+    int end;           // keys that its last row looks at
+    bool nothing;      // rows that belong to no sequence: zeros
+    int piece;
+};
+
+__device__ __forceinline__ int bound(const Args &a, int i) // of the sequences, and of what is in front of the first and behind the last
+{
+    if (i <= 0)
+        return 0;
+    return i > a.n_seq + 1 ? a.Tq : min(max(a.bounds[i - 1], 0), a.Tq);
+}
+
+// Of packed sequences the host knows neither how many blocks each has nor where they begin: sequence i's are from (its first row) / EACH + i on, which
+// leaves room for all of them and some empty ones in between.
+template <int EACH>
+__device__ __forceinline__ bool find(const Args &a, int block, int lane, Job &j)
+{
+    int lo = 0, hi = a.n_seq + 2; // the last i whose place is not behind `block`
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 63) / 64, at = lo + lane * step;
+        const bool before = at < hi && (int)((int64_t)bound(a, at) * a.g / EACH) + at <= block;
+        const uint64_t which = __ballot(before);
+        const int last = which ? 63 - __builtin_clzll(which) : 0;
+        lo += last * step;
+        hi = min(hi, lo + step);
+    }
+    const int x = bound(a, lo), y = bound(a, lo + 1);
+    j.n = j.m = max(y - x, 0);
+    j.q0 = j.k0 = x;
+    j.rows = j.n * a.g;
+    j.first = (block - (int)((int64_t)x * a.g / EACH) - lo) * EACH;
+    j.nothing = lo == 0 || lo == a.n_seq + 1;
+    return j.first < j.rows;
+}
+
+__device__ __forceinline__ int token(const Args &a, int r) { return a.g == 1 ? r : (int)__umulhi((uint32_t)r, a.by_g); }
+
+template <int EACH>
+__device__ __forceinline__ bool place(const Args &a, int i, int lane, Job &j)
+{
+    if (a.bounds != nullptr) {
+        // one after the other, all heads of a block together
+        const int block = i / (a.H * a.pieces), rest = i - block * a.H * a.pieces;
+        j.h = rest / a.pieces;
+        j.piece = rest - j.h * a.pieces;
+        j.b = 0;
+        if (!find<EACH>(a, a.blocks - 1 - block, lane, j))
+            return false;
+    } else {
+        // `together` units at a time, their longest rows first; consecutive units are on different XCDs, and a unit's blocks on one if
+        // there are eight of them or a multiple of that
+        j.piece = i % a.pieces;
+        i /= a.pieces;
+        const int batch = i / (a.together * a.blocks), here = min(a.together, a.units - batch * a.together);
+        i -= batch * a.together * a.blocks;
+        const int back = i / here, unit = batch * a.together + i - back * here;
+        j.b = unit / a.H;
+        j.h = unit - j.b * a.H;
+        j.q0 = j.k0 = 0;
+        j.n = a.Tq;
+        j.m = a.Tk;
+        j.rows = j.n * a.g;
+        j.first = (a.blocks - 1 - back) * EACH;
+        j.nothing = false;
+    }
+    j.end = j.nothing ? 0 : j.m - j.n + token(a, min(j.first + EACH, j.rows) - 1) + 1;
+    return true;
+}
+
+// A wave's 32 rows
+template <int TYPE, int DP, int MASK>
+struct Wave {
+    using Hf = Half<TYPE>;
+    static constexpr int STEPS = DP / 16, CB = DP / 32;
+    u4v q[STEPS];
+    f16v o[CB];
+    float m, l;      // of row lane % 32: reference, in powers of two; this half's sum
+    int row;         // of the sequence
+    int limit;       // keys that it looks at
+    int low, high;   // least and most of the wave's rows
+    const char *mask;
+    float c;
+    int lane;
+
+    __device__ __forceinline__ void open(const Args &a, const Job &j, int first, int lane_)
+    {
+        lane = lane_;
+        row = first + (lane & 31);
+        const int r = min(row, j.rows - 1), t = token(a, r), head = j.h * a.g + r - t * a.g;
+        limit = j.m - j.n + t + 1;
+        low = j.m - j.n + token(a, min(first, j.rows - 1)) + 1;
+        high = first < j.rows ? j.m - j.n + token(a, min(first + ROWS, j.rows) - 1) + 1 : 0;
+        low = __builtin_amdgcn_readfirstlane(low);
+        high = __builtin_amdgcn_readfirstlane(high);
+        const char *src = a.q.p + j.b * a.q.sb + head * a.q.sh + (long)(j.q0 + t) * a.q.st;
+        const uint32_t sign = a.scaling < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) {
+            const int piece = 2 * s + (lane >> 5);
+            u4v u = {0, 0, 0, 0};
+            if (piece * 8 < a.D)
+                u = *(const GLOBAL u4v *)(src + piece * 16);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                u[e] ^= sign;
+            q[s] = u;
+        }
+        c = fabsf(a.scaling) * LOG2E;
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int cb = 0; cb < CB; cb++)
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                o[cb][e] = 0.0f;
+        if constexpr (MASK != 0) {
+            const int size = a.mask_dt == 0 ? 4 : a.mask_dt == 3 ? 1 : 2;
+            mask = a.mask + (j.b * a.m_sb + head * a.m_sh + (long)t * a.m_st) * size;
+        }
+    }
+
+    // what is added to the scores of keys k.. k + 3, in powers of two; -inf for what is hidden
+    __device__ __forceinline__ void added(const Args &a, int k, int there, float *to) const
+    {
+        const int dt = a.mask_dt;
+        const int size = dt == 0 ? 4 : dt == 3 ? 1 : 2;
+        const GLOBAL char *p = (const GLOBAL char *)mask + (long)k * size;
+        uint32_t w[4];
+        typedef uint32_t u1 __attribute__((aligned(1)));
+        typedef uint32_t u2a __attribute__((ext_vector_type(2), aligned(2)));
+        typedef uint32_t u4a __attribute__((ext_vector_type(4), aligned(4)));
+        if (there >= 4) {
+            if (dt == 0) {
+                const u4a u = *(const GLOBAL u4a *)p;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    w[e] = u[e];
+            } else if (dt == 3) {
+                const uint32_t u = *(const GLOBAL u1 *)p;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    w[e] = u >> 8 * e & 255u;
+            } else {
+                const u2a u = *(const GLOBAL u2a *)p;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    w[e] = e & 1 ? u[e >> 1] >> 16 : u[e >> 1] & 0xFFFFu;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                w[e] = 0;
+                if (e < there)
+                    w[e] = dt == 0 ? ((const GLOBAL uint32_t *)p)[e] : dt == 3 ? (uint32_t)((const GLOBAL uint8_t *)p)[e] : (uint32_t)((const GLOBAL uint16_t *)p)[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (dt == 3)
+                to[e] = w[e] ? 0.0f : -INFINITY;
+            else
+                to[e] = dt == 0 ? __uint_as_float(w[e]) : dt == BF16 ? __uint_as_float(w[e] << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)w[e]);
+        }
+    }
+
+    // Score s of a key whose mask is x, in powers of two.  A type's lowest value times log2(e) would be -inf, which stands for hidden keys only: rows of
+    // nothing but lowest values look at all of them alike.
+    __device__ __forceinline__ float with(float s, float x) const
+    {
+        const float y = __builtin_fmaf(x, LOG2E, s * c);
+        return x == -INFINITY ? -INFINITY : y < -3.0e38f ? -3.0e38f : y; // what is no number stays that
+    }
+
+    // KB * 32 keys from k on, keys and values in the LDS
+    template <int KB>
+    __device__ __forceinline__ void tile(const Args &a, uint32_t keys, uint32_t values, int k)
+    {
+        const int r32 = lane & 31, h = lane >> 5, i16 = lane & 15;
+        f16v sc[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; kb++) {
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                sc[kb][e] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < STEPS; s++) {
+                const uint32_t at = keys + (kb * 32 + r32) * (DP * 2) + ((2 * s + h) ^ turn<DP>(r32)) * 16;
+                const u4v key = *shared<u4v>(at);
+                sc[kb] = Hf::mfma(key, q[s], sc[kb]);
+            }
+        }
+        float x[KB * 16];
+#pragma unroll
+        for (int e = 0; e < KB * 16; e++)
+            x[e] = sc[e >> 4][e & 15];
+        if constexpr (MASK != 0) {
+#pragma unroll
+            for (int e = 0; e < KB * 16; e += 4) {
+                const int at = k + (e >> 2) * 8 + 4 * h;
+                float add[4];
+                added(a, at, a.Tk - at, add);
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    x[e + i] = with(x[e + i], add[i]);
+            }
+        }
+        if (k + KB * 32 > low) {
+#pragma unroll
+            for (int e = 0; e < KB * 16; e++)
+                x[e] = k + (e >> 2) * 8 + 4 * h + (e & 3) < limit ? x[e] : -INFINITY;
+        }
+        float top = x[0];
+#pragma unroll
+        for (int e = 1; e < KB * 16; e++)
+            top = fmaxf(top, x[e]);
+        if (MASK == 0)
+            top *= c;
+        if (__any(top > m + SLACK)) {
+            const float to = fmaxf(m, other_half(top, true));
+            const float shrink = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - to);
+            m = to;
+            l *= shrink;
+#pragma unroll
+            for (int cb = 0; cb < CB; cb++)
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    o[cb][e] *= shrink;
+        }
+        const float ref = m == -INFINITY ? 0.0f : m - Hf::BIAS; // nothing yet: all weights are zero
+        uint32_t w[KB * 8];
+#pragma unroll
+        for (int e = 0; e < KB * 16; e += 2) {
+            float p[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                p[i] = __builtin_amdgcn_exp2f(MASK != 0 ? x[e + i] - ref : __builtin_fmaf(x[e + i], c, -ref));
+            w[e >> 1] = Hf::pack(p[0], p[1]);
+            l = Hf::add(w[e >> 1], l);
+        }
+#pragma unroll
+        for (int kk = 0; kk < KB * 2; kk++) {
+            const u4v p = {w[kk * 4], w[kk * 4 + 1], w[kk * 4 + 2], w[kk * 4 + 3]};
+#pragma unroll
+            for (int cb = 0; cb < CB; cb++) {
+                u2v half[2];
+#pragma unroll
+                for (int d = 0; d < 2; d++) {
+                    const int key = kk * 16 + 8 * d + 4 * h + (i16 >> 2), piece = cb * 4 + (lane >> 4 & 1) * 2 + (i16 >> 1 & 1);
+                    const uint32_t at = values + key * (DP * 2) + (piece ^ turn<DP>(key)) * 16 + (i16 & 1) * 8;
+                    half[d] = __builtin_bit_cast(u2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16(shared<s4v>(at)));
+                }
+                o[cb] = Hf::mfma((u4v){half[0].x, half[0].y, half[1].x, half[1].y}, p, o[cb]);
+            }
+        }
+    }
+
+    __device__ __forceinline__ bool strange() const
+    {
+        bool nan = l != l;
+#pragma unroll
+        for (int cb = 0; cb < CB; cb++)
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                nan |= o[cb][e] != o[cb][e];
+        return __any(nan);
+    }
+
+    // To the LDS: 32 rows of DP sums, in pieces of four at place piece ^ row, then the rows' m and l
+    __device__ __forceinline__ void leave(uint32_t to)
+    {
+        const int r32 = lane & 31, h = lane >> 5;
+        const float sum = other_half(l, false);
+#pragma unroll
+        for (int cb = 0; cb < CB; cb++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int piece = cb * 8 + (e >> 2) * 2 + h;
+                *shared<f4v>(to + (r32 * (DP / 4) + (piece ^ (r32 & 15))) * 16) = (f4v){o[cb][e], o[cb][e + 1], o[cb][e + 2], o[cb][e + 3]};
+            }
+        if (h == 0)
+            *shared<f2v>(to + ROWS * DP * 4 + r32 * 8) = (f2v){m, sum};
+    }
+};
+
+constexpr int result_bytes(int DP) { return ROWS * DP * 4 + ROWS * 8; }
+
+// The same as tile() and leave() for keys k0..k1, a row after the other and without a look at what is hidden: a hidden value that is infinite or not a
+// number meets a weight of zero in a matrix product, and leaves nothing of the row.  Taken where a product's results are no numbers.
+template <int TYPE, int DP, int MASK>
+__device__ __forceinline__ void carefully(const Args &a, const Job &j, int first, int k0, int k1, int lane, uint32_t to)
+{
+    using Hf = Half<TYPE>;
+    constexpr int N = DP / 64;
+    const float c = a.scaling * LOG2E;
+#pragma unroll 1
+    for (int i = 0; i < ROWS; i++) {
+        float o[N], m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int n = 0; n < N; n++)
+            o[n] = 0.0f;
+        const int r = min(first + i, j.rows - 1), t = token(a, r), head = j.h * a.g + r - t * a.g;
+        const int end = min(k1, j.m - j.n + t + 1);
+        const char *q = a.q.p + j.b * a.q.sb + head * a.q.sh + (long)(j.q0 + t) * a.q.st;
+#pragma unroll 1
+        for (int k = k0; k < end; k += 64) {
+            const int key = k + lane;
+            float x = -INFINITY;
+            if (key < end) {
+                const char *kp = a.k.p + j.b * a.k.sb + j.h * a.k.sh + (long)(j.k0 + key) * a.k.st;
+                float s = 0.0f;
+#pragma unroll 1
+                for (int d = 0; d < a.D; d++)
+                    s = __builtin_fmaf(Hf::number(((const GLOBAL uint16_t *)q)[d]), Hf::number(((const GLOBAL uint16_t *)kp)[d]), s);
+                if constexpr (MASK != 0) {
+                    Wave<TYPE, DP, MASK> w;
+                    w.c = c;
+                    w.mask = a.mask + (j.b * a.m_sb + head * a.m_sh + (long)t * a.m_st) * (a.mask_dt == 0 ? 4 : a.mask_dt == 3 ? 1 : 2);
+                    float add[4];
+                    w.added(a, key, 1, add);
+                    x = w.with(s, add[0]);
+                } else {
+                    x = s * c;
+                }
+            }
+            const uint64_t seen = __ballot(!(x == -INFINITY));
+            float top = x;
+            for (int d = 32; d; d >>= 1)
+                top = fmaxf(top, __shfl_xor(top, d));
+            const float now = fmaxf(m, top), shrink = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - now);
+            m = now;
+            const float ref = m == -INFINITY ? 0.0f : m - Hf::BIAS, p = x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - ref);
+            float sum = p;
+            for (int d = 32; d; d >>= 1)
+                sum += __shfl_xor(sum, d);
+            l = l * shrink + sum;
+#pragma unroll
+            for (int n = 0; n < N; n++)
+                o[n] *= shrink;
+#pragma unroll 1
+            for (int e = 0; e < 64; e++) {
+                if (!(seen >> e & 1))
+                    continue;
+                const float w = __shfl(p, e);
+                const char *vp = a.v.p + j.b * a.v.sb + j.h * a.v.sh + (long)(j.k0 + k + e) * a.v.st;
+#pragma unroll
+                for (int n = 0; n < N; n++)
+                    if (lane * N + n < a.D)
+                        o[n] = __builtin_fmaf(w, Hf::number(((const GLOBAL uint16_t *)vp)[lane * N + n]), o[n]);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const int d = lane * N + n;
+            *shared<float>(to + (i * (DP / 4) + ((d >> 2) ^ (i & 15))) * 16 + (d & 3) * 4) = o[n];
+        }
+        if (lane == 0)
+            *shared<f2v>(to + ROWS * DP * 4 + i * 8) = (f2v){m, l};
+    }
+}
+
+// Rows first.. first + n of what is left in the LDS by `from` waves for the same rows, joined and written; lanes take four channels each
+template <int TYPE, int DP, int FROM>
+__device__ __forceinline__ void deliver(const Args &a, const Job &j, uint32_t at, int row0, int first, int n, int lane)
+{
+    using Hf = Half<TYPE>;
+    constexpr int LANES = DP / 4, EACH = 64 / LANES;
+    const int piece = lane % LANES;
+    for (int i = first + lane / LANES; i < first + n; i += EACH) {
+        if (row0 + i >= j.rows)
+            break;
+        float M = -INFINITY, L = 0.0f;
+        f2v ml[FROM];
+#pragma unroll
+        for (int w = 0; w < FROM; w++) {
+            ml[w] = *shared<f2v>(at + w * result_bytes(DP) + ROWS * DP * 4 + i * 8);
+            M = fmaxf(M, ml[w].x);
+        }
+        const float ref = M == -INFINITY ? 0.0f : M;
+        f4v o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < FROM; w++) {
+            const f4v v = *shared<f4v>(at + w * result_bytes(DP) + (i * (DP / 4) + (piece ^ (i & 15))) * 16);
+            const float e = FROM == 1 ? 1.0f : __builtin_amdgcn_exp2f(ml[w].x - ref);
+            L = __builtin_fmaf(ml[w].y, e, L);
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                o[k] = __builtin_fmaf(v[k], e, o[k]);
+        }
+        if (piece * 4 >= a.D)
+            continue;
+        const int t = token(a, row0 + i), head = j.h * a.g + row0 + i - t * a.g;
+        const long r = ((long)j.b * a.Tq + j.q0 + t) * (a.H * a.g) + head;
+        if (a.pieces > 1) {
+            if (piece == 0)
+                *(GLOBAL f2v *)(a.ml + j.piece * a.all + r) = (f2v){M, L};
+            *(GLOBAL f4v *)(a.partial + (j.piece * a.all + r) * a.D + piece * 4) = o;
+            continue;
+        }
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        *(GLOBAL u2v *)(a.out + (r * a.D + piece * 4) * 2) = (u2v){Hf::pack(o[0] * inv, o[1] * inv), Hf::pack(o[2] * inv, o[3] * inv)};
+    }
+}
+
+template <int DP> constexpr int many_lds() { return std::max(2 * 64 * DP * 2 * 2, WAVES * result_bytes(DP)); }
+
+template <int TYPE, int DP, int MASK>
+__global__ __launch_bounds__(NT, DP > 128 ? 1 : 2) void many_kernel(const Args a)
+{
+    __shared__ uint4 smem[many_lds<DP>() / 16];
+    const uint32_t lds = (uint32_t)(uintptr_t)(LDS char *)(char *)smem;
+    constexpr int TILE = 64, BYTES = TILE * DP * 2;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    Job j;
+    if (!place<WAVES * ROWS>(a, blockIdx.x, lane, j))
+        return;
+    const int first = j.first + wave * ROWS;
+    Wave<TYPE, DP, MASK> w;
+    w.open(a, j, first, lane);
+    const char *kp = a.k.p + j.b * a.k.sb + j.h * a.k.sh + (long)j.k0 * a.k.st, *vp = a.v.p + j.b * a.v.sb + j.h * a.v.sh + (long)j.k0 * a.v.st;
+    auto load = [&](int k, uint32_t to) __attribute__((always_inline)) {
+        fetch<DP>(to, rows_from(kp, a.k.st, k, j.end - k, a.D), a.k.st, wave * 16, 16, lane, a.D);
+        fetch<DP>(to + BYTES, rows_from(vp, a.v.st, k, j.end - k, a.D), a.v.st, wave * 16, 16, lane, a.D);
+    };
+    if (j.end > 0)
+        load(0, lds);
+    int buffer = 0;
+    for (int k = 0; k < j.end; k += TILE) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); // the tile is there, and nobody reads the one before it any more
+        if (k + TILE < j.end)
+            load(k + TILE, lds + (buffer ^ 1) * 2 * BYTES);
+        if (k < w.high)
+            w.template tile<2>(a, lds + buffer * 2 * BYTES, lds + buffer * 2 * BYTES + BYTES, k);
+        buffer ^= 1;
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); // the tiles' place is free
+    const uint32_t mine = lds + wave * result_bytes(DP);
+    if (w.strange())
+        carefully<TYPE, DP, MASK>(a, j, first, 0, j.end, lane, mine);
+    else
+        w.leave(mine);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    deliver<TYPE, DP, 1>(a, j, mine, first, 0, ROWS, lane);
+}
+
+template <int DP> constexpr int few_stages() { return DP > 128 ? 1 : 2; }
+template <int DP> constexpr int few_lds() { return std::max(WAVES * few_stages<DP>() * 32 * DP * 2 * 2, WAVES * result_bytes(DP)); }
+
+template <int TYPE, int DP, int MASK>
+__global__ __launch_bounds__(NT, 1) void few_kernel(const Args a)
+{
+    __shared__ uint4 smem[few_lds<DP>() / 16];
+    const uint32_t lds = (uint32_t)(uintptr_t)(LDS char *)(char *)smem;
+    constexpr int TILE = 32, BYTES = TILE * DP * 2, STAGES = few_stages<DP>();
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    Job j;
+    if (!place<ROWS>(a, blockIdx.x, lane, j))
+        return;
+    Wave<TYPE, DP, MASK> w;
+    w.open(a, j, j.first, lane);
+    const int tiles = (j.end + TILE - 1) / TILE, parts = a.pieces * WAVES, part = j.piece * WAVES + wave;
+    const int k0 = (int)((int64_t)tiles * part / parts) * TILE, k1 = min((int)((int64_t)tiles * (part + 1) / parts) * TILE, j.end);
+    const char *kp = a.k.p + j.b * a.k.sb + j.h * a.k.sh + (long)j.k0 * a.k.st, *vp = a.v.p + j.b * a.v.sb + j.h * a.v.sh + (long)j.k0 * a.v.st;
+    const uint32_t own = lds + wave * (STAGES * 2 * BYTES);
+    auto load = [&](int k, uint32_t to) __attribute__((always_inline)) {
+        fetch<DP>(to, rows_from(kp, a.k.st, k, j.end - k, a.D), a.k.st, 0, TILE, lane, a.D);
+        fetch<DP>(to + BYTES, rows_from(vp, a.v.st, k, j.end - k, a.D), a.v.st, 0, TILE, lane, a.D);
+    };
+    if (k0 < k1)
+        load(k0, own);
+    int stage = 0;
+    for (int k = k0; k < k1; k += TILE) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // what was read of the tile that is overwritten now
+        if (STAGES > 1 && k + TILE < k1) {
+            load(k + TILE, own + (stage ^ 1) * 2 * BYTES);
+            if (DP == 64)
+                asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+            else
+                asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        w.template tile<1>(a, own + stage * 2 * BYTES, own + stage * 2 * BYTES + BYTES, k);
+        if (STAGES > 1) {
+            stage ^= 1;
+        } else if (k + TILE < k1) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            load(k + TILE, own);
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const uint32_t mine = lds + wave * result_bytes(DP);
+    if (w.strange())
+        carefully<TYPE, DP, MASK>(a, j, j.first, k0, k1, lane, mine);
+    else
+        w.leave(mine);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    deliver<TYPE, DP, WAVES>(a, j, lds, j.first, wave * (ROWS / WAVES), ROWS / WAVES, lane);
+}
+
+// Pieces of a row to its output, four channels per lane
+template <int TYPE>
+__global__ __launch_bounds__(256) void join_kernel(const Args a)
+{
+    const int lanes = a.D / 4;
+    const long i = (long)blockIdx.x * 256 + threadIdx.x, r = i / lanes;
+    const int piece = (int)(i - r * lanes);
+    if (r >= a.all)
+        return;
+    float M = -INFINITY;
+    for (int p = 0; p < a.pieces; p++)
+        M = fmaxf(M, a.ml[p * a.all + r].x);
+    const float ref = M == -INFINITY ? 0.0f : M;
+    float L = 0.0f;
+    f4v o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int p = 0; p < a.pieces; p++) {
+        const f2v ml = a.ml[p * a.all + r];
+        const f4v v = *(const GLOBAL f4v *)(a.partial + (p * a.all + r) * a.D + piece * 4);
+        const float e = __builtin_amdgcn_exp2f(ml.x - ref);
+        L = __builtin_fmaf(ml.y, e, L);
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            o[k] = __builtin_fmaf(v[k], e, o[k]);
+    }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    *(GLOBAL u2v *)(a.out + (r * a.D + piece * 4) * 2) = (u2v){Half<TYPE>::pack(o[0] * inv, o[1] * inv), Half<TYPE>::pack(o[2] * inv, o[3] * inv)};
+}
+
+// ------------------------------------------------------------------------------------------------------------------------- host
+
+struct Plan {
+    bool many;
+    int blocks, units, together, pieces;
+};
+
+static Plan plan(int B, int Hq, int H, int Tq, int Tk, int n_seq)
+{
+    const int g = Hq / H, cus = std::max(1, cu_count());
+    const int64_t rows = (int64_t)Tq * g;
+    Plan p;
+    p.units = n_seq ? H : B * H;
+    const auto blocks = [&](int each) { return (int)(n_seq ? rows / each + n_seq + 2 : (rows + each - 1) / each); };
+    p.many = (int64_t)p.units * blocks(WAVES * ROWS) >= cus;
+    p.blocks = blocks(p.many ? WAVES * ROWS : ROWS);
+    p.pieces = 1;
+    p.together = p.units;
+    if (p.many) {
+        // as many units at a time as fill the device twice, so that their blocks find their keys in the XCDs' caches
+        const int64_t fill = (4ll * cus + p.blocks - 1) / p.blocks;
+        p.together = (int)std::min<int64_t>(p.units, (fill + 7) / 8 * 8);
+    } else {
+        const int64_t wide = (int64_t)p.units * p.blocks, tiles = (Tk + 31) / 32;
+        p.pieces = (int)std::max<int64_t>(1, std::min<int64_t>(cus / wide, tiles / (2 * WAVES)));
+    }
+    return p;
+}
+
+static int checked(int B, int Hq, int H, int Tq, int Tk, int D, int n_seq)
+{
+    if (B <= 0 || Hq <= 0 || H <= 0 || Tq <= 0 || Tk < Tq || n_seq < 0 || Hq % H)
+        return ADKV_E_SHAPE;
+    if (n_seq && (B != 1 || Tq != Tk))
+        return ADKV_E_SHAPE;
+    if (D <= 0 || D > 256 || D % 8)
+        return ADKV_E_DIM;
+    const int64_t g = Hq / H;
+    // rows are counted in 31 bits and divided by g in 32; a grid is 2^32 threads at most
+    if (Tq * g * g > INT32_MAX || Tk > INT32_MAX - 256 || (Tq * g / ROWS + n_seq + 3) * B * H > (1 << 24) - 1 || (int64_t)B * Tq * Hq > INT32_MAX)
+        return ADKV_E_SHAPE;
+    return ADKV_OK;
+}
+
+template <int TYPE, int MASK> static auto many_of(int D) { return D > 128 ? many_kernel<TYPE, 256, MASK> : D > 64 ? many_kernel<TYPE, 128, MASK> : many_kernel<TYPE, 64, MASK>; }
+template <int TYPE, int MASK> static auto few_of(int D) { return D > 128 ? few_kernel<TYPE, 256, MASK> : D > 64 ? few_kernel<TYPE, 128, MASK> : few_kernel<TYPE, 64, MASK>; }
+
+} // namespace adkv_prompt
+
+extern "C" int64_t adkv_prompt_attention_workspace_bytes(int B, int Hq, int H, int Tq, int Tk, int D, int n_seq)
+{
+    using namespace adkv_prompt;
+    if (int rc = checked(B, Hq, H, Tq, Tk, D, n_seq))
+        return rc;
+    if (cu_count() <= 0)
+        return ADKV_E_DEVICE;
+    const Plan p = plan(B, Hq, H, Tq, Tk, n_seq);
+    return p.pieces > 1 ? (int64_t)p.pieces * B * Tq * Hq * (D * 4 + 8) : 0;
+}
+
+extern "C" int adkv_prompt_attention(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides, const void *v,
+                                     const int64_t *v_strides, const void *mask, const int64_t *mask_strides, float scaling, const int *bounds,
+                                     int n_seq, void *out, int B, int Hq, int H, int Tq, int Tk, int D, int dtype, void *workspace,
+                                     int64_t workspace_bytes, void *stream)
+{
+    using namespace adkv_prompt;
+    if (!q || !k || !v || !out || !q_strides || !k_strides || !v_strides || (mask && !mask_strides) || (n_seq > 0 && !bounds))
+        return ADKV_E_NULL;
+    if (int rc = checked(B, Hq, H, Tq, Tk, D, n_seq))
+        return rc;
+    const int type = dtype & 255, mask_dt = dtype >> 8;
+    if ((type != F16 && type != BF16) || mask_dt < 0 || mask_dt > ADKV_DT_BOOL || (mask && n_seq))
+        return ADKV_E_UNSUPPORTED;
+    uint64_t bits = (uint64_t)q | (uint64_t)k | (uint64_t)v | (uint64_t)out;
+    const int64_t *const strides[] = {q_strides, k_strides, v_strides};
+    for (const int64_t *s : strides) {
+        bits |= (uint64_t)(s[0] | s[1] | s[2]) * 2;
+        // tiles of 64 rows are addressed in 31 bits
+        if (s[0] < 0 || s[1] < 0 || s[2] < 0 || s[2] * 2 > 0x3FFFFFFF / 64)
+            return ADKV_E_SHAPE;
+    }
+    if (bits & 15)
+        return ADKV_E_ALIGN;
+    const int size = mask_dt == 0 ? 4 : mask_dt == ADKV_DT_BOOL ? 1 : 2;
+    if ((uint64_t)mask & (size - 1))
+        return ADKV_E_ALIGN;
+    if (cu_count() <= 0)
+        return ADKV_E_DEVICE;
+    const Plan p = plan(B, Hq, H, Tq, Tk, n_seq);
+    const int64_t all = (int64_t)B * Tq * Hq, need = p.pieces > 1 ? p.pieces * all * (D * 4 + 8) : 0;
+    if (need && (!workspace || workspace_bytes < need))
+        return ADKV_E_WORKSPACE;
+    if (need && (uint64_t)workspace & 15)
+        return ADKV_E_ALIGN;
+    Args a = {};
+    const auto rows = [](const void *p, const int64_t *s) { return Rows{(const char *)p, (long)s[0] * 2, (long)s[1] * 2, (int)(s[2] * 2)}; };
+    a.q = rows(q, q_strides);
+    a.k = rows(k, k_strides);
+    a.v = rows(v, v_strides);
+    a.out = (char *)out;
+    a.mask = (const char *)mask;
+    if (mask) {
+        a.m_sb = mask_strides[0];
+        a.m_sh = mask_strides[1];
+        a.m_st = mask_strides[2];
+    }
+    a.bounds = n_seq ? bounds : nullptr;
+    a.partial = (float *)workspace;
+    a.ml = (f2v *)((char *)workspace + (int64_t)p.pieces * all * D * 4);
+    a.all = all;
+    a.B = B;
+    a.H = H;
+    a.g = Hq / H;
+    a.Tq = Tq;
+    a.Tk = Tk;
+    a.D = D;
+    a.n_seq = n_seq;
+    a.mask_dt = mask_dt;
+    a.pieces = p.pieces;
+    a.blocks = p.blocks;
+    a.units = p.units;
+    a.together = p.together;
+    a.scaling = scaling;
+    a.by_g = (uint32_t)(((1ull << 32) + a.g - 1) / a.g);
+    const auto kernel = p.many ? (type == F16 ? (mask ? many_of<F16, 1>(D) : many_of<F16, 0>(D)) : (mask ? many_of<BF16, 1>(D) : many_of<BF16, 0>(D)))
+                               : (type == F16 ? (mask ? few_of<F16, 1>(D) : few_of<F16, 0>(D)) : (mask ? few_of<BF16, 1>(D) : few_of<BF16, 0>(D)));
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((int64_t)p.blocks * p.units * p.pieces)), dim3(NT), 0, (hipStream_t)stream, a);
+    if (int rc = check_launch())
+        return rc;
+    if (p.pieces > 1) {
+        const auto join = type == F16 ? join_kernel<F16> : join_kernel<BF16>;
+        hipLaunchKernelGGL(join, dim3((unsigned)((all * (D / 4) + 255) / 256)), dim3(256), 0, (hipStream_t)stream, a);
+        return check_launch();
+    }
+    return ADKV_OK;
+}

@@ -620,6 +620,95 @@ def rope_norm_qk(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch
     return (_RopeNorm.apply if wanted else _rope_norm_forward)(q, k, cos, sin, q_weight, k_weight, float(eps))
 
 
+_PROMPT_MASK_DT = {torch.float32: 0, torch.float16: _DT_F16, torch.bfloat16: _DT_BF16, torch.bool: 3}     # ADKV_DT_*
+
+
+def _no_derivatives(name: str, *tensors: torch.Tensor) -> None:
+    _chk(not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)), f"{name} has no gradient")
+    _chk(all(forward_ad.unpack_dual(t).tangent is None for t in tensors), f"{name} has no forward derivatives")
+
+
+def _prompt_rows(t: torch.Tensor):
+    """``t`` if ``adkv_prompt_attention`` can read it in place, else a copy; and its strides."""
+    ok = t.stride(3) == 1 and all(st % 8 == 0 for n, st in zip(t.shape[:3], t.stride()) if n > 1) \
+        and t.data_ptr() % 16 == 0 and (t.shape[2] == 1 or t.stride(2) < 1 << 23)
+    t = t if ok else t.clone(memory_format=torch.contiguous_format)
+    return t, _stride3(t)
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scaling: float, mask: torch.Tensor | None = None, *,
+                     bounds: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention over the dense rows of a prompt, as prefill and the evaluation model need it: ``q [B, Hq, Tq, D]`` are the last
+    ``Tq`` of ``Tk`` tokens, ``k``, ``v`` ``[B, H, Tk, D]``; returns ``[B, Tq, Hq, D]`` in their type.
+
+    ``out_i = sum_t softmax(scaling * q_i . k_t + mask_it) v_t`` over every token ``t`` up to query ``i``'s own; rows that look at nothing are
+    zeros.  (The reference calls transformers' attention here, src/adkv/hf/llama_adkv.py:365-378; queries of a single token over many are
+    its evaluation model's steps, src/adkv/hf/llama_adkv_eval.py:400-420.)
+
+    Args:
+        q, k, v: float16 or bfloat16, ``H`` dividing ``Hq``, ``D`` a multiple of 8 up to 256; any batch / head / token strides with
+            contiguous channels are read in place where rows are 16-byte aligned, and copied first where not.
+        mask: ``[B or 1, Hq or 1, Tq or 1, Tk]``, boolean (true where a token is looked at) or additive (any float type; minus infinity hides a
+            token whatever its key and value hold, a row of nothing but the type's lowest value looks at all tokens up to its own alike).
+        bounds: ``n`` sequences of different lengths share the row axis (``B == 1``, ``Tq == Tk``, no mask): int32 ``[n + 1]``, ascending, sequence
+            ``i`` is rows ``bounds[i] .. bounds[i+1]-1`` and looks at itself only; rows of no sequence are zeros.  On the device the values are
+            not checked (that would wait for it); what is read and written stays inside the tensors whatever they are.  On the
+            host they are checked and copied.
+
+    No gradient: refused where one is wanted.  Weights are rounded to the tensors' type; scores, sums and outputs are fp32.
+    """
+    _chk(q.dim() == 4 and k.dim() == 4 and v.dim() == 4, "q must be [B, Hq, Tq, D], k and v [B, H, Tk, D]")
+    B, Hq, Tq, D = q.shape
+    H, Tk = k.shape[1], k.shape[2]
+    _chk(k.shape == (B, H, Tk, D) and v.shape == k.shape, "q, k and v disagree in shape")
+    _chk(q.dtype in (torch.float16, torch.bfloat16), "q must be float16 or bfloat16")
+    _chk(k.dtype == q.dtype and v.dtype == q.dtype, "q, k and v must share one dtype")
+    _chk(0 < D <= 256 and D % 8 == 0, "head dim must be a multiple of 8 up to 256")
+    _chk(H > 0 and Hq > 0 and Hq % H == 0, "the number of query heads must be a multiple of that of KV heads")
+    _chk(Tq <= Tk, "the queries are the last of the tokens: there cannot be more of them")
+    _no_derivatives("prompt_attention", q, k, v)
+    n_seq = 0
+    if bounds is not None:
+        _chk(B == 1 and Tq == Tk and mask is None, "packed sequences need B == 1, as many queries as keys and no mask")
+        _chk(bounds.dim() == 1 and bounds.numel() >= 1 and not bounds.is_floating_point(), "bounds must be [n + 1] whole numbers")
+        n_seq = bounds.numel() - 1
+        if not bounds.is_cuda:
+            e = bounds.tolist()
+            _chk(0 <= e[0] and e[-1] <= Tq and all(x <= y for x, y in zip(e, e[1:])), "bounds must ascend within the rows")
+    if mask is not None:
+        _chk(mask.dim() == 4 and mask.shape[3] == Tk and mask.shape[0] in (1, B) and mask.shape[1] in (1, Hq) and mask.shape[2] in (1, Tq),
+             "mask must broadcast to [B, Hq, Tq, Tk]")
+        _chk(mask.dtype == torch.bool or mask.is_floating_point(), "mask must be boolean or additive")
+        _no_derivatives("prompt_attention", mask)
+    dev = _need_device(q, k, v)
+    out = torch.empty((B, Tq, Hq, D), dtype=q.dtype, device=dev)
+    if out.numel() == 0:
+        return out
+    if bounds is not None:
+        if n_seq == 0:
+            return out.zero_()
+        bounds = bounds.to(device=dev, dtype=torch.int32).contiguous()
+    mst, mdt = None, 0
+    if mask is not None:
+        mdt = _PROMPT_MASK_DT.get(mask.dtype, 0)
+        mask = mask.to(device=dev, dtype=mask.dtype if mask.dtype in _PROMPT_MASK_DT else torch.float32)
+        if mask.stride(3) != 1 and Tk > 1:
+            mask = mask.contiguous()
+        mst = _stride3(mask)
+    (q, qs), (k, ks), (v, vs) = _prompt_rows(q), _prompt_rows(k), _prompt_rows(v)
+    L = _lib.lib()
+    with _lib.device_guard(dev):
+        size = L.adkv_prompt_attention_workspace_bytes(B, Hq, H, Tq, Tk, D, n_seq)
+        _lib.check(min(size, 0), "prompt_attention")
+        workspace = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+        rc = L.adkv_prompt_attention(q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, _ptr(mask), mst, float(scaling), _ptr(bounds),
+                                     n_seq, out.data_ptr(), B, Hq, H, Tq, Tk, D,
+                                     (_DT_BF16 if q.dtype == torch.bfloat16 else _DT_F16) | mdt << 8, _ptr(workspace), size,
+                                     _lib.current_stream_ptr(dev))
+    _lib.check(rc, "prompt_attention")
+    return out
+
+
 def softmax_scale_mask(logits: torch.Tensor, scaling: float,
                        mask: torch.Tensor | None = None) -> torch.Tensor:
     """``softmax(logits.float()*scaling + mask) -> fp16`` in one launch.

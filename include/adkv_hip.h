@@ -379,6 +379,7 @@ void adkv_set_stage_events(void *const *events);
 #define ADKV_DT_F32 0
 #define ADKV_DT_F16 1
 #define ADKV_DT_BF16 2
+#define ADKV_DT_BOOL 3 /* masks of adkv_prompt_attention: a byte per key, 0 where it is hidden */
 #define ADKV_MASK_DT(dt) ((dt) << 8) /* in act_dtype of adkv_decode_step: the mask's type */
 #define ADKV_PARAMS_FREE 256         /* in x_dtype of adkv_quant_f32 */
 int adkv_quant_f32(const void *x, void *xhat, void *codes, void *zp_state, void *sc_state,
@@ -495,6 +496,28 @@ int adkv_extend(const void *q, const int64_t *q_strides, void *k_cache, void *v_
 int64_t adkv_fp16_decode_workspace_bytes(int B, int H, int T);
 int adkv_fp16_decode(const void *q, const void *K, const void *V, void *out, void *workspace,
                      int64_t workspace_bytes, int B, int H, int T, int D, float scaling, void *stream);
+
+/*
+ * Causal attention over the dense rows of a prompt (the attention of the reference's prefill and of its evaluation model,
+ * src/adkv/hf/llama_adkv.py:365-378, src/adkv/hf/llama_adkv_eval.py:400-420, which go through transformers'):
+ *   out[b, i, hq] = sum_t softmax_t(scaling * q[b, hq, i] . k[b, hq / (Hq / H), t] + mask[b, hq, i, t]) v[b, hq / (Hq / H), t]
+ * over t <= i + Tk - Tq, the queries being the last Tq of Tk tokens (Tq <= Tk); rows that look at nothing are zeros.
+ *   q [B, Hq, Tq, D], k, v [B, H, Tk, D] of fp16 or bfloat16, H dividing Hq, D a multiple of 8 up to 256; rows contiguous, 16-byte aligned,
+ *   element strides of batch, head and token in *_strides (multiples of 8).  out [B, Tq, Hq, D], packed, 16-byte aligned, of their type.
+ *   mask (may be NULL): element strides of batch, head and query token in mask_strides (0 where it is the same for all), keys contiguous; added
+ *   to the scores (fp16, bfloat16, fp32; minus infinity hides a key whatever it and its value hold), or ADKV_DT_BOOL.  A row of nothing but
+ *   its type's lowest value looks at all keys up to its own alike.
+ *   bounds (n_seq > 0): n_seq sequences share the row axis, B = 1, Tq = Tk, no mask: sequence i is rows bounds[i] .. bounds[i + 1] - 1,
+ *   n_seq + 1 ascending int32 from 0 to Tq; other rows are zeros.  A sequence may be empty.
+ *   dtype: of q, k, v, out, plus the mask's << 8.
+ *   workspace: adkv_prompt_attention_workspace_bytes() (0: none is needed), 16-byte aligned.
+ * Scores, maxima, sums and outputs are fp32; weights are rounded to the tensors' type.
+ */
+int64_t adkv_prompt_attention_workspace_bytes(int B, int Hq, int H, int Tq, int Tk, int D, int n_seq);
+int adkv_prompt_attention(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides, const void *v,
+                          const int64_t *v_strides, const void *mask, const int64_t *mask_strides, float scaling, const int *bounds,
+                          int n_seq, void *out, int B, int Hq, int H, int Tq, int Tk, int D, int dtype, void *workspace,
+                          int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }
