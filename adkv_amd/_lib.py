@@ -65,14 +65,22 @@ PROTOTYPES = {
     "adkv_extend": (_i, [_vp] * 12 + [_f, _vp] + [_i] * 9 + [_vp, _vp, _i, _i, _vp, _vp, C.c_int64, _vp]),
     "adkv_prompt_attention_workspace_bytes": (C.c_int64, [_i] * 7),
     "adkv_prompt_attention": (_i, [_vp] * 8 + [_f, _vp, _i, _vp] + [_i] * 7 + [_vp, C.c_int64, _vp]),
+    "adkv_take_sequences": (_i, [_vp, _i, _vp, _i, _i, _vp]),
+    "adkv_token_logprobs": (_i, [_vp, C.c_int64, C.c_int64, _vp] + [_i] * 5 + [_vp] * 5),
     "adkv_fp16_decode_workspace_bytes": (C.c_int64, [_i] * 3),
     "adkv_fp16_decode": (_i, [_vp] * 5 + [C.c_int64] + [_i] * 4 + [_f, _vp]),
 }
+
 
 class Prefix(C.Structure):
     """``adkv_prefix`` of include/adkv_hip.h."""
     _fields_ = [(n, _vp) for n in ("k_codes", "v_codes", "k_params", "v_params", "k_ckpt", "v_ckpt")] + \
         [(n, _i) for n in ("tokens", "n_super", "n_ckpt_cap", "ckpt_interval")]
+
+
+class Rows(C.Structure):
+    """``adkv_rows`` of include/adkv_hip.h."""
+    _fields_ = [("data", _vp), ("into", _vp)] + [(n, C.c_int64) for n in ("segments", "pitch", "into_pitch", "used")]
 
 
 _lib = None

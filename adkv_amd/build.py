@@ -16,7 +16,9 @@ SOURCES = [os.path.join(_DIR, "csrc", "adkv_kernels.hip"),
            os.path.join(_DIR, "csrc", "adkv_extend.hip"),
            os.path.join(_DIR, "csrc", "fp16_baseline.hip")]
 # The operators around a prompt are a library of their own, which the first one brings along: they are built and looked at without it.
-PROMPT_SOURCES = [os.path.join(_DIR, "csrc", "adkv_prompt.hip")]
+PROMPT_SOURCES = [os.path.join(_DIR, "csrc", "adkv_prompt.hip"),
+                  os.path.join(_DIR, "csrc", "adkv_logprobs.hip"),
+                  os.path.join(_DIR, "csrc", "adkv_sequences.hip")]
 HEADERS = sorted(glob.glob(os.path.join(_DIR, "csrc", "*.h"))) + \
     [os.path.join(_DIR, "..", "include", "adkv_hip.h")]
 LIB_PATH = os.path.join(_DIR, "libadkv_hip.so")

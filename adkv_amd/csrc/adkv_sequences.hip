@@ -1,0 +1,204 @@
+// Sequences of a cache copied over one another: row r of every tensor becomes what row index[r] was, all layers' tensors in a launch or two.
+//
+// Nothing but memory: a row that moves is read and written once, one that stays is not touched.  In place any map is taken, whatever the order in
+// which rows overwrite each other: a wave takes a column of the tensors (1 KB or less, of all rows), and has read what it needs of it before it
+// writes.  Columns are independent, so that there is nothing to wait for between waves.  32 loads of 1 KB are in flight per wave: the moved rows of as
+// many columns as that gives, or, with more than 32 rows, of a narrower column.
+// One of four beams of 603 tokens, 32 layers of 32 heads (166 MB read and written): see take_kernel.
+#include <algorithm>
+
+#include "adkv_device.h"
+
+#include "../../include/adkv_hip.h"
+
+namespace adkv_sequences {
+using adkv::check_launch;
+
+typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+#define GLOBAL __attribute__((address_space(1)))
+
+constexpr int WAVES = 4, SLOTS = 32, BLOCK = 1024; // bytes of a column
+constexpr int TENSORS = 96;                         // of a launch
+constexpr int MOST = 2048;                          // rows: with all of them moved a column is 16 bytes
+
+struct Tensor {
+    const char *from;
+    char *to;
+    int segments;        // of a row (heads)
+    int pitch, to_pitch; // of a segment, bytes
+    int used, width;     // columns up to `used` are copied, from there to `width` they are zeros
+    int first;           // job
+};
+struct Args {
+    const int64_t *index;
+    int rows, batch, n, jobs;
+    Tensor t[TENSORS];
+};
+static_assert(sizeof(Args) <= 4096, "kernel arguments");
+
+// A row may be another one's source: what is read of a column is there before any of it is written.
+__device__ __forceinline__ void all_read() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+template <bool INTO>
+__global__ __launch_bounds__(WAVES * 64) void take_kernel(const Args a)
+{
+    __shared__ int2 list[MOST];
+    __shared__ int count;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    if (threadIdx.x == 0)
+        count = 0;
+    __syncthreads();
+    // the rows that move, in any order
+    for (int r = threadIdx.x; r < a.rows; r += WAVES * 64) {
+        int64_t from = a.index[r];
+        const bool there = from >= 0 && from < a.batch;
+        if (INTO || (there && from != r))
+            list[atomicAdd(&count, 1)] = make_int2(r, there ? (int)from : -1);
+    }
+    __syncthreads();
+    const int m = __builtin_amdgcn_readfirstlane(count), job = (int)blockIdx.x * WAVES + wave;
+    if (m == 0 || job >= a.jobs)
+        return;
+    int which = 0;
+    for (int i = 0; i < a.n; i += 64)
+        which += __popcll(__ballot(i + lane < a.n && a.t[min(i + lane, TENSORS - 1)].first <= job));
+    which--;
+    const Tensor t = a.t[which];
+    const int blocks = (t.width + BLOCK - 1) / BLOCK; // columns of a segment
+    const long from_row = (long)t.segments * t.pitch, to_row = (long)t.segments * t.to_pitch;
+    int unit = (job - t.first) * SLOTS;
+    const int end = min(unit + SLOTS, t.segments * blocks);
+    u4v x[SLOTS];
+    if (m <= SLOTS) {
+        int log = 0; // 2^log slots are a column's
+        while (1 << log < m)
+            log++;
+        const int2 mine = list[min(lane, m - 1)];
+        for (; unit < end; unit += SLOTS >> log) {
+            const int seg0 = unit / blocks, block0 = unit - seg0 * blocks;
+            auto each = [&](auto &&f) __attribute__((always_inline)) {
+                int seg = seg0, block = block0;
+#pragma unroll
+                for (int i = 0; i < SLOTS; i++) {
+                    const int row = i & ((1 << log) - 1);
+                    if (i > 0 && row == 0 && ++block == blocks) {
+                        block = 0;
+                        seg++;
+                    }
+                    if (row < m && unit + (i >> log) < end)
+                        f(i, __builtin_amdgcn_readlane(mine.x, row), __builtin_amdgcn_readlane(mine.y, row), seg, block * BLOCK + lane * 16);
+                }
+            };
+            each([&](int i, int, int from, int seg, int at) __attribute__((always_inline)) {
+                x[i] = (u4v){0, 0, 0, 0};
+                if ((!INTO || from >= 0) && at < t.used)
+                    x[i] = *(const GLOBAL u4v *)(t.from + from * from_row + (long)seg * t.pitch + at);
+            });
+            all_read();
+            each([&](int i, int to, int, int seg, int at) __attribute__((always_inline)) {
+                if (at < t.width)
+                    *(GLOBAL u4v *)(t.to + to * to_row + (long)seg * t.to_pitch + at) = x[i];
+            });
+        }
+        return;
+    }
+    int log = 1; // 2^log rows to a slot
+    while (SLOTS << log < m)
+        log++;
+    const int wide = BLOCK >> log, sub = lane >> (6 - log), in = (lane & ((64 >> log) - 1)) * 16;
+    for (; unit < end; unit++) {
+        const int seg = unit / blocks, block = unit - seg * blocks;
+        for (int part = 0; part < 1 << log; part++) {
+            const int at = block * BLOCK + part * wide + in;
+#pragma unroll
+            for (int i = 0; i < SLOTS; i++) {
+                const int p = (i << log) + sub;
+                x[i] = (u4v){0, 0, 0, 0};
+                if (p < m && at < t.used) {
+                    const int from = list[p].y;
+                    if (!INTO || from >= 0)
+                        x[i] = *(const GLOBAL u4v *)(t.from + from * from_row + (long)seg * t.pitch + at);
+                }
+            }
+            all_read();
+#pragma unroll
+            for (int i = 0; i < SLOTS; i++) {
+                const int p = (i << log) + sub;
+                if (p < m && at < t.width)
+                    *(GLOBAL u4v *)(t.to + list[p].x * to_row + (long)seg * t.to_pitch + at) = x[i];
+            }
+        }
+    }
+}
+
+} // namespace adkv_sequences
+
+extern "C" int adkv_take_sequences(const adkv_rows *tensors, int n, const int64_t *index, int rows, int batch, void *stream)
+{
+    using namespace adkv_sequences;
+    if (n < 0 || rows < 0 || batch <= 0 || rows > MOST)
+        return ADKV_E_SHAPE;
+    if ((n > 0 && !tensors) || (rows > 0 && !index))
+        return ADKV_E_NULL;
+    bool into = false;
+    for (int i = 0; i < n; i++) {
+        const adkv_rows &t = tensors[i];
+        if (!t.data)
+            return ADKV_E_NULL;
+        if (i == 0)
+            into = t.into != nullptr;
+        if (into != (t.into != nullptr))
+            return ADKV_E_UNSUPPORTED;
+        if (t.segments < 0 || t.used < 0 || t.pitch < t.used || (into && t.into_pitch < t.used) || (!into && rows > batch) || t.pitch > INT32_MAX - BLOCK ||
+            t.into_pitch > INT32_MAX - BLOCK)
+            return ADKV_E_SHAPE;
+        if (((uint64_t)t.data | (uint64_t)t.into | (uint64_t)t.pitch | (uint64_t)(into ? t.into_pitch : 0) | (uint64_t)t.used) & 15)
+            return ADKV_E_ALIGN;
+    }
+    for (int at = 0; at < n && rows > 0;) {
+        Args a = {};
+        a.index = index;
+        a.rows = rows;
+        a.batch = batch;
+        int64_t jobs = 0;
+        for (; at < n && a.n < TENSORS; at++) {
+            const adkv_rows &r = tensors[at];
+            Tensor t = {};
+            t.from = (const char *)r.data;
+            t.to = into ? (char *)r.into : (char *)r.data;
+            t.pitch = (int)r.pitch;
+            t.to_pitch = into ? (int)r.into_pitch : t.pitch;
+            int64_t used = r.used, width = into ? t.to_pitch : used, segments = r.segments;
+            if (used == t.pitch && used == t.to_pitch && segments * used <= INT32_MAX - BLOCK) { // one piece
+                width = used *= segments;
+                t.pitch = t.to_pitch = (int)used;
+                segments = 1;
+            }
+            t.segments = (int)segments;
+            t.used = (int)used;
+            t.width = (int)width;
+            const int64_t blocks = (width + BLOCK - 1) / BLOCK;
+            if (segments * blocks > INT32_MAX - SLOTS)
+                return ADKV_E_SHAPE;
+            const int64_t more = (segments * blocks + SLOTS - 1) / SLOTS;
+            if (more == 0)
+                continue;
+            if (jobs + more > 1 << 26) { // a grid is 2^32 threads at most
+                if (more > 1 << 26)
+                    return ADKV_E_SHAPE;
+                break;
+            }
+            t.first = (int)jobs;
+            a.t[a.n++] = t;
+            jobs += more;
+        }
+        if (a.n == 0)
+            continue;
+        a.jobs = (int)jobs;
+        const auto kernel = into ? take_kernel<true> : take_kernel<false>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((jobs + WAVES - 1) / WAVES)), dim3(WAVES * 64), 0, (hipStream_t)stream, a);
+        if (int rc = check_launch())
+            return rc;
+    }
+    return ADKV_OK;
+}

@@ -13,6 +13,7 @@ by hand-written gfx950 kernels behind ``libadkv_hip.so``.  Differences, all on t
 from __future__ import annotations
 
 import functools
+import math
 from typing import NamedTuple
 
 import torch
@@ -707,6 +708,107 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scaling:
                                      _lib.current_stream_ptr(dev))
     _lib.check(rc, "prompt_attention")
     return out
+
+
+class TokenLogprobs(NamedTuple):
+    """What ``token_logprobs`` returns, shaped as the tokens are; ``top_*`` have one more axis (None without ``top``)."""
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    top_logprobs: torch.Tensor | None = None
+    top_tokens: torch.Tensor | None = None
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) -> TokenLogprobs:
+    """Log probabilities of ``tokens [...]`` under ``softmax(logits [..., V])``, the rows' entropy (nats) and their ``top`` likeliest
+    tokens, in one pass over the logits (what the reference's evaluation, tools/lm_eval_adkv.py, asks its model for).
+
+    Logits: float16, bfloat16 or float32, read in place whatever the strides of up to two leading axes are.  Tokens: whole numbers; a negative one
+    stands for none (its log probability is 0), one from ``V`` on gives NaN.  ``top``: 0 to 32; equal logits come lowest token first.
+    Everything is computed in fp32 or more and returned in fp32 (``top_tokens`` int64), with the digits of probabilities near one kept.  Minus
+    infinity is a probability of zero; a row with a NaN or plus infinity, or of nothing but minus infinity, gives NaN, and its
+    likeliest tokens in order, NaN first.  No gradient: refused where one is wanted.
+    """
+    _chk(logits.dim() >= 1 and tokens.shape == logits.shape[:-1], "tokens must have the shape of logits without its last axis")
+    V = logits.shape[-1]
+    _chk(logits.dtype in _NORM_DT, "logits must be float16, bfloat16 or float32")
+    _chk(not (tokens.is_floating_point() or tokens.is_complex() or tokens.dtype == torch.bool), "tokens must be whole numbers")
+    _chk(V > 0, "logits must have at least one column")
+    _chk(0 <= top <= 32 and top <= V, "top must be 0 to 32, and at most the vocabulary")
+    _no_derivatives("token_logprobs", logits)
+    dev = _need_device(logits, tokens)
+    shape = tokens.shape
+    made = lambda *s, dtype=torch.float32: torch.empty((*shape, *s), dtype=dtype, device=dev)
+    out = TokenLogprobs(made(), made(), *((made(top), made(top, dtype=torch.int64)) if top else ()))
+    if out.logprobs.numel() == 0:
+        return out
+    x = logits if logits.stride(-1) == 1 or V == 1 else logits.contiguous()
+    x = x.reshape(1, -1, V) if x.dim() < 3 else x if x.dim() == 3 else x.reshape(1, -1, V)
+    tokens = tokens.to(torch.int64).contiguous()
+    with _lib.device_guard(dev):
+        rc = _lib.lib().adkv_token_logprobs(
+            x.data_ptr(), x.stride(0) if x.shape[0] > 1 else 0, x.stride(1) if x.shape[1] > 1 else 0, tokens.data_ptr(), x.shape[0], x.shape[1], V,
+            _NORM_DT[x.dtype], top, *[_ptr(t) for t in out], _lib.current_stream_ptr(dev))
+    _lib.check(rc, "token_logprobs")
+    return out
+
+
+def take_sequences(tensors, index: torch.Tensor, *, used=None, into=None) -> None:
+    """Sequences of a cache copied over one another: row ``r`` of every tensor becomes what its row ``index[r]`` was (extension: the reference's
+    cache cannot be reordered).  Beams that go on from another one, finished sequences that leave a batch (the first ``len(index)`` rows are then
+    what is left), one prompt that several answers begin with.
+
+    Args:
+        tensors: any number of contiguous tensors ``[B, H, n, ...]`` of one device, a cache's codes, checkpoints and states, of one layer or of all:
+            one or two launches for all of them.  They begin at multiples of 16 bytes, and a head's entries (``[n, ...]``), those that are used too, are
+            such multiples.
+        index: ``[R]`` whole numbers, ``R <= 2048``; the same one may come several times.  On the device they are not checked (that would wait for it): a
+            row whose index is none of the rows stays as it is, or is zeros in ``into``.  On the host they are checked and copied.
+        used: how many entries along the third axis hold anything, one number per tensor (all): what is behind them is neither read nor written.
+        into: as many tensors ``[R, H, m, ...]``, ``m >= used``, to write instead, which share no memory with ``tensors``; what is behind the entries that are
+            used becomes zero.  Without it ``R <= B``, rows may be one another's sources in any way, and no two tensors may share memory.
+    """
+    tensors = list(tensors)
+    _chk(index.dim() == 1 and not (index.is_floating_point() or index.is_complex() or index.dtype == torch.bool), "index must be [R] whole numbers")
+    R = index.shape[0]
+    _chk(R <= 2048, "at most 2048 sequences")
+    used = [None] * len(tensors) if used is None else list(used)
+    into = None if into is None else list(into)
+    _chk(len(used) == len(tensors), "used must have a number for every tensor")
+    _chk(into is None or len(into) == len(tensors), "into must have a tensor for every tensor")
+    if not tensors:
+        return
+    B = tensors[0].shape[0] if tensors[0].dim() else 0
+    _chk(into is not None or R <= B, "in place there are at most as many sequences as before")
+    rows = []
+    for i, t in enumerate(tensors):
+        _chk(t.dim() >= 3 and t.shape[0] == B and t.is_contiguous(), "tensors must be contiguous [B, H, n, ...]")
+        entry = t.element_size() * math.prod(t.shape[3:])
+        n = t.shape[2] if used[i] is None else int(used[i])
+        _chk(0 <= n <= t.shape[2], "used must be between 0 and the third axis's length")
+        _chk(t.shape[2] * entry % 16 == 0 and n * entry % 16 == 0 and t.data_ptr() % 16 == 0, "heads and what is used of them must be multiples of 16 bytes")
+        _no_derivatives("take_sequences", t)
+        if into is None:
+            if t.numel():
+                rows.append(_lib.Rows(t.data_ptr(), None, t.shape[1], t.shape[2] * entry, 0, n * entry))
+        else:
+            to = into[i]
+            _chk(to.dtype == t.dtype and to.dim() == t.dim() and to.shape[0] == R and to.shape[1] == t.shape[1] and to.shape[2] >= n
+                 and to.shape[3:] == t.shape[3:] and to.is_contiguous() and to.data_ptr() % 16 == 0 and to.shape[2] * entry % 16 == 0,
+                 "into must be contiguous [R, H, m, ...] of the tensors' types, with room for what is used")
+            _chk(to.numel() == 0 or t.numel() == 0 or to.data_ptr() + to.numel() * to.element_size() <= t.data_ptr()
+                 or t.data_ptr() + t.numel() * t.element_size() <= to.data_ptr(), "into must not share memory with the tensors")
+            _no_derivatives("take_sequences", to)
+            if to.numel():       # nothing is read where nothing is used
+                rows.append(_lib.Rows((t if t.numel() else to).data_ptr(), to.data_ptr(), t.shape[1], t.shape[2] * entry, to.shape[2] * entry, n * entry))
+    if not index.is_cuda:
+        _chk(all(0 <= r < B for r in index.tolist()), "index must be of the sequences")
+    dev = _need_device(*tensors, *(into or ()))
+    if R == 0 or B == 0 or not rows:
+        return
+    index = index.to(device=dev, dtype=torch.int64).contiguous()
+    with _lib.device_guard(dev):
+        rc = _lib.lib().adkv_take_sequences((_lib.Rows * len(rows))(*rows), len(rows), index.data_ptr(), R, B, _lib.current_stream_ptr(dev))
+    _lib.check(rc, "take_sequences")
 
 
 def softmax_scale_mask(logits: torch.Tensor, scaling: float,

@@ -519,6 +519,36 @@ int adkv_prompt_attention(const void *q, const int64_t *q_strides, const void *k
                           int n_seq, void *out, int B, int Hq, int H, int Tq, int Tk, int D, int dtype, void *workspace,
                           int64_t workspace_bytes, void *stream);
 
+/*
+ * Sequences of a cache copied over one another, any number of tensors in a call: row r < rows of each becomes what its row index[r] was (device,
+ * int64; 0 <= index[r] < batch; a row with another one is left as it is, or zeros in `into`).  The reference has no counterpart: its cache cannot
+ * be reordered.
+ *   data      [batch, segments, pitch bytes], packed: a cache's codes or checkpoints with a segment per head
+ *   into      NULL: in place, whatever the map (a row may be several rows' source), rows <= batch.  Else [rows, segments, into_pitch bytes], packed,
+ *             for every tensor of the call, which do not overlap data
+ *   used      bytes of a segment that are copied, the same in all rows; what is behind them is left as it is in place, zeros in `into`
+ * Pointers and sizes are multiples of 16 bytes; at most 2048 rows.  The array is host memory and may be reused after the call.
+ */
+typedef struct {
+    void *data, *into;
+    int64_t segments, pitch, into_pitch, used;
+} adkv_rows;
+int adkv_take_sequences(const adkv_rows *tensors, int n, const int64_t *index, int rows, int batch, void *stream);
+
+/*
+ * Log probabilities of given tokens from rows of logits (what the reference's evaluation asks its model for, tools/lm_eval_adkv.py), the rows'
+ * entropy and their likeliest tokens, in one pass over the logits:
+ *   logprobs[r] = log softmax(x_r)[tokens[r]], entropy[r] = -sum_i p_i log p_i (nats), top_tokens[r, j] the j-th largest logit's index (the lowest of
+ *   equal ones first), top_logprobs[r, j] its log probability.
+ *   logits [n0, n1, V] of dtype (ADKV_DT_F32, F16, BF16), element strides stride0, stride1, V contiguous, aligned as its elements; tokens int64
+ *   [n0 * n1], packed: a negative one stands for none (0 is returned), one from V on gives NaN; outputs fp32 (top_tokens int64), packed; top 0..32, at
+ *   most V, top_* unused if 0.
+ * Minus infinity is a probability of zero; beside others, logits beyond +-1.7e38 weigh as that.  A row with a NaN or plus infinity, or of nothing but minus infinity, gives NaN; its likeliest tokens are in
+ * order all the same, NaN first.
+ */
+int adkv_token_logprobs(const void *logits, int64_t stride0, int64_t stride1, const int64_t *tokens, int n0, int n1, int V, int dtype,
+                        int top, float *logprobs, float *entropy, float *top_logprobs, int64_t *top_tokens, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
