@@ -15,7 +15,9 @@ reference's cache object works unchanged.  What differs is underneath:
 * the filter state after the last prompt token is carried, so a prompt may be prefilled in chunks
   (the reference refuses: llama_adkv.py:195-197);
 * several new tokens may be attended with at once (``extend``), and a batch may go on from one prefilled sequence whose codes it
-  shares (``share``); the reference has neither.
+  shares (``share``); the reference has neither;
+* sequences may take each other's place, leave the batch or multiply (``reorder_cache``, ``batch_select_indices``,
+  ``batch_repeat_interleave``, what ``generate`` asks of a cache), all layers in a launch or two.
 """
 from __future__ import annotations
 
@@ -24,7 +26,7 @@ import math
 import torch
 
 from .. import _lib
-from ..kernel.gemv import SharedPrefix, append_kv_pair, decode_step, decode_step_workspace_bytes, extend
+from ..kernel.gemv import SharedPrefix, append_kv_pair, decode_step, decode_step_workspace_bytes, extend, take_sequences
 
 SCALE_MIN = math.exp(-4.0)  # kept for API parity; the fp16 recurrence never clamps
 SCALE_MAX = math.exp(4.0)
@@ -417,6 +419,32 @@ class KVCacheLayer_ADKV:
         self._state_valid = False
         return out if out.dtype == query_states.dtype else out.to(query_states.dtype)
 
+    # ------------------------------------------------------------------ sequences that take each other's place
+    def _tensors(self):
+        """The layer's tensors with a row per sequence, and how many entries of each head hold anything."""
+        T, S = self._quant_len, self._ckpt_interval
+        found = [(t, self._n_super(T)) for t in (self._key_buf, self._value_buf)]
+        if self._key_ckpt is not None:
+            found += [(t, T // S) for t in (self._key_ckpt, self._value_ckpt)]
+        return found + [(t, self._C) for t in (self._key_state, self._value_state)]
+
+    def _now_hold(self, tensors, rows: int, where) -> None:
+        """The layer's tensors and its sequences' bookkeeping; ``where``: each one's row before, or None where the host does not know it."""
+        self._key_buf, self._value_buf, *rest = tensors
+        if self._key_ckpt is not None:
+            self._key_ckpt, self._value_ckpt, *rest = rest
+        self._key_state, self._value_state = rest
+        old = self._valid[self._span]
+        if where is not None:
+            new = bytes(old[r] for r in where)
+        else:
+            new = bytes(rows) if 0 in old else b"\1" * rows       # of some it is not: of none then
+        if self._shares_storage:
+            self._valid[self._span] = new
+        else:
+            self._valid, self._span = bytearray(new), slice(0, rows)
+        self._B = rows
+
     # ------------------------------------------------------------------ save / restore
     def state_dict(self) -> dict:
         """Everything needed to continue decoding elsewhere: the used part of the code buffers, the
@@ -523,6 +551,60 @@ class KVCache_ADKV(list):
         shared = KVCache_ADKV(0)
         shared.extend(layer.share(B, tokens) for layer in self)
         return shared
+
+    # ------------------------------------------------------------------ sequences that take each other's place
+    def _take(self, index: torch.Tensor, rows: int, fresh: bool) -> None:
+        layers = [layer for layer in self if layer._key_buf is not None]
+        if not layers:
+            return
+        B, dev = layers[0]._B, layers[0]._device
+        if any(layer._B != B for layer in layers):
+            raise ValueError("the layers hold different numbers of sequences")
+        if any(layer._shares_storage for layer in layers) and (fresh or rows != B):
+            raise ValueError("a batch view has as many sequences as it was made with")
+        where = None
+        if not index.is_cuda:
+            where = index.tolist()
+            if any(not 0 <= r < B for r in where):
+                raise IndexError(f"a cache of {B} sequences has no others")
+        held = [layer._tensors() for layer in layers]
+        flat = [t for layer in held for t, _ in layer]
+        used = [n for layer in held for _, n in layer]
+        into = [torch.empty((rows, *t.shape[1:]), dtype=t.dtype, device=t.device) for t in flat] if fresh else None
+        take_sequences(flat, index.to(dev), used=used, into=into)
+        flat = into if fresh else [t[:rows] for t in flat]
+        for layer, tensors in zip(layers, held):
+            layer._now_hold(flat[:len(tensors)], rows, where)
+            flat = flat[len(tensors):]
+
+    def reorder_cache(self, beam_idx: torch.Tensor) -> None:
+        """Sequence ``i`` goes on from what sequence ``beam_idx[i]`` holds (beam search), in place.  An index on the device is not looked at by the host: if
+        only some of the sequences can be prefilled further, afterwards none can."""
+        B = max((layer._B for layer in self if layer._key_buf is not None), default=0)
+        if beam_idx.dim() != 1 or (B and beam_idx.shape[0] != B):
+            raise ValueError("reorder_cache needs an index for every sequence")
+        self._take(beam_idx, B, False)
+
+    def batch_select_indices(self, indices: torch.Tensor) -> None:
+        """The sequences ``indices``, in that order, are the batch from now on: in place where there are not more of them than before (the memory of the
+        others is the cache's still), else in new memory."""
+        B = max((layer._B for layer in self if layer._key_buf is not None), default=0)
+        if indices.dtype == torch.bool:
+            if indices.shape != (B,) and B:
+                raise ValueError("a mask of sequences needs an entry for each")
+            indices = indices.nonzero().flatten()
+        if indices.dim() != 1 or indices.shape[0] == 0:
+            raise ValueError("batch_select_indices needs one sequence at least")
+        self._take(indices, indices.shape[0], indices.shape[0] > B)
+
+    def batch_repeat_interleave(self, repeats: int) -> None:
+        """Every sequence ``repeats`` times, one after the other, in new memory: several answers to each prompt that go different ways (``share`` keeps one
+        prompt once where all of them begin with it)."""
+        if repeats < 1:
+            raise ValueError("batch_repeat_interleave needs one of each at least")
+        B = max((layer._B for layer in self if layer._key_buf is not None), default=0)
+        if repeats > 1:
+            self._take(torch.arange(B).repeat_interleave(repeats), B * repeats, True)
 
     def get_mask_sizes(self, cache_position, layer_idx: int) -> tuple[int, int]:
         return self[layer_idx].get_mask_sizes(cache_position)

@@ -24,9 +24,10 @@ from transformers.models.llama.modeling_llama import (
 )
 from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
 
-from ..kernel.gemv import rope_norm_qk, rope_qk
+from ..kernel.gemv import prompt_attention, rope_norm_qk, rope_qk
 from .cache import (CAP_LEN, INIT_SEQ_LEN, SCALE_MAX, SCALE_MIN, KVCache_ADKV,  # noqa: F401
                     KVCacheLayer_ADKV)
+from .score import Scores
 
 # the five per-(head, channel) quantities, for K and for V (reference llama_adkv.py:27)
 ADKV_PARAM_FIELDS = ("zp_init", "scale_init", "alpha", "beta", "quant_target")
@@ -57,6 +58,28 @@ def norm_and_rotate(attn, q, k, cos, sin):
         # one launch for both norms and the rotation, and one for their gradients
         return rope_norm_qk(q, k, cos, sin, wq, wk, attn.q_norm.variance_epsilon)
     return apply_rotary_pos_emb(attn.q_norm(q), attn.k_norm(k), cos, sin)
+
+
+def prompt_ctx(attn, q, k, v, attention_mask, cached: bool, kwargs) -> torch.Tensor | None:
+    """config.adkv_prompt: the dense rows' attention ``[B, T, Hq, C]`` by the framework's own kernel, without weights; None where transformers' is to
+    run (without the flag, on the host, for other types and head sizes, where a gradient, dropout or the weights are wanted).  With
+    ``cu_seq_lens_q`` (transformers' name for the bounds of sequences packed into one row axis) each sequence looks at itself only."""
+    if not getattr(attn.config, "adkv_prompt", False):
+        return None
+    bounds = kwargs.get("cu_seq_lens_q")
+    if bounds is not None and cached:
+        raise ValueError("packed sequences have no cache: pass use_cache=False")
+    if not (q.is_cuda and q.dtype in (torch.float16, torch.bfloat16) and k.dtype == v.dtype == q.dtype and q.shape[-1] % 8 == 0 and q.shape[-1] <= 256) \
+            or (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v))) or (attn.training and attn.attention_dropout > 0) \
+            or kwargs.get("output_attentions") or getattr(attn.config, "output_attentions", False):
+        return None
+    if bounds is not None:
+        return prompt_attention(q, k, v, attn.scaling, bounds=bounds)
+    if attention_mask is not None:
+        if attention_mask.dim() != 4 or attention_mask.shape[-1] < k.shape[2]:
+            return None
+        attention_mask = attention_mask[..., :k.shape[2]]
+    return prompt_attention(q, k, v, attn.scaling, attention_mask)
 
 
 class LlamaAttention_ADKV(LlamaAttention):
@@ -149,8 +172,11 @@ class LlamaAttention_ADKV(LlamaAttention):
             ctx = torch.stack(steps, dim=1)                      # [B, Tq, Hq, C]
             return self.o_proj(ctx.reshape(*lead, -1)), None
 
+        ctx = prompt_ctx(self, q, k, v, attention_mask, layer_cache is not None, kwargs)
         if layer_cache is not None:
             layer_cache.prefill(k, v, *self._adkv_params("key"), *self._adkv_params("value"))
+        if ctx is not None:
+            return self.o_proj(ctx.reshape(*lead, -1)), None
 
         attend = eager_attention_forward
         if self.config._attn_implementation != "eager":
@@ -191,7 +217,7 @@ class LlamaModel_ADKV(LlamaModel):
                                use_cache=use_cache, **kwargs)
 
 
-class LlamaForCausalLM_ADKV(LlamaForCausalLM):
+class LlamaForCausalLM_ADKV(Scores, LlamaForCausalLM):
     _no_split_modules = ["LlamaDecoderLayer_ADKV"]
 
     def __init__(self, config):

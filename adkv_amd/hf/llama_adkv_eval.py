@@ -25,8 +25,10 @@ from transformers.models.llama.modeling_llama import (
 )
 from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
 
+from ..kernel.gemv import take_sequences
 from ..train.train_model import quant_f32_pair
-from .llama_adkv import ADKV_PARAM_FIELDS, ADKVConfig, make_head_norms, norm_and_rotate  # noqa: F401
+from .llama_adkv import ADKV_PARAM_FIELDS, ADKVConfig, make_head_norms, norm_and_rotate, prompt_ctx  # noqa: F401
+from .score import Scores
 
 SCALE_MIN = math.exp(-4.0)
 SCALE_MAX = math.exp(4.0)
@@ -177,6 +179,19 @@ class KVCache_ADKV(list):
     def get_max_length(self) -> int:
         return -1
 
+    def reorder_cache(self, beam_idx: torch.Tensor) -> None:
+        """Sequence ``i`` goes on from what sequence ``beam_idx[i]`` holds (beam search), in place, all layers in a launch or two."""
+        layers = [layer for layer in self if layer._key_buf is not None]
+        if beam_idx.dim() != 1 or any(beam_idx.shape[0] != layer._key_buf.shape[0] for layer in layers):
+            raise ValueError("reorder_cache needs an index for every sequence")
+        tensors, used = [], []
+        for layer in layers:
+            tensors += [t[:, None] for t in (layer._key_buf, layer._value_buf)]
+            tensors += [t[:, None, None] for t in (layer.key_dc, layer.key_scale, layer.value_dc, layer.value_scale)]
+            used += [layer._recent_len] * 2 + [1] * 4
+        if tensors:
+            take_sequences(tensors, beam_idx.to(tensors[0].device), used=used)
+
     is_sliding = [False]
     is_compileable = False
 
@@ -244,6 +259,9 @@ class LlamaAttention_ADKV(LlamaAttention):
                 n = layer.get_seq_length()
                 k, v = heads(layer.key_states, n), heads(layer.value_states, n)
 
+        out = prompt_ctx(self, q, k, v, attention_mask, past_key_values is not None, kwargs)
+        if out is not None:
+            return self.o_proj(out.reshape(*lead, -1)), None
         attend = eager_attention_forward
         if self.config._attn_implementation != "eager":
             attend = ALL_ATTENTION_FUNCTIONS[self.config._attn_implementation]
@@ -281,8 +299,9 @@ class LlamaModel_ADKV(LlamaModel):
                                use_cache=use_cache, **kwargs)
 
 
-class LlamaForCausalLM_ADKV(LlamaForCausalLM):
+class LlamaForCausalLM_ADKV(Scores, LlamaForCausalLM):
     _no_split_modules = ["LlamaDecoderLayer_ADKV"]
+    scores_with_cache = True
 
     def __init__(self, config):
         super().__init__(config)

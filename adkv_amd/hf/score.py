@@ -1,0 +1,46 @@
+"""Log probabilities of texts under a model (what the reference's evaluation asks for, tools/lm_eval_adkv.py), for both of its Llama flavours."""
+from __future__ import annotations
+
+import torch
+
+from ..kernel.gemv import TokenLogprobs, token_logprobs
+
+
+class Scores:
+    """``score`` for a causal language model with ``model``, ``lm_head`` and ``config``."""
+
+    @torch.no_grad()
+    def score(self, sequences, *, top: int = 0, rows: int = 4096) -> list[TokenLogprobs]:
+        """Of every sequence (token ids ``[n]``, ``n >= 1``, of any lengths) the log probability of each of its tokens but the first, given those in
+        front of it: ``n - 1`` of them, with the distributions' entropy and their ``top`` likeliest tokens.  ``rows`` of logits are made at a time.
+
+        The evaluation flavour scores with its fake-quantised cache, in one batch padded behind the texts, where nothing looks at it.  The deployment
+        flavour's prompts are attended with as they are; with ``config.adkv_prompt`` they are packed into one row axis without padding."""
+        dev = self.lm_head.weight.device
+        ids = [torch.as_tensor(s, dtype=torch.int64, device=dev).reshape(-1) for s in sequences]
+        if not ids:
+            return []
+        lengths = [s.shape[0] for s in ids]
+        if min(lengths) < 1:
+            raise ValueError("a sequence needs one token at least")
+        quantised = getattr(self, "scores_with_cache", False)
+        if getattr(self.config, "adkv_prompt", False) and not quantised and dev.type == "cuda":
+            ends = torch.tensor([0, *lengths], device="cpu").cumsum(0)
+            at = torch.cat([torch.arange(n) for n in lengths]).to(dev)[None]
+            total = int(ends[-1])
+            # a mask of four axes is the attention's own affair: here it says nothing
+            hidden = self.model(input_ids=torch.cat(ids)[None], position_ids=at, attention_mask=torch.ones(1, 1, 1, total, dtype=torch.bool, device=dev),
+                                cu_seq_lens_q=ends.to(dev, torch.int32), use_cache=False).last_hidden_state[0]
+            keep = torch.ones(total, dtype=torch.bool)
+            keep[ends[1:] - 1] = False
+            hidden = hidden[keep.to(dev)]
+        else:
+            batch = torch.nn.utils.rnn.pad_sequence(ids, batch_first=True)
+            extra = {"prefill_full_precision": getattr(self.config, "prefill_full_precision", True)} if quantised else {}
+            hidden = self.model(input_ids=batch, use_cache=quantised, **extra).last_hidden_state
+            hidden = torch.cat([h[:n - 1] for h, n in zip(hidden, lengths)])
+        given = torch.cat([s[1:] for s in ids])
+        parts = [token_logprobs(self.lm_head(h), t, top=top) for h, t in zip(hidden.split(rows), given.split(rows))]
+        whole = [None if p[0] is None else torch.cat(p) for p in zip(*parts)]
+        each = zip(*([None] * len(ids) if w is None else w.split([n - 1 for n in lengths]) for w in whole))
+        return [TokenLogprobs(*e) for e in each]
