@@ -1,4 +1,4 @@
-// The library calls of an attention layer, and of the fp32 quantiser, from Python without Python: rotary embedding,
+// The library calls of an attention layer, of the operators around a prompt and of the fp32 quantiser, from Python without Python: rotary embedding,
 // attention of one token, quantising of new tokens.  On few sequences a step is over on the device in 10 to 20 us,
 // and the checks, views, allocations and argument conversions of the Python functions took twice that on the host
 // (1 x 32 heads x 603 tokens with its rotary embedding: 38.2 us per step in Python, now 13.1, as long as the device is busy with it).
@@ -693,6 +693,188 @@ PyObject *quant_f32_pair(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     return PyLong_FromLong(rc);
 }
 
+// Nobody wants a derivative of it.
+bool constant(const at::Tensor &t) { return !(t.requires_grad() && c10::GradMode::is_enabled()) && !t._fw_grad(0).defined(); }
+
+// prompt_attention(q, k, v, scaling, mask or None, bounds or None)
+PyObject *prompt_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    if (nargs != 6 || !unwatched() || !PyFloat_CheckExact(args[3]))
+        Py_RETURN_NONE;
+    const at::Tensor *t[3];
+    int64_t strides[3][3];
+    for (int i = 0; i < 3; i++) {
+        if (!(t[i] = plain(args[i])) || t[i]->device() != t[0]->device() || t[i]->scalar_type() != t[0]->scalar_type() || t[i]->dim() != 4 || !constant(*t[i]) ||
+            t[i]->stride(3) != 1 || (uintptr_t)t[i]->const_data_ptr() % 16)
+            Py_RETURN_NONE;
+        for (int j = 0; j < 3; j++) {
+            strides[i][j] = t[i]->size(j) > 1 ? t[i]->stride(j) : 0;
+            if (strides[i][j] % 8 || (j == 2 && strides[i][j] >= 1 << 23))
+                Py_RETURN_NONE;
+        }
+    }
+    const at::Tensor &q = *t[0], &k = *t[1];
+    const int64_t B = q.size(0), Hq = q.size(1), Tq = q.size(2), D = q.size(3), H = k.size(1), Tk = k.size(2);
+    if (!half_type(q) || k.sizes() != t[2]->sizes() || k.size(0) != B || k.size(3) != D || B <= 0 || Tq <= 0 || Tk < Tq || H <= 0 || Hq <= 0 || Hq % H || D <= 0 || D > 256 ||
+        D % 8 || B > INT32_MAX || Hq > INT32_MAX || Tk > INT32_MAX)
+        Py_RETURN_NONE;
+    const void *mask = nullptr;
+    const int *bounds = nullptr;
+    int64_t ms[3] = {}, n_seq = 0;
+    int mask_type = 0;
+    if (args[4] != Py_None) {
+        const at::Tensor *m = plain(args[4]);
+        if (!m || m->device() != q.device() || !constant(*m) || m->dim() != 4 || m->size(3) != Tk || (m->size(0) != 1 && m->size(0) != B) || (m->size(1) != 1 && m->size(1) != Hq) ||
+            (m->size(2) != 1 && m->size(2) != Tq) || (m->stride(3) != 1 && Tk > 1) || (!half_type(*m) && m->scalar_type() != at::kFloat && m->scalar_type() != at::kBool))
+            Py_RETURN_NONE;
+        for (int j = 0; j < 3; j++)
+            ms[j] = m->size(j) > 1 ? m->stride(j) : 0;
+        mask_type = m->scalar_type() == at::kFloat ? ADKV_DT_F32 : m->scalar_type() == at::kHalf ? ADKV_DT_F16 : m->scalar_type() == at::kBool ? ADKV_DT_BOOL : ADKV_DT_BF16;
+        mask = m->const_data_ptr();
+    }
+    if (args[5] != Py_None) {
+        const at::Tensor *b = plain(args[5]);
+        if (!b || b->device() != q.device() || b->scalar_type() != at::kInt || b->dim() != 1 || !b->is_contiguous() || b->size(0) < 2 || b->size(0) > INT32_MAX || mask || B != 1 || Tq != Tk)
+            Py_RETURN_NONE;
+        n_seq = b->size(0) - 1;
+        bounds = (const int *)b->const_data_ptr();
+    }
+    void *stream;
+    if (!current(q.device(), stream))
+        Py_RETURN_NONE;
+    const int64_t bytes = adkv_prompt_attention_workspace_bytes((int)B, (int)Hq, (int)H, (int)Tq, (int)Tk, (int)D, (int)n_seq);
+    if (bytes < 0)
+        Py_RETURN_NONE;
+    at::Tensor out = fresh({B, Tq, Hq, D}, q, q.scalar_type()), work;
+    if (bytes)
+        work = fresh({bytes}, q, at::kByte);
+    if (!out.has_storage() || (bytes && !work.has_storage()))
+        Py_RETURN_NONE;
+    void *op = out.mutable_data_ptr(), *wp = bytes ? work.mutable_data_ptr() : nullptr;
+    const void *in[3] = {q.const_data_ptr(), k.const_data_ptr(), t[2]->const_data_ptr()};
+    const float scaling = (float)PyFloat_AS_DOUBLE(args[3]);
+    const int type = (q.scalar_type() == at::kHalf ? ADKV_DT_F16 : ADKV_DT_BF16) | mask_type << 8;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = adkv_prompt_attention(in[0], strides[0], in[1], strides[1], in[2], strides[2], mask, ms, scaling, bounds, (int)n_seq, op, (int)B, (int)Hq, (int)H, (int)Tq, (int)Tk, (int)D,
+                               type, wp, bytes, stream);
+    Py_END_ALLOW_THREADS
+    return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(std::move(out));
+}
+
+// token_logprobs(logits, tokens, top) -> (log probabilities, entropy[, of the likeliest, the likeliest])
+PyObject *token_logprobs(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    if (nargs != 3 || !unwatched())
+        Py_RETURN_NONE;
+    const at::Tensor *x = plain(args[0]), *tokens = plain(args[1]);
+    const long top = PyLong_AsLong(args[2]);
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    if (!x || !tokens || x->device() != tokens->device() || !constant(*x) || (!half_type(*x) && x->scalar_type() != at::kFloat) || x->dim() < 1 || x->dim() > 3 ||
+        tokens->dim() != x->dim() - 1 || tokens->scalar_type() != at::kLong || !tokens->is_contiguous())
+        Py_RETURN_NONE;
+    const int d = (int)x->dim();
+    const int64_t V = x->size(d - 1), n0 = d == 3 ? x->size(0) : 1, n1 = d >= 2 ? x->size(d - 2) : 1;
+    for (int i = 0; i < d - 1; i++)
+        if (tokens->size(i) != x->size(i))
+            Py_RETURN_NONE;
+    if (V <= 0 || V > INT32_MAX || n0 <= 0 || n1 <= 0 || n0 > INT32_MAX || n1 > INT32_MAX || top < 0 || top > 32 || top > V || x->stride(d - 1) != 1)
+        Py_RETURN_NONE;
+    void *stream;
+    if (!current(x->device(), stream))
+        Py_RETURN_NONE;
+    std::vector<int64_t> shape(tokens->sizes().begin(), tokens->sizes().end());
+    at::Tensor out[4];
+    for (int i = 0; i < (top ? 4 : 2); i++) {
+        if (i == 2)
+            shape.push_back(top);
+        out[i] = fresh(shape, *x, i == 3 ? at::kLong : at::kFloat);
+        if (!out[i].has_storage())
+            Py_RETURN_NONE;
+    }
+    void *op[4] = {};
+    for (int i = 0; i < (top ? 4 : 2); i++)
+        op[i] = out[i].mutable_data_ptr();
+    const void *xp = x->const_data_ptr();
+    const int64_t *tp = (const int64_t *)tokens->const_data_ptr(), s0 = n0 > 1 ? x->stride(0) : 0, s1 = n1 > 1 ? x->stride(d - 2) : 0;
+    const int type = x->scalar_type() == at::kFloat ? ADKV_DT_F32 : x->scalar_type() == at::kHalf ? ADKV_DT_F16 : ADKV_DT_BF16;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = adkv_token_logprobs(xp, s0, s1, tp, (int)n0, (int)n1, (int)V, type, (int)top, (float *)op[0], (float *)op[1], (float *)op[2], (int64_t *)op[3], stream);
+    Py_END_ALLOW_THREADS
+    if (rc)
+        return PyLong_FromLong(rc);
+    PyObject *r = PyTuple_New(top ? 4 : 2);
+    for (int i = 0; r && i < (top ? 4 : 2); i++) {
+        PyObject *o = THPVariable_Wrap(std::move(out[i]));
+        if (!o) {
+            Py_CLEAR(r);
+            break;
+        }
+        PyTuple_SET_ITEM(r, i, o);
+    }
+    return r;
+}
+
+// take_sequences(list of tensors, index, list of numbers or None, list of tensors or None) -> return code
+PyObject *take_sequences(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    if (nargs != 4 || !unwatched() || !PyList_CheckExact(args[0]) || (args[2] != Py_None && !PyList_CheckExact(args[2])) || (args[3] != Py_None && !PyList_CheckExact(args[3])))
+        Py_RETURN_NONE;
+    const Py_ssize_t n = PyList_GET_SIZE(args[0]);
+    const bool some = args[2] != Py_None, into = args[3] != Py_None;
+    const at::Tensor *index = plain(args[1]);
+    if (n == 0 || !index || index->scalar_type() != at::kLong || index->dim() != 1 || !index->is_contiguous() || index->size(0) <= 0 || index->size(0) > 2048 ||
+        (some && PyList_GET_SIZE(args[2]) != n) || (into && PyList_GET_SIZE(args[3]) != n))
+        Py_RETURN_NONE;
+    const int64_t R = index->size(0);
+    int64_t B = 0;
+    std::vector<adkv_rows> rows;
+    rows.reserve(n);
+    for (Py_ssize_t i = 0; i < n; i++) {
+        const at::Tensor *t = plain(PyList_GET_ITEM(args[0], i)), *to = into ? plain(PyList_GET_ITEM(args[3], i)) : nullptr;
+        if (!t || (into && !to) || t->dim() < 3 || t->numel() == 0 || !t->is_contiguous() || t->device() != index->device() || !constant(*t))
+            Py_RETURN_NONE;
+        if (i == 0)
+            B = t->size(0);
+        const int64_t most = t->size(2), entry = t->numel() / (t->size(0) * t->size(1) * most) * (int64_t)t->element_size();
+        int64_t used = most;
+        if (some) {
+            used = PyLong_AsLong(PyList_GET_ITEM(args[2], i));
+            if (PyErr_Occurred()) {
+                PyErr_Clear();
+                Py_RETURN_NONE;
+            }
+        }
+        adkv_rows r = {t->mutable_data_ptr(), nullptr, t->size(1), most * entry, 0, used * entry};
+        if (t->size(0) != B || used < 0 || used > most || r.pitch % 16 || r.used % 16 || (uintptr_t)r.data % 16)
+            Py_RETURN_NONE;
+        if (into) {
+            if (to->dim() != t->dim() || to->numel() == 0 || !to->is_contiguous() || to->device() != t->device() || to->scalar_type() != t->scalar_type() || to->size(0) != R ||
+                to->size(1) != t->size(1) || to->size(2) < used || to->sizes().slice(3) != t->sizes().slice(3) || !constant(*to))
+                Py_RETURN_NONE;
+            r.into = to->mutable_data_ptr();
+            r.into_pitch = to->size(2) * entry;
+            const char *a = (const char *)r.data, *b = (const char *)r.into;
+            if (r.into_pitch % 16 || (uintptr_t)b % 16 || !(b + to->nbytes() <= a || a + t->nbytes() <= b))
+                Py_RETURN_NONE;
+        }
+        rows.push_back(r);
+    }
+    void *stream;
+    if ((!into && R > B) || B > INT32_MAX || !current(index->device(), stream))
+        Py_RETURN_NONE;
+    const int64_t *ip = (const int64_t *)index->const_data_ptr();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = adkv_take_sequences(rows.data(), (int)n, ip, (int)R, (int)B, stream);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+
 // No C++ exception reaches Python's frames.
 template <PyObject *(*CALL)(PyObject *, PyObject *const *, Py_ssize_t)>
 PyObject *guarded(PyObject *self, PyObject *const *args, Py_ssize_t n)
@@ -722,6 +904,9 @@ PyMethodDef methods[] = {
     {"extend", (PyCFunction)(void (*)(void))guarded<extend>, METH_FASTCALL, nullptr},
     {"rope_norm_qk", (PyCFunction)(void (*)(void))guarded<rope_norm_qk>, METH_FASTCALL, nullptr},
     {"append", (PyCFunction)(void (*)(void))guarded<append>, METH_FASTCALL, nullptr},
+    {"prompt_attention", (PyCFunction)(void (*)(void))guarded<prompt_attention>, METH_FASTCALL, nullptr},
+    {"token_logprobs", (PyCFunction)(void (*)(void))guarded<token_logprobs>, METH_FASTCALL, nullptr},
+    {"take_sequences", (PyCFunction)(void (*)(void))guarded<take_sequences>, METH_FASTCALL, nullptr},
     {"quant_f32", (PyCFunction)(void (*)(void))guarded<quant_f32>, METH_FASTCALL, nullptr},
     {"quant_f32_pair", (PyCFunction)(void (*)(void))guarded<quant_f32_pair>, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -658,6 +658,11 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scaling:
 
     No gradient: refused where one is wanted.  Weights are rounded to the tensors' type; scores, sums and outputs are fp32.
     """
+    r = _lib.host().prompt_attention(q, k, v, scaling, mask, bounds)      # None: something to check, convert or complain about below
+    if r is not None:
+        if isinstance(r, int):
+            _lib.check(r, "prompt_attention")
+        return r
     _chk(q.dim() == 4 and k.dim() == 4 and v.dim() == 4, "q must be [B, Hq, Tq, D], k and v [B, H, Tk, D]")
     B, Hq, Tq, D = q.shape
     H, Tk = k.shape[1], k.shape[2]
@@ -728,6 +733,11 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
     infinity is a probability of zero; a row with a NaN or plus infinity, or of nothing but minus infinity, gives NaN, and its
     likeliest tokens in order, NaN first.  No gradient: refused where one is wanted.
     """
+    r = _lib.host().token_logprobs(logits, tokens, top)      # None: something to check, convert or complain about below
+    if r is not None:
+        if isinstance(r, int):
+            _lib.check(r, "token_logprobs")
+        return TokenLogprobs(*r)
     _chk(logits.dim() >= 1 and tokens.shape == logits.shape[:-1], "tokens must have the shape of logits without its last axis")
     V = logits.shape[-1]
     _chk(logits.dtype in _NORM_DT, "logits must be float16, bfloat16 or float32")
@@ -768,11 +778,16 @@ def take_sequences(tensors, index: torch.Tensor, *, used=None, into=None) -> Non
             used becomes zero.  Without it ``R <= B``, rows may be one another's sources in any way, and no two tensors may share memory.
     """
     tensors = list(tensors)
+    used = None if used is None else list(used)
+    into = None if into is None else list(into)
+    rc = _lib.host().take_sequences(tensors, index, used, into)      # None: something to check, convert or complain about below
+    if rc is not None:
+        _lib.check(rc, "take_sequences")
+        return
     _chk(index.dim() == 1 and not (index.is_floating_point() or index.is_complex() or index.dtype == torch.bool), "index must be [R] whole numbers")
     R = index.shape[0]
     _chk(R <= 2048, "at most 2048 sequences")
-    used = [None] * len(tensors) if used is None else list(used)
-    into = None if into is None else list(into)
+    used = [None] * len(tensors) if used is None else used
     _chk(len(used) == len(tensors), "used must have a number for every tensor")
     _chk(into is None or len(into) == len(tensors), "into must have a tensor for every tensor")
     if not tensors:
