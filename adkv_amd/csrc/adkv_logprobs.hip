@@ -4,18 +4,20 @@
 //   log p_token = d_token - log(1 + S),   entropy = log(1 + S) - T / (1 + S)
 // The largest is left out of the sums, so that log(1 + S) keeps its digits where one token is nearly certain, and T is a sum of numbers of one sign.
 // A lane holds back the largest it has seen, adds the smaller of it and the next one, and sums relative to a reference r of its own, the largest of its
-// first logits (replaced where a logit is more than FAR larger); the difference is taken before anything else, so that logits of any size keep theirs.
-// Logits beyond +-MOST count as that beside others.  The last steps, once a row, are in 64 bits.  NaN and infinities are looked for beside it: v_max drops a NaN.
+// first logits (replaced where a logit is more than 2^FAR larger), all in powers of two: x log2(e) - r is one multiply-add, and r log2(e) - M log2(e) another
+// at the end, so that neither r nor log2(e) need be exact.  Logits below FLOOR, minus infinity among them, weigh nothing; rows whose largest is beyond
+// +-FLOOR are gone through again.  NaN is looked for beside it: v_med3 and v_max drop it.
 //
 // The likeliest: a key is the logit's bits in the order of numbers with the index, backwards, behind them, so that all keys differ and equal logits
 // come lowest index first.  The lanes' maxima of the first step, 64 groups of them, give a bound that at least `top` keys reach; what reaches it goes to a
-// list in the LDS, some 1.2 to 1.7 times `top` per step, and a list of more than REFINE keys raises the bound the same way.  At the end each key of
-// the list counts the larger ones.  Rows whose keys overrun the list (ascending logits) or that have a NaN are searched a key at a time instead.
+// list in the LDS, some 1.2 to 1.7 times `top` per step, and after one, two, four.. steps a list of more than REFINE keys raises the bound the same way.  At
+// the end each key of the list counts the larger ones.  Rows whose keys overrun the list (ascending logits) or that have a NaN are searched a key at a time instead.
 //
 // A workgroup per row.  Bound by memory where rows are many; see the launcher for the size of the workgroups.
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "adkv_device.h"
 
@@ -28,16 +30,15 @@ using adkv::check_launch;
 using adkv::cu_count;
 
 typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+typedef uint32_t u2v __attribute__((ext_vector_type(2)));
 #define GLOBAL __attribute__((address_space(1)))
 
 constexpr int F32 = ADKV_DT_F32, F16 = ADKV_DT_F16, BF16 = ADKV_DT_BF16;
-constexpr int STEP = 4;                 // vectors of 16 bytes of a lane's step
-constexpr int CAP = 1024, REFINE = 256; // keys of a list; above which it is looked through
+constexpr int CAP = 1024, REFINE = 128; // keys of a list; above which it is looked through
 constexpr int TOP = 32;
 constexpr float L2E = 1.44269504088896340736f;
-constexpr float MOST = 1.7e38f;         // stands for everything above it, -MOST for everything below: differences are finite
-constexpr float NONE = -3.0e38f;        // a reference before there is one
-constexpr float FAR = 40.0f;
+constexpr float FLOOR = -0x1p126f; // times log2(e) it is exact, and its difference from itself zero
+constexpr float FAR = 60.0f;
 
 struct Args {
     const char *x;
@@ -49,14 +50,12 @@ struct Args {
 };
 
 struct Sums {
-    float big, s, t, r; // the largest so far, which is not in the sums; sum e^d, sum e^d d, d = x - r
+    float big, s, t, r; // the largest so far, which is not in the sums; sum 2^d, sum 2^d d, d = x log2(e) - r
 };
-
-__device__ __forceinline__ float within(float x) { return __builtin_amdgcn_fmed3f(x, -MOST, MOST); }
 
 __device__ __forceinline__ void add(Sums &a, float x)
 {
-    const float d = fminf(x, a.big) - a.r, e = __builtin_amdgcn_exp2f(d * L2E);
+    const float d = __builtin_fmaf(__builtin_amdgcn_fmed3f(x, FLOOR, a.big), L2E, -a.r), e = __builtin_amdgcn_exp2f(d);
     a.big = fmaxf(a.big, x);
     a.s += e;
     a.t = __builtin_fmaf(e, d, a.t);
@@ -64,26 +63,59 @@ __device__ __forceinline__ void add(Sums &a, float x)
 
 __device__ __forceinline__ void refer(Sums &a, float r)
 {
-    const float shift = a.r - r, e = __builtin_amdgcn_exp2f(shift * L2E);
-    a.t = e == 0.0f ? 0.0f : e * __builtin_fmaf(shift, a.s, a.t); // the difference of a lowest value may be infinite
+    const float shift = a.r - r, e = __builtin_amdgcn_exp2f(shift);
+    a.t = e == 0.0f ? 0.0f : e * __builtin_fmaf(shift, a.s, a.t); // relative to FLOOR the product may be infinite
     a.s *= e;
     a.r = r;
 }
 
-__device__ __forceinline__ void merge(Sums &a, Sums b)
+// Over a wave, in all of its lanes: within four lanes, eight, sixteen, then between rows of sixteen
+template <typename F>
+__device__ __forceinline__ uint32_t fold(uint32_t v, F f)
 {
-    const float r = fmaxf(a.r, b.r);
-    refer(a, r);
-    refer(b, r);
-    a.s += b.s;
-    a.t += b.t;
-    const float smaller = fminf(a.big, b.big);
-    a.big = fmaxf(a.big, b.big);
-    if (smaller == -INFINITY) // one of them has seen nothing
-        return;
-    const float d = smaller - r, e = __builtin_amdgcn_exp2f(d * L2E);
-    a.s += e;
-    a.t = __builtin_fmaf(e, d, a.t);
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false));  // lane ^ 1
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false));  // lane ^ 2
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, false)); // 7 - lane of eight
+    v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, false)); // 15 - lane of sixteen
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        unsigned x = v, y = v;
+        asm volatile("" : "+v"(y)); // two copies: the compiler folds a swap of a register with itself
+        const u2v r = i ? __builtin_amdgcn_permlane32_swap(x, y, false, false) : __builtin_amdgcn_permlane16_swap(x, y, false, false);
+        x = r.x;
+        y = r.y;
+        asm volatile("" : "+v"(x), "+v"(y));
+        v = f(x, y);
+    }
+    return v;
+}
+__device__ __forceinline__ float largest(float v)
+{
+    return __uint_as_float(fold(__float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }));
+}
+__device__ __forceinline__ float sum(float v)
+{
+    return __uint_as_float(fold(__float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
+}
+__device__ __forceinline__ uint32_t smallest(uint32_t v)
+{
+    return fold(v, [](uint32_t a, uint32_t b) { return std::min(a, b); });
+}
+
+// The sums of all lanes, in all of them; one that has seen nothing has FLOOR for its largest
+__device__ __forceinline__ void together(Sums &a, int lane)
+{
+    refer(a, largest(a.r));
+    const float big = largest(a.big);
+    const uint64_t holders = __ballot(a.big == big);
+    if (lane != __builtin_ctzll(holders)) { // what others held back is not the largest, or not the one of them that is left out
+        const float d = __builtin_fmaf(a.big, L2E, -a.r), e = __builtin_amdgcn_exp2f(d);
+        a.s += e;
+        a.t = __builtin_fmaf(e, d, a.t);
+    }
+    a.big = big;
+    a.s = sum(a.s);
+    a.t = sum(a.t);
 }
 
 __device__ __forceinline__ uint64_t key(float x, int i)
@@ -131,80 +163,75 @@ template <int TYPE> struct Piece {
 };
 
 struct List {
-    uint64_t keys[2][CAP];
-    uint64_t groups[64];
-    uint64_t bound;
-    int n[2], overrun;
+    uint64_t keys[CAP];
+    uint64_t raised;
+    int n, overrun;
 };
 
-// The top-th largest of the groups' largest keys: at least `top` keys reach it.  0 where fewer groups have any.  A wave's work.
-__device__ __forceinline__ uint64_t bound_of(uint64_t mine, int top)
+__device__ __forceinline__ uint64_t of_lane(uint64_t k, int i)
 {
-    int larger = 0;
-    for (int i = 0; i < 64; i++) {
-        const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), i) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)mine, i);
-        larger += other > mine;
-    }
-    const uint64_t is = __ballot(larger == top - 1 && mine != 0);
-    if (is == 0)
-        return 0;
-    const int at = __builtin_ctzll(is);
-    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), at) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)mine, at);
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), i) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)k, i);
 }
 
-// Leaves those of the list `from` in the other one that reach a bound found from its groups; all threads of the workgroup
-template <int NT>
-__device__ void refine(List &l, int from, int top)
+// A bound that at least `top` of all keys reach, from the largest keys of 2 * top or more groups of lanes (0: none): the least of those that hold the
+// top-th largest value of them.  0 where fewer groups have any.
+__device__ __forceinline__ uint64_t bound_of(uint64_t mine, int top)
 {
-    const int n = min(l.n[from], CAP);
-    if (threadIdx.x < 64)
-        l.groups[threadIdx.x] = 0;
-    if (threadIdx.x == 0)
-        l.n[from ^ 1] = 0;
-    __syncthreads();
-    uint64_t most = 0;
-    for (int i = threadIdx.x; i < n; i += NT)
-        most = std::max(most, l.keys[from][i]);
-    if (most)
-        atomicMax((unsigned long long *)&l.groups[threadIdx.x & 63], (unsigned long long)most);
-    __syncthreads();
-    if (threadIdx.x < 64) {
-        const uint64_t b = bound_of(l.groups[threadIdx.x], top);
-        if (threadIdx.x == 0)
-            l.bound = b;
+    // 16 groups of four lanes for up to 8, 32 of two for up to 16: what reaches the bound is 1.1 to 1.4 times `top` then
+    for (int d = 32; d >= 16 && top * 4 <= 2 * d; d /= 2) {
+        const uint64_t other = (uint64_t)(uint32_t)__shfl_xor((int)(mine >> 32), d) << 32 | (uint32_t)__shfl_xor((int)mine, d);
+        mine = std::max(mine, other);
     }
-    __syncthreads();
-    const uint64_t bound = l.bound;
-    for (int i = threadIdx.x; i < n; i += NT)
-        if (l.keys[from][i] >= bound)
-            l.keys[from ^ 1][atomicAdd(&l.n[from ^ 1], 1)] = l.keys[from][i];
-    __syncthreads();
+    const int groups = top <= 8 ? 16 : top <= 16 ? 32 : 64;
+    const uint32_t value = (uint32_t)(mine >> 32);
+    int larger = 0;
+    for (int i = 0; i < groups; i += 16)
+#pragma unroll
+        for (int j = 0; j < 16; j++)
+            larger += (uint32_t)__builtin_amdgcn_readlane((int)value, i + j) > value;
+    const bool among = larger < top && mine != 0;
+    if (__popcll(__ballot(among)) * groups < top * 64)
+        return 0;
+    const uint32_t least = smallest(among ? value : ~0u);
+    return (uint64_t)least << 32 | smallest(among && value == least ? (uint32_t)mine : ~0u);
+}
+
+// A wave's work: of the list's n keys those that reach a bound found from them stay
+__device__ __forceinline__ uint64_t refine(List &l, int &n, int top, int lane)
+{
+    uint64_t most = 0;
+    for (int i = lane; i < n; i += 64)
+        most = std::max(most, l.keys[i]);
+    const uint64_t bound = bound_of(most, top);
+    int kept = 0;
+    for (int i = lane; __any(i < n); i += 64) {
+        const uint64_t k = i < n ? l.keys[i] : 0;
+        const uint64_t stay = __ballot(i < n && k >= bound);
+        if (i < n && k >= bound)
+            l.keys[kept + __popcll(stay & ((1ull << lane) - 1))] = k;
+        kept += __popcll(stay);
+    }
+    n = kept;
+    return bound;
 }
 
 template <int TYPE, int NT, bool WITH_TOP>
-__global__ __launch_bounds__(NT) void logprobs_kernel(const Args a)
+__global__ __launch_bounds__(NT, WITH_TOP ? 6 : 8) void logprobs_kernel(const Args a)
 {
     using P = Piece<TYPE>;
+    constexpr int NW = NT / 64;
+    constexpr int STEP = WITH_TOP && NT == 256 ? 4 : 2; // vectors of 16 bytes of a lane's step
     __shared__ List list[1];
-    __shared__ Sums left[NT / 64];
-    __shared__ int strange;
-    __shared__ double result[2]; // M, log(1 + S)
+    __shared__ uint64_t first[NT];
+    __shared__ Sums left[NW];
+    __shared__ bool strange[NW];
     __shared__ uint64_t best;
-    const int tid = threadIdx.x, lane = tid & 63;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid / 64;
     const long r = blockIdx.x;
     const char *row = a.x + r / a.n1 * a.s0 + r % a.n1 * a.s1;
-    if (tid == 0)
-        strange = 0;
-    if constexpr (WITH_TOP)
-        if (tid == 0) {
-            list->n[0] = list->n[1] = 0;
-            list->overrun = 0;
-        }
     // whole vectors between the first and the last aligned one; single logits in front of and behind them
     const int head = std::min(a.V, (int)((16 - ((uintptr_t)row & 15)) & 15) / P::SIZE), vectors = (a.V - head) / P::N, tail = a.V - head - vectors * P::N;
     const char *body = row + (long)head * P::SIZE;
-    const int lone = tid < head ? tid : tid >= NT - tail ? a.V - (NT - tid) : -1; // NT > 14
-    const float single = lone >= 0 ? P::one(row, lone) : -INFINITY;
     u4v now[STEP], next[STEP];
     const auto load = [&](int v0, u4v *to) __attribute__((always_inline)) {
 #pragma unroll
@@ -216,172 +243,170 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const Args a)
         }
     };
     load(0, now);
-    Sums sums = {-INFINITY, 0.0f, 0.0f, NONE};
-    bool first = true, nan = single != single;
+    const int lone = tid < head ? tid : tid >= NT - tail ? a.V - (NT - tid) : -1; // NT > 14
+    const float single = lone >= 0 ? P::one(row, lone) : -INFINITY;
+    const int64_t token = a.tokens[r];
+    const float given = token >= 0 && token < a.V ? P::one(row, (int)token) : NAN;
+    Sums sums = {fmaxf(single, FLOOR), 0.0f, 0.0f, fminf(fmaxf(single, FLOOR), -FLOOR) * L2E};
+    bool nan = single != single;
     uint64_t bound = 0;
     float bound_value = -INFINITY;
-    int from = 0;
     const auto take = [&](float x, int i) __attribute__((always_inline)) {
-        if constexpr (WITH_TOP) {
-            const uint64_t k = key(x, i);
-            if (k >= bound) {
-                const int at = atomicAdd(&list->n[from], 1);
-                if (at < CAP)
-                    list->keys[from][at] = k;
-                else
-                    list->overrun = 1;
-            }
+        const uint64_t k = key(x, i);
+        if (k >= bound) {
+            const int at = atomicAdd(&list->n, 1);
+            if (at < CAP)
+                list->keys[at] = k;
+            else
+                list->overrun = 1;
         }
     };
-    for (int v0 = 0; first || v0 < vectors; v0 += STEP * NT) {
-        load(v0 + STEP * NT, next);
-        float x[STEP][P::N], most[STEP];
+    if constexpr (WITH_TOP) {
+        if (tid == 0)
+            list->n = list->overrun = 0;
+        // the lane's largest logit of the first step, the first of equal ones
+        float most = -INFINITY;
+        int at = -1;
 #pragma unroll
         for (int i = 0; i < STEP; i++) {
-            P::open(now[i], x[i]);
-            most[i] = x[i][0];
+            float x[P::N];
+            P::open(now[i], x);
+            const int v = i * NT + tid;
+#pragma unroll
+            for (int e = 0; e < P::N; e++)
+                if (v < vectors && (at < 0 || x[e] > most)) {
+                    most = x[e];
+                    at = v * P::N + e;
+                }
+        }
+        const uint64_t mine = at >= 0 ? key(most, head + at) : 0;
+        first[tid] = lone >= 0 ? std::max(mine, key(single, lone)) : mine;
+        __syncthreads();
+        uint64_t group = 0;
+#pragma unroll
+        for (int w = 0; w < NW; w++)
+            group = std::max(group, first[w * 64 + lane]);
+        bound = bound_of(group, a.top);
+        bound_value = bound ? number(bound) : -INFINITY;
+        if (lone >= 0)
+            take(single, lone);
+    }
+    int step = 0;
+    for (int v0 = 0; v0 < vectors; v0 += STEP * NT) {
+        load(v0 + STEP * NT, next);
+#pragma unroll
+        for (int i = 0; i < STEP; i++) {
+            float x[P::N];
+            P::open(now[i], x);
+            const int v = v0 + i * NT + tid;
+            float most = x[0];
 #pragma unroll
             for (int e = 1; e < P::N; e++)
-                most[i] = fmaxf(most[i], x[i][e]);
-        }
-        if (WITH_TOP && first) {
-            // the lane's largest key
-            uint64_t mine = lone >= 0 ? key(single, lone) : 0;
+                most = fmaxf(most, x[e]);
+            if (WITH_TOP && __any(most >= bound_value)) {
 #pragma unroll
-            for (int i = 0; i < STEP; i++)
+                for (int e = 0; e < P::N; e++)
+                    if (x[e] >= bound_value && v < vectors)
+                        take(x[e], head + v * P::N + e);
+            }
+            if (__any(most * L2E > sums.r + FAR)) {
+                if (most * L2E > sums.r + FAR)
+                    refer(sums, fminf(most, -FLOOR) * L2E);
+            }
+            // what is behind the row is minus infinity, and weighs nothing
 #pragma unroll
-                for (int e = 0; e < P::N; e++) {
-                    const int v = v0 + i * NT + tid;
-                    if (v < vectors)
-                        mine = std::max(mine, key(x[i][e], head + v * P::N + e));
-                }
-            if (tid < 64)
-                list->groups[tid] = 0;
-            __syncthreads();
-            if (mine)
-                atomicMax((unsigned long long *)&list->groups[lane], (unsigned long long)mine);
-            __syncthreads();
-            bound = bound_of(list->groups[lane], a.top);
-            bound_value = bound ? number(bound) : -INFINITY;
-            if (lone >= 0)
-                take(single, lone);
+            for (int e = 0; e < P::N; e++) {
+                nan |= x[e] != x[e];
+                add(sums, x[e]);
+            }
         }
+        step++;
         if constexpr (WITH_TOP) {
-#pragma unroll
-            for (int i = 0; i < STEP; i++)
-                if (__any(most[i] >= bound_value)) {
-#pragma unroll
-                    for (int e = 0; e < P::N; e++) {
-                        const int v = v0 + i * NT + tid;
-                        if (x[i][e] >= bound_value && v < vectors)
-                            take(x[i][e], head + v * P::N + e);
+            // seldom: after four, eight, sixteen.. steps
+            if (step >= 4 && (step & (step - 1)) == 0 && v0 + STEP * NT < vectors) {
+                __syncthreads();
+                if (wave == 0) {
+                    int n = std::min(list->n, CAP);
+                    const uint64_t raised = n > REFINE ? refine(*list, n, a.top, lane) : 0;
+                    if (lane == 0) {
+                        list->n = n;
+                        list->raised = raised;
                     }
                 }
-        }
-        if (first) {
-            if (lone >= 0) {
-                sums.big = sums.r = within(single);
-            }
-            first = false;
-        }
-#pragma unroll
-        for (int i = 0; i < STEP; i++) {
-            const float top = within(most[i]);
-            if (__any(top > sums.r + FAR)) {
-                if (top > sums.r + FAR)
-                    refer(sums, top);
-            }
-            const int v = v0 + i * NT + tid;
-            if (v < vectors) {
-#pragma unroll
-                for (int e = 0; e < P::N; e++) {
-                    nan |= x[i][e] != x[i][e];
-                    const float y = within(x[i][e]);
-                    if (e == 0 && sums.big == -INFINITY)
-                        sums.big = y; // the lane's first
-                    else
-                        add(sums, y);
-                }
-            }
-        }
-        if constexpr (WITH_TOP) {
-            __syncthreads();
-            if (list->n[from] > REFINE) {
-                refine<NT>(*list, from, a.top);
-                from ^= 1;
-                bound = std::max(bound, list->bound);
+                __syncthreads();
+                bound = std::max(bound, list->raised);
                 bound_value = bound ? number(bound) : -INFINITY;
             }
-            __syncthreads();
         }
 #pragma unroll
         for (int i = 0; i < STEP; i++)
             now[i] = next[i];
     }
-    if (__any(nan) && lane == 0)
-        strange = 1;
-    for (int d = 32; d; d >>= 1) {
-        Sums o;
-        o.big = __shfl_xor(sums.big, d);
-        o.s = __shfl_xor(sums.s, d);
-        o.t = __shfl_xor(sums.t, d);
-        o.r = __shfl_xor(sums.r, d);
-        merge(sums, o);
-    }
-    if (lane == 0)
-        left[tid / 64] = sums;
-    __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < NT / 64; w++)
-            merge(sums, left[w]);
-        left[0] = sums;
+    nan = __any(nan);
+    together(sums, lane);
+    if (lane == 0) {
+        strange[wave] = nan;
+        left[wave] = sums;
     }
     __syncthreads();
-    sums = left[0];
+    const bool odd = __any(lane < NW && strange[lane % NW]), slow = WITH_TOP && (odd || list->overrun);
+    sums = lane < NW ? left[lane] : (Sums){FLOOR, 0.0f, 0.0f, FLOOR * L2E};
+    together(sums, lane);
     float M = sums.big;
-    if (fabsf(M) >= MOST) {
-        // nothing but what may be minus infinity, or plus infinity
+    const bool again = !(fabsf(M) < -FLOOR);
+    if (wave != 0 && !slow && !again)
+        return; // the rest is the first wave's
+    const float shift = __builtin_fmaf(-M, L2E, sums.r), scale = __builtin_amdgcn_exp2f(shift);
+    float S = scale * sums.s, T = scale * __builtin_fmaf(shift, sums.s, sums.t) * 0.69314718055994530942f;
+    if (again) {
+        // logits of the type's lowest value only, or of minus or plus infinity: the definition, in two passes more
         M = -INFINITY;
         for (int i = tid; i < a.V; i += NT)
             M = fmaxf(M, P::one(row, i));
-        for (int d = 32; d; d >>= 1)
-            M = fmaxf(M, __shfl_xor(M, d));
+        M = largest(M);
         __syncthreads();
         if (lane == 0)
-            left[tid / 64].big = M;
+            left[wave].big = M;
         __syncthreads();
-        for (int w = 0; w < NT / 64; w++)
-            M = fmaxf(M, left[w].big);
-        if (tid == 0 && fabsf(M) == INFINITY)
-            strange |= 2;
+        M = largest(left[lane % NW].big);
+        S = T = 0.0f;
+        for (int i = tid; i < a.V; i += NT) {
+            const double d = (double)P::one(row, i) - M;
+            const float e = d > -200.0 ? expf((float)d) : 0.0f;
+            S += e;
+            T += e > 0.0f ? e * (float)d : 0.0f;
+        }
+        S = sum(S);
+        T = sum(T);
+        if (lane == 0)
+            left[wave].s = S, left[wave].t = T;
+        __syncthreads();
+        S = sum(lane < NW ? left[lane].s : 0.0f) - 1.0f;
+        T = sum(lane < NW ? left[lane].t : 0.0f);
     }
+    const float log1 = odd || fabsf(M) == INFINITY ? NAN : log1pf(S);
+    const auto log_of = [&](float x) { return (float)((double)x - M - log1); };
     if (tid == 0) {
-        const double shift = (double)sums.r - (double)sums.big, scale = exp(shift), S = scale * sums.s, T = scale * ((double)sums.t + shift * sums.s);
-        const double log1 = strange ? (double)NAN : log1p(S);
-        result[0] = M;
-        result[1] = log1;
-        const int64_t token = a.tokens[r];
-        a.logprobs[r] = token < 0 ? 0.0f : token < a.V ? (float)((double)P::one(row, (int)token) - M - log1) : NAN;
-        a.entropy[r] = (float)(log1 - T / (1.0 + S));
+        a.logprobs[r] = token < 0 ? 0.0f : token < a.V ? log_of(given) : NAN;
+        a.entropy[r] = log1 - T / (1.0f + S);
     }
     if constexpr (WITH_TOP) {
-        __syncthreads();
         const auto put = [&](int rank, uint64_t k) {
-            const float x = number(k);
             a.top_tokens[r * a.top + rank] = (int64_t)(0xFFFFFFFFu - (uint32_t)k);
-            a.top_logprobs[r * a.top + rank] = (float)((double)x - result[0] - result[1]);
+            a.top_logprobs[r * a.top + rank] = log_of(number(k));
         };
-        if (!(strange & 1) && !list->overrun) {
-            if (list->n[from] > 2 * TOP) {
-                refine<NT>(*list, from, a.top);
-                from ^= 1;
-            }
-            const int n = list->n[from];
-            for (int i = tid; i < n; i += NT) {
-                const uint64_t k = list->keys[from][i];
+        if (!slow) {
+            if (wave != 0)
+                return;
+            int n = list->n;
+            if (n > 64)
+                refine(*list, n, a.top, lane);
+            for (int i = lane; i < n; i += 64) {
+                const uint64_t k = list->keys[i];
                 int rank = 0;
+#pragma unroll 8
                 for (int j = 0; j < n; j++)
-                    rank += list->keys[from][j] > k;
+                    rank += list->keys[j] > k;
                 if (rank < a.top)
                     put(rank, k);
             }
@@ -412,6 +437,8 @@ template <int TYPE> static auto kernel_of(int threads, bool top)
 {
     if (threads == 256)
         return top ? logprobs_kernel<TYPE, 256, true> : logprobs_kernel<TYPE, 256, false>;
+    if (threads == 512)
+        return top ? logprobs_kernel<TYPE, 512, true> : logprobs_kernel<TYPE, 512, false>;
     return top ? logprobs_kernel<TYPE, 1024, true> : logprobs_kernel<TYPE, 1024, false>;
 }
 
@@ -436,7 +463,11 @@ extern "C" int adkv_token_logprobs(const void *logits, int64_t stride0, int64_t 
     if (((uint64_t)logprobs | (uint64_t)entropy | (uint64_t)top_logprobs) & 3 || ((uint64_t)tokens | (uint64_t)top_tokens) & 7)
         return ADKV_E_ALIGN;
     Args a = {(const char *)logits, (long)stride0 * size, (long)stride1 * size, tokens, n1, V, top, logprobs, entropy, top_logprobs, top_tokens};
-    const int threads = rows >= 4ll * cu_count() ? 256 : 1024;
+    // The smallest workgroups that fill the device: few rows are over sooner with more lanes, many have less to put together with fewer.  us with 256, 512
+    // and 1024 lanes: 4 rows of 32 000 logits with 8 alternatives 16.3, 10.5, 10.3; 512 of 128 000 48.4, 37.8, 34.8; 1000 of 128 000 with 20 72, 67, 74;
+    // 4096 of 32 000 with 5 61, 66, 93
+    const int64_t cus = cu_count();
+    const int threads = rows > 6 * cus ? 256 : rows > 2 * cus ? 512 : 1024;
     const auto kernel = dtype == F32 ? kernel_of<F32>(threads, top > 0) : dtype == F16 ? kernel_of<F16>(threads, top > 0) : kernel_of<BF16>(threads, top > 0);
     hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(threads), 0, (hipStream_t)stream, a);
     return check_launch();

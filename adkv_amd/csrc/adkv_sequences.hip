@@ -13,13 +13,15 @@
 
 namespace adkv_sequences {
 using adkv::check_launch;
+using adkv::cu_count;
 
 typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 #define GLOBAL __attribute__((address_space(1)))
 
-constexpr int WAVES = 4, SLOTS = 32, BLOCK = 1024; // bytes of a column
+constexpr int WAVES = 4, SLOTS = 16, BLOCK = 1024; // bytes of a column
+constexpr int PER_CU = 12;                          // waves: all of them at once, three to a SIMD by their registers
 constexpr int TENSORS = 96;                         // of a launch
-constexpr int MOST = 2048;                          // rows: with all of them moved a column is 16 bytes
+constexpr int MOST = 1024;                          // rows: with all of them moved a column is 16 bytes
 
 struct Tensor {
     const char *from;
@@ -27,11 +29,11 @@ struct Tensor {
     int segments;        // of a row (heads)
     int pitch, to_pitch; // of a segment, bytes
     int used, width;     // columns up to `used` are copied, from there to `width` they are zeros
-    int first;           // job
+    int first;           // column of all
 };
 struct Args {
     const int64_t *index;
-    int rows, batch, n, jobs;
+    int rows, batch, n, units, waves;
     Tensor t[TENSORS];
 };
 static_assert(sizeof(Args) <= 4096, "kernel arguments");
@@ -50,82 +52,83 @@ __global__ __launch_bounds__(WAVES * 64) void take_kernel(const Args a)
     __syncthreads();
     // the rows that move, in any order
     for (int r = threadIdx.x; r < a.rows; r += WAVES * 64) {
-        int64_t from = a.index[r];
+        const int64_t from = a.index[r];
         const bool there = from >= 0 && from < a.batch;
         if (INTO || (there && from != r))
             list[atomicAdd(&count, 1)] = make_int2(r, there ? (int)from : -1);
     }
     __syncthreads();
-    const int m = __builtin_amdgcn_readfirstlane(count), job = (int)blockIdx.x * WAVES + wave;
-    if (m == 0 || job >= a.jobs)
+    const int m = __builtin_amdgcn_readfirstlane(count), me = (int)blockIdx.x * WAVES + wave;
+    if (m == 0 || me >= a.waves)
         return;
+    // this wave's share of the columns, which may be of several tensors
+    int unit = (int)((int64_t)a.units * me / a.waves);
+    const int last = (int)((int64_t)a.units * (me + 1) / a.waves);
     int which = 0;
     for (int i = 0; i < a.n; i += 64)
-        which += __popcll(__ballot(i + lane < a.n && a.t[min(i + lane, TENSORS - 1)].first <= job));
+        which += __popcll(__ballot(i + lane < a.n && a.t[min(i + lane, TENSORS - 1)].first <= unit));
     which--;
-    const Tensor t = a.t[which];
-    const int blocks = (t.width + BLOCK - 1) / BLOCK; // columns of a segment
-    const long from_row = (long)t.segments * t.pitch, to_row = (long)t.segments * t.to_pitch;
-    int unit = (job - t.first) * SLOTS;
-    const int end = min(unit + SLOTS, t.segments * blocks);
+    int log = 0; // up to SLOTS rows: 2^log slots are a column's; more: 2^log rows are a slot's
+    while ((m <= SLOTS ? 1 : SLOTS) << log < m)
+        log++;
+    const int2 mine = list[min(lane, m - 1)];
     u4v x[SLOTS];
-    if (m <= SLOTS) {
-        int log = 0; // 2^log slots are a column's
-        while (1 << log < m)
-            log++;
-        const int2 mine = list[min(lane, m - 1)];
-        for (; unit < end; unit += SLOTS >> log) {
-            const int seg0 = unit / blocks, block0 = unit - seg0 * blocks;
-            auto each = [&](auto &&f) __attribute__((always_inline)) {
-                int seg = seg0, block = block0;
+    for (; unit < last; which++) {
+        const Tensor t = a.t[which];
+        const int blocks = (t.width + BLOCK - 1) / BLOCK; // columns of a segment
+        const long from_row = (long)t.segments * t.pitch, to_row = (long)t.segments * t.to_pitch;
+        const int end = min(last, t.first + t.segments * blocks);
+        if (m <= SLOTS) {
+            for (; unit < end; unit = min(unit + (SLOTS >> log), end)) {
+                const int seg0 = (unit - t.first) / blocks, block0 = unit - t.first - seg0 * blocks;
+                auto each = [&](auto &&f) __attribute__((always_inline)) {
+                    int seg = seg0, block = block0;
+#pragma unroll
+                    for (int i = 0; i < SLOTS; i++) {
+                        const int row = i & ((1 << log) - 1);
+                        if (i > 0 && row == 0 && ++block == blocks) {
+                            block = 0;
+                            seg++;
+                        }
+                        if (row < m && unit + (i >> log) < end)
+                            f(i, __builtin_amdgcn_readlane(mine.x, row), __builtin_amdgcn_readlane(mine.y, row), seg, block * BLOCK + lane * 16);
+                    }
+                };
+                each([&](int i, int, int from, int seg, int at) __attribute__((always_inline)) {
+                    x[i] = (u4v){0, 0, 0, 0};
+                    if ((!INTO || from >= 0) && at < t.used)
+                        x[i] = *(const GLOBAL u4v *)(t.from + from * from_row + (long)seg * t.pitch + at);
+                });
+                all_read();
+                each([&](int i, int to, int, int seg, int at) __attribute__((always_inline)) {
+                    if (at < t.width)
+                        __builtin_nontemporal_store(x[i], (GLOBAL u4v *)(t.to + to * to_row + (long)seg * t.to_pitch + at));
+                });
+            }
+            continue;
+        }
+        const int wide = BLOCK >> log, sub = lane >> (6 - log), in = (lane & ((64 >> log) - 1)) * 16;
+        for (; unit < end; unit++) {
+            const int seg = (unit - t.first) / blocks, block = unit - t.first - seg * blocks;
+            for (int part = 0; part < 1 << log; part++) {
+                const int at = block * BLOCK + part * wide + in;
 #pragma unroll
                 for (int i = 0; i < SLOTS; i++) {
-                    const int row = i & ((1 << log) - 1);
-                    if (i > 0 && row == 0 && ++block == blocks) {
-                        block = 0;
-                        seg++;
+                    const int p = (i << log) + sub;
+                    x[i] = (u4v){0, 0, 0, 0};
+                    if (p < m && at < t.used) {
+                        const int from = list[p].y;
+                        if (!INTO || from >= 0)
+                            x[i] = *(const GLOBAL u4v *)(t.from + from * from_row + (long)seg * t.pitch + at);
                     }
-                    if (row < m && unit + (i >> log) < end)
-                        f(i, __builtin_amdgcn_readlane(mine.x, row), __builtin_amdgcn_readlane(mine.y, row), seg, block * BLOCK + lane * 16);
                 }
-            };
-            each([&](int i, int, int from, int seg, int at) __attribute__((always_inline)) {
-                x[i] = (u4v){0, 0, 0, 0};
-                if ((!INTO || from >= 0) && at < t.used)
-                    x[i] = *(const GLOBAL u4v *)(t.from + from * from_row + (long)seg * t.pitch + at);
-            });
-            all_read();
-            each([&](int i, int to, int, int seg, int at) __attribute__((always_inline)) {
-                if (at < t.width)
-                    *(GLOBAL u4v *)(t.to + to * to_row + (long)seg * t.to_pitch + at) = x[i];
-            });
-        }
-        return;
-    }
-    int log = 1; // 2^log rows to a slot
-    while (SLOTS << log < m)
-        log++;
-    const int wide = BLOCK >> log, sub = lane >> (6 - log), in = (lane & ((64 >> log) - 1)) * 16;
-    for (; unit < end; unit++) {
-        const int seg = unit / blocks, block = unit - seg * blocks;
-        for (int part = 0; part < 1 << log; part++) {
-            const int at = block * BLOCK + part * wide + in;
+                all_read();
 #pragma unroll
-            for (int i = 0; i < SLOTS; i++) {
-                const int p = (i << log) + sub;
-                x[i] = (u4v){0, 0, 0, 0};
-                if (p < m && at < t.used) {
-                    const int from = list[p].y;
-                    if (!INTO || from >= 0)
-                        x[i] = *(const GLOBAL u4v *)(t.from + from * from_row + (long)seg * t.pitch + at);
+                for (int i = 0; i < SLOTS; i++) {
+                    const int p = (i << log) + sub;
+                    if (p < m && at < t.width)
+                        __builtin_nontemporal_store(x[i], (GLOBAL u4v *)(t.to + list[p].x * to_row + (long)seg * t.to_pitch + at));
                 }
-            }
-            all_read();
-#pragma unroll
-            for (int i = 0; i < SLOTS; i++) {
-                const int p = (i << log) + sub;
-                if (p < m && at < t.width)
-                    *(GLOBAL u4v *)(t.to + list[p].x * to_row + (long)seg * t.to_pitch + at) = x[i];
             }
         }
     }
@@ -160,7 +163,7 @@ extern "C" int adkv_take_sequences(const adkv_rows *tensors, int n, const int64_
         a.index = index;
         a.rows = rows;
         a.batch = batch;
-        int64_t jobs = 0;
+        int64_t units = 0;
         for (; at < n && a.n < TENSORS; at++) {
             const adkv_rows &r = tensors[at];
             Tensor t = {};
@@ -178,25 +181,23 @@ extern "C" int adkv_take_sequences(const adkv_rows *tensors, int n, const int64_
             t.used = (int)used;
             t.width = (int)width;
             const int64_t blocks = (width + BLOCK - 1) / BLOCK;
-            if (segments * blocks > INT32_MAX - SLOTS)
-                return ADKV_E_SHAPE;
-            const int64_t more = (segments * blocks + SLOTS - 1) / SLOTS;
-            if (more == 0)
+            if (segments * blocks == 0)
                 continue;
-            if (jobs + more > 1 << 26) { // a grid is 2^32 threads at most
-                if (more > 1 << 26)
+            if (units + segments * blocks > INT32_MAX / 2) {
+                if (units == 0)
                     return ADKV_E_SHAPE;
                 break;
             }
-            t.first = (int)jobs;
+            t.first = (int)units;
             a.t[a.n++] = t;
-            jobs += more;
+            units += segments * blocks;
         }
         if (a.n == 0)
             continue;
-        a.jobs = (int)jobs;
+        a.units = (int)units;
+        a.waves = (int)std::min<int64_t>(units, (int64_t)PER_CU * cu_count());
         const auto kernel = into ? take_kernel<true> : take_kernel<false>;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)((jobs + WAVES - 1) / WAVES)), dim3(WAVES * 64), 0, (hipStream_t)stream, a);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((a.waves + WAVES - 1) / WAVES)), dim3(WAVES * 64), 0, (hipStream_t)stream, a);
         if (int rc = check_launch())
             return rc;
     }

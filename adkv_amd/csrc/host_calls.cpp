@@ -827,7 +827,7 @@ PyObject *take_sequences(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     const Py_ssize_t n = PyList_GET_SIZE(args[0]);
     const bool some = args[2] != Py_None, into = args[3] != Py_None;
     const at::Tensor *index = plain(args[1]);
-    if (n == 0 || !index || index->scalar_type() != at::kLong || index->dim() != 1 || !index->is_contiguous() || index->size(0) <= 0 || index->size(0) > 2048 ||
+    if (n == 0 || !index || index->scalar_type() != at::kLong || index->dim() != 1 || !index->is_contiguous() || index->size(0) <= 0 || index->size(0) > 1024 ||
         (some && PyList_GET_SIZE(args[2]) != n) || (into && PyList_GET_SIZE(args[3]) != n))
         Py_RETURN_NONE;
     const int64_t R = index->size(0);

@@ -771,7 +771,7 @@ def take_sequences(tensors, index: torch.Tensor, *, used=None, into=None) -> Non
         tensors: any number of contiguous tensors ``[B, H, n, ...]`` of one device, a cache's codes, checkpoints and states, of one layer or of all:
             one or two launches for all of them.  They begin at multiples of 16 bytes, and a head's entries (``[n, ...]``), those that are used too, are
             such multiples.
-        index: ``[R]`` whole numbers, ``R <= 2048``; the same one may come several times.  On the device they are not checked (that would wait for it): a
+        index: ``[R]`` whole numbers, ``R <= 1024``; the same one may come several times.  On the device they are not checked (that would wait for it): a
             row whose index is none of the rows stays as it is, or is zeros in ``into``.  On the host they are checked and copied.
         used: how many entries along the third axis hold anything, one number per tensor (all): what is behind them is neither read nor written.
         into: as many tensors ``[R, H, m, ...]``, ``m >= used``, to write instead, which share no memory with ``tensors``; what is behind the entries that are
@@ -786,7 +786,7 @@ def take_sequences(tensors, index: torch.Tensor, *, used=None, into=None) -> Non
         return
     _chk(index.dim() == 1 and not (index.is_floating_point() or index.is_complex() or index.dtype == torch.bool), "index must be [R] whole numbers")
     R = index.shape[0]
-    _chk(R <= 2048, "at most 2048 sequences")
+    _chk(R <= 1024, "at most 1024 sequences")
     used = [None] * len(tensors) if used is None else used
     _chk(len(used) == len(tensors), "used must have a number for every tensor")
     _chk(into is None or len(into) == len(tensors), "into must have a tensor for every tensor")

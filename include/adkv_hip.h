@@ -527,7 +527,7 @@ int adkv_prompt_attention(const void *q, const int64_t *q_strides, const void *k
  *   into      NULL: in place, whatever the map (a row may be several rows' source), rows <= batch.  Else [rows, segments, into_pitch bytes], packed,
  *             for every tensor of the call, which do not overlap data
  *   used      bytes of a segment that are copied, the same in all rows; what is behind them is left as it is in place, zeros in `into`
- * Pointers and sizes are multiples of 16 bytes; at most 2048 rows.  The array is host memory and may be reused after the call.
+ * Pointers and sizes are multiples of 16 bytes; at most 1024 rows.  The array is host memory and may be reused after the call.
  */
 typedef struct {
     void *data, *into;
@@ -543,7 +543,7 @@ int adkv_take_sequences(const adkv_rows *tensors, int n, const int64_t *index, i
  *   logits [n0, n1, V] of dtype (ADKV_DT_F32, F16, BF16), element strides stride0, stride1, V contiguous, aligned as its elements; tokens int64
  *   [n0 * n1], packed: a negative one stands for none (0 is returned), one from V on gives NaN; outputs fp32 (top_tokens int64), packed; top 0..32, at
  *   most V, top_* unused if 0.
- * Minus infinity is a probability of zero; beside others, logits beyond +-1.7e38 weigh as that.  A row with a NaN or plus infinity, or of nothing but minus infinity, gives NaN; its likeliest tokens are in
+ * Minus infinity is a probability of zero.  A row with a NaN or plus infinity, or of nothing but minus infinity, gives NaN; its likeliest tokens are in
  * order all the same, NaN first.
  */
 int adkv_token_logprobs(const void *logits, int64_t stride0, int64_t stride1, const int64_t *tokens, int n0, int n1, int V, int dtype,
