@@ -61,6 +61,7 @@ struct Args {
     Rows q, k, v;
     char *out;                // [B, Tq, H * g, D]
     const char *mask;
+    const char *mask_end;     // behind its last element
     long m_sb, m_sh, m_st;    // elements
     const int *bounds;        // of packed sequences, n_seq + 1, or null
     float *partial;           // [pieces][rows of all][D], few rows in pieces
@@ -221,7 +222,99 @@ __device__ __forceinline__ bool place(const Args &a, int i, int lane, Job &j)
     return true;
 }
 
-// A wave's 32 rows
+// The mask of a lane's row for KB * 32 keys: SIZE bytes per key, as it is in memory.  Half h of the lanes loads keys 16 * KB * h.. of them, 16 bytes at a
+// time, whatever their alignment; an exchange with the other half leaves both with the keys whose scores they have.
+template <int SIZE, int KB>
+struct Mask {
+    static constexpr int WORDS = KB * 4 * SIZE;
+    uint32_t w[WORDS];
+    // row: the lane's; keys k.., of `there` that the mask has
+    __device__ __forceinline__ void load(const Args &a, const char *row, int k, int lane)
+    {
+        typedef uint32_t u4a __attribute__((ext_vector_type(4), aligned(4)));
+        const int first = k + (lane >> 5) * KB * 16;
+        const char *p = row + (long)first * SIZE;
+        // rows may begin between two words; loads that do so cost more than the shifts (1023 tokens, 16 bits: 97 us)
+        const GLOBAL char *from = (const GLOBAL char *)((uintptr_t)p & ~(uintptr_t)3);
+        constexpr int MORE = SIZE < 4 ? 1 : 0;
+        if (__all((const char *)from + (WORDS + MORE) * 4 <= a.mask_end)) {
+            uint32_t u[WORDS + 1];
+#pragma unroll
+            for (int i = 0; i < WORDS; i += 4) {
+                const u4a four = *(const GLOBAL u4a *)(from + i * 4);
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    u[i + e] = four[e];
+            }
+            if (MORE)
+                u[WORDS] = *(const GLOBAL uint32_t *)(from + WORDS * 4);
+#pragma unroll
+            for (int i = 0; i < WORDS; i++)
+                w[i] = MORE ? __builtin_amdgcn_alignbyte(u[i + 1], u[i], (uint32_t)(uintptr_t)p & 3) : u[i];
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < WORDS; i++) {
+            w[i] = 0;
+#pragma unroll
+            for (int e = 0; e < 4 / SIZE; e++)
+                if (first + i * 4 / SIZE + e < a.Tk) {
+                    if constexpr (SIZE == 4)
+                        w[i] = *(const GLOBAL uint32_t *)(p + i * 4);
+                    else if constexpr (SIZE == 2)
+                        w[i] |= (uint32_t)*(const GLOBAL uint16_t *)(p + i * 4 + e * 2) << e * 16;
+                    else
+                        w[i] |= (uint32_t)*(const GLOBAL uint8_t *)(p + i * 4 + e) << e * 8;
+                }
+        }
+    }
+    // what all of the wave's keys have, and any: 1 where nothing is added or hidden, -1 where all of them are hidden
+    __device__ __forceinline__ int alike(int dt) const
+    {
+        uint32_t all = ~0u, any = 0;
+#pragma unroll
+        for (int i = 0; i < WORDS; i++) {
+            all &= w[i];
+            any |= w[i];
+        }
+        const uint32_t none = SIZE == 1 ? 0 : SIZE == 4 ? 0xFF800000u : dt == F16 ? 0xFC00FC00u : 0xFF80FF80u, whole = SIZE == 1 ? 0x01010101u : 0;
+        return __all(all == whole && any == whole) ? 1 : __all(all == none && any == none) ? -1 : 0;
+    }
+    __device__ __forceinline__ void exchange()
+    {
+#pragma unroll
+        for (int i = 0; i < 2 * KB; i++)
+#pragma unroll
+            for (int e = 0; e < SIZE; e++) {
+                const u2v r = __builtin_amdgcn_permlane32_swap(w[i * 2 * SIZE + e], w[i * 2 * SIZE + SIZE + e], false, false);
+                w[i * 2 * SIZE + e] = r.x;
+                w[i * 2 * SIZE + SIZE + e] = r.y;
+            }
+    }
+    // of score e of the lane, after the exchange: what is added, or whether the key is looked at
+    template <int E> __device__ __forceinline__ float of(int dt) const
+    {
+        constexpr int G = E >> 2, AT = G < 2 * KB ? G * 2 * SIZE : (G - 2 * KB) * 2 * SIZE + SIZE;
+        if constexpr (SIZE == 1) {
+            return w[AT] & 0xFFu << 8 * (E & 3) ? 1.0f : 0.0f;
+        } else if constexpr (SIZE == 4) {
+            return __uint_as_float(w[AT + (E & 3)]);
+        } else {
+            const uint32_t u = w[AT + (E >> 1 & 1)], half = E & 1 ? u >> 16 : u & 0xFFFFu;
+            return dt == BF16 ? __uint_as_float(half << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)half);
+        }
+    }
+};
+
+// Score s of a key to which x is added, c being the scaling, all in powers of two.  A type's lowest value times log2(e) would be -inf, which stands for
+// hidden keys only: rows of nothing but lowest values look at all of them alike.
+__device__ __forceinline__ float with(float s, float x, float c)
+{
+    const float y = __builtin_fmaf(x, LOG2E, s * c);
+    return x == -INFINITY ? -INFINITY : y < -3.0e38f ? -3.0e38f : y; // what is no number stays that
+}
+
+// A wave's 32 rows; MASK: bytes of a key's mask, 0 without one
 template <int TYPE, int DP, int MASK>
 struct Wave {
     using Hf = Half<TYPE>;
@@ -267,68 +360,17 @@ struct Wave {
 #pragma unroll
             for (int e = 0; e < 16; e++)
                 o[cb][e] = 0.0f;
-        if constexpr (MASK != 0) {
-            const int size = a.mask_dt == 0 ? 4 : a.mask_dt == 3 ? 1 : 2;
-            mask = a.mask + (j.b * a.m_sb + head * a.m_sh + (long)t * a.m_st) * size;
-        }
-    }
-
-    // what is added to the scores of keys k.. k + 3, in powers of two; -inf for what is hidden
-    __device__ __forceinline__ void added(const Args &a, int k, int there, float *to) const
-    {
-        const int dt = a.mask_dt;
-        const int size = dt == 0 ? 4 : dt == 3 ? 1 : 2;
-        const GLOBAL char *p = (const GLOBAL char *)mask + (long)k * size;
-        uint32_t w[4];
-        typedef uint32_t u1 __attribute__((aligned(1)));
-        typedef uint32_t u2a __attribute__((ext_vector_type(2), aligned(2)));
-        typedef uint32_t u4a __attribute__((ext_vector_type(4), aligned(4)));
-        if (there >= 4) {
-            if (dt == 0) {
-                const u4a u = *(const GLOBAL u4a *)p;
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    w[e] = u[e];
-            } else if (dt == 3) {
-                const uint32_t u = *(const GLOBAL u1 *)p;
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    w[e] = u >> 8 * e & 255u;
-            } else {
-                const u2a u = *(const GLOBAL u2a *)p;
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    w[e] = e & 1 ? u[e >> 1] >> 16 : u[e >> 1] & 0xFFFFu;
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                w[e] = 0;
-                if (e < there)
-                    w[e] = dt == 0 ? ((const GLOBAL uint32_t *)p)[e] : dt == 3 ? (uint32_t)((const GLOBAL uint8_t *)p)[e] : (uint32_t)((const GLOBAL uint16_t *)p)[e];
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            if (dt == 3)
-                to[e] = w[e] ? 0.0f : -INFINITY;
-            else
-                to[e] = dt == 0 ? __uint_as_float(w[e]) : dt == BF16 ? __uint_as_float(w[e] << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)w[e]);
-        }
-    }
-
-    // Score s of a key whose mask is x, in powers of two.  A type's lowest value times log2(e) would be -inf, which stands for hidden keys only: rows of
-    // nothing but lowest values look at all of them alike.
-    __device__ __forceinline__ float with(float s, float x) const
-    {
-        const float y = __builtin_fmaf(x, LOG2E, s * c);
-        return x == -INFINITY ? -INFINITY : y < -3.0e38f ? -3.0e38f : y; // what is no number stays that
+        if constexpr (MASK != 0)
+            mask = a.mask + (j.b * a.m_sb + head * a.m_sh + (long)t * a.m_st) * MASK;
     }
 
     // KB * 32 keys from k on, keys and values in the LDS
     template <int KB>
-    __device__ __forceinline__ void tile(const Args &a, uint32_t keys, uint32_t values, int k)
+    __device__ __forceinline__ void tile(const Args &a, uint32_t keys, uint32_t values, int k, Mask<MASK ? MASK : 1, KB> &masked)
     {
+        const int all = MASK != 0 ? masked.alike(a.mask_dt) : 1;
+        if (MASK != 0 && all < 0)
+            return; // nothing to look at
         const int r32 = lane & 31, h = lane >> 5, i16 = lane & 15;
         f16v sc[KB];
 #pragma unroll
@@ -347,15 +389,17 @@ struct Wave {
 #pragma unroll
         for (int e = 0; e < KB * 16; e++)
             x[e] = sc[e >> 4][e & 15];
+        float unit = c; // of x; with something added they are in powers of two
         if constexpr (MASK != 0) {
-#pragma unroll
-            for (int e = 0; e < KB * 16; e += 4) {
-                const int at = k + (e >> 2) * 8 + 4 * h;
-                float add[4];
-                added(a, at, a.Tk - at, add);
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    x[e + i] = with(x[e + i], add[i]);
+            if (all == 0) {
+                masked.exchange();
+                if (MASK != 1)
+                    unit = 1.0f;
+                adkv::static_for<KB * 16>([&](auto i) {
+                    constexpr int E = decltype(i)::value;
+                    const float y = masked.template of<E>(a.mask_dt);
+                    x[E] = MASK == 1 ? (y != 0.0f ? x[E] : -INFINITY) : with(x[E], y, c);
+                });
             }
         }
         if (k + KB * 32 > low) {
@@ -367,8 +411,7 @@ struct Wave {
 #pragma unroll
         for (int e = 1; e < KB * 16; e++)
             top = fmaxf(top, x[e]);
-        if (MASK == 0)
-            top *= c;
+        top *= unit;
         if (__any(top > m + SLACK)) {
             const float to = fmaxf(m, other_half(top, true));
             const float shrink = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - to);
@@ -387,7 +430,7 @@ struct Wave {
             float p[2];
 #pragma unroll
             for (int i = 0; i < 2; i++)
-                p[i] = __builtin_amdgcn_exp2f(MASK != 0 ? x[e + i] - ref : __builtin_fmaf(x[e + i], c, -ref));
+                p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e + i], unit, -ref));
             w[e >> 1] = Hf::pack(p[0], p[1]);
             l = Hf::add(w[e >> 1], l);
         }
@@ -465,15 +508,15 @@ __device__ __forceinline__ void carefully(const Args &a, const Job &j, int first
 #pragma unroll 1
                 for (int d = 0; d < a.D; d++)
                     s = __builtin_fmaf(Hf::number(((const GLOBAL uint16_t *)q)[d]), Hf::number(((const GLOBAL uint16_t *)kp)[d]), s);
+                x = s * c;
                 if constexpr (MASK != 0) {
-                    Wave<TYPE, DP, MASK> w;
-                    w.c = c;
-                    w.mask = a.mask + (j.b * a.m_sb + head * a.m_sh + (long)t * a.m_st) * (a.mask_dt == 0 ? 4 : a.mask_dt == 3 ? 1 : 2);
-                    float add[4];
-                    w.added(a, key, 1, add);
-                    x = w.with(s, add[0]);
-                } else {
-                    x = s * c;
+                    const GLOBAL char *mp = (const GLOBAL char *)(a.mask + (j.b * a.m_sb + head * a.m_sh + (long)t * a.m_st + key) * MASK);
+                    if constexpr (MASK == 1)
+                        x = *mp ? x : -INFINITY;
+                    else if constexpr (MASK == 4)
+                        x = with(s, *(const GLOBAL float *)mp, c);
+                    else
+                        x = with(s, a.mask_dt == BF16 ? Half<BF16>::number(*(const GLOBAL uint16_t *)mp) : Half<F16>::number(*(const GLOBAL uint16_t *)mp), c);
                 }
             }
             const uint64_t seen = __ballot(!(x == -INFINITY));
@@ -575,15 +618,19 @@ __global__ __launch_bounds__(NT, DP > 128 ? 1 : 2) void many_kernel(const Args a
         fetch<DP>(to, rows_from(kp, a.k.st, k, j.end - k, a.D), a.k.st, wave * 16, 16, lane, a.D);
         fetch<DP>(to + BYTES, rows_from(vp, a.v.st, k, j.end - k, a.D), a.v.st, wave * 16, 16, lane, a.D);
     };
+    Mask<MASK ? MASK : 1, 2> masked;
     if (j.end > 0)
         load(0, lds);
     int buffer = 0;
     for (int k = 0; k < j.end; k += TILE) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); // the tile is there, and nobody reads the one before it any more
+        // in front of the next tile's loads, which are waited for with whatever comes behind them
+        if (MASK != 0 && k < w.high)
+            masked.load(a, w.mask, k, lane);
         if (k + TILE < j.end)
             load(k + TILE, lds + (buffer ^ 1) * 2 * BYTES);
         if (k < w.high)
-            w.template tile<2>(a, lds + buffer * 2 * BYTES, lds + buffer * 2 * BYTES + BYTES, k);
+            w.template tile<2>(a, lds + buffer * 2 * BYTES, lds + buffer * 2 * BYTES + BYTES, k, masked);
         buffer ^= 1;
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); // the tiles' place is free
@@ -619,10 +666,13 @@ __global__ __launch_bounds__(NT, 1) void few_kernel(const Args a)
         fetch<DP>(to, rows_from(kp, a.k.st, k, j.end - k, a.D), a.k.st, 0, TILE, lane, a.D);
         fetch<DP>(to + BYTES, rows_from(vp, a.v.st, k, j.end - k, a.D), a.v.st, 0, TILE, lane, a.D);
     };
+    Mask<MASK ? MASK : 1, 1> masked;
     if (k0 < k1)
         load(k0, own);
     int stage = 0;
     for (int k = k0; k < k1; k += TILE) {
+        if (MASK != 0)
+            masked.load(a, w.mask, k, lane);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // what was read of the tile that is overwritten now
         if (STAGES > 1 && k + TILE < k1) {
             load(k + TILE, own + (stage ^ 1) * 2 * BYTES);
@@ -633,7 +683,7 @@ __global__ __launch_bounds__(NT, 1) void few_kernel(const Args a)
         } else {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
-        w.template tile<1>(a, own + stage * 2 * BYTES, own + stage * 2 * BYTES + BYTES, k);
+        w.template tile<1>(a, own + stage * 2 * BYTES, own + stage * 2 * BYTES + BYTES, k, masked);
         if (STAGES > 1) {
             stage ^= 1;
         } else if (k + TILE < k1) {
@@ -698,9 +748,10 @@ static Plan plan(int B, int Hq, int H, int Tq, int Tk, int n_seq)
     p.pieces = 1;
     p.together = p.units;
     if (p.many) {
-        // as many units at a time as fill the device twice, so that their blocks find their keys in the XCDs' caches
-        const int64_t fill = (4ll * cus + p.blocks - 1) / p.blocks;
-        p.together = (int)std::min<int64_t>(p.units, (fill + 7) / 8 * 8);
+        // Many blocks: as many units at a time as fill the device once, so that their blocks find their keys in the XCDs' caches (128 sequences of 512
+        // tokens, 32 heads: 653 us; with eight units at a time 737, with all of them 807).  Else all of them, the longest first everywhere.
+        if ((int64_t)p.units * p.blocks > 8ll * cus)
+            p.together = (int)std::min<int64_t>(p.units, (cus / p.blocks + 8) / 8 * 8);
     } else {
         const int64_t wide = (int64_t)p.units * p.blocks, tiles = (Tk + 31) / 32;
         p.pieces = (int)std::max<int64_t>(1, std::min<int64_t>(cus / wide, tiles / (2 * WAVES)));
@@ -784,6 +835,9 @@ extern "C" int adkv_prompt_attention(const void *q, const int64_t *q_strides, co
         a.m_sb = mask_strides[0];
         a.m_sh = mask_strides[1];
         a.m_st = mask_strides[2];
+        if (a.m_sb < 0 || a.m_sh < 0 || a.m_st < 0)
+            return ADKV_E_SHAPE;
+        a.mask_end = a.mask + ((B - 1) * a.m_sb + (Hq - 1) * a.m_sh + (Tq - 1) * a.m_st + Tk) * size;
     }
     a.bounds = n_seq ? bounds : nullptr;
     a.partial = (float *)workspace;
@@ -803,8 +857,13 @@ extern "C" int adkv_prompt_attention(const void *q, const int64_t *q_strides, co
     a.together = p.together;
     a.scaling = scaling;
     a.by_g = (uint32_t)(((1ull << 32) + a.g - 1) / a.g);
-    const auto kernel = p.many ? (type == F16 ? (mask ? many_of<F16, 1>(D) : many_of<F16, 0>(D)) : (mask ? many_of<BF16, 1>(D) : many_of<BF16, 0>(D)))
-                               : (type == F16 ? (mask ? few_of<F16, 1>(D) : few_of<F16, 0>(D)) : (mask ? few_of<BF16, 1>(D) : few_of<BF16, 0>(D)));
+    const int masked = !mask ? 0 : size;
+    const auto of = [&](auto type_) {
+        constexpr int TYPE = decltype(type_)::value;
+        return p.many ? (masked == 0 ? many_of<TYPE, 0>(D) : masked == 1 ? many_of<TYPE, 1>(D) : masked == 2 ? many_of<TYPE, 2>(D) : many_of<TYPE, 4>(D))
+                      : (masked == 0 ? few_of<TYPE, 0>(D) : masked == 1 ? few_of<TYPE, 1>(D) : masked == 2 ? few_of<TYPE, 2>(D) : few_of<TYPE, 4>(D));
+    };
+    const auto kernel = type == F16 ? of(std::integral_constant<int, F16>{}) : of(std::integral_constant<int, BF16>{});
     hipLaunchKernelGGL(kernel, dim3((unsigned)((int64_t)p.blocks * p.units * p.pieces)), dim3(NT), 0, (hipStream_t)stream, a);
     if (int rc = check_launch())
         return rc;
