@@ -144,7 +144,7 @@ __device__ __forceinline__ void fetch(uint32_t lds, rsrc4 buffer, int st, int fi
     for (int i = 0; i < n; i += EACH) {
         const int row = first + i + r, piece = c ^ turn<DP>(row);
         const uint32_t at = piece * 8 < D ? (uint32_t)(row * st + piece * 16) : 0x7FFFFFF0u;
-        load_to_lds(lds + (uint32_t)(first + i) * (DP * 2), at, buffer);
+        load_to_lds(__builtin_amdgcn_readfirstlane(lds + (uint32_t)(first + i) * (DP * 2)), at, buffer);
     }
 }
 
@@ -328,10 +328,18 @@ struct Wave {
     const char *mask;
     float c;
     int lane;
+    uint32_t key_at[STEPS], value_at[STEPS]; // in a tile: of key lane % 32, and of the four tokens and channels of a transposing read
 
     __device__ __forceinline__ void open(const Args &a, const Job &j, int first, int lane_)
     {
         lane = lane_;
+        const int r32 = lane & 31, half = lane >> 5, i16 = lane & 15;
+#pragma unroll
+        for (int i = 0; i < STEPS; i++) {
+            key_at[i] = r32 * (DP * 2) + ((2 * i + half) ^ turn<DP>(r32)) * 16;
+            const int of = 8 * (i & 1) + 4 * half + (i16 >> 2), piece = (i >> 1) * 4 + (lane >> 4 & 1) * 2 + (i16 >> 1 & 1);
+            value_at[i] = of * (DP * 2) + (piece ^ turn<DP>(of)) * 16 + (i16 & 1) * 8;
+        }
         row = first + (lane & 31);
         const int r = min(row, j.rows - 1), t = token(a, r), head = j.h * a.g + r - t * a.g;
         limit = j.m - j.n + t + 1;
@@ -364,48 +372,30 @@ struct Wave {
             mask = a.mask + (j.b * a.m_sb + head * a.m_sh + (long)t * a.m_st) * MASK;
     }
 
-    // KB * 32 keys from k on, keys and values in the LDS
-    template <int KB>
-    __device__ __forceinline__ void tile(const Args &a, uint32_t keys, uint32_t values, int k, Mask<MASK ? MASK : 1, KB> &masked)
+    // q . k of KB * 32 keys in the LDS
+    template <int KB> __device__ __forceinline__ void scores(uint32_t keys, f16v *sc) const
     {
-        const int all = MASK != 0 ? masked.alike(a.mask_dt) : 1;
-        if (MASK != 0 && all < 0)
-            return; // nothing to look at
-        const int r32 = lane & 31, h = lane >> 5, i16 = lane & 15;
-        f16v sc[KB];
 #pragma unroll
-        for (int kb = 0; kb < KB; kb++) {
+        for (int kb = 0; kb < KB; kb++)
 #pragma unroll
             for (int e = 0; e < 16; e++)
                 sc[kb][e] = 0.0f;
 #pragma unroll
-            for (int s = 0; s < STEPS; s++) {
-                const uint32_t at = keys + (kb * 32 + r32) * (DP * 2) + ((2 * s + h) ^ turn<DP>(r32)) * 16;
-                const u4v key = *shared<u4v>(at);
-                sc[kb] = Hf::mfma(key, q[s], sc[kb]);
-            }
-        }
-        float x[KB * 16];
+        for (int s = 0; s < STEPS; s++)
 #pragma unroll
-        for (int e = 0; e < KB * 16; e++)
-            x[e] = sc[e >> 4][e & 15];
-        float unit = c; // of x; with something added they are in powers of two
-        if constexpr (MASK != 0) {
-            if (all == 0) {
-                masked.exchange();
-                if (MASK != 1)
-                    unit = 1.0f;
-                adkv::static_for<KB * 16>([&](auto i) {
-                    constexpr int E = decltype(i)::value;
-                    const float y = masked.template of<E>(a.mask_dt);
-                    x[E] = MASK == 1 ? (y != 0.0f ? x[E] : -INFINITY) : with(x[E], y, c);
-                });
-            }
-        }
+            for (int kb = 0; kb < KB; kb++)
+                sc[kb] = Hf::mfma(*shared<u4v>(key_at[s] + keys + kb * 32 * (DP * 2)), q[s], sc[kb]);
+    }
+
+    // What keys k.. are hidden behind a row's own, and the row's reference, which goes along with its sum and outputs; unit: of the scores x
+    template <int KB> __device__ __forceinline__ void settle(float *x, int k, float unit)
+    {
         if (k + KB * 32 > low) {
+            int left = limit - k - 4 * (lane >> 5);
+            asm volatile("" : "+v"(left)); // a branch, not two operations more for every score of every tile
 #pragma unroll
             for (int e = 0; e < KB * 16; e++)
-                x[e] = k + (e >> 2) * 8 + 4 * h + (e & 3) < limit ? x[e] : -INFINITY;
+                x[e] = (e >> 2) * 8 + (e & 3) < left ? x[e] : -INFINITY;
         }
         float top = x[0];
 #pragma unroll
@@ -423,17 +413,20 @@ struct Wave {
                 for (int e = 0; e < 16; e++)
                     o[cb][e] *= shrink;
         }
+    }
+
+    template <int KB> __device__ __forceinline__ void weights(const float *x, float unit, uint32_t *w)
+    {
         const float ref = m == -INFINITY ? 0.0f : m - Hf::BIAS; // nothing yet: all weights are zero
-        uint32_t w[KB * 8];
 #pragma unroll
         for (int e = 0; e < KB * 16; e += 2) {
-            float p[2];
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-                p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e + i], unit, -ref));
-            w[e >> 1] = Hf::pack(p[0], p[1]);
+            w[e >> 1] = Hf::pack(__builtin_amdgcn_exp2f(__builtin_fmaf(x[e], unit, -ref)), __builtin_amdgcn_exp2f(__builtin_fmaf(x[e + 1], unit, -ref)));
             l = Hf::add(w[e >> 1], l);
         }
+    }
+
+    template <int KB> __device__ __forceinline__ void outputs(uint32_t values, const uint32_t *w)
+    {
 #pragma unroll
         for (int kk = 0; kk < KB * 2; kk++) {
             const u4v p = {w[kk * 4], w[kk * 4 + 1], w[kk * 4 + 2], w[kk * 4 + 3]};
@@ -441,14 +434,57 @@ struct Wave {
             for (int cb = 0; cb < CB; cb++) {
                 u2v half[2];
 #pragma unroll
-                for (int d = 0; d < 2; d++) {
-                    const int key = kk * 16 + 8 * d + 4 * h + (i16 >> 2), piece = cb * 4 + (lane >> 4 & 1) * 2 + (i16 >> 1 & 1);
-                    const uint32_t at = values + key * (DP * 2) + (piece ^ turn<DP>(key)) * 16 + (i16 & 1) * 8;
-                    half[d] = __builtin_bit_cast(u2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16(shared<s4v>(at)));
-                }
+                for (int d = 0; d < 2; d++)
+                    half[d] = __builtin_bit_cast(u2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16(shared<s4v>(value_at[cb * 2 + d] + values + kk * 16 * (DP * 2))));
                 o[cb] = Hf::mfma((u4v){half[0].x, half[0].y, half[1].x, half[1].y}, p, o[cb]);
             }
         }
+    }
+
+    // KB * 32 keys from k on, keys and values in the LDS
+    template <int KB>
+    __device__ __forceinline__ void tile(const Args &a, uint32_t keys, uint32_t values, int k, Mask<MASK ? MASK : 1, KB> &masked)
+    {
+        const int all = MASK != 0 ? masked.alike(a.mask_dt) : 1;
+        if (MASK != 0 && all < 0)
+            return; // nothing to look at
+        f16v sc[KB];
+        scores<KB>(keys, sc);
+        float x[KB * 16];
+#pragma unroll
+        for (int e = 0; e < KB * 16; e++)
+            x[e] = sc[e >> 4][e & 15];
+        float unit = c; // of x; with something added they are in powers of two
+        if constexpr (MASK != 0) {
+            if (all == 0) {
+                masked.exchange();
+                if (MASK != 1)
+                    unit = 1.0f;
+                adkv::static_for<KB * 16>([&](auto i) {
+                    constexpr int E = decltype(i)::value;
+                    const float y = masked.template of<E>(a.mask_dt);
+                    x[E] = MASK == 1 ? (y != 0.0f ? x[E] : -INFINITY) : with(x[E], y, c);
+                });
+            }
+        }
+        settle<KB>(x, k, unit);
+        uint32_t w[KB * 8];
+        weights<KB>(x, unit, w);
+        outputs<KB>(values, w);
+    }
+
+    // 32 keys whose scores are there already, beside the scores of the next 32, which are put into `next`
+    __device__ __forceinline__ void beside(const f16v *sc, f16v *next, uint32_t values, int k, uint32_t next_keys)
+    {
+        float x[16];
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+            x[e] = sc[0][e];
+        settle<1>(x, k, c);
+        scores<1>(next_keys, next);
+        uint32_t w[8];
+        weights<1>(x, c, w);
+        outputs<1>(values, w);
     }
 
     __device__ __forceinline__ bool strange() const
@@ -614,24 +650,64 @@ __global__ __launch_bounds__(NT, DP > 128 ? 1 : 2) void many_kernel(const Args a
     Wave<TYPE, DP, MASK> w;
     w.open(a, j, first, lane);
     const char *kp = a.k.p + j.b * a.k.sb + j.h * a.k.sh + (long)j.k0 * a.k.st, *vp = a.v.p + j.b * a.v.sb + j.h * a.v.sh + (long)j.k0 * a.v.st;
-    auto load = [&](int k, uint32_t to) __attribute__((always_inline)) {
-        fetch<DP>(to, rows_from(kp, a.k.st, k, j.end - k, a.D), a.k.st, wave * 16, 16, lane, a.D);
-        fetch<DP>(to + BYTES, rows_from(vp, a.v.st, k, j.end - k, a.D), a.v.st, wave * 16, 16, lane, a.D);
-    };
-    Mask<MASK ? MASK : 1, 2> masked;
-    if (j.end > 0)
-        load(0, lds);
-    int buffer = 0;
-    for (int k = 0; k < j.end; k += TILE) {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); // the tile is there, and nobody reads the one before it any more
-        // in front of the next tile's loads, which are waited for with whatever comes behind them
-        if (MASK != 0 && k < w.high)
-            masked.load(a, w.mask, k, lane);
-        if (k + TILE < j.end)
-            load(k + TILE, lds + (buffer ^ 1) * 2 * BYTES);
-        if (k < w.high)
-            w.template tile<2>(a, lds + buffer * 2 * BYTES, lds + buffer * 2 * BYTES + BYTES, k, masked);
-        buffer ^= 1;
+    if constexpr (MASK == 0) {
+        // The weights of 32 keys are made beside the products of the next 32 keys' scores, so that keys are half a tile ahead of the values: tile k / 64
+        // of them in the LDS begins with key k + 32.  (16384 tokens, 32 heads of 128: 2.05 ms instead of the 2.21 of a tile's scores, weights and
+        // outputs one after the other, 1.07 PFLOP/s; with all of it zeros 1.7: what is left is the clock that the matrix cores' power allows.)
+        const auto keys = [&](int k) __attribute__((always_inline)) {
+            fetch<DP>(lds + (k / TILE & 1) * BYTES, rows_from(kp, a.k.st, k + 32, j.end - k - 32, a.D), a.k.st, wave * 16, 16, lane, a.D);
+        };
+        const auto values = [&](int k) __attribute__((always_inline)) {
+            fetch<DP>(lds + (2 + (k / TILE & 1)) * BYTES, rows_from(vp, a.v.st, k, j.end - k, a.D), a.v.st, wave * 16, 16, lane, a.D);
+        };
+        f16v even[1], odd[1];
+        if (j.end > 0) {
+            // the first 32, where the second tile of keys will be
+            if (wave < 2)
+                fetch<DP>(lds + BYTES, rows_from(kp, a.k.st, 0, j.end, a.D), a.k.st, wave * 16, 16, lane, a.D);
+            asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+            values(0);
+            keys(0);
+            if (w.high > 0)
+                w.template scores<1>(lds + BYTES, even);
+        }
+        const auto step = [&](int k, auto parity) __attribute__((always_inline)) {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); // this tile is there, and nobody reads the one in front of it
+            if (k + TILE < j.end) {
+                values(k + TILE);
+                keys(k + TILE);
+            }
+            if (k < w.high) { // behind the last of its keys a wave makes scores that nobody looks at
+                constexpr uint32_t NEXT = decltype(parity)::value * BYTES, V = NEXT + 2 * BYTES, HALF = BYTES / 2;
+                w.beside(even, odd, lds + V, k, lds + NEXT);
+                w.beside(odd, even, lds + V + HALF, k + 32, lds + NEXT + HALF);
+            }
+        };
+        for (int k = 0; k < j.end; k += 2 * TILE) { // where the LDS is read is part of the instructions
+            step(k, std::integral_constant<int, 0>{});
+            if (k + TILE < j.end)
+                step(k + TILE, std::integral_constant<int, 1>{});
+        }
+    } else {
+        auto load = [&](int k, uint32_t to) __attribute__((always_inline)) {
+            fetch<DP>(to, rows_from(kp, a.k.st, k, j.end - k, a.D), a.k.st, wave * 16, 16, lane, a.D);
+            fetch<DP>(to + BYTES, rows_from(vp, a.v.st, k, j.end - k, a.D), a.v.st, wave * 16, 16, lane, a.D);
+        };
+        Mask<MASK ? MASK : 1, 2> masked;
+        if (j.end > 0)
+            load(0, lds);
+        int buffer = 0;
+        for (int k = 0; k < j.end; k += TILE) {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); // the tile is there, and nobody reads the one before it any more
+            // in front of the next tile's loads, which are waited for with whatever comes behind them
+            if (k < w.high)
+                masked.load(a, w.mask, k, lane);
+            if (k + TILE < j.end)
+                load(k + TILE, lds + (buffer ^ 1) * 2 * BYTES);
+            if (k < w.high)
+                w.template tile<2>(a, lds + buffer * 2 * BYTES, lds + buffer * 2 * BYTES + BYTES, k, masked);
+            buffer ^= 1;
+        }
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); // the tiles' place is free
     const uint32_t mine = lds + wave * result_bytes(DP);
@@ -663,8 +739,11 @@ __global__ __launch_bounds__(NT, 1) void few_kernel(const Args a)
     const char *kp = a.k.p + j.b * a.k.sb + j.h * a.k.sh + (long)j.k0 * a.k.st, *vp = a.v.p + j.b * a.v.sb + j.h * a.v.sh + (long)j.k0 * a.v.st;
     const uint32_t own = lds + wave * (STAGES * 2 * BYTES);
     auto load = [&](int k, uint32_t to) __attribute__((always_inline)) {
-        fetch<DP>(to, rows_from(kp, a.k.st, k, j.end - k, a.D), a.k.st, 0, TILE, lane, a.D);
-        fetch<DP>(to + BYTES, rows_from(vp, a.v.st, k, j.end - k, a.D), a.v.st, 0, TILE, lane, a.D);
+        int l = lane;
+        if (DP > 128 && MASK != 0)
+            asm volatile("" : "+v"(l)); // 32 addresses in a tile are made again for every tile: there is no room to keep them
+        fetch<DP>(to, rows_from(kp, a.k.st, k, j.end - k, a.D), a.k.st, 0, TILE, l, a.D);
+        fetch<DP>(to + BYTES, rows_from(vp, a.v.st, k, j.end - k, a.D), a.v.st, 0, TILE, l, a.D);
     };
     Mask<MASK ? MASK : 1, 1> masked;
     if (k0 < k1)
