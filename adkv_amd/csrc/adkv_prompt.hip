@@ -170,16 +170,20 @@ __device__ __forceinline__ int bound(const Args &a, int i) // of the sequences, 
 template <int EACH>
 __device__ __forceinline__ bool find(const Args &a, int block, int lane, Job &j)
 {
-    int lo = 0, hi = a.n_seq + 2; // the last i whose place is not behind `block`
-    while (hi - lo > 1) {
-        const int step = (hi - lo + 63) / 64, at = lo + lane * step;
-        const bool before = at < hi && (int)((int64_t)bound(a, at) * a.g / EACH) + at <= block;
+    int lo = 0, hi = a.n_seq + 2, x, y; // the last i whose place is not behind `block`
+    while (true) {
+        const int step = (hi - lo + 62) / 63, at = lo + lane * step, here = bound(a, at);
+        const bool before = lane < 63 && at < hi && (int)((int64_t)here * a.g / EACH) + at <= block;
         const uint64_t which = __ballot(before);
         const int last = which ? 63 - __builtin_clzll(which) : 0;
         lo += last * step;
         hi = min(hi, lo + step);
+        if (step == 1) { // the one behind it is on the next lane
+            x = __builtin_amdgcn_readlane(here, last);
+            y = __builtin_amdgcn_readlane(here, last + 1);
+            break;
+        }
     }
-    const int x = bound(a, lo), y = bound(a, lo + 1);
     j.n = j.m = max(y - x, 0);
     j.q0 = j.k0 = x;
     j.rows = j.n * a.g;
@@ -348,18 +352,19 @@ struct Wave {
         low = __builtin_amdgcn_readfirstlane(low);
         high = __builtin_amdgcn_readfirstlane(high);
         const char *src = a.q.p + j.b * a.q.sb + head * a.q.sh + (long)(j.q0 + t) * a.q.st;
-        const uint32_t sign = a.scaling < 0.0f ? 0x80008000u : 0u;
 #pragma unroll
         for (int s = 0; s < STEPS; s++) {
-            const int piece = 2 * s + (lane >> 5);
-            u4v u = {0, 0, 0, 0};
-            if (piece * 8 < a.D)
-                u = *(const GLOBAL u4v *)(src + piece * 16);
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                u[e] ^= sign;
-            q[s] = u;
+            const int piece = min(2 * s + half, a.D / 8 - 1); // channels behind the last are zeros in the keys
+            q[s] = *(const GLOBAL u4v *)(src + piece * 16);
         }
+        // here and for all: else the first use inside a loop waits, and for the tiles that are on their way there (vmcnt 0)
+        __builtin_amdgcn_s_waitcnt(0x0F70);
+        if (a.scaling < 0.0f)
+#pragma unroll
+            for (int s = 0; s < STEPS; s++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    q[s][e] ^= 0x80008000u;
         c = fabsf(a.scaling) * LOG2E;
         m = -INFINITY;
         l = 0.0f;
@@ -648,7 +653,6 @@ __global__ __launch_bounds__(NT, DP > 128 ? 1 : 2) void many_kernel(const Args a
         return;
     const int first = j.first + wave * ROWS;
     Wave<TYPE, DP, MASK> w;
-    w.open(a, j, first, lane);
     const char *kp = a.k.p + j.b * a.k.sb + j.h * a.k.sh + (long)j.k0 * a.k.st, *vp = a.v.p + j.b * a.v.sb + j.h * a.v.sh + (long)j.k0 * a.v.st;
     if constexpr (MASK == 0) {
         // The weights of 32 keys are made beside the products of the next 32 keys' scores, so that keys are half a tile ahead of the values: tile k / 64
@@ -665,9 +669,12 @@ __global__ __launch_bounds__(NT, DP > 128 ? 1 : 2) void many_kernel(const Args a
             // the first 32, where the second tile of keys will be
             if (wave < 2)
                 fetch<DP>(lds + BYTES, rows_from(kp, a.k.st, 0, j.end, a.D), a.k.st, wave * 16, 16, lane, a.D);
-            asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
             values(0);
             keys(0);
+        }
+        w.open(a, j, first, lane); // behind the loads of the tiles: all are on their way together
+        if (j.end > 0) {
+            asm volatile("s_barrier" ::: "memory"); // open() has waited
             if (w.high > 0)
                 w.template scores<1>(lds + BYTES, even);
         }
@@ -696,6 +703,7 @@ __global__ __launch_bounds__(NT, DP > 128 ? 1 : 2) void many_kernel(const Args a
         Mask<MASK ? MASK : 1, 2> masked;
         if (j.end > 0)
             load(0, lds);
+        w.open(a, j, first, lane);
         int buffer = 0;
         for (int k = 0; k < j.end; k += TILE) {
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); // the tile is there, and nobody reads the one before it any more
@@ -733,7 +741,6 @@ __global__ __launch_bounds__(NT, 1) void few_kernel(const Args a)
     if (!place<ROWS>(a, blockIdx.x, lane, j))
         return;
     Wave<TYPE, DP, MASK> w;
-    w.open(a, j, j.first, lane);
     const int tiles = (j.end + TILE - 1) / TILE, parts = a.pieces * WAVES, part = j.piece * WAVES + wave;
     const int k0 = (int)((int64_t)tiles * part / parts) * TILE, k1 = min((int)((int64_t)tiles * (part + 1) / parts) * TILE, j.end);
     const char *kp = a.k.p + j.b * a.k.sb + j.h * a.k.sh + (long)j.k0 * a.k.st, *vp = a.v.p + j.b * a.v.sb + j.h * a.v.sh + (long)j.k0 * a.v.st;
@@ -748,6 +755,7 @@ __global__ __launch_bounds__(NT, 1) void few_kernel(const Args a)
     Mask<MASK ? MASK : 1, 1> masked;
     if (k0 < k1)
         load(k0, own);
+    w.open(a, j, j.first, lane);
     int stage = 0;
     for (int k = k0; k < k1; k += TILE) {
         if (MASK != 0)
