@@ -492,15 +492,44 @@ struct Wave {
         outputs<1>(values, w);
     }
 
+    // whether a product's result, or the sum, is infinite or no number
     __device__ __forceinline__ bool strange() const
     {
-        bool nan = l != l;
+        float nothing[4] = {l * 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int cb = 0; cb < CB; cb++)
 #pragma unroll
             for (int e = 0; e < 16; e++)
-                nan |= o[cb][e] != o[cb][e];
-        return __any(nan);
+                nothing[e & 3] = __builtin_fmaf(o[cb][e], 0.0f, nothing[e & 3]);
+        return __any((nothing[0] + nothing[1]) + (nothing[2] + nothing[3]) != 0.0f);
+    }
+
+    // To the output, 16 bytes at a time: two lanes have four channels each of the same eight of a row; an exchange leaves one of them with these and
+    // the other with the next eight.
+    __device__ __forceinline__ void deliver(const Args &a, const Job &j)
+    {
+        const float sum = other_half(l, false), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int t = token(a, row), head = j.h * a.g + row - t * a.g, half = lane >> 5;
+        char *to = a.out + (((long)j.b * a.Tq + j.q0 + t) * (a.H * a.g) + head) * (a.D * 2) + half * 16;
+        if (row >= j.rows)
+            return;
+#pragma unroll
+        for (int cb = 0; cb < CB; cb++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 8) {
+                uint32_t u[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    u[i] = Hf::pack(o[cb][e + 2 * i] * inv, o[cb][e + 2 * i + 1] * inv);
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const u2v r = __builtin_amdgcn_permlane32_swap(u[i], u[2 + i], false, false);
+                    u[i] = r.x;
+                    u[2 + i] = r.y;
+                }
+                if (cb * 32 + e * 2 + half * 8 < a.D)
+                    *(GLOBAL u4v *)(to + (cb * 32 + e * 2) * 2) = (u4v){u[0], u[1], u[2], u[3]};
+            }
     }
 
     // To the LDS: 32 rows of DP sums, in pieces of four at place piece ^ row, then the rows' m and l
@@ -524,7 +553,8 @@ constexpr int result_bytes(int DP) { return ROWS * DP * 4 + ROWS * 8; }
 
 // The same as tile() and leave() for keys k0..k1, a row after the other and without a look at what is hidden: a hidden value that is infinite or not a
 // number meets a weight of zero in a matrix product, and leaves nothing of the row.  Taken where a product's results are no numbers.
-template <int TYPE, int DP, int MASK>
+// WHOLE: all keys, straight to the output
+template <int TYPE, int DP, int MASK, bool WHOLE>
 __device__ __forceinline__ void carefully(const Args &a, const Job &j, int first, int k0, int k1, int lane, uint32_t to)
 {
     using Hf = Half<TYPE>;
@@ -586,6 +616,15 @@ __device__ __forceinline__ void carefully(const Args &a, const Job &j, int first
                         o[n] = __builtin_fmaf(w, Hf::number(((const GLOBAL uint16_t *)vp)[lane * N + n]), o[n]);
             }
         }
+        if (WHOLE) {
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            GLOBAL uint16_t *out = (GLOBAL uint16_t *)a.out + (((long)j.b * a.Tq + j.q0 + t) * (a.H * a.g) + head) * a.D;
+#pragma unroll
+            for (int n = 0; n < N; n++)
+                if (first + i < j.rows && lane * N + n < a.D)
+                    out[lane * N + n] = (uint16_t)Hf::pack(o[n] * inv, 0.0f);
+            continue;
+        }
 #pragma unroll
         for (int n = 0; n < N; n++) {
             const int d = lane * N + n;
@@ -618,7 +657,7 @@ __device__ __forceinline__ void deliver(const Args &a, const Job &j, uint32_t at
 #pragma unroll
         for (int w = 0; w < FROM; w++) {
             const f4v v = *shared<f4v>(at + w * result_bytes(DP) + (i * (DP / 4) + (piece ^ (i & 15))) * 16);
-            const float e = FROM == 1 ? 1.0f : __builtin_amdgcn_exp2f(ml[w].x - ref);
+            const float e = __builtin_amdgcn_exp2f(ml[w].x - ref);
             L = __builtin_fmaf(ml[w].y, e, L);
 #pragma unroll
             for (int k = 0; k < 4; k++)
@@ -639,7 +678,7 @@ __device__ __forceinline__ void deliver(const Args &a, const Job &j, uint32_t at
     }
 }
 
-template <int DP> constexpr int many_lds() { return std::max(2 * 64 * DP * 2 * 2, WAVES * result_bytes(DP)); }
+template <int DP> constexpr int many_lds() { return 2 * 64 * DP * 2 * 2; }
 
 template <int TYPE, int DP, int MASK>
 __global__ __launch_bounds__(NT, DP > 128 ? 1 : 2) void many_kernel(const Args a)
@@ -717,14 +756,11 @@ __global__ __launch_bounds__(NT, DP > 128 ? 1 : 2) void many_kernel(const Args a
             buffer ^= 1;
         }
     }
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); // the tiles' place is free
-    const uint32_t mine = lds + wave * result_bytes(DP);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if (w.strange())
-        carefully<TYPE, DP, MASK>(a, j, first, 0, j.end, lane, mine);
+        carefully<TYPE, DP, MASK, true>(a, j, first, 0, j.end, lane, 0);
     else
-        w.leave(mine);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    deliver<TYPE, DP, 1>(a, j, mine, first, 0, ROWS, lane);
+        w.deliver(a, j);
 }
 
 template <int DP> constexpr int few_stages() { return DP > 128 ? 1 : 2; }
@@ -781,7 +817,7 @@ __global__ __launch_bounds__(NT, 1) void few_kernel(const Args a)
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     const uint32_t mine = lds + wave * result_bytes(DP);
     if (w.strange())
-        carefully<TYPE, DP, MASK>(a, j, j.first, k0, k1, lane, mine);
+        carefully<TYPE, DP, MASK, false>(a, j, j.first, k0, k1, lane, mine);
     else
         w.leave(mine);
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
