@@ -11,8 +11,9 @@
 // operands' type for the matrix cores (fp16: after a factor of 2^7, which keeps 2^7 more of the small ones out of the subnormals); the sum that
 // divides them is that of the rounded ones.  Scores, m, sums and outputs are fp32.
 //
-// Two forms:
+// Three forms:
 //   many  a workgroup is four waves of 32 rows each over shared tiles of 64 keys and values, two tiles in the LDS, a barrier per tile
+//   some  a workgroup is 64 rows, eight waves: each has 32 rows and every fourth 32 keys of them, over shared tiles of 128; joined in the LDS
 //   few   a workgroup is 32 rows, its four waves walk through a quarter of the keys each in tiles of their own and are joined in the LDS; where
 //         that leaves CUs without work the keys are cut into pieces for several workgroups, joined by a second kernel
 #include <math.h>
@@ -126,27 +127,38 @@ template <int DP> __device__ __forceinline__ constexpr int turn(int r)
     return DP == 64 ? (r >> 1 & 1) << 2 | (r >> 2 & 3) : (r & 3) << 2 | (r >> 2 & 3);
 }
 
-// The memory of a row axis from row `first` on, of which `there` rows may be read; what is behind them reads as zeros.
-__device__ __forceinline__ rsrc4 rows_from(const char *p, int st, int first, int there, int D)
-{
-    const uint64_t base = (uint64_t)p + (int64_t)first * st;
-    const int64_t bytes = there > 0 ? (int64_t)(there - 1) * st + D * 2 : 0;
-    return (rsrc4){(uint32_t)base, (uint32_t)(base >> 32) & 0xFFFFu, (uint32_t)(bytes < 0x40000000 ? bytes : 0x40000000), 0x00027000u};
-}
-
-// `n` rows straight to the LDS, 1 KB an instruction: rows first, first + 1.. of a tile, whose row 0 the buffer begins with
+// Rows of keys or values one tile after the other, straight to the LDS, 1 KB an instruction; what is behind the last reads as zeros
 template <int DP>
-__device__ __forceinline__ void fetch(uint32_t lds, rsrc4 buffer, int st, int first, int n, int lane, int D)
-{
-    constexpr int PIECES = DP / 8, EACH = 64 / PIECES;
-    const int r = lane / PIECES, c = lane % PIECES;
-#pragma unroll
-    for (int i = 0; i < n; i += EACH) {
-        const int row = first + i + r, piece = c ^ turn<DP>(row);
-        const uint32_t at = piece * 8 < D ? (uint32_t)(row * st + piece * 16) : 0x7FFFFFF0u;
-        load_to_lds(__builtin_amdgcn_readfirstlane(lds + (uint32_t)(first + i) * (DP * 2)), at, buffer);
+struct Stream {
+    static constexpr int PIECES = DP / 8, EACH = 64 / PIECES; // of a row; rows per instruction
+    uint64_t base;
+    int left, st; // rows
+    // from row `first` of `rows` on
+    __device__ __forceinline__ void open(const char *p, int st_, int first, int rows)
+    {
+        base = (uint64_t)p + (int64_t)first * st_;
+        left = rows - first;
+        st = st_;
     }
-}
+    // N rows, whose first is at a multiple of 16 in its tile, to `lds`
+    template <int N> __device__ __forceinline__ void ask(uint32_t lds, int lane, int D) const
+    {
+        const int bytes = left > 0 ? (min(left, N) - 1) * st + D * 2 : 0;
+        const rsrc4 buffer = {(uint32_t)base, (uint32_t)(base >> 32), (uint32_t)bytes, 0x00027000u};
+        const int r = lane / PIECES, c = lane % PIECES;
+#pragma unroll
+        for (int i = 0; i < N; i += EACH) {
+            const int piece = c ^ turn<DP>(i + r);
+            const uint32_t at = piece * 8 < D ? (uint32_t)((i + r) * st + piece * 16) : 0x7FFFFFF0u;
+            load_to_lds(__builtin_amdgcn_readfirstlane(lds + (uint32_t)i * (DP * 2)), at, buffer);
+        }
+    }
+    __device__ __forceinline__ void skip(int rows)
+    {
+        base += (int64_t)rows * st;
+        left -= rows;
+    }
+};
 
 // Where a workgroup's rows are
 struct Job {
@@ -230,9 +242,10 @@ __device__ __forceinline__ bool place(const Args &a, int i, int lane, Job &j)
 // time, whatever their alignment; an exchange with the other half leaves both with the keys whose scores they have.
 template <int SIZE, int KB>
 struct Mask {
-    static constexpr int WORDS = KB * 4 * SIZE;
-    uint32_t w[WORDS];
-    // row: the lane's; keys k.., of `there` that the mask has
+    static constexpr int WORDS = KB * 4 * SIZE, MORE = SIZE < 4 ? 1 : 0;
+    uint32_t w[WORDS + MORE];
+    uint32_t shift; // bytes in front of the lane's first
+    // row: the lane's; keys k.. Nothing here waits for what is loaded.
     __device__ __forceinline__ void load(const Args &a, const char *row, int k, int lane)
     {
         typedef uint32_t u4a __attribute__((ext_vector_type(4), aligned(4)));
@@ -240,23 +253,22 @@ struct Mask {
         const char *p = row + (long)first * SIZE;
         // rows may begin between two words; loads that do so cost more than the shifts (1023 tokens, 16 bits: 97 us)
         const GLOBAL char *from = (const GLOBAL char *)((uintptr_t)p & ~(uintptr_t)3);
-        constexpr int MORE = SIZE < 4 ? 1 : 0;
         if (__all((const char *)from + (WORDS + MORE) * 4 <= a.mask_end)) {
-            uint32_t u[WORDS + 1];
+            shift = (uint32_t)(uintptr_t)p & 3;
 #pragma unroll
             for (int i = 0; i < WORDS; i += 4) {
                 const u4a four = *(const GLOBAL u4a *)(from + i * 4);
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    u[i + e] = four[e];
+                    w[i + e] = four[e];
             }
             if (MORE)
-                u[WORDS] = *(const GLOBAL uint32_t *)(from + WORDS * 4);
-#pragma unroll
-            for (int i = 0; i < WORDS; i++)
-                w[i] = MORE ? __builtin_amdgcn_alignbyte(u[i + 1], u[i], (uint32_t)(uintptr_t)p & 3) : u[i];
+                w[WORDS] = *(const GLOBAL uint32_t *)(from + WORDS * 4);
             return;
         }
+        shift = 0;
+        if (MORE)
+            w[WORDS] = 0;
 #pragma unroll
         for (int i = 0; i < WORDS; i++) {
             w[i] = 0;
@@ -271,6 +283,13 @@ struct Mask {
                         w[i] |= (uint32_t)*(const GLOBAL uint8_t *)(p + i * 4 + e) << e * 8;
                 }
         }
+    }
+    __device__ __forceinline__ void align()
+    {
+        if (MORE)
+#pragma unroll
+            for (int i = 0; i < WORDS; i++)
+                w[i] = __builtin_amdgcn_alignbyte(w[i + MORE], w[i], shift);
     }
     // what all of the wave's keys have, and any: 1 where nothing is added or hidden, -1 where all of them are hidden
     __device__ __forceinline__ int alike(int dt) const
@@ -357,8 +376,6 @@ struct Wave {
             const int piece = min(2 * s + half, a.D / 8 - 1); // channels behind the last are zeros in the keys
             q[s] = *(const GLOBAL u4v *)(src + piece * 16);
         }
-        // here and for all: else the first use inside a loop waits, and for the tiles that are on their way there (vmcnt 0)
-        __builtin_amdgcn_s_waitcnt(0x0F70);
         if (a.scaling < 0.0f)
 #pragma unroll
             for (int s = 0; s < STEPS; s++)
@@ -450,6 +467,8 @@ struct Wave {
     template <int KB>
     __device__ __forceinline__ void tile(const Args &a, uint32_t keys, uint32_t values, int k, Mask<MASK ? MASK : 1, KB> &masked)
     {
+        if (MASK != 0)
+            masked.align();
         const int all = MASK != 0 ? masked.alike(a.mask_dt) : 1;
         if (MASK != 0 && all < 0)
             return; // nothing to look at
@@ -553,8 +572,8 @@ constexpr int result_bytes(int DP) { return ROWS * DP * 4 + ROWS * 8; }
 
 // The same as tile() and leave() for keys k0..k1, a row after the other and without a look at what is hidden: a hidden value that is infinite or not a
 // number meets a weight of zero in a matrix product, and leaves nothing of the row.  Taken where a product's results are no numbers.
-// WHOLE: all keys, straight to the output
-template <int TYPE, int DP, int MASK, bool WHOLE>
+// WHOLE: all keys, straight to the output; else WIDTH keys of every STEP
+template <int TYPE, int DP, int MASK, bool WHOLE, int WIDTH = 64, int STEP = 64>
 __device__ __forceinline__ void carefully(const Args &a, const Job &j, int first, int k0, int k1, int lane, uint32_t to)
 {
     using Hf = Half<TYPE>;
@@ -570,10 +589,10 @@ __device__ __forceinline__ void carefully(const Args &a, const Job &j, int first
         const int end = min(k1, j.m - j.n + t + 1);
         const char *q = a.q.p + j.b * a.q.sb + head * a.q.sh + (long)(j.q0 + t) * a.q.st;
 #pragma unroll 1
-        for (int k = k0; k < end; k += 64) {
+        for (int k = k0; k < end; k += STEP) {
             const int key = k + lane;
             float x = -INFINITY;
-            if (key < end) {
+            if (lane < WIDTH && key < end) {
                 const char *kp = a.k.p + j.b * a.k.sb + j.h * a.k.sh + (long)(j.k0 + key) * a.k.st;
                 float s = 0.0f;
 #pragma unroll 1
@@ -678,6 +697,10 @@ __device__ __forceinline__ void deliver(const Args &a, const Job &j, uint32_t at
     }
 }
 
+// All that was asked for is there, for the compiler too: what it does not know to be there it waits for at its first use, and with it for all that
+// load_to_lds() has been told since.
+__device__ __forceinline__ void arrive() { __builtin_amdgcn_s_waitcnt(0x0F70); } // vmcnt(0)
+
 template <int DP> constexpr int many_lds() { return 2 * 64 * DP * 2 * 2; }
 
 template <int TYPE, int DP, int MASK>
@@ -685,7 +708,7 @@ __global__ __launch_bounds__(NT, DP > 128 ? 1 : 2) void many_kernel(const Args a
 {
     __shared__ uint4 smem[many_lds<DP>() / 16];
     const uint32_t lds = (uint32_t)(uintptr_t)(LDS char *)(char *)smem;
-    constexpr int TILE = 64, BYTES = TILE * DP * 2;
+    constexpr int TILE = 64, BYTES = TILE * DP * 2, EACH = TILE / WAVES;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     Job j;
     if (!place<WAVES * ROWS>(a, blockIdx.x, lane, j))
@@ -693,38 +716,41 @@ __global__ __launch_bounds__(NT, DP > 128 ? 1 : 2) void many_kernel(const Args a
     const int first = j.first + wave * ROWS;
     Wave<TYPE, DP, MASK> w;
     const char *kp = a.k.p + j.b * a.k.sb + j.h * a.k.sh + (long)j.k0 * a.k.st, *vp = a.v.p + j.b * a.v.sb + j.h * a.v.sh + (long)j.k0 * a.v.st;
+    Stream<DP> keys, values;
+    values.open(vp, a.v.st, wave * EACH, j.end);
+    const uint32_t mine = lds + wave * EACH * DP * 2;
     if constexpr (MASK == 0) {
         // The weights of 32 keys are made beside the products of the next 32 keys' scores, so that keys are half a tile ahead of the values: tile k / 64
         // of them in the LDS begins with key k + 32.  (16384 tokens, 32 heads of 128: 2.05 ms instead of the 2.21 of a tile's scores, weights and
         // outputs one after the other, 1.07 PFLOP/s; with all of it zeros 1.7: what is left is the clock that the matrix cores' power allows.)
-        const auto keys = [&](int k) __attribute__((always_inline)) {
-            fetch<DP>(lds + (k / TILE & 1) * BYTES, rows_from(kp, a.k.st, k + 32, j.end - k - 32, a.D), a.k.st, wave * 16, 16, lane, a.D);
-        };
-        const auto values = [&](int k) __attribute__((always_inline)) {
-            fetch<DP>(lds + (2 + (k / TILE & 1)) * BYTES, rows_from(vp, a.v.st, k, j.end - k, a.D), a.v.st, wave * 16, 16, lane, a.D);
-        };
         f16v even[1], odd[1];
         if (j.end > 0) {
             // the first 32, where the second tile of keys will be
-            if (wave < 2)
-                fetch<DP>(lds + BYTES, rows_from(kp, a.k.st, 0, j.end, a.D), a.k.st, wave * 16, 16, lane, a.D);
-            values(0);
-            keys(0);
+            if (wave < 2) {
+                keys.open(kp, a.k.st, wave * EACH, j.end);
+                keys.template ask<EACH>(mine + BYTES, lane, a.D);
+            }
+            keys.open(kp, a.k.st, 32 + wave * EACH, j.end);
+            keys.template ask<EACH>(mine, lane, a.D);
+            values.template ask<EACH>(mine + 2 * BYTES, lane, a.D);
         }
         w.open(a, j, first, lane); // behind the loads of the tiles: all are on their way together
+        arrive();
         if (j.end > 0) {
-            asm volatile("s_barrier" ::: "memory"); // open() has waited
+            asm volatile("s_barrier" ::: "memory");
             if (w.high > 0)
                 w.template scores<1>(lds + BYTES, even);
         }
         const auto step = [&](int k, auto parity) __attribute__((always_inline)) {
+            constexpr uint32_t NEXT = decltype(parity)::value * BYTES, OTHER = BYTES - NEXT, V = NEXT + 2 * BYTES, HALF = BYTES / 2;
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); // this tile is there, and nobody reads the one in front of it
             if (k + TILE < j.end) {
-                values(k + TILE);
-                keys(k + TILE);
+                keys.skip(TILE);
+                values.skip(TILE);
+                keys.template ask<EACH>(mine + OTHER, lane, a.D);
+                values.template ask<EACH>(mine + OTHER + 2 * BYTES, lane, a.D);
             }
             if (k < w.high) { // behind the last of its keys a wave makes scores that nobody looks at
-                constexpr uint32_t NEXT = decltype(parity)::value * BYTES, V = NEXT + 2 * BYTES, HALF = BYTES / 2;
                 w.beside(even, odd, lds + V, k, lds + NEXT);
                 w.beside(odd, even, lds + V + HALF, k + 32, lds + NEXT + HALF);
             }
@@ -735,32 +761,97 @@ __global__ __launch_bounds__(NT, DP > 128 ? 1 : 2) void many_kernel(const Args a
                 step(k + TILE, std::integral_constant<int, 1>{});
         }
     } else {
-        auto load = [&](int k, uint32_t to) __attribute__((always_inline)) {
-            fetch<DP>(to, rows_from(kp, a.k.st, k, j.end - k, a.D), a.k.st, wave * 16, 16, lane, a.D);
-            fetch<DP>(to + BYTES, rows_from(vp, a.v.st, k, j.end - k, a.D), a.v.st, wave * 16, 16, lane, a.D);
-        };
-        Mask<MASK ? MASK : 1, 2> masked;
-        if (j.end > 0)
-            load(0, lds);
+        Mask<MASK ? MASK : 1, 2> masked, next;
+        keys.open(kp, a.k.st, wave * EACH, j.end);
+        if (j.end > 0) {
+            keys.template ask<EACH>(mine, lane, a.D);
+            values.template ask<EACH>(mine + BYTES, lane, a.D);
+        }
         w.open(a, j, first, lane);
+        if (0 < w.high)
+            next.load(a, w.mask, 0, lane);
         int buffer = 0;
         for (int k = 0; k < j.end; k += TILE) {
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); // the tile is there, and nobody reads the one before it any more
-            // in front of the next tile's loads, which are waited for with whatever comes behind them
-            if (k < w.high)
-                masked.load(a, w.mask, k, lane);
-            if (k + TILE < j.end)
-                load(k + TILE, lds + (buffer ^ 1) * 2 * BYTES);
+            arrive();
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); // the tile is there, and nobody reads the one before it any more
+            masked = next;
+            if (k + TILE < w.high)
+                next.load(a, w.mask, k + TILE, lane);
+            if (k + TILE < j.end) {
+                keys.skip(TILE);
+                values.skip(TILE);
+                keys.template ask<EACH>(mine + (buffer ^ 1) * 2 * BYTES, lane, a.D);
+                values.template ask<EACH>(mine + (buffer ^ 1) * 2 * BYTES + BYTES, lane, a.D);
+            }
             if (k < w.high)
                 w.template tile<2>(a, lds + buffer * 2 * BYTES, lds + buffer * 2 * BYTES + BYTES, k, masked);
             buffer ^= 1;
         }
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    arrive();
     if (w.strange())
         carefully<TYPE, DP, MASK, true>(a, j, first, 0, j.end, lane, 0);
     else
         w.deliver(a, j);
+}
+
+constexpr int PARTS = 4; // of the keys
+template <int DP> constexpr int some_lds() { return std::max(2 * PARTS * 32 * DP * 2 * 2, 2 * PARTS * result_bytes(DP)); }
+
+template <int TYPE, int DP, int MASK>
+__global__ __launch_bounds__(2 * NT, 1) void some_kernel(const Args a)
+{
+    __shared__ uint4 smem[some_lds<DP>() / 16];
+    const uint32_t lds = (uint32_t)(uintptr_t)(LDS char *)(char *)smem;
+    constexpr int TILE = PARTS * 32, BYTES = TILE * DP * 2, EACH = 16;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), part = wave % PARTS, rows = wave / PARTS;
+    Job j;
+    if (!place<2 * ROWS>(a, blockIdx.x, lane, j))
+        return;
+    const int first = j.first + rows * ROWS;
+    Wave<TYPE, DP, MASK> w;
+    Stream<DP> keys, values;
+    keys.open(a.k.p + j.b * a.k.sb + j.h * a.k.sh + (long)j.k0 * a.k.st, a.k.st, wave * EACH, j.end);
+    values.open(a.v.p + j.b * a.v.sb + j.h * a.v.sh + (long)j.k0 * a.v.st, a.v.st, wave * EACH, j.end);
+    const uint32_t mine = lds + wave * EACH * DP * 2;
+    Mask<MASK ? MASK : 1, 1> masked, next;
+    if (j.end > 0) {
+        keys.template ask<EACH>(mine, lane, a.D);
+        values.template ask<EACH>(mine + BYTES, lane, a.D);
+    }
+    w.open(a, j, first, lane);
+    if (MASK != 0 && part * 32 < w.high)
+        next.load(a, w.mask, part * 32, lane);
+    int buffer = 0;
+    for (int k = part * 32; k - part * 32 < j.end; k += TILE) {
+        arrive();
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); // the tile is there, and nobody reads the one before it any more
+        if (MASK != 0) {
+            masked = next;
+            if (k + TILE < w.high)
+                next.load(a, w.mask, k + TILE, lane);
+        }
+        if (k - part * 32 + TILE < j.end) {
+            keys.skip(TILE);
+            values.skip(TILE);
+            keys.template ask<EACH>(mine + (buffer ^ 1) * 2 * BYTES, lane, a.D);
+            values.template ask<EACH>(mine + (buffer ^ 1) * 2 * BYTES + BYTES, lane, a.D);
+        }
+        if (k < w.high) {
+            const uint32_t at = lds + buffer * 2 * BYTES + part * 32 * DP * 2;
+            w.template tile<1>(a, at, at + BYTES, k, masked);
+        }
+        buffer ^= 1;
+    }
+    arrive();
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); // the tiles' place is free
+    const uint32_t result = lds + wave * result_bytes(DP);
+    if (w.strange())
+        carefully<TYPE, DP, MASK, false, 32, TILE>(a, j, first, part * 32, j.end, lane, result);
+    else
+        w.leave(result);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    deliver<TYPE, DP, PARTS>(a, j, lds + rows * PARTS * result_bytes(DP), first, part * (ROWS / PARTS), ROWS / PARTS, lane);
 }
 
 template <int DP> constexpr int few_stages() { return DP > 128 ? 1 : 2; }
@@ -779,42 +870,46 @@ __global__ __launch_bounds__(NT, 1) void few_kernel(const Args a)
     Wave<TYPE, DP, MASK> w;
     const int tiles = (j.end + TILE - 1) / TILE, parts = a.pieces * WAVES, part = j.piece * WAVES + wave;
     const int k0 = (int)((int64_t)tiles * part / parts) * TILE, k1 = min((int)((int64_t)tiles * (part + 1) / parts) * TILE, j.end);
-    const char *kp = a.k.p + j.b * a.k.sb + j.h * a.k.sh + (long)j.k0 * a.k.st, *vp = a.v.p + j.b * a.v.sb + j.h * a.v.sh + (long)j.k0 * a.v.st;
+    Stream<DP> keys, values;
+    keys.open(a.k.p + j.b * a.k.sb + j.h * a.k.sh + (long)j.k0 * a.k.st, a.k.st, k0, j.end);
+    values.open(a.v.p + j.b * a.v.sb + j.h * a.v.sh + (long)j.k0 * a.v.st, a.v.st, k0, j.end);
     const uint32_t own = lds + wave * (STAGES * 2 * BYTES);
-    auto load = [&](int k, uint32_t to) __attribute__((always_inline)) {
+    const auto ask = [&](uint32_t to) __attribute__((always_inline)) {
         int l = lane;
         if (DP > 128 && MASK != 0)
             asm volatile("" : "+v"(l)); // 32 addresses in a tile are made again for every tile: there is no room to keep them
-        fetch<DP>(to, rows_from(kp, a.k.st, k, j.end - k, a.D), a.k.st, 0, TILE, l, a.D);
-        fetch<DP>(to + BYTES, rows_from(vp, a.v.st, k, j.end - k, a.D), a.v.st, 0, TILE, l, a.D);
+        keys.template ask<TILE>(to, l, a.D);
+        values.template ask<TILE>(to + BYTES, l, a.D);
+        keys.skip(TILE);
+        values.skip(TILE);
     };
-    Mask<MASK ? MASK : 1, 1> masked;
+    Mask<MASK ? MASK : 1, 1> masked, next;
     if (k0 < k1)
-        load(k0, own);
+        ask(own);
     w.open(a, j, j.first, lane);
+    if (MASK != 0 && k0 < k1)
+        next.load(a, w.mask, k0, lane);
     int stage = 0;
     for (int k = k0; k < k1; k += TILE) {
-        if (MASK != 0)
-            masked.load(a, w.mask, k, lane);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // what was read of the tile that is overwritten now
-        if (STAGES > 1 && k + TILE < k1) {
-            load(k + TILE, own + (stage ^ 1) * 2 * BYTES);
-            if (DP == 64)
-                asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-            else
-                asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
-        } else {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        arrive();
+        if (MASK != 0) {
+            masked = next;
+            if (k + TILE < k1)
+                next.load(a, w.mask, k + TILE, lane);
         }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // what was read of the tile that is overwritten now
+        if (STAGES > 1 && k + TILE < k1)
+            ask(own + (stage ^ 1) * 2 * BYTES);
         w.template tile<1>(a, own + stage * 2 * BYTES, own + stage * 2 * BYTES + BYTES, k, masked);
         if (STAGES > 1) {
             stage ^= 1;
         } else if (k + TILE < k1) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            load(k + TILE, own);
+            ask(own);
         }
     }
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    arrive();
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     const uint32_t mine = lds + wave * result_bytes(DP);
     if (w.strange())
         carefully<TYPE, DP, MASK, false>(a, j, j.first, k0, k1, lane, mine);
@@ -833,20 +928,38 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a)
     const int piece = (int)(i - r * lanes);
     if (r >= a.all)
         return;
-    float M = -INFINITY;
-    for (int p = 0; p < a.pieces; p++)
-        M = fmaxf(M, a.ml[p * a.all + r].x);
-    const float ref = M == -INFINITY ? 0.0f : M;
-    float L = 0.0f;
+    constexpr int EACH = 8; // loads on their way together
+    float M = -INFINITY, L = 0.0f;
     f4v o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int p = 0; p < a.pieces; p++) {
-        const f2v ml = a.ml[p * a.all + r];
-        const f4v v = *(const GLOBAL f4v *)(a.partial + (p * a.all + r) * a.D + piece * 4);
-        const float e = __builtin_amdgcn_exp2f(ml.x - ref);
-        L = __builtin_fmaf(ml.y, e, L);
+    for (int p0 = 0; p0 < a.pieces; p0 += EACH) {
+        f2v ml[EACH];
+        f4v v[EACH];
+        float top = M;
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            const int p = min(p0 + i, a.pieces - 1);
+            ml[i] = *(const GLOBAL f2v *)(a.ml + p * a.all + r);
+            v[i] = *(const GLOBAL f4v *)(a.partial + (p * a.all + r) * a.D + piece * 4);
+        }
+#pragma unroll
+        for (int i = 0; i < EACH; i++)
+            top = fmaxf(top, ml[i].x);
+        if (top == -INFINITY)
+            continue; // nothing yet
+        const float shrink = __builtin_amdgcn_exp2f(M - top);
+        M = top;
+        L *= shrink;
 #pragma unroll
         for (int k = 0; k < 4; k++)
-            o[k] = __builtin_fmaf(v[k], e, o[k]);
+            o[k] *= shrink;
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            const float e = p0 + i < a.pieces ? __builtin_amdgcn_exp2f(ml[i].x - M) : 0.0f;
+            L = __builtin_fmaf(ml[i].y, e, L);
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                o[k] = __builtin_fmaf(v[i][k], e, o[k]);
+        }
     }
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     *(GLOBAL u2v *)(a.out + (r * a.D + piece * 4) * 2) = (u2v){Half<TYPE>::pack(o[0] * inv, o[1] * inv), Half<TYPE>::pack(o[2] * inv, o[3] * inv)};
@@ -854,30 +967,45 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a)
 
 // ------------------------------------------------------------------------------------------------------------------------- host
 
+enum { MANY_ROWS = WAVES * ROWS, SOME_ROWS = 2 * ROWS, FEW_ROWS = ROWS };
 struct Plan {
-    bool many;
+    int rows; // of a workgroup: the form
     int blocks, units, together, pieces;
 };
 
-static Plan plan(int B, int Hq, int H, int Tq, int Tk, int n_seq)
+static Plan plan(int B, int Hq, int H, int Tq, int Tk, int D, int n_seq)
 {
     const int g = Hq / H, cus = std::max(1, cu_count());
     const int64_t rows = (int64_t)Tq * g;
     Plan p;
     p.units = n_seq ? H : B * H;
     const auto blocks = [&](int each) { return (int)(n_seq ? rows / each + n_seq + 2 : (rows + each - 1) / each); };
-    p.many = (int64_t)p.units * blocks(WAVES * ROWS) >= cus;
-    p.blocks = blocks(p.many ? WAVES * ROWS : ROWS);
+    // Where 128 rows at a time leave CUs without work, or with the longest rows alone at the end, more waves share a row's keys.  Workgroups of the forms
+    // for that have a CU to themselves, or share it with one more (64 channels), and two rounds of them still pay where a unit has long rows beside short
+    // ones.  us of many, some, few, bf16, channels: units x tokens
+    //    64: 16 x 512  10.4, 7.9, 7.0     32 x 512  10.6, 8.3, 7.9     32 x 1024  18, 14, 18     16 x 4096  59, 55, 75     64 x 1024  19, 23, 32
+    //   128: 16 x 512  13.7, 11.5, 9.8    32 x 512  13.8, 11.9, 15.7   16 x 1024  23, 17, 20     16 x 2048  41, 34, 53     64 x 512   16, 20, 30
+    //   256: 16 x 512  27, 25, 16         32 x 512  28, 26, 26         16 x 1024  46, 42, 34     64 x 256   19, 19, 22     32 x 1024  50, 53, 66
+    const int64_t slots = D > 64 ? cus : 2ll * cus;
+    const auto fits = [&](int each, int length) { // once, or twice with so many blocks of a sequence
+        const int64_t all = (int64_t)p.units * blocks(each);
+        return all <= slots || (all <= 2 * slots && blocks(each) >= (int64_t)length * std::max(1, n_seq));
+    };
+    // A tile of keys leaves nothing to share: 64 tokens of 128 channels 5.6, 7.9, 6.4 us.
+    p.rows = Tk <= 64 && D <= 128 ? MANY_ROWS : fits(FEW_ROWS, D > 128 ? 16 : INT32_MAX) ? FEW_ROWS : D <= 128 && fits(SOME_ROWS, 32) ? SOME_ROWS : MANY_ROWS;
+    p.blocks = blocks(p.rows);
     p.pieces = 1;
     p.together = p.units;
-    if (p.many) {
+    if (p.rows == MANY_ROWS) {
         // Many blocks: as many units at a time as fill the device once, so that their blocks find their keys in the XCDs' caches (128 sequences of 512
         // tokens, 32 heads: 653 us; with eight units at a time 737, with all of them 807).  Else all of them, the longest first everywhere.
         if ((int64_t)p.units * p.blocks > 8ll * cus)
             p.together = (int)std::min<int64_t>(p.units, (cus / p.blocks + 8) / 8 * 8);
-    } else {
+    } else if (p.rows == FEW_ROWS) {
         const int64_t wide = (int64_t)p.units * p.blocks, tiles = (Tk + 31) / 32;
-        p.pieces = (int)std::max<int64_t>(1, std::min<int64_t>(cus / wide, tiles / (2 * WAVES)));
+        // two tiles a wave at least, and none for few keys (us, 8 units of 128 channels: 512 tokens in two pieces 12.5, in one 9.8; a token behind 1000 in
+        // four 9.4, in two 11.4)
+        p.pieces = tiles < 24 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(cus / wide, tiles / (2 * WAVES)));
     }
     return p;
 }
@@ -897,8 +1025,17 @@ static int checked(int B, int Hq, int H, int Tq, int Tk, int D, int n_seq)
     return ADKV_OK;
 }
 
-template <int TYPE, int MASK> static auto many_of(int D) { return D > 128 ? many_kernel<TYPE, 256, MASK> : D > 64 ? many_kernel<TYPE, 128, MASK> : many_kernel<TYPE, 64, MASK>; }
-template <int TYPE, int MASK> static auto few_of(int D) { return D > 128 ? few_kernel<TYPE, 256, MASK> : D > 64 ? few_kernel<TYPE, 128, MASK> : few_kernel<TYPE, 64, MASK>; }
+template <int TYPE, int DP, int MASK> static auto form_of(int rows)
+{
+    if constexpr (DP <= 128)
+        if (rows == SOME_ROWS)
+            return some_kernel<TYPE, DP, MASK>;
+    return rows == MANY_ROWS ? many_kernel<TYPE, DP, MASK> : few_kernel<TYPE, DP, MASK>;
+}
+template <int TYPE, int MASK> static auto kernel_of(int D, int rows)
+{
+    return D > 128 ? form_of<TYPE, 256, MASK>(rows) : D > 64 ? form_of<TYPE, 128, MASK>(rows) : form_of<TYPE, 64, MASK>(rows);
+}
 
 } // namespace adkv_prompt
 
@@ -909,7 +1046,7 @@ extern "C" int64_t adkv_prompt_attention_workspace_bytes(int B, int Hq, int H, i
         return rc;
     if (cu_count() <= 0)
         return ADKV_E_DEVICE;
-    const Plan p = plan(B, Hq, H, Tq, Tk, n_seq);
+    const Plan p = plan(B, Hq, H, Tq, Tk, D, n_seq);
     return p.pieces > 1 ? (int64_t)p.pieces * B * Tq * Hq * (D * 4 + 8) : 0;
 }
 
@@ -941,7 +1078,7 @@ extern "C" int adkv_prompt_attention(const void *q, const int64_t *q_strides, co
         return ADKV_E_ALIGN;
     if (cu_count() <= 0)
         return ADKV_E_DEVICE;
-    const Plan p = plan(B, Hq, H, Tq, Tk, n_seq);
+    const Plan p = plan(B, Hq, H, Tq, Tk, D, n_seq);
     const int64_t all = (int64_t)B * Tq * Hq, need = p.pieces > 1 ? p.pieces * all * (D * 4 + 8) : 0;
     if (need && (!workspace || workspace_bytes < need))
         return ADKV_E_WORKSPACE;
@@ -983,11 +1120,13 @@ extern "C" int adkv_prompt_attention(const void *q, const int64_t *q_strides, co
     const int masked = !mask ? 0 : size;
     const auto of = [&](auto type_) {
         constexpr int TYPE = decltype(type_)::value;
-        return p.many ? (masked == 0 ? many_of<TYPE, 0>(D) : masked == 1 ? many_of<TYPE, 1>(D) : masked == 2 ? many_of<TYPE, 2>(D) : many_of<TYPE, 4>(D))
-                      : (masked == 0 ? few_of<TYPE, 0>(D) : masked == 1 ? few_of<TYPE, 1>(D) : masked == 2 ? few_of<TYPE, 2>(D) : few_of<TYPE, 4>(D));
+        return masked == 0 ? kernel_of<TYPE, 0>(D, p.rows)
+            : masked == 1  ? kernel_of<TYPE, 1>(D, p.rows)
+            : masked == 2  ? kernel_of<TYPE, 2>(D, p.rows)
+                           : kernel_of<TYPE, 4>(D, p.rows);
     };
     const auto kernel = type == F16 ? of(std::integral_constant<int, F16>{}) : of(std::integral_constant<int, BF16>{});
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((int64_t)p.blocks * p.units * p.pieces)), dim3(NT), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((int64_t)p.blocks * p.units * p.pieces)), dim3(p.rows == SOME_ROWS ? 2 * NT : NT), 0, (hipStream_t)stream, a);
     if (int rc = check_launch())
         return rc;
     if (p.pieces > 1) {
