@@ -120,6 +120,9 @@ __device__ __forceinline__ float other_half(float v, bool max)
     return max ? fmaxf(__uint_as_float(x), __uint_as_float(y)) : __uint_as_float(x) + __uint_as_float(y);
 }
 
+// Channels that are multiplied, and that a tile's row has room for.  (80 channels, 997 tokens, 50 x 8 heads: with 96 of them 101 us, with all 128 115.)
+constexpr int room(int CH) { return CH > 128 ? 256 : CH > 64 ? 128 : 64; }
+
 // Rows of a tile are DP * 2 bytes in pieces of 16, piece c of row r at place c ^ turn(r), so that neither sixteen rows' reads of one piece
 // nor a transposing read (four consecutive rows, 64 bytes of each) meet in a bank.
 template <int DP> __device__ __forceinline__ constexpr int turn(int r)
@@ -338,10 +341,10 @@ __device__ __forceinline__ float with(float s, float x, float c)
 }
 
 // A wave's 32 rows; MASK: bytes of a key's mask, 0 without one
-template <int TYPE, int DP, int MASK>
+template <int TYPE, int CH, int MASK>
 struct Wave {
     using Hf = Half<TYPE>;
-    static constexpr int STEPS = DP / 16, CB = DP / 32;
+    static constexpr int DP = room(CH), STEPS = CH / 16, CB = CH / 32;
     u4v q[STEPS];
     f16v o[CB];
     float m, l;      // of row lane % 32: reference, in powers of two; this half's sum
@@ -703,9 +706,10 @@ __device__ __forceinline__ void arrive() { __builtin_amdgcn_s_waitcnt(0x0F70); }
 
 template <int DP> constexpr int many_lds() { return 2 * 64 * DP * 2 * 2; }
 
-template <int TYPE, int DP, int MASK>
-__global__ __launch_bounds__(NT, DP > 128 ? 1 : 2) void many_kernel(const Args a)
+template <int TYPE, int CH, int MASK>
+__global__ __launch_bounds__(NT, CH > 128 ? 1 : 2) void many_kernel(const Args a)
 {
+    constexpr int DP = room(CH);
     __shared__ uint4 smem[many_lds<DP>() / 16];
     const uint32_t lds = (uint32_t)(uintptr_t)(LDS char *)(char *)smem;
     constexpr int TILE = 64, BYTES = TILE * DP * 2, EACH = TILE / WAVES;
@@ -714,7 +718,7 @@ __global__ __launch_bounds__(NT, DP > 128 ? 1 : 2) void many_kernel(const Args a
     if (!place<WAVES * ROWS>(a, blockIdx.x, lane, j))
         return;
     const int first = j.first + wave * ROWS;
-    Wave<TYPE, DP, MASK> w;
+    Wave<TYPE, CH, MASK> w;
     const char *kp = a.k.p + j.b * a.k.sb + j.h * a.k.sh + (long)j.k0 * a.k.st, *vp = a.v.p + j.b * a.v.sb + j.h * a.v.sh + (long)j.k0 * a.v.st;
     Stream<DP> keys, values;
     values.open(vp, a.v.st, wave * EACH, j.end);
@@ -798,9 +802,10 @@ __global__ __launch_bounds__(NT, DP > 128 ? 1 : 2) void many_kernel(const Args a
 constexpr int PARTS = 4; // of the keys
 template <int DP> constexpr int some_lds() { return std::max(2 * PARTS * 32 * DP * 2 * 2, 2 * PARTS * result_bytes(DP)); }
 
-template <int TYPE, int DP, int MASK>
+template <int TYPE, int CH, int MASK>
 __global__ __launch_bounds__(2 * NT, 1) void some_kernel(const Args a)
 {
+    constexpr int DP = room(CH);
     __shared__ uint4 smem[some_lds<DP>() / 16];
     const uint32_t lds = (uint32_t)(uintptr_t)(LDS char *)(char *)smem;
     constexpr int TILE = PARTS * 32, BYTES = TILE * DP * 2, EACH = 16;
@@ -809,7 +814,7 @@ __global__ __launch_bounds__(2 * NT, 1) void some_kernel(const Args a)
     if (!place<2 * ROWS>(a, blockIdx.x, lane, j))
         return;
     const int first = j.first + rows * ROWS;
-    Wave<TYPE, DP, MASK> w;
+    Wave<TYPE, CH, MASK> w;
     Stream<DP> keys, values;
     keys.open(a.k.p + j.b * a.k.sb + j.h * a.k.sh + (long)j.k0 * a.k.st, a.k.st, wave * EACH, j.end);
     values.open(a.v.p + j.b * a.v.sb + j.h * a.v.sh + (long)j.k0 * a.v.st, a.v.st, wave * EACH, j.end);
@@ -857,9 +862,10 @@ __global__ __launch_bounds__(2 * NT, 1) void some_kernel(const Args a)
 template <int DP> constexpr int few_stages() { return DP > 128 ? 1 : 2; }
 template <int DP> constexpr int few_lds() { return std::max(WAVES * few_stages<DP>() * 32 * DP * 2 * 2, WAVES * result_bytes(DP)); }
 
-template <int TYPE, int DP, int MASK>
+template <int TYPE, int CH, int MASK>
 __global__ __launch_bounds__(NT, 1) void few_kernel(const Args a)
 {
+    constexpr int DP = room(CH);
     __shared__ uint4 smem[few_lds<DP>() / 16];
     const uint32_t lds = (uint32_t)(uintptr_t)(LDS char *)(char *)smem;
     constexpr int TILE = 32, BYTES = TILE * DP * 2, STAGES = few_stages<DP>();
@@ -867,7 +873,7 @@ __global__ __launch_bounds__(NT, 1) void few_kernel(const Args a)
     Job j;
     if (!place<ROWS>(a, blockIdx.x, lane, j))
         return;
-    Wave<TYPE, DP, MASK> w;
+    Wave<TYPE, CH, MASK> w;
     const int tiles = (j.end + TILE - 1) / TILE, parts = a.pieces * WAVES, part = j.piece * WAVES + wave;
     const int k0 = (int)((int64_t)tiles * part / parts) * TILE, k1 = min((int)((int64_t)tiles * (part + 1) / parts) * TILE, j.end);
     Stream<DP> keys, values;
@@ -1025,16 +1031,16 @@ static int checked(int B, int Hq, int H, int Tq, int Tk, int D, int n_seq)
     return ADKV_OK;
 }
 
-template <int TYPE, int DP, int MASK> static auto form_of(int rows)
+template <int TYPE, int CH, int MASK> static auto form_of(int rows)
 {
-    if constexpr (DP <= 128)
+    if constexpr (CH <= 128)
         if (rows == SOME_ROWS)
-            return some_kernel<TYPE, DP, MASK>;
-    return rows == MANY_ROWS ? many_kernel<TYPE, DP, MASK> : few_kernel<TYPE, DP, MASK>;
+            return some_kernel<TYPE, CH, MASK>;
+    return rows == MANY_ROWS ? many_kernel<TYPE, CH, MASK> : few_kernel<TYPE, CH, MASK>;
 }
 template <int TYPE, int MASK> static auto kernel_of(int D, int rows)
 {
-    return D > 128 ? form_of<TYPE, 256, MASK>(rows) : D > 64 ? form_of<TYPE, 128, MASK>(rows) : form_of<TYPE, 64, MASK>(rows);
+    return D > 128 ? form_of<TYPE, 256, MASK>(rows) : D > 96 ? form_of<TYPE, 128, MASK>(rows) : D > 64 ? form_of<TYPE, 96, MASK>(rows) : form_of<TYPE, 64, MASK>(rows);
 }
 
 } // namespace adkv_prompt
