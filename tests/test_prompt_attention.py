@@ -1,4 +1,4 @@
-"""gemv.prompt_attention against its formula in 64 bits: sizes around tiles and waves, both forms of the kernel, packed sequences, masks, strides,
+"""gemv.prompt_attention against its formula in 64 bits: sizes around tiles and waves, the kernel's forms, packed sequences, masks, strides,
 numbers that are none in hidden places, streams and graphs.
 
 Tolerances: with u half a step of the type, a weight is off by u from its rounding and by the error of its score, which is a sum of D products in
@@ -98,6 +98,55 @@ def test_sizes(gpu, size, dtype):
     B, H, g, Tq, Tk, D = size
     q, k, v = qkv(*size, dtype, gpu)
     check(gemv.prompt_attention(q, k, v, D ** -0.5), *plain(q, k, v, D ** -0.5))
+
+
+# For as many rows as keep the device busy with 128 at a time, with 64 and with 32
+FORMS = [(40, 8, 1, 130, 131, 64), (20, 16, 1, 70, 200, 80), (20, 16, 1, 129, 129, 128), (64, 9, 1, 40, 65, 256),
+         (2, 8, 1, 1100, 1100, 64), (1, 8, 1, 1101, 1101, 96), (1, 8, 4, 300, 2000, 128),
+         (2, 4, 2, 300, 301, 64), (1, 3, 2, 200, 900, 88), (1, 4, 1, 515, 515, 128), (1, 2, 4, 100, 400, 256)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["none", "bool", "bool_heads", "bias", "fp16", "bf16", "fp64", "inf"])
+@pytest.mark.parametrize("size", FORMS, ids=str)
+def test_forms(gpu, size, kind):
+    B, H, g, Tq, Tk, D = size
+    dtype = BF16 if kind == "bf16" else F16
+    q, k, v = qkv(*size, dtype, gpu)
+    m = None if kind == "none" else masks(kind, B, H * g, Tq, Tk, gpu)
+    got = gemv.prompt_attention(q, k, v, D ** -0.5, m)
+    picks = sorted({0, B // 2, B - 1})          # sequences; the formula takes its time
+    of = lambda t: t if t is None or t.shape[0] == 1 else t[picks]
+    check(got[picks], *plain(of(q) if B > 1 else q, of(k), of(v), D ** -0.5, of(m)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["none", "bool", "inf"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("size", [(40, 8, 1, 100, 131, 64), (20, 16, 1, 129, 129, 96), (2, 8, 1, 1100, 1100, 64), (1, 8, 1, 1101, 1101, 128), (1, 4, 1, 200, 515, 128)], ids=str)
+def test_forms_with_numbers_that_are_none_behind_a_row(gpu, size, bad, kind):
+    B, H, g, Tq, Tk, D = size
+    q, k, v = qkv(*size, F16, gpu)
+    at = Tk - 20
+    m = None if kind == "none" else masks(kind, B, H * g, Tq, Tk, gpu)
+    v[:, :, at, 5] = bad
+    k[:, :, at + 1:] = math.nan
+    got = gemv.prompt_attention(q, k, v, D ** -0.5, m)
+    n = Tq - 19          # rows that do not look at what is no key
+    pick = slice(B - 1, B)
+    m = m if m is None else m[pick, :, :n, :at + 1]
+    check(got[pick, :n], *plain(q[pick, :, :n], k[pick, :, :at + 1], v[pick, :, :at + 1], D ** -0.5, m))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,g,D,ends", [(8, 1, 128, [0, 700, 701, 1100]), (16, 1, 64, [3, 500, 700, 1090]), (3, 2, 96, [0, 100, 333, 350])], ids=str)
+def test_forms_of_packed_sequences(gpu, H, g, D, ends):
+    T = ends[-1] + 3
+    q, k, v = qkv(1, H, g, T, T, D, F16, gpu)
+    bounds = torch.tensor(ends, dtype=torch.int32)
+    got = gemv.prompt_attention(q, k, v, D ** -0.5, bounds=bounds.to(gpu))
+    check(got, *plain(q, k, v, D ** -0.5, bounds=bounds))
+    assert not got[:, ends[-1]:].any() and not got[:, :ends[0]].any()
 
 
 @pytest.mark.gpu
