@@ -599,8 +599,12 @@ __device__ __forceinline__ void carefully(const Args &a, const Job &j, int first
                 const char *kp = a.k.p + j.b * a.k.sb + j.h * a.k.sh + (long)(j.k0 + key) * a.k.st;
                 float s = 0.0f;
 #pragma unroll 1
-                for (int d = 0; d < a.D; d++)
-                    s = __builtin_fmaf(Hf::number(((const GLOBAL uint16_t *)q)[d]), Hf::number(((const GLOBAL uint16_t *)kp)[d]), s);
+                for (int d = 0; d < a.D; d += 8) {
+                    const u4v x8 = *(const GLOBAL u4v *)(q + d * 2), y8 = *(const GLOBAL u4v *)(kp + d * 2);
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        s = __builtin_fmaf(Hf::number((uint16_t)(x8[e >> 1] >> (e & 1) * 16)), Hf::number((uint16_t)(y8[e >> 1] >> (e & 1) * 16)), s);
+                }
                 x = s * c;
                 if constexpr (MASK != 0) {
                     const GLOBAL char *mp = (const GLOBAL char *)(a.mask + (j.b * a.m_sb + head * a.m_sh + (long)t * a.m_st + key) * MASK);
@@ -626,16 +630,16 @@ __device__ __forceinline__ void carefully(const Args &a, const Job &j, int first
 #pragma unroll
             for (int n = 0; n < N; n++)
                 o[n] *= shrink;
-#pragma unroll 1
-            for (int e = 0; e < 64; e++) {
-                if (!(seen >> e & 1))
-                    continue;
-                const float w = __shfl(p, e);
-                const char *vp = a.v.p + j.b * a.v.sb + j.h * a.v.sh + (long)(j.k0 + k + e) * a.v.st;
+#pragma unroll 8
+            for (int e = 0; e < WIDTH; e++) {
+                const bool look = seen >> e & 1;
+                const float w = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(p), e));
+                const char *vp = a.v.p + j.b * a.v.sb + j.h * a.v.sh + (long)(j.k0 + min(k + e, end - 1)) * a.v.st;
 #pragma unroll
-                for (int n = 0; n < N; n++)
-                    if (lane * N + n < a.D)
-                        o[n] = __builtin_fmaf(w, Hf::number(((const GLOBAL uint16_t *)vp)[lane * N + n]), o[n]);
+                for (int n = 0; n < N; n++) {
+                    const float y = Hf::number(((const GLOBAL uint16_t *)vp)[min(lane * N + n, a.D - 1)]);
+                    o[n] = look ? __builtin_fmaf(w, y, o[n]) : o[n];
+                }
             }
         }
         if (WHOLE) {

@@ -6,6 +6,8 @@
 // many columns as that gives, or, with more than 32 rows, of a narrower column.
 // One of four beams of 603 tokens, 32 layers of 32 heads (166 MB read and written): see take_kernel.
 #include <algorithm>
+#include <memory>
+#include <new>
 
 #include "adkv_device.h"
 
@@ -134,6 +136,27 @@ __global__ __launch_bounds__(WAVES * 64) void take_kernel(const Args a)
     }
 }
 
+struct Extent {
+    uint64_t begin, end;
+    bool written;
+};
+
+// whether any that is written shares memory with another one
+static bool overlapping(Extent *first, Extent *last)
+{
+    std::sort(first, last, [](const Extent &a, const Extent &b) { return a.begin < b.begin; });
+    uint64_t any = 0, written = 0; // ends of what is in front
+    for (; first != last; first++) {
+        const Extent &e = *first;
+        if (e.begin < written || (e.written && e.begin < any))
+            return true;
+        any = std::max(any, e.end);
+        if (e.written)
+            written = std::max(written, e.end);
+    }
+    return false;
+}
+
 } // namespace adkv_sequences
 
 extern "C" int adkv_take_sequences(const adkv_rows *tensors, int n, const int64_t *index, int rows, int batch, void *stream)
@@ -158,6 +181,20 @@ extern "C" int adkv_take_sequences(const adkv_rows *tensors, int n, const int64_
         if (((uint64_t)t.data | (uint64_t)t.into | (uint64_t)t.pitch | (uint64_t)(into ? t.into_pitch : 0) | (uint64_t)t.used) & 15)
             return ADKV_E_ALIGN;
     }
+    // rows that are written while another tensor's are read
+    const std::unique_ptr<Extent[]> all(new (std::nothrow) Extent[2 * (size_t)n]);
+    if (!all)
+        return ADKV_E_WORKSPACE;
+    size_t extents = 0;
+    for (int i = 0; i < n && rows > 0; i++) {
+        const adkv_rows &t = tensors[i];
+        if (t.segments * t.used > 0)
+            all[extents++] = {(uint64_t)t.data, (uint64_t)t.data + (uint64_t)batch * t.segments * t.pitch, !into};
+        if (into && t.segments * t.into_pitch > 0)
+            all[extents++] = {(uint64_t)t.into, (uint64_t)t.into + (uint64_t)rows * t.segments * t.into_pitch, true};
+    }
+    if (overlapping(all.get(), all.get() + extents))
+        return ADKV_E_UNSUPPORTED;
     for (int at = 0; at < n && rows > 0;) {
         Args a = {};
         a.index = index;

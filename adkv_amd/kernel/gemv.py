@@ -697,6 +697,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scaling:
     mst, mdt = None, 0
     if mask is not None:
         mdt = _PROMPT_MASK_DT.get(mask.dtype, 0)
+        if mask.dtype == torch.float64:        # its lowest value is no minus infinity in fp32 either
+            most = torch.finfo(torch.float32).max
+            mask = torch.where(mask.isinf(), mask, mask.clamp(-most, most))
         mask = mask.to(device=dev, dtype=mask.dtype if mask.dtype in _PROMPT_MASK_DT else torch.float32)
         if mask.stride(3) != 1 and Tk > 1:
             mask = mask.contiguous()
@@ -775,7 +778,8 @@ def take_sequences(tensors, index: torch.Tensor, *, used=None, into=None) -> Non
             row whose index is none of the rows stays as it is, or is zeros in ``into``.  On the host they are checked and copied.
         used: how many entries along the third axis hold anything, one number per tensor (all): what is behind them is neither read nor written.
         into: as many tensors ``[R, H, m, ...]``, ``m >= used``, to write instead, which share no memory with ``tensors``; what is behind the entries that are
-            used becomes zero.  Without it ``R <= B``, rows may be one another's sources in any way, and no two tensors may share memory.
+            used becomes zero.  Without it ``R <= B``, rows may be one another's sources in any way, and no two tensors may share memory
+            (refused).
     """
     tensors = list(tensors)
     used = None if used is None else list(used)

@@ -527,7 +527,8 @@ int adkv_prompt_attention(const void *q, const int64_t *q_strides, const void *k
  *   into      NULL: in place, whatever the map (a row may be several rows' source), rows <= batch.  Else [rows, segments, into_pitch bytes], packed,
  *             for every tensor of the call, which do not overlap data
  *   used      bytes of a segment that are copied, the same in all rows; what is behind them is left as it is in place, zeros in `into`
- * Pointers and sizes are multiples of 16 bytes; at most 1024 rows.  The array is host memory and may be reused after the call.
+ * Pointers and sizes are multiples of 16 bytes; at most 1024 rows.  What is written shares no memory with another tensor (ADKV_E_UNSUPPORTED).  The array
+ * is host memory and may be reused after the call.
  */
 typedef struct {
     void *data, *into;

@@ -285,6 +285,19 @@ def test_masked_tokens_leave_nothing_behind(gpu, kind):
 
 
 @pytest.mark.gpu
+def test_lowest_values_of_64_bits(gpu):
+    """They are the lowest of 32 bits to the kernel, not minus infinity: rows of nothing else look at all tokens up to their own alike."""
+    q, k, v = qkv(2, 2, 1, 50, 50, 64, F16, gpu)
+    m = torch.zeros(2, 1, 50, 50, dtype=torch.float64, device=gpu)
+    m[0, :, :, :20] = torch.finfo(torch.float64).min
+    m[1, :, 30:, 10] = -math.inf
+    low = m.clamp(min=torch.finfo(torch.float32).min).float().masked_fill_(m == -math.inf, -math.inf)
+    got = gemv.prompt_attention(q, k, v, 0.125, m)
+    assert torch.equal(got, gemv.prompt_attention(q, k, v, 0.125, low))
+    check(got, *plain(q, k, v, 0.125, low))
+
+
+@pytest.mark.gpu
 def test_layouts(gpu):
     """Heads first, a slice of a fused projection, one key head for all sequences, rows that begin between two pieces of 16 bytes."""
     base = qkv(2, 2, 2, 40, 40, 64, F16, gpu)

@@ -163,4 +163,24 @@ def test_the_library_refuses_what_it_cannot_take():
         assert call(**change) == code, change
     both = (_lib.Rows * 2)(_lib.Rows(4096, None, 1, 64, 0, 64), _lib.Rows(4096, 8192, 1, 64, 64, 64))
     assert L.adkv_take_sequences(both, 2, 4096, 1, 1, None) == -6
+    # what is written shares memory with another tensor: twice the same, one inside another, into what is read or written elsewhere
+    for a, b in [((4096, None, 2, 64, 0, 64),) * 2, ((4096, None, 2, 64, 0, 64), (4096 + 192, None, 1, 32, 0, 16)),
+                 ((4096, 8192, 1, 64, 64, 64), (16384, 4096 + 64, 1, 64, 64, 64)), ((4096, 8192, 1, 64, 64, 64), (16384, 8192, 1, 64, 64, 64)),
+                 ((4096, 8192, 1, 64, 64, 64), (8192 + 64, 16384, 1, 64, 64, 64))]:
+        for two in ((a, b), (b, a)):
+            assert L.adkv_take_sequences((_lib.Rows * 2)(*(_lib.Rows(*t) for t in two)), 2, 4096, 2, 2, None) == -6
     assert L.adkv_take_sequences(None, 0, 4096, 1, 1, None) == 0 and L.adkv_take_sequences(both, 2, None, 0, 1, None) == -6
+
+
+@pytest.mark.gpu
+def test_tensors_that_share_memory(gpu):
+    """Refused where one of them is written; several of them may be copied from one."""
+    t, = tensors_of(4, 2, [("codes", 6)], gpu)
+    i = torch.tensor([1, 0], device=gpu)
+    for pair in ([t, t], [t, t[:]]):
+        with pytest.raises(RuntimeError):
+            gemv.take_sequences(pair, i)
+    into = torch.empty(2, 2, 6, 32, 4, 4, dtype=torch.uint8, device=gpu)
+    with pytest.raises(RuntimeError):
+        gemv.take_sequences([t, t], i, into=[into, into])
+    check([t, t], i, None, [into, into.clone()])
