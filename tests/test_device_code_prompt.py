@@ -9,6 +9,8 @@ import subprocess
 import pytest
 
 from adkv_amd.build import PROMPT_PATH
+from test_device_code import _registers, early_sources, kernels
+from test_lane_swaps import early_exchanges
 
 LLVM = "/opt/rocm/llvm/bin"
 
@@ -70,3 +72,12 @@ def test_nothing_waits_for_tiles_on_their_way_but_the_barriers(listings):
             assert len(barriers) == 3 and len(waits) == 1 and code[waits[0] + 1][0] == "s_barrier", (name, [code[i] for i in waits])
             seen += 1
     assert seen == 8
+
+
+def test_distances_between_dependent_instructions(listings):
+    """Matrix instructions and exchanges between lanes read what was written two wait states before; a swap is between two registers."""
+    assert sum(t.count("\tv_mfma") for t, _ in listings) > 1000 and sum(t.count("_swap_b32") for t, _ in listings) > 100
+    assert not [v for t, _ in listings for v in early_sources(t)][:5]
+    assert not [v for t, _ in listings for v in early_exchanges(t)][:5]
+    swaps = [(name, a) for t, _ in listings for name, code, _ in kernels(t, "v_permlane") for o, a, _ in code if o.endswith("_swap_b32_e32")]
+    assert not [f for f in swaps if len(_registers(f[1])) != 2][:5]
