@@ -2,9 +2,11 @@
 //
 // Nothing but memory: a row that moves is read and written once, one that stays is not touched.  In place any map is taken, whatever the order in
 // which rows overwrite each other: a wave takes a column of the tensors (1 KB or less, of all rows), and has read what it needs of it before it
-// writes.  Columns are independent, so that there is nothing to wait for between waves.  32 loads of 1 KB are in flight per wave: the moved rows of as
-// many columns as that gives, or, with more than 32 rows, of a narrower column.
-// One of four beams of 603 tokens, 32 layers of 32 heads (166 MB read and written): see take_kernel.
+// writes.  Columns are independent, so that there is nothing to wait for between waves.  A wave has 8 or 16 loads of up to 1 KB in flight: the moved rows of
+// as many columns as that gives, or, with more rows, of a narrower column.  All waves are resident, each with an equal share of the columns; stores go past
+// the caches.
+// MI355X, one layer's worth after another's so that nothing is in a cache: one of four beams of 603 tokens, 32 layers of 32 heads (166 MB read and written)
+// 38 us, 4.4 TB/s; 12 of 64 sequences of 4096 tokens (416 MB) 88, 4.7 TB/s; sixteen of one of 8001 (368 MB) 75, 4.9 TB/s; a large copy runs at 5.15.
 #include <algorithm>
 #include <memory>
 #include <new>
@@ -20,10 +22,13 @@ using adkv::cu_count;
 typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 #define GLOBAL __attribute__((address_space(1)))
 
-constexpr int WAVES = 4, SLOTS = 16, BLOCK = 1024; // bytes of a column
-constexpr int PER_CU = 12;                          // waves: all of them at once, three to a SIMD by their registers
+constexpr int WAVES = 4, BLOCK = 1024; // bytes of a column
+// Rows up to which a wave has 8 slots, and five fit a SIMD by their registers; with more rows it has 16, and three fit.  us with 8 and 16: 4 rows 38, 51;
+// 48 rows, 12 of them moved, 88, 105; 50 21, 21; 78 42, 31; 122 104, 78.  (4 slots, six waves: 42, 88; 29; 165; 387.)
+constexpr int FEW = 64;
+constexpr int waves_per_cu(int SLOTS) { return SLOTS == 8 ? 20 : 12; }
 constexpr int TENSORS = 96;                         // of a launch
-constexpr int MOST = 1024;                          // rows: with all of them moved a column is 16 bytes
+constexpr int MOST = 1024;                          // rows: with all of them moved 16 slots have columns of 16 bytes
 
 struct Tensor {
     const char *from;
@@ -43,7 +48,7 @@ static_assert(sizeof(Args) <= 4096, "kernel arguments");
 // A row may be another one's source: what is read of a column is there before any of it is written.
 __device__ __forceinline__ void all_read() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-template <bool INTO>
+template <bool INTO, int SLOTS>
 __global__ __launch_bounds__(WAVES * 64) void take_kernel(const Args a)
 {
     __shared__ int2 list[MOST];
@@ -232,8 +237,9 @@ extern "C" int adkv_take_sequences(const adkv_rows *tensors, int n, const int64_
         if (a.n == 0)
             continue;
         a.units = (int)units;
-        a.waves = (int)std::min<int64_t>(units, (int64_t)PER_CU * cu_count());
-        const auto kernel = into ? take_kernel<true> : take_kernel<false>;
+        const bool few = rows <= FEW;
+        a.waves = (int)std::min<int64_t>(units, (int64_t)waves_per_cu(few ? 8 : 16) * cu_count());
+        const auto kernel = into ? (few ? take_kernel<true, 8> : take_kernel<true, 16>) : few ? take_kernel<false, 8> : take_kernel<false, 16>;
         hipLaunchKernelGGL(kernel, dim3((unsigned)((a.waves + WAVES - 1) / WAVES)), dim3(WAVES * 64), 0, (hipStream_t)stream, a);
         if (int rc = check_launch())
             return rc;
