@@ -357,7 +357,8 @@ __global__ __launch_bounds__(NT, WITH_TOP ? 6 : 8) void logprobs_kernel(const Ar
     if (wave != 0 && !slow && !again)
         return; // the rest is the first wave's
     const float shift = __builtin_fmaf(-M, L2E, sums.r), scale = __builtin_amdgcn_exp2f(shift);
-    float S = scale * sums.s, T = scale * __builtin_fmaf(shift, sums.s, sums.t) * 0.69314718055994530942f;
+    // T is the small difference of two large ones where the reference is not the largest
+    float S = scale * sums.s, T = (float)(0.69314718055994530942 * ((double)scale * ((double)shift * sums.s + sums.t)));
     if (again) {
         // logits of the type's lowest value only, or of minus or plus infinity: the definition, in two passes more
         M = -INFINITY;
@@ -388,7 +389,7 @@ __global__ __launch_bounds__(NT, WITH_TOP ? 6 : 8) void logprobs_kernel(const Ar
     const auto log_of = [&](float x) { return (float)((double)x - M - log1); };
     if (tid == 0) {
         a.logprobs[r] = token < 0 ? 0.0f : token < a.V ? log_of(given) : NAN;
-        a.entropy[r] = log1 - T / (1.0f + S);
+        a.entropy[r] = (float)((double)log1 - (double)T / (1.0 + (double)S));
     }
     if constexpr (WITH_TOP) {
         const auto put = [&](int rank, uint64_t k) {
