@@ -16,6 +16,12 @@
 //   some  a workgroup is 64 rows, eight waves: each has 32 rows and every fourth 32 keys of them, over shared tiles of 128; joined in the LDS
 //   few   a workgroup is 32 rows, its four waves walk through a quarter of the keys each in tiles of their own and are joined in the LDS; where
 //         that leaves CUs without work the keys are cut into pieces for several workgroups, joined by a second kernel
+// plan() says which, and what each takes.
+//
+// What bounds it, MI355X: long prompts the clock that the matrix cores' power allows (16384 tokens, 32 heads on 8, bf16: 1.98 ms, 1.11 PFLOP/s, matrix cores
+// busy for 61 % of the time at 1.67 GHz; a library's product of 8192^3 runs at 1.40).  Batches of short ones memory and the way in and out of a workgroup
+// (128 of 512 tokens, 32 heads: 554 us, 3.9 TB/s, the matrix cores 33 % busy; of 128 tokens 112 us, 4.8 TB/s; a copy runs at 5.15), and few blocks the
+// chain of a single one.  A row over many keys: memory (8 x 8 heads of four, 4097 tokens: 31 us, 4.4 TB/s).
 #include <math.h>
 
 #include <algorithm>
@@ -1007,8 +1013,9 @@ static Plan plan(int B, int Hq, int H, int Tq, int Tk, int D, int n_seq)
     p.pieces = 1;
     p.together = p.units;
     if (p.rows == MANY_ROWS) {
-        // Many blocks: as many units at a time as fill the device once, so that their blocks find their keys in the XCDs' caches (128 sequences of 512
-        // tokens, 32 heads: 653 us; with eight units at a time 737, with all of them 807).  Else all of them, the longest first everywhere.
+        // Many blocks: as many units at a time as fill the device once, so that their blocks find their keys in the XCDs' caches (us with that many, twice
+        // and four times as many, bf16: 128 sequences of 512 tokens, 32 heads 607, 585, 633; 64 of 300, eight heads of four queries 122, 129, 124; 101 of 278,
+        // 16 heads 124, 131, 138).  Else all of them, the longest first everywhere.
         if ((int64_t)p.units * p.blocks > 8ll * cus)
             p.together = (int)std::min<int64_t>(p.units, (cus / p.blocks + 8) / 8 * 8);
     } else if (p.rows == FEW_ROWS) {
