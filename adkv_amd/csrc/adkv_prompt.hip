@@ -735,8 +735,7 @@ __global__ __launch_bounds__(NT, CH > 128 ? 1 : 2) void many_kernel(const Args a
     const uint32_t mine = lds + wave * EACH * DP * 2;
     if constexpr (MASK == 0) {
         // The weights of 32 keys are made beside the products of the next 32 keys' scores, so that keys are half a tile ahead of the values: tile k / 64
-        // of them in the LDS begins with key k + 32.  (16384 tokens, 32 heads of 128: 2.05 ms instead of the 2.21 of a tile's scores, weights and
-        // outputs one after the other, 1.07 PFLOP/s; with all of it zeros 1.7: what is left is the clock that the matrix cores' power allows.)
+        // of them in the LDS begins with key k + 32.  (16384 tokens, 32 heads of 128: a tile's scores, weights and outputs one after the other take 7 % longer.)
         f16v even[1], odd[1];
         if (j.end > 0) {
             // the first 32, where the second tile of keys will be
