@@ -234,8 +234,10 @@ __device__ __forceinline__ bool place(const Args &a, int i, int lane, Job &j)
         const int batch = i / (a.together * a.blocks), here = min(a.together, a.units - batch * a.together);
         i -= batch * a.together * a.blocks;
         const int back = i / here, unit = batch * a.together + i - back * here;
-        j.b = unit / a.H;
-        j.h = unit - j.b * a.H;
+        // eight sequences side by side, so that all heads of one are on an XCD, which is the only one to read their mask then
+        const int eight = unit / (8 * a.H), of = unit - eight * 8 * a.H, beside = min(8, a.B - 8 * eight);
+        j.h = of / beside;
+        j.b = 8 * eight + of - j.h * beside;
         j.q0 = j.k0 = 0;
         j.n = a.Tq;
         j.m = a.Tk;
@@ -300,7 +302,7 @@ struct Mask {
             for (int i = 0; i < WORDS; i++)
                 w[i] = __builtin_amdgcn_alignbyte(w[i + MORE], w[i], shift);
     }
-    // what all of the wave's keys have, and any: 1 where nothing is added or hidden, -1 where all of them are hidden
+    // Of all of the wave's keys: 1 where nothing is added or hidden, -1 where all of them are hidden, 2 where the same is added to all, else 0
     __device__ __forceinline__ int alike(int dt) const
     {
         uint32_t all = ~0u, any = 0;
@@ -309,8 +311,11 @@ struct Mask {
             all &= w[i];
             any |= w[i];
         }
+        const uint32_t one = __builtin_amdgcn_readfirstlane(w[0]);
+        if (!__all(all == one && any == one))
+            return 0;
         const uint32_t none = SIZE == 1 ? 0 : SIZE == 4 ? 0xFF800000u : dt == F16 ? 0xFC00FC00u : 0xFF80FF80u, whole = SIZE == 1 ? 0x01010101u : 0;
-        return __all(all == whole && any == whole) ? 1 : __all(all == none && any == none) ? -1 : 0;
+        return one == whole ? 1 : one == none ? -1 : SIZE == 4 || (SIZE == 2 && one >> 16 == (one & 0xFFFFu)) ? 2 : 0;
     }
     __device__ __forceinline__ void exchange()
     {
@@ -418,8 +423,8 @@ struct Wave {
                 sc[kb] = Hf::mfma(*shared<u4v>(key_at[s] + keys + kb * 32 * (DP * 2)), q[s], sc[kb]);
     }
 
-    // What keys k.. are hidden behind a row's own, and the row's reference, which goes along with its sum and outputs; unit: of the scores x
-    template <int KB> __device__ __forceinline__ void settle(float *x, int k, float unit)
+    // What keys k.. are hidden behind a row's own, and the row's reference, which goes along with its sum and outputs; unit: of the scores x, more: added to them
+    template <int KB> __device__ __forceinline__ void settle(float *x, int k, float unit, float more = 0.0f)
     {
         if (k + KB * 32 > low) {
             int left = limit - k - 4 * (lane >> 5);
@@ -432,7 +437,7 @@ struct Wave {
 #pragma unroll
         for (int e = 1; e < KB * 16; e++)
             top = fmaxf(top, x[e]);
-        top *= unit;
+        top = MASK > 1 ? __builtin_fmaf(top, unit, more) : top * unit;
         if (__any(top > m + SLACK)) {
             const float to = fmaxf(m, other_half(top, true));
             const float shrink = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - to);
@@ -446,9 +451,9 @@ struct Wave {
         }
     }
 
-    template <int KB> __device__ __forceinline__ void weights(const float *x, float unit, uint32_t *w)
+    template <int KB> __device__ __forceinline__ void weights(const float *x, float unit, uint32_t *w, float more = 0.0f)
     {
-        const float ref = m == -INFINITY ? 0.0f : m - Hf::BIAS; // nothing yet: all weights are zero
+        const float ref = m == -INFINITY ? 0.0f : MASK > 1 ? m - Hf::BIAS - more : m - Hf::BIAS; // nothing yet: all weights are zero
 #pragma unroll
         for (int e = 0; e < KB * 16; e += 2) {
             w[e >> 1] = Hf::pack(__builtin_amdgcn_exp2f(__builtin_fmaf(x[e], unit, -ref)), __builtin_amdgcn_exp2f(__builtin_fmaf(x[e + 1], unit, -ref)));
@@ -478,7 +483,7 @@ struct Wave {
     {
         if (MASK != 0)
             masked.align();
-        const int all = MASK != 0 ? masked.alike(a.mask_dt) : 1;
+        int all = MASK != 0 ? masked.alike(a.mask_dt) : 1;
         if (MASK != 0 && all < 0)
             return; // nothing to look at
         f16v sc[KB];
@@ -487,7 +492,19 @@ struct Wave {
 #pragma unroll
         for (int e = 0; e < KB * 16; e++)
             x[e] = sc[e >> 4][e & 15];
-        float unit = c; // of x; with something added they are in powers of two
+        float unit = c, more = 0.0f; // of x; with something added they are in powers of two
+        if (MASK > 1 && all == 2) {
+            // The same for all keys, a type's lowest value in front of a padded text: added to the reference, not to every score.  Where that leaves nothing of
+            // the scores they are next to nothing, where it would leave little of them they are rounded one by one, as beside other masks.
+            more = masked.template of<0>(a.mask_dt) * LOG2E;
+            if (more < -1e30f) {
+                more = -3.0e38f;
+                unit = 1e-30f;
+            } else if (!(fabsf(more) < 131072.0f)) {
+                more = 0.0f;
+                all = 0;
+            }
+        }
         if constexpr (MASK != 0) {
             if (all == 0) {
                 masked.exchange();
@@ -500,9 +517,9 @@ struct Wave {
                 });
             }
         }
-        settle<KB>(x, k, unit);
+        settle<KB>(x, k, unit, more);
         uint32_t w[KB * 8];
-        weights<KB>(x, unit, w);
+        weights<KB>(x, unit, w, more);
         outputs<KB>(values, w);
     }
 
