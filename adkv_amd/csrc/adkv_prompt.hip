@@ -234,7 +234,8 @@ __device__ __forceinline__ bool place(const Args &a, int i, int lane, Job &j)
         const int batch = i / (a.together * a.blocks), here = min(a.together, a.units - batch * a.together);
         i -= batch * a.together * a.blocks;
         const int back = i / here, unit = batch * a.together + i - back * here;
-        // eight sequences side by side, so that all heads of one are on an XCD, which is the only one to read their mask then
+        // eight sequences side by side, so that all heads of one are on an XCD, which is the only one to read their mask then (32 sequences of 700 tokens, eight
+        // heads of 64 channels, bool: 35 us instead of 50; 128 of 512 without a mask: 538 instead of 550)
         const int eight = unit / (8 * a.H), of = unit - eight * 8 * a.H, beside = min(8, a.B - 8 * eight);
         j.h = of / beside;
         j.b = 8 * eight + of - j.h * beside;
