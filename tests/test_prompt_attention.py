@@ -285,14 +285,12 @@ def test_masked_tokens_leave_nothing_behind(gpu, kind):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("value", [-10000.0, -1e9, 3.0, -6.5, "lowest", -math.inf])
-@pytest.mark.parametrize("dtype", [F16, BF16, torch.float32], ids=["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("dtype,value", [(d, x) for d in (F16, BF16, torch.float32) for x in (-10000.0, -1e9, 3.0, -6.5, "lowest", -math.inf) if d != F16 or x != -1e9],
+                         ids=lambda x: str(x).replace("torch.", ""))
 @pytest.mark.parametrize("size", [(20, 16, 1, 129, 300, 128), (2, 8, 1, 1100, 1100, 64), (2, 4, 2, 100, 401, 64)], ids=str)
 def test_the_same_added_to_many_keys(gpu, size, dtype, value):
     """Whole tiles of it, at the edge of one and from one head to the next; every row looks at a key that it is not added to."""
     B, H, g, Tq, Tk, D = size
-    if dtype == F16 and value == -1e9:
-        pytest.skip("no such value")
     q, k, v = qkv(*size, F16 if dtype == torch.float32 else dtype, gpu)
     m = torch.zeros(B, 1, 1, Tk, dtype=dtype, device=gpu).expand(B, 1, Tq, Tk).contiguous()
     value = torch.finfo(dtype).min if value == "lowest" else value
