@@ -27,6 +27,7 @@ from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
 from ..kernel.gemv import prompt_attention, rope_norm_qk, rope_qk
 from .cache import (CAP_LEN, INIT_SEQ_LEN, SCALE_MAX, SCALE_MIN, KVCache_ADKV,  # noqa: F401
                     KVCacheLayer_ADKV)
+from .packed import packed_mask, says_nothing, takes_prompts
 from .score import Scores
 
 # the five per-(head, channel) quantities, for K and for V (reference llama_adkv.py:27)
@@ -62,19 +63,22 @@ def norm_and_rotate(attn, q, k, cos, sin):
 
 def prompt_ctx(attn, q, k, v, attention_mask, cached: bool, kwargs) -> torch.Tensor | None:
     """config.adkv_prompt: the dense rows' attention ``[B, T, Hq, C]`` by the framework's own kernel, without weights; None where transformers' is to
-    run (without the flag, on the host, for other types and head sizes, where a gradient, dropout or the weights are wanted).  With
-    ``cu_seq_lens_q`` (transformers' name for the bounds of sequences packed into one row axis) each sequence looks at itself only."""
+    run (``takes_prompts``; where a gradient is wanted).  With ``cu_seq_lens_q`` (transformers' name for the bounds of sequences packed into one row
+    axis) each sequence looks at itself only."""
     if not getattr(attn.config, "adkv_prompt", False):
         return None
     bounds = kwargs.get("cu_seq_lens_q")
     if bounds is not None and cached:
         raise ValueError("packed sequences have no cache: pass use_cache=False")
-    if not (q.is_cuda and q.dtype in (torch.float16, torch.bfloat16) and k.dtype == v.dtype == q.dtype and q.shape[-1] % 8 == 0 and q.shape[-1] <= 256) \
-            or (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v))) or (attn.training and attn.attention_dropout > 0) \
-            or kwargs.get("output_attentions") or getattr(attn.config, "output_attentions", False):
+    apart = says_nothing(attention_mask)
+    if not takes_prompts(attn, q.dtype, q.device, kwargs) or not k.dtype == v.dtype == q.dtype \
+            or (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v))):
+        if apart:
+            raise ValueError("packed sequences that nothing keeps apart: give their mask, or call the model without one")
         return None
     if bounds is not None:
-        return prompt_attention(q, k, v, attn.scaling, bounds=bounds)
+        # with a mask of its own transformers' attention runs, which goes by that
+        return prompt_attention(q, k, v, attn.scaling, bounds=bounds) if apart or attention_mask is None else None
     if attention_mask is not None:
         if attention_mask.dim() != 4 or attention_mask.shape[-1] < k.shape[2]:
             return None
@@ -211,6 +215,7 @@ class LlamaModel_ADKV(LlamaModel):
             # config.adkv_bits = 2 selects the 2-bit code format (extension; default 4 as the reference)
             past_key_values = KVCache_ADKV(self.config.num_hidden_layers,
                                            bits=getattr(self.config, "adkv_bits", 4))
+        attention_mask = packed_mask(self, input_ids if inputs_embeds is None else inputs_embeds, attention_mask, kwargs)
         return super().forward(input_ids=input_ids, attention_mask=attention_mask,
                                position_ids=position_ids, past_key_values=past_key_values,
                                inputs_embeds=inputs_embeds, cache_position=cache_position,

@@ -28,6 +28,7 @@ from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
 from ..kernel.gemv import take_sequences
 from ..train.train_model import quant_f32_pair
 from .llama_adkv import ADKV_PARAM_FIELDS, ADKVConfig, make_head_norms, norm_and_rotate, prompt_ctx  # noqa: F401
+from .packed import packed_mask
 from .score import Scores
 
 SCALE_MIN = math.exp(-4.0)
@@ -293,6 +294,7 @@ class LlamaModel_ADKV(LlamaModel):
             use_cache = getattr(self.config, "use_cache", True)
         if use_cache and past_key_values is None:
             past_key_values = KVCache_ADKV(self.config.num_hidden_layers)
+        attention_mask = packed_mask(self, input_ids if inputs_embeds is None else inputs_embeds, attention_mask, kwargs)
         return super().forward(input_ids=input_ids, attention_mask=attention_mask,
                                position_ids=position_ids, past_key_values=past_key_values,
                                inputs_embeds=inputs_embeds, cache_position=cache_position,

@@ -4,6 +4,7 @@ from __future__ import annotations
 import torch
 
 from ..kernel.gemv import TokenLogprobs, token_logprobs
+from .packed import packs
 
 
 class Scores:
@@ -15,7 +16,7 @@ class Scores:
         front of it: ``n - 1`` of them, with the distributions' entropy and their ``top`` likeliest tokens.  ``rows`` of logits are made at a time.
 
         The evaluation flavour scores with its fake-quantised cache, in one batch padded behind the texts, where nothing looks at it.  The deployment
-        flavour's prompts are attended with as they are; with ``config.adkv_prompt`` they are packed into one row axis without padding."""
+        flavour's prompts are attended with as they are; where ``config.adkv_prompt`` has its own attention run they are packed into one row axis without padding."""
         dev = self.lm_head.weight.device
         ids = [torch.as_tensor(s, dtype=torch.int64, device=dev).reshape(-1) for s in sequences]
         if not ids:
@@ -24,13 +25,11 @@ class Scores:
         if min(lengths) < 1:
             raise ValueError("a sequence needs one token at least")
         quantised = getattr(self, "scores_with_cache", False)
-        if getattr(self.config, "adkv_prompt", False) and not quantised and dev.type == "cuda":
+        if not quantised and packs(self.model, {}):
             ends = torch.tensor([0, *lengths], device="cpu").cumsum(0)
             at = torch.cat([torch.arange(n) for n in lengths]).to(dev)[None]
             total = int(ends[-1])
-            # a mask of four axes is the attention's own affair: here it says nothing
-            hidden = self.model(input_ids=torch.cat(ids)[None], position_ids=at, attention_mask=torch.ones(1, 1, 1, total, dtype=torch.bool, device=dev),
-                                cu_seq_lens_q=ends.to(dev, torch.int32), use_cache=False).last_hidden_state[0]
+            hidden = self.model(input_ids=torch.cat(ids)[None], position_ids=at, cu_seq_lens_q=ends.to(dev, torch.int32), use_cache=False).last_hidden_state[0]
             keep = torch.ones(total, dtype=torch.bool)
             keep[ends[1:] - 1] = False
             hidden = hidden[keep.to(dev)]

@@ -1,0 +1,108 @@
+"""Sequences that share a row axis (cu_seq_lens_q, score()) under config.adkv_prompt, where the framework's attention runs and where transformers' does: each of
+them is what it is by itself."""
+import pytest
+import torch
+
+pytest.importorskip("transformers")
+
+from test_hf_prompt import both, ids_of, make, config, near  # noqa: E402
+
+from adkv_amd.hf import llama_adkv, llama_adkv_eval  # noqa: E402
+from adkv_amd.hf.packed import says_nothing, takes_prompts  # noqa: E402
+
+ENDS = [0, 5, 6, 17]
+FLAVOURS = {"deployment": llama_adkv, "evaluation": llama_adkv_eval}
+
+
+def packed(device):
+    at = torch.cat([torch.arange(b - a) for a, b in zip(ENDS, ENDS[1:])])[None]
+    return dict(position_ids=at.to(device), cu_seq_lens_q=torch.tensor(ENDS, dtype=torch.int32, device=device), use_cache=False)
+
+
+@pytest.mark.parametrize("positions", [True, False])
+@pytest.mark.parametrize("implementation", ["sdpa", "eager"])
+@pytest.mark.parametrize("flavour", FLAVOURS)
+def test_packed_sequences_on_the_host(flavour, implementation, positions):
+    """Transformers' attention runs, in 64 bits: off by some hundred roundings of 2^-53 of numbers of size one."""
+    m = make(FLAVOURS[flavour].LlamaForCausalLM_ADKV, config(adkv_prompt=True, attn_implementation=implementation), torch.float64, "cpu")
+    ids, how = ids_of(1, ENDS[-1]), packed("cpu")
+    if not positions:
+        del how["position_ids"]      # rotations are relative
+    with torch.no_grad():
+        got = m(ids, **how).logits[0]
+        for a, b in zip(ENDS, ENDS[1:]):
+            # rotary angles are of 32 bits, 2^-24 of 17 radians, and the eager attention's softmax is
+            off = 1e-12 if positions and implementation == "sdpa" else 17 * 2.0 ** -18
+            assert (got[a:b] - m(ids[:, a:b], use_cache=False).logits[0]).abs().max() <= off
+
+
+def test_refused_with_packed_sequences():
+    m = make(llama_adkv.LlamaForCausalLM_ADKV, config(adkv_prompt=True), torch.float32, "cpu")
+    with pytest.raises(ValueError, match="no padding"):
+        m(ids_of(1, ENDS[-1]), attention_mask=torch.ones(1, ENDS[-1], dtype=torch.int64), **packed("cpu"))
+    with pytest.raises(ValueError, match="batch of one"):
+        m(ids_of(2, ENDS[-1]), **packed("cpu"))
+    # a mask that says nothing has nothing to say where the kernel does not run
+    assert says_nothing(torch.empty(1, 1, 0, 0, dtype=torch.bool)) and not says_nothing(torch.ones(1, 1, 1, 17)) and not says_nothing(None)
+    with pytest.raises(ValueError, match="apart"):
+        m(ids_of(1, ENDS[-1]), attention_mask=torch.empty(1, 1, 0, 0, dtype=torch.bool), **packed("cpu"))
+
+
+def test_what_the_kernel_takes():
+    at = lambda **how: make(llama_adkv.LlamaForCausalLM_ADKV, config(adkv_prompt=True, **how), torch.float32, "cpu").model.layers[0].self_attn
+    dev, attn = torch.device("cuda"), at()
+    assert takes_prompts(attn, torch.float16, dev, {}) and takes_prompts(attn, torch.bfloat16, dev, {})
+    assert not takes_prompts(attn, torch.float32, dev, {}) and not takes_prompts(attn, torch.float16, torch.device("cpu"), {})
+    assert not takes_prompts(attn, torch.float16, dev, dict(output_attentions=True)) and not takes_prompts(at(head_dim=36), torch.float16, dev, {})
+    assert not takes_prompts(at(head_dim=264), torch.float16, dev, {}) and not takes_prompts(at(output_attentions=True, attn_implementation="eager"), torch.float16, dev, {})
+    attn = at(attention_dropout=0.1)
+    assert takes_prompts(attn, torch.float16, dev, {}) and not takes_prompts(attn.train(), torch.float16, dev, {})
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("flavour", FLAVOURS)
+@pytest.mark.parametrize("why", ["type", "head size", "weights", "dropout"])
+def test_scores_by_transformers_attention(gpu, flavour, why):
+    """(Dropout of 1e-9 drops nothing.)"""
+    how = {"type": {}, "head size": dict(head_dim=36), "weights": dict(output_attentions=True, attn_implementation="eager"),
+           "dropout": dict(attention_dropout=1e-9, attn_implementation="eager")}[why]
+    if flavour == "evaluation" and why == "head size":
+        how = dict(head_dim=264)
+    mine, other, host = both(flavour, torch.float32 if why == "type" else torch.float16, gpu, **how)
+    if why == "dropout":
+        mine.train(), other.train()
+    texts = [ids_of(1, n, n)[0] for n in (40, 1, 7, 33)]
+    got, ref = mine.score(texts), other.score(texts)
+    for text, g, r in zip(texts, got, ref):
+        if len(text) > 1:
+            with torch.no_grad():
+                log = torch.log_softmax(host(text[None], use_cache=False).logits[0, :-1], -1)
+            kind = torch.float32 if why == "type" else torch.float16
+            near(g.logprobs.to(kind), r.logprobs.to(kind), log.gather(1, text[1:, None])[:, 0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("flavour", FLAVOURS)
+@pytest.mark.parametrize("why", ["", "type", "gradient", "autocast", "mask"])
+def test_packed_sequences(gpu, flavour, why, monkeypatch):
+    mine, other, host = both(flavour, torch.float32 if why in ("type", "autocast") else torch.float16, gpu)
+    ids, how = ids_of(1, ENDS[-1]), packed(gpu)
+    calls = []
+    real = llama_adkv.prompt_attention
+    monkeypatch.setattr(llama_adkv, "prompt_attention", lambda *a, **k: calls.append(k) or real(*a, **k))
+    if why == "mask":           # which goes on: the first two are one sequence then
+        of = torch.tensor([0] * ENDS[2] + [1] * (ENDS[3] - ENDS[2]))
+        how["attention_mask"] = ((of[:, None] == of) & torch.ones(17, 17).tril().bool())[None, None].to(gpu)
+    with torch.set_grad_enabled(why == "gradient"), torch.autocast("cuda", torch.float16, enabled=why == "autocast"):
+        got = mine(ids.to(gpu), **how).logits[0].detach()
+        ends = [0, ENDS[2], ENDS[3]] if why == "mask" else ENDS
+        if why == "mask":
+            how["position_ids"][:, :ENDS[2]] = torch.arange(ENDS[2])
+            got = mine(ids.to(gpu), **how).logits[0]
+        ref = torch.cat([other(ids[:, a:b].to(gpu), use_cache=False).logits[0] for a, b in zip(ends, ends[1:])]).detach()
+    assert len(calls) == (2 if why == "" else 0) and all("bounds" in k for k in calls)
+    with torch.no_grad():
+        exact = torch.cat([host(ids[:, a:b], use_cache=False).logits[0] for a, b in zip(ends, ends[1:])])
+    if why == "autocast":
+        got, ref = got.half(), ref.half()
+    near(got, ref, exact)
