@@ -100,6 +100,11 @@ class KVCacheLayer_ADKV:
         if self._valid:      # there are buffers
             self._valid[self._span] = b"\1" * self._B if valid else bytes(self._B)
 
+    def _look(self) -> None:
+        """A batch view is one of what its parent holds; the parent empties the bytes when its sequences leave that memory."""
+        if self._shares_storage and not self._valid:
+            raise RuntimeError("the cache that this is a view of holds other sequences by now")
+
     # ------------------------------------------------------------------ HF cache protocol
     def get_seq_length(self) -> int:
         return self._quant_len + self._prefix_len()
@@ -197,6 +202,7 @@ class KVCacheLayer_ADKV:
         through it, then ``commit`` the parent."""
         if self._key_buf is None or not 0 <= b0 < b1 <= self._B:
             raise ValueError("batch_view needs a reserved cache and a slice inside its batch")
+        self._look()
         v = KVCacheLayer_ADKV(self._bits)
         v._B, v._H, v._C, v._device = b1 - b0, self._H, self._C, self._device
         v._ckpt_interval, v._cap_len, v._quant_len = self._ckpt_interval, self._cap_len, self._quant_len
@@ -221,6 +227,7 @@ class KVCacheLayer_ADKV:
             raise NotImplementedError("a cache is shared before it is decoded with")
         if B < 1:
             raise ValueError("share needs at least one sequence")
+        self._look()
         v = KVCacheLayer_ADKV(self._bits)
         v._ckpt_interval = self._ckpt_interval
         ends = [tuple(st[0, :, :, i].contiguous() for i in range(2)) for st in (self._key_state, self._value_state)]
@@ -231,6 +238,7 @@ class KVCacheLayer_ADKV:
     def commit(self, tokens: int) -> None:
         """Declare that every sequence now holds ``tokens`` quantised tokens (all slices prefilled).  The carried state goes along
         unless a slice was decoded or extended with."""
+        self._look()
         tokens -= self._prefix_len()
         if tokens > self._cap_len:
             raise ValueError("more tokens than the cache holds")
@@ -285,6 +293,7 @@ class KVCacheLayer_ADKV:
                 key_zp_init, key_scale_init, key_alpha, key_beta, key_quant_target,
                 value_zp_init, value_scale_init, value_alpha, value_beta, value_quant_target):
         """Quantise the prompt into the cache.  No attention is computed here."""
+        self._look()
         B, H, T, C = key_states.shape
         if value_states.shape != key_states.shape:
             raise ValueError("key/value shapes differ")
@@ -327,6 +336,7 @@ class KVCacheLayer_ADKV:
         """One causal decode step: attend over the cached tokens and the new one, append the new
         K/V codes, return ``(output [B,H,C] in the query's dtype, weights [B,H,ctx+1] fp16)``
         (weights ``None`` behind a shared prefix).  A mask is additive, or boolean (true where a token is looked at)."""
+        self._look()
         ctx = self._quant_len
         if self._prefix is not None:
             if query_states.shape[2] != 1 or key_states.shape[2] != 1:
@@ -395,6 +405,7 @@ class KVCacheLayer_ADKV:
         drafted tokens to be checked, the questions behind a shared prompt.  Queries ``[B, Hq, n, C]``, keys and values
         ``[B, H, n, C]``; returns ``[B, n, Hq, C]`` in the query's dtype.  ``n`` calls of ``decode`` append the same codes and
         give the same outputs up to rounding.  A mask is additive, or boolean (true where a token is looked at)."""
+        self._look()
         B, _, n, C = query_states.shape
         H = key_states.shape[1]
         if key_states.shape != value_states.shape or key_states.shape[2] != n:
@@ -422,6 +433,7 @@ class KVCacheLayer_ADKV:
     # ------------------------------------------------------------------ sequences that take each other's place
     def _tensors(self):
         """The layer's tensors with a row per sequence, and how many entries of each head hold anything."""
+        self._look()
         T, S = self._quant_len, self._ckpt_interval
         found = [(t, self._n_super(T)) for t in (self._key_buf, self._value_buf)]
         if self._key_ckpt is not None:
@@ -439,9 +451,10 @@ class KVCacheLayer_ADKV:
             new = bytes(old[r] for r in where)
         else:
             new = bytes(rows) if 0 in old else b"\1" * rows       # of some it is not: of none then
-        if self._shares_storage:
+        if rows == self._B:      # in place: slices of it go on, and mark the same bytes
             self._valid[self._span] = new
         else:
+            self._valid.clear()
             self._valid, self._span = bytearray(new), slice(0, rows)
         self._B = rows
 
@@ -450,6 +463,7 @@ class KVCacheLayer_ADKV:
         """Everything needed to continue decoding elsewhere: the used part of the code buffers, the
         state checkpoints that go with them and, while it is still valid, the carried filter state.
         Plain tensors and ints, so ``torch.save`` / ``torch.load(weights_only=True)`` round-trip it."""
+        self._look()
         if self._key_buf is None:
             return {"quant_len": 0}
         ns = self._n_super(self._quant_len)
@@ -587,7 +601,7 @@ class KVCache_ADKV(list):
 
     def batch_select_indices(self, indices: torch.Tensor) -> None:
         """The sequences ``indices``, in that order, are the batch from now on: in place where there are not more of them than before (the memory of the
-        others is the cache's still), else in new memory."""
+        others is the cache's still), else in new memory.  Batch views made before can't be used any more if the number of sequences changes."""
         B = max((layer._B for layer in self if layer._key_buf is not None), default=0)
         if indices.dtype == torch.bool:
             if indices.shape != (B,) and B:
@@ -599,7 +613,7 @@ class KVCache_ADKV(list):
 
     def batch_repeat_interleave(self, repeats: int) -> None:
         """Every sequence ``repeats`` times, one after the other, in new memory: several answers to each prompt that go different ways (``share`` keeps one
-        prompt once where all of them begin with it)."""
+        prompt once where all of them begin with it).  Batch views made before can't be used any more."""
         if repeats < 1:
             raise ValueError("batch_repeat_interleave needs one of each at least")
         B = max((layer._B for layer in self if layer._key_buf is not None), default=0)

@@ -205,6 +205,36 @@ def test_what_is_known_of_the_states(monkeypatch):
     same(c, filled(4), 4, torch.tensor([0, 2, 1, 3]))
 
 
+def test_views_of_what_moved(monkeypatch):
+    """A slice that is stepped after its parent's sequences took each other's place is known to be; one of a batch that is another one by now is refused."""
+    monkeypatch.setattr(cache_module, "take_sequences", as_indexing)
+    for change in (lambda c: c.reorder_cache(torch.tensor([3, 2, 1, 0])), lambda c: c.batch_select_indices(torch.tensor([1, 0, 3, 2])), lambda c: c.batch_repeat_interleave(1)):
+        c = filled(4)
+        view = c.batch_view(1, 3)
+        change(c)
+        assert view[0].key_states.data_ptr() == c[0].key_states[1:].data_ptr()
+        view[0]._state_valid = False                                # stepped
+        assert not c[0]._state_valid and bytes(c[0]._valid) == b"\1\0\0\1" and c[1]._state_valid
+        view.batch_view(1, 2)[1]._state_valid = False
+        assert bytes(c[1]._valid) == b"\1\1\0\1"
+    x = torch.zeros(2, 2, 1, D)
+    for change in (lambda c: c.batch_select_indices(torch.tensor([0, 1])), lambda c: c.batch_repeat_interleave(2), lambda c: c.batch_select_indices(torch.arange(4).repeat(2))):
+        c = filled(4)
+        view, part = c.batch_view(1, 3), c.batch_view(0, 3).batch_view(1, 2)
+        change(c)
+        assert c[0]._state_valid and c.batch_view(0, 2)[0]._state_valid
+        for v in (view, part):
+            for use in (lambda: v[0].prefill(x, x, *[None] * 10), lambda: v[0].decode(x, x, x, *[None] * 10), lambda: v[0].extend(x, x, x, *[None] * 10), lambda: v.batch_view(0, 1),
+                        lambda: v.commit(300), lambda: v.reorder_cache(torch.arange(v[0]._B)), lambda: v[0].state_dict()):
+                with pytest.raises(RuntimeError, match="other sequences"):
+                    use()
+    c = filled(1)
+    view = c.batch_view(0, 1)
+    c.batch_repeat_interleave(2)
+    with pytest.raises(RuntimeError, match="other sequences"):
+        view.share(2)
+
+
 def test_refused_moves(monkeypatch):
     monkeypatch.setattr(cache_module, "take_sequences", as_indexing)
     c = filled(3)
