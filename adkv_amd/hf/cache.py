@@ -80,6 +80,7 @@ class KVCacheLayer_ADKV:
         # whether a sequence's is that behind its last token, a byte per sequence, and the sequences that are this object's: a batch_view()
         # has its parent's bytes, which is how the parent knows that a slice was stepped
         self._valid, self._span = bytearray(), slice(0, 0)
+        self._reached: list = []  # tokens that a slice had of each sequence when it was last stepped, shared in the same way
         self._quant_len = 0
         self._cap_len = 0
         self._B = self._H = self._C = 0
@@ -104,6 +105,12 @@ class KVCacheLayer_ADKV:
         """A batch view is one of what its parent holds; the parent empties the bytes when its sequences leave that memory."""
         if self._shares_storage and not self._valid:
             raise RuntimeError("the cache that this is a view of holds other sequences by now")
+
+    def _stepped(self, tokens: int, state_valid: bool) -> None:
+        self._quant_len += tokens
+        self._state_valid = state_valid
+        if self._shares_storage:
+            self._reached[self._span] = [self._quant_len] * self._B
 
     # ------------------------------------------------------------------ HF cache protocol
     def get_seq_length(self) -> int:
@@ -166,7 +173,7 @@ class KVCacheLayer_ADKV:
          self._key_ckpt, self._value_ckpt) = self._new_buffers(tokens, alloc)
         mk = lambda: alloc((B, H, C, 2), dtype=torch.float16, device=device)
         self._key_state, self._value_state = mk(), mk()
-        self._valid, self._span = bytearray(b"\1" * B), slice(0, B)
+        self._valid, self._span, self._reached = bytearray(b"\1" * B), slice(0, B), [0] * B
 
     def _cap_buffers(self, T: int):
         """Make room for ``T`` tokens.  New slots are zero, as the append kernels expect."""
@@ -210,6 +217,7 @@ class KVCacheLayer_ADKV:
         if self._key_ckpt is not None:
             v._key_ckpt, v._value_ckpt = self._key_ckpt[b0:b1], self._value_ckpt[b0:b1]
         v._key_state, v._value_state = self._key_state[b0:b1], self._value_state[b0:b1]
+        v._reached = self._reached
         v._valid, v._span = self._valid, slice(self._span.start + b0, self._span.start + b1)
         v._shares_storage = True
         v._prefix = self._prefix
@@ -286,8 +294,7 @@ class KVCacheLayer_ADKV:
             self._own((value_zp_init, value_scale_init, value_alpha, value_beta, value_quant_target), 1),
             self._quant_len, self._key_state, self._value_state,
             k_ckpt=self._key_ckpt, v_ckpt=self._value_ckpt, ckpt_interval=self._ckpt_interval, bits=self._bits, fresh=fresh)
-        self._quant_len += key_states.shape[2]
-        self._state_valid = True
+        self._stepped(key_states.shape[2], True)
 
     def prefill(self, key_states, value_states,
                 key_zp_init, key_scale_init, key_alpha, key_beta, key_quant_target,
@@ -336,7 +343,8 @@ class KVCacheLayer_ADKV:
         """One causal decode step: attend over the cached tokens and the new one, append the new
         K/V codes, return ``(output [B,H,C] in the query's dtype, weights [B,H,ctx+1] fp16)``
         (weights ``None`` behind a shared prefix).  A mask is additive, or boolean (true where a token is looked at)."""
-        self._look()
+        if self._shares_storage:
+            self._look()
         ctx = self._quant_len
         if self._prefix is not None:
             if query_states.shape[2] != 1 or key_states.shape[2] != 1:
@@ -357,7 +365,10 @@ class KVCacheLayer_ADKV:
             if r is not None:      # None: something to check, convert, allocate or complain about below
                 if isinstance(r, int):
                     _lib.check(r, "decode_step")
-                self._quant_len, self._state_valid = ctx + 1, False
+                if self._shares_storage:
+                    self._stepped(1, False)
+                else:
+                    self._quant_len, self._state_valid = ctx + 1, False
                 return r
         B, Hq, Tq, C = query_states.shape
         H, Tk = key_states.shape[1], key_states.shape[2]
@@ -387,8 +398,7 @@ class KVCacheLayer_ADKV:
             ctx, scaling, attention_mask,
             k_ckpt=self._key_ckpt, v_ckpt=self._value_ckpt, ckpt_interval=S, bits=self._bits,
             workspace=ws)
-        self._quant_len = ctx + 1
-        self._state_valid = False
+        self._stepped(1, False)
         return (out if out.dtype == query_states.dtype else out.to(query_states.dtype)), weights
 
     # ------------------------------------------------------------------ several tokens
@@ -426,8 +436,7 @@ class KVCacheLayer_ADKV:
         out = extend(act(query_states), self._key_buf, self._value_buf, act(key_states), act(value_states),
                      self._own(key, 0), self._own(value, 1), self._quant_len, scaling, attention_mask, prefix=prefix,
                      k_ckpt=self._key_ckpt, v_ckpt=self._value_ckpt, ckpt_interval=self._ckpt_interval, bits=self._bits)
-        self._quant_len += n
-        self._state_valid = False
+        self._stepped(n, False)
         return out if out.dtype == query_states.dtype else out.to(query_states.dtype)
 
     # ------------------------------------------------------------------ sequences that take each other's place
@@ -455,7 +464,7 @@ class KVCacheLayer_ADKV:
             self._valid[self._span] = new
         else:
             self._valid.clear()
-            self._valid, self._span = bytearray(new), slice(0, rows)
+            self._valid, self._span, self._reached = bytearray(new), slice(0, rows), [0] * rows
         self._B = rows
 
     # ------------------------------------------------------------------ save / restore
@@ -576,6 +585,8 @@ class KVCache_ADKV(list):
             raise ValueError("the layers hold different numbers of sequences")
         if any(layer._shares_storage for layer in layers) and (fresh or rows != B):
             raise ValueError("a batch view has as many sequences as it was made with")
+        if any(n > layer._quant_len for layer in layers for n in layer._reached[layer._span]):
+            raise ValueError("slices of the batch hold more tokens than it knows of: commit() them first")
         where = None
         if not index.is_cuda:
             where = index.tolist()

@@ -235,6 +235,30 @@ def test_views_of_what_moved(monkeypatch):
         view.share(2)
 
 
+def test_slices_that_are_further_than_their_batch(monkeypatch):
+    """What a slice has been prefilled or stepped with does not move before the batch knows of it: the states would move without the codes."""
+    monkeypatch.setattr(cache_module, "take_sequences", as_indexing)
+    monkeypatch.setattr(cache_module, "append_kv_pair", lambda *a, **k: None)
+    x = torch.zeros(2, 2, 7, D)
+    moves = (lambda c: c.reorder_cache(torch.tensor([3, 2, 1, 0])), lambda c: c.batch_select_indices(torch.tensor([0, 3])), lambda c: c.batch_repeat_interleave(2))
+    for move in moves:
+        c, was = filled(4), filled(4)
+        c.batch_view(0, 2)[0].prefill(x, x, *[None] * 10)
+        with pytest.raises(ValueError, match="commit"):
+            move(c)
+        same(c, was, 4, torch.arange(4))
+        c.batch_view(2, 4)[0].prefill(x, x, *[None] * 10)
+        c.commit(307)
+        move(c)
+        c.batch_view(0, 2).reorder_cache(torch.tensor([1, 0]))
+    c = filled(4)
+    for layer in c.batch_view(1, 3):
+        layer.prefill(x, x, *[None] * 10)
+    c.batch_view(0, 1).reorder_cache(torch.tensor([0]))             # another slice
+    with pytest.raises(ValueError, match="commit"):
+        c.batch_view(0, 2).reorder_cache(torch.tensor([1, 0]))
+
+
 def test_refused_moves(monkeypatch):
     monkeypatch.setattr(cache_module, "take_sequences", as_indexing)
     c = filled(3)
