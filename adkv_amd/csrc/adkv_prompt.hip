@@ -344,12 +344,14 @@ struct Mask {
     }
 };
 
+constexpr float LOWEST = -3.0e38f; // of scores, in powers of two
+
 // Score s of a key to which x is added, c being the scaling, all in powers of two.  A type's lowest value times log2(e) would be -inf, which stands for
 // hidden keys only: rows of nothing but lowest values look at all of them alike.
 __device__ __forceinline__ float with(float s, float x, float c)
 {
     const float y = __builtin_fmaf(x, LOG2E, s * c);
-    return x == -INFINITY ? -INFINITY : y < -3.0e38f ? -3.0e38f : y; // what is no number stays that
+    return x == -INFINITY ? -INFINITY : y < LOWEST ? LOWEST : y; // what is no number stays that
 }
 
 // A wave's 32 rows; MASK: bytes of a key's mask, 0 without one
@@ -495,11 +497,12 @@ struct Wave {
             x[e] = sc[e >> 4][e & 15];
         float unit = c, more = 0.0f; // of x; with something added they are in powers of two
         if (MASK > 1 && all == 2) {
-            // The same for all keys, a type's lowest value in front of a padded text: added to the reference, not to every score.  Where that leaves nothing of
-            // the scores they are next to nothing, where it would leave little of them they are rounded one by one, as beside other masks.
+            // The same for all keys, a type's lowest value in front of a padded text: added to the reference, not to every score.  Where it would leave little
+            // or nothing of the scores they are rounded one by one, as beside other masks, so that a row's keys are alike whatever tile they are in; where
+            // with() makes the same of all of them the scores are next to nothing.
             more = masked.template of<0>(a.mask_dt) * LOG2E;
-            if (more < -1e30f) {
-                more = -3.0e38f;
+            if (more < LOWEST) {
+                more = LOWEST;
                 unit = 1e-30f;
             } else if (!(fabsf(more) < 131072.0f)) {
                 more = 0.0f;

@@ -506,7 +506,7 @@ int adkv_fp16_decode(const void *q, const void *K, const void *V, void *out, voi
  *   element strides of batch, head and token in *_strides (multiples of 8).  out [B, Tq, Hq, D], packed, 16-byte aligned, of their type.
  *   mask (may be NULL): element strides of batch, head and query token in mask_strides (0 where it is the same for all), keys contiguous; added
  *   to the scores (fp16, bfloat16, fp32; minus infinity hides a key whatever it and its value hold), or ADKV_DT_BOOL.  A row of nothing but
- *   its type's lowest value looks at all keys up to its own alike.
+ *   its type's lowest value looks at all keys up to its own alike.  What is below -2e38 is taken for the lowest.
  *   bounds (n_seq > 0): n_seq sequences share the row axis, B = 1, Tq = Tk, no mask: sequence i is rows bounds[i] .. bounds[i + 1] - 1,
  *   n_seq + 1 ascending int32 from 0 to Tq; other rows are zeros.  A sequence may be empty.
  *   dtype: of q, k, v, out, plus the mask's << 8.

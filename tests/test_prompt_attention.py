@@ -303,6 +303,32 @@ def test_the_same_added_to_many_keys(gpu, size, dtype, value):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("value", [-1e29, -1e30, -1e32, -2e38, -2.2e38, -3e38])
+@pytest.mark.parametrize("dtype", [torch.float32, BF16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("size", [(20, 16, 1, 300, 300, 128), (2, 8, 1, 1101, 1101, 96), (1, 4, 2, 300, 301, 64), (1, 2, 1, 260, 300, 256)], ids=str)
+def test_large_values_that_stand_for_hidden_keys(gpu, size, dtype, value):
+    """In front of every text, over whole tiles and the beginning of one: rows that look at nothing else look at all of it alike, whatever tile a key is in.
+
+    The scores are less than half a step of such a value, so that these rows' weights are equal: the output is a mean, of sums with a rounding of 2^-24 for each key,
+    divided and rounded once more.  Other rows see nothing of it."""
+    B, H, g, Tq, Tk, D = size
+    q, k, v = qkv(*size, F16, gpu)
+    n = 100
+    m = torch.zeros(B, 1, Tq, Tk, dtype=dtype, device=gpu)
+    m[..., :n] = value
+    got = gemv.prompt_attention(q, k, v, D ** -0.5, m).cpu().double()
+    first = n - (Tk - Tq)
+    of = v[0].cpu().double().repeat_interleave(g, 0)[:, :n]
+    seen = torch.arange(1, n + 1)[:, None]
+    mean, size_of = of.cumsum(1) / seen, of.abs().cumsum(1) / seen
+    want, off = (t[:, n - first:].transpose(0, 1) for t in (mean, 2.0 ** -11 * mean.abs() + (seen + 4) * 2.0 ** -24 * size_of + 2.0 ** -25))
+    d = (got[0, :first] - want).abs() - off
+    assert d.max() <= 0, f"{float((got[0, :first] - want).abs().max()):.3e}, {float(d.max()):.3e} more than may be"
+    want, off = plain(q[:1], k[:1], v[:1], D ** -0.5, m[:1].masked_fill(m[:1] != 0, -math.inf))
+    check(got[:1, first:], want[:, first:], off[:, first:])
+
+
+@pytest.mark.gpu
 def test_lowest_values_of_64_bits(gpu):
     """They are the lowest of 32 bits to the kernel, not minus infinity: rows of nothing else look at all tokens up to their own alike."""
     q, k, v = qkv(2, 2, 1, 50, 50, 64, F16, gpu)
