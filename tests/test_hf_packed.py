@@ -106,3 +106,36 @@ def test_packed_sequences(gpu, flavour, why, monkeypatch):
     if why == "autocast":
         got, ref = got.half(), ref.half()
     near(got, ref, exact)
+
+
+def test_scores_of_quantised_prompts_are_the_evaluation_models():
+    m = make(llama_adkv.LlamaForCausalLM_ADKV, config(), torch.float32, "cpu")
+    with pytest.raises(ValueError, match="evaluation"):
+        m.score([[1, 2]], prefill_full_precision=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("prompt", [True, False])
+def test_scores_show_what_quantisation_costs(gpu, prompt):
+    """What the model itself gives for the same batch; other parameters of the quantiser give other scores, and none where prompts are attended with as they are."""
+    mine = make(llama_adkv_eval.LlamaForCausalLM_ADKV, config(adkv_prompt=prompt), torch.float32, gpu)
+    texts = [ids_of(1, n, n)[0] for n in (40, 1, 7, 33)]
+    batch = torch.nn.utils.rnn.pad_sequence(texts, batch_first=True).to(gpu)
+    found = {}
+    for target in (3.5, 0.5):
+        for layer in mine.model.layers:
+            for side in ("key", "value"):
+                getattr(layer.self_attn, f"{side}_quant_target").fill_(target)
+        for full in (True, False, None):
+            found[target, full] = torch.cat([s.logprobs for s in mine.score(texts, prefill_full_precision=full)])
+        with torch.no_grad():
+            logits = mine(batch, use_cache=True, prefill_full_precision=False).logits
+        want = torch.cat([torch.log_softmax(x[:len(t) - 1].double(), -1).gather(1, t[1:, None].to(gpu))[:, 0] for x, t in zip(logits, texts)])
+        # one logit per token from a product of other rows: 256 roundings of 2^-24 of numbers of size one
+        assert (found[target, False] - want).abs().max() <= 2.0 ** -14
+        assert torch.equal(found[target, True], found[target, None])
+        mine.config.prefill_full_precision = False
+        assert torch.equal(found[target, False], torch.cat([s.logprobs for s in mine.score(texts)]))
+        del mine.config.prefill_full_precision
+    assert torch.equal(found[3.5, True], found[0.5, True])
+    assert (found[3.5, False] - found[0.5, False]).abs().max() > 2.0 ** -10 and (found[3.5, False] - found[3.5, True]).abs().max() > 2.0 ** -10
