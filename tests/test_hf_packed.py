@@ -108,6 +108,32 @@ def test_packed_sequences(gpu, flavour, why, monkeypatch):
     near(got, ref, exact)
 
 
+def test_groups_of_sequences():
+    from adkv_amd.hf.score import _groups
+    lengths = [3, 9, 1, 30, 9, 2, 1]
+    assert list(_groups(lengths, 20, True)) == [[3], [1, 4], [0, 5, 2, 6]] and list(_groups(lengths, 20, False)) == [[3], [1, 4], [0, 5, 2, 6]]
+    assert list(_groups(lengths, 10, False)) == [[3], [1], [4], [0, 5, 2], [6]] and list(_groups(lengths, 10, True)) == [[3], [1], [4], [0, 5, 2, 6]]
+    assert list(_groups([5] * 4, 10, True)) == [[0, 1], [2, 3]] and list(_groups([], 10, True)) == [] and list(_groups([4, 4], 1, False)) == [[0], [1]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("flavour,how", [("deployment", {}), ("deployment", dict(adkv_prompt=True)), ("evaluation", {}), ("evaluation", dict(prefill_full_precision=False))], ids=str)
+def test_scores_a_few_texts_at_a_time(gpu, flavour, how, monkeypatch):
+    """No run of the model has more tokens than were asked for, and all of them are scored: as by themselves, but for the roundings of products over other rows
+    (and for what these change in codes)."""
+    m = make(FLAVOURS[flavour].LlamaForCausalLM_ADKV, config(**how), torch.float16, gpu)
+    texts = [ids_of(1, n, n)[0] for n in (40, 1, 7, 133, 2, 41, 39)]
+    shapes, real = [], m.model.forward
+    monkeypatch.setattr(m.model, "forward", lambda *a, **k: shapes.append(k["input_ids"].shape) or real(*a, **k))
+    got = m.score(texts, top=2, tokens=90)
+    assert [tuple(s) for s in shapes] == ([(1, 133), (1, 81), (1, 49)] if "adkv_prompt" in how else [(1, 133), (2, 41), (2, 39), (2, 2)])
+    for t, g in zip(texts, got):
+        alone = m.score([t], top=2)[0]
+        assert g.logprobs.shape == (len(t) - 1,) and g.top_tokens.shape == (len(t) - 1, 2)
+        if len(t) > 1 and how.get("prefill_full_precision", True):
+            assert (g.logprobs - alone.logprobs).abs().max() <= 2.0 ** -6 and (g.entropy - alone.entropy).abs().max() <= 2.0 ** -6
+
+
 def test_scores_of_quantised_prompts_are_the_evaluation_models():
     m = make(llama_adkv.LlamaForCausalLM_ADKV, config(), torch.float32, "cpu")
     with pytest.raises(ValueError, match="evaluation"):
