@@ -27,7 +27,7 @@ from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
 from ..kernel.gemv import prompt_attention, rope_norm_qk, rope_qk
 from .cache import (CAP_LEN, INIT_SEQ_LEN, SCALE_MAX, SCALE_MIN, KVCache_ADKV,  # noqa: F401
                     KVCacheLayer_ADKV)
-from .packed import packed_mask, says_nothing, takes_prompts
+from .packed import derivatives_wanted, packed_mask, says_nothing, takes_prompts
 from .score import Scores
 
 # the five per-(head, channel) quantities, for K and for V (reference llama_adkv.py:27)
@@ -63,7 +63,7 @@ def norm_and_rotate(attn, q, k, cos, sin):
 
 def prompt_ctx(attn, q, k, v, attention_mask, cached: bool, kwargs) -> torch.Tensor | None:
     """config.adkv_prompt: the dense rows' attention ``[B, T, Hq, C]`` by the framework's own kernel, without weights; None where transformers' is to
-    run (``takes_prompts``; where a gradient is wanted).  With ``cu_seq_lens_q`` (transformers' name for the bounds of sequences packed into one row
+    run (``takes_prompts``; where a derivative is wanted).  With ``cu_seq_lens_q`` (transformers' name for the bounds of sequences packed into one row
     axis) each sequence looks at itself only."""
     if not getattr(attn.config, "adkv_prompt", False):
         return None
@@ -71,8 +71,7 @@ def prompt_ctx(attn, q, k, v, attention_mask, cached: bool, kwargs) -> torch.Ten
     if bounds is not None and cached:
         raise ValueError("packed sequences have no cache: pass use_cache=False")
     apart = says_nothing(attention_mask)
-    if not takes_prompts(attn, q.dtype, q.device, kwargs) or not k.dtype == v.dtype == q.dtype \
-            or (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v))):
+    if not takes_prompts(attn, q.dtype, q.device, kwargs) or not k.dtype == v.dtype == q.dtype or derivatives_wanted(q, k, v, attention_mask):
         if apart:
             raise ValueError("packed sequences that nothing keeps apart: give their mask, or call the model without one")
         return None

@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 
 def takes_prompts(attn, dtype, device, kwargs) -> bool:
@@ -10,6 +11,12 @@ def takes_prompts(attn, dtype, device, kwargs) -> bool:
     return bool(getattr(attn.config, "adkv_prompt", False) and device.type == "cuda" and dtype in (torch.float16, torch.bfloat16)
                 and attn.head_dim % 8 == 0 and attn.head_dim <= 256 and not (attn.training and attn.attention_dropout > 0)
                 and not kwargs.get("output_attentions") and not getattr(attn.config, "output_attentions", False))
+
+
+def derivatives_wanted(*tensors) -> bool:
+    """Of what is computed from them: backward, forward, or a transform's."""
+    return any((t.requires_grad and torch.is_grad_enabled()) or torch._C._functorch.is_functorch_wrapped_tensor(t) or forward_ad.unpack_dual(t).tangent is not None
+               for t in tensors if isinstance(t, torch.Tensor))
 
 
 def packs(model, kwargs) -> bool:

@@ -165,3 +165,36 @@ def test_scores_show_what_quantisation_costs(gpu, prompt):
         del mine.config.prefill_full_precision
     assert torch.equal(found[3.5, True], found[0.5, True])
     assert (found[3.5, False] - found[0.5, False]).abs().max() > 2.0 ** -10 and (found[3.5, False] - found[3.5, True]).abs().max() > 2.0 ** -10
+
+
+# ------------------------------------------------------------------------------------------------ where transformers' attention runs without packed sequences
+def rows_of(gpu, T=9, seed=0):
+    g = torch.Generator(device=gpu).manual_seed(seed)
+    return tuple(torch.randn(1, h, T, 128, generator=g, device=gpu).half() for h in (4, 2, 2))
+
+
+@pytest.mark.gpu
+def test_derivatives_are_transformers(gpu, monkeypatch):
+    """A tangent of the activations, a transform around the call, a mask that is learned; the evaluation model's tangents are those without the flag."""
+    mine, other, _ = both("evaluation", torch.float16, gpu, attn_implementation="eager")
+    monkeypatch.setattr(llama_adkv, "prompt_attention", lambda *a, **k: pytest.fail("not for this call"))
+    attn = mine.model.layers[0].self_attn
+    q, k, v = rows_of(gpu)
+    with torch.no_grad(), torch.autograd.forward_ad.dual_level():
+        for i in range(3):
+            t = [q, k, v]
+            t[i] = torch.autograd.forward_ad.make_dual(t[i], torch.ones_like(t[i]))
+            assert llama_adkv.prompt_ctx(attn, *t, None, False, {}) is None
+    with torch.no_grad():
+        none = []
+        torch.func.vmap(lambda x: none.append(llama_adkv.prompt_ctx(attn, x, k, v, None, False, {})) or x)(q[None])
+        torch.func.jvp(lambda x: none.append(llama_adkv.prompt_ctx(attn, q, k, x, None, False, {})) or x, (v,), (v,))
+        assert none == [None, None]
+    assert llama_adkv.prompt_ctx(attn, q, k, v, torch.zeros(1, 1, 9, 9, device=gpu, requires_grad=True), False, {}) is None
+    found = []
+    for m in (mine, other):
+        with torch.no_grad(), torch.autograd.forward_ad.dual_level():
+            x = m.model.embed_tokens(ids_of(1, 9).to(gpu))
+            out = m(inputs_embeds=torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)), use_cache=False).logits
+            found += list(torch.autograd.forward_ad.unpack_dual(out))
+    assert found[1] is not None and torch.equal(found[0], found[2]) and torch.equal(found[1], found[3])
