@@ -79,8 +79,8 @@ def prompt_ctx(attn, q, k, v, attention_mask, cached: bool, kwargs) -> torch.Ten
         # with a mask of its own transformers' attention runs, which goes by that
         return prompt_attention(q, k, v, attn.scaling, bounds=bounds) if apart or attention_mask is None else None
     if attention_mask is not None:
-        if attention_mask.dim() != 4 or attention_mask.shape[-1] < k.shape[2]:
-            return None
+        if not isinstance(attention_mask, torch.Tensor) or attention_mask.dim() != 4 or attention_mask.shape[-1] < k.shape[2]:
+            return None                # flex_attention's masks are objects of its own
         attention_mask = attention_mask[..., :k.shape[2]]
     return prompt_attention(q, k, v, attn.scaling, attention_mask)
 

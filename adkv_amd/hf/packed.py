@@ -35,7 +35,7 @@ def packed_mask(model, tokens: torch.Tensor, attention_mask, kwargs):
     """The mask for a model's ``tokens [1, T, ..]`` where config.adkv_prompt has each of the sequences that ``cu_seq_lens_q`` bounds look at itself only: one
     that says nothing where ``prompt_attention`` sees to that, else what transformers' own attention needs for it, ``[1, 1, T, T]``."""
     bounds = kwargs.get("cu_seq_lens_q")
-    if bounds is None or not getattr(model.config, "adkv_prompt", False) or (attention_mask is not None and attention_mask.ndim != 2):
+    if bounds is None or not getattr(model.config, "adkv_prompt", False) or (attention_mask is not None and getattr(attention_mask, "ndim", 4) != 2):
         return attention_mask
     if attention_mask is not None:
         raise ValueError("packed sequences have no padding: pass no attention_mask")

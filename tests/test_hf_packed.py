@@ -8,7 +8,7 @@ pytest.importorskip("transformers")
 from test_hf_prompt import both, ids_of, make, config, near  # noqa: E402
 
 from adkv_amd.hf import llama_adkv, llama_adkv_eval  # noqa: E402
-from adkv_amd.hf.packed import says_nothing, takes_prompts  # noqa: E402
+from adkv_amd.hf.packed import packed_mask, says_nothing, takes_prompts  # noqa: E402
 
 ENDS = [0, 5, 6, 17]
 FLAVOURS = {"deployment": llama_adkv, "evaluation": llama_adkv_eval}
@@ -42,6 +42,8 @@ def test_refused_with_packed_sequences():
         m(ids_of(1, ENDS[-1]), attention_mask=torch.ones(1, ENDS[-1], dtype=torch.int64), **packed("cpu"))
     with pytest.raises(ValueError, match="batch of one"):
         m(ids_of(2, ENDS[-1]), **packed("cpu"))
+    theirs = object()                  # a mask that is no tensor goes on
+    assert packed_mask(m.model, ids_of(1, 17), theirs, packed("cpu")) is theirs
     # a mask that says nothing has nothing to say where the kernel does not run
     assert says_nothing(torch.empty(1, 1, 0, 0, dtype=torch.bool)) and not says_nothing(torch.ones(1, 1, 1, 17)) and not says_nothing(None)
     with pytest.raises(ValueError, match="apart"):
@@ -198,3 +200,16 @@ def test_derivatives_are_transformers(gpu, monkeypatch):
             out = m(inputs_embeds=torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)), use_cache=False).logits
             found += list(torch.autograd.forward_ad.unpack_dual(out))
     assert found[1] is not None and torch.equal(found[0], found[2]) and torch.equal(found[1], found[3])
+
+
+@pytest.mark.gpu
+def test_masks_of_other_kinds_are_transformers(gpu, monkeypatch):
+    """flex_attention's, and those that are not of four axes or too short."""
+    from torch.nn.attention.flex_attention import create_block_mask
+    attn = make(llama_adkv.LlamaForCausalLM_ADKV, config(adkv_prompt=True), torch.float16, gpu).model.layers[0].self_attn
+    monkeypatch.setattr(llama_adkv, "prompt_attention", lambda *a, **k: pytest.fail("not for this call"))
+    rows = rows_of(gpu)
+    with torch.no_grad():
+        for mask in (create_block_mask(lambda b, h, i, j: i >= j, 1, 1, 9, 9, device=gpu), torch.ones(1, 9, dtype=torch.bool, device=gpu), torch.ones(1, 1, 9, 8, dtype=torch.bool, device=gpu)):
+            for how in ({}, dict(cu_seq_lens_q=torch.tensor([0, 4, 9], dtype=torch.int32, device=gpu))):
+                assert llama_adkv.prompt_ctx(attn, *rows, mask, False, how) is None
