@@ -27,7 +27,7 @@ from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
 from ..kernel.gemv import prompt_attention, rope_norm_qk, rope_qk
 from .cache import (CAP_LEN, INIT_SEQ_LEN, SCALE_MAX, SCALE_MIN, KVCache_ADKV,  # noqa: F401
                     KVCacheLayer_ADKV)
-from .packed import derivatives_wanted, packed_mask, says_nothing, takes_prompts
+from .packed import derivatives_wanted, packed_mask, refuse_cache, says_nothing, takes_prompts
 from .score import Scores
 
 # the five per-(head, channel) quantities, for K and for V (reference llama_adkv.py:27)
@@ -61,15 +61,13 @@ def norm_and_rotate(attn, q, k, cos, sin):
     return apply_rotary_pos_emb(attn.q_norm(q), attn.k_norm(k), cos, sin)
 
 
-def prompt_ctx(attn, q, k, v, attention_mask, cached: bool, kwargs) -> torch.Tensor | None:
+def prompt_ctx(attn, q, k, v, attention_mask, kwargs) -> torch.Tensor | None:
     """config.adkv_prompt: the dense rows' attention ``[B, T, Hq, C]`` by the framework's own kernel, without weights; None where transformers' is to
     run (``takes_prompts``; where a derivative is wanted).  With ``cu_seq_lens_q`` (transformers' name for the bounds of sequences packed into one row
     axis) each sequence looks at itself only."""
     if not getattr(attn.config, "adkv_prompt", False):
         return None
     bounds = kwargs.get("cu_seq_lens_q")
-    if bounds is not None and cached:
-        raise ValueError("packed sequences have no cache: pass use_cache=False")
     apart = says_nothing(attention_mask)
     if not takes_prompts(attn, q.dtype, q.device, kwargs) or not k.dtype == v.dtype == q.dtype or derivatives_wanted(q, k, v, attention_mask):
         if apart:
@@ -129,6 +127,7 @@ class LlamaAttention_ADKV(LlamaAttention):
 
     def forward(self, hidden_states, position_embeddings=None, attention_mask=None,
                 past_key_values=None, cache_position=None, use_cache: bool = True, **kwargs):
+        refuse_cache(self, use_cache and past_key_values is not None, kwargs)
         lead = hidden_states.shape[:-1]
         split = (*lead, -1, self.head_dim)
         q = self.q_proj(hidden_states).view(split).transpose(1, 2)
@@ -175,7 +174,7 @@ class LlamaAttention_ADKV(LlamaAttention):
             ctx = torch.stack(steps, dim=1)                      # [B, Tq, Hq, C]
             return self.o_proj(ctx.reshape(*lead, -1)), None
 
-        ctx = prompt_ctx(self, q, k, v, attention_mask, layer_cache is not None, kwargs)
+        ctx = prompt_ctx(self, q, k, v, attention_mask, kwargs)
         if layer_cache is not None:
             layer_cache.prefill(k, v, *self._adkv_params("key"), *self._adkv_params("value"))
         if ctx is not None:

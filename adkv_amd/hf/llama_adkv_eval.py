@@ -28,7 +28,7 @@ from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
 from ..kernel.gemv import take_sequences
 from ..train.train_model import quant_f32_pair
 from .llama_adkv import ADKV_PARAM_FIELDS, ADKVConfig, make_head_norms, norm_and_rotate, prompt_ctx  # noqa: F401
-from .packed import packed_mask
+from .packed import packed_mask, refuse_cache
 from .score import Scores
 
 SCALE_MIN = math.exp(-4.0)
@@ -232,6 +232,7 @@ class LlamaAttention_ADKV(LlamaAttention):
     def forward(self, hidden_states, position_embeddings=None, attention_mask=None,
                 past_key_values=None, cache_position=None, use_cache: bool = True,
                 prefill_full_precision: bool = True, **kwargs):
+        refuse_cache(self, past_key_values is not None, kwargs)
         lead = hidden_states.shape[:-1]
         shape = (*lead, -1, self.head_dim)
         q = self.q_proj(hidden_states).view(shape).transpose(1, 2)
@@ -260,7 +261,7 @@ class LlamaAttention_ADKV(LlamaAttention):
                 n = layer.get_seq_length()
                 k, v = heads(layer.key_states, n), heads(layer.value_states, n)
 
-        out = prompt_ctx(self, q, k, v, attention_mask, past_key_values is not None, kwargs)
+        out = prompt_ctx(self, q, k, v, attention_mask, kwargs)
         if out is not None:
             return self.o_proj(out.reshape(*lead, -1)), None
         attend = eager_attention_forward

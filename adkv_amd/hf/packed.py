@@ -13,6 +13,12 @@ def takes_prompts(attn, dtype, device, kwargs) -> bool:
                 and not kwargs.get("output_attentions") and not getattr(attn.config, "output_attentions", False))
 
 
+def refuse_cache(attn, cached: bool, kwargs) -> None:
+    """Ahead of anything that is written to a cache: it keeps sequences of one length, each a row of its batch."""
+    if cached and kwargs.get("cu_seq_lens_q") is not None and getattr(attn.config, "adkv_prompt", False):
+        raise ValueError("packed sequences have no cache: pass use_cache=False")
+
+
 def derivatives_wanted(*tensors) -> bool:
     """Of what is computed from them: backward, forward, or a transform's."""
     return any((t.requires_grad and torch.is_grad_enabled()) or torch._C._functorch.is_functorch_wrapped_tensor(t) or forward_ad.unpack_dual(t).tangent is not None

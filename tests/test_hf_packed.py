@@ -50,6 +50,21 @@ def test_refused_with_packed_sequences():
         m(ids_of(1, ENDS[-1]), attention_mask=torch.empty(1, 1, 0, 0, dtype=torch.bool), **packed("cpu"))
 
 
+@pytest.mark.parametrize("flavour", FLAVOURS)
+def test_a_cache_is_refused_before_it_is_written(flavour, monkeypatch):
+    """A new one, and one that holds a prompt already (one more token, and several)."""
+    module = FLAVOURS[flavour]
+    m = make(module.LlamaForCausalLM_ADKV, config(adkv_prompt=True), torch.float32, "cpu")
+    for name in ("update", "prefill", "decode", "extend"):
+        monkeypatch.setattr(module.KVCacheLayer_ADKV, name, lambda *a, **k: pytest.fail("written"), raising=False)
+    for length, n in ((0, ENDS[-1]), (30, ENDS[-1]), (30, 1)):
+        cache = module.KVCache_ADKV(2)
+        for layer in cache:
+            layer._quant_len = layer._recent_len = length
+        with torch.no_grad(), pytest.raises(ValueError, match="no cache"):
+            m(ids_of(1, n), past_key_values=cache, use_cache=True, cu_seq_lens_q=torch.tensor([0, n], dtype=torch.int32))
+
+
 def test_what_the_kernel_takes():
     at = lambda **how: make(llama_adkv.LlamaForCausalLM_ADKV, config(adkv_prompt=True, **how), torch.float32, "cpu").model.layers[0].self_attn
     dev, attn = torch.device("cuda"), at()
@@ -186,13 +201,13 @@ def test_derivatives_are_transformers(gpu, monkeypatch):
         for i in range(3):
             t = [q, k, v]
             t[i] = torch.autograd.forward_ad.make_dual(t[i], torch.ones_like(t[i]))
-            assert llama_adkv.prompt_ctx(attn, *t, None, False, {}) is None
+            assert llama_adkv.prompt_ctx(attn, *t, None, {}) is None
     with torch.no_grad():
         none = []
-        torch.func.vmap(lambda x: none.append(llama_adkv.prompt_ctx(attn, x, k, v, None, False, {})) or x)(q[None])
-        torch.func.jvp(lambda x: none.append(llama_adkv.prompt_ctx(attn, q, k, x, None, False, {})) or x, (v,), (v,))
+        torch.func.vmap(lambda x: none.append(llama_adkv.prompt_ctx(attn, x, k, v, None, {})) or x)(q[None])
+        torch.func.jvp(lambda x: none.append(llama_adkv.prompt_ctx(attn, q, k, x, None, {})) or x, (v,), (v,))
         assert none == [None, None]
-    assert llama_adkv.prompt_ctx(attn, q, k, v, torch.zeros(1, 1, 9, 9, device=gpu, requires_grad=True), False, {}) is None
+    assert llama_adkv.prompt_ctx(attn, q, k, v, torch.zeros(1, 1, 9, 9, device=gpu, requires_grad=True), {}) is None
     found = []
     for m in (mine, other):
         with torch.no_grad(), torch.autograd.forward_ad.dual_level():
@@ -212,4 +227,4 @@ def test_masks_of_other_kinds_are_transformers(gpu, monkeypatch):
     with torch.no_grad():
         for mask in (create_block_mask(lambda b, h, i, j: i >= j, 1, 1, 9, 9, device=gpu), torch.ones(1, 9, dtype=torch.bool, device=gpu), torch.ones(1, 1, 9, 8, dtype=torch.bool, device=gpu)):
             for how in ({}, dict(cu_seq_lens_q=torch.tensor([0, 4, 9], dtype=torch.int32, device=gpu))):
-                assert llama_adkv.prompt_ctx(attn, *rows, mask, False, how) is None
+                assert llama_adkv.prompt_ctx(attn, *rows, mask, how) is None
