@@ -63,8 +63,8 @@ def norm_and_rotate(attn, q, k, cos, sin):
 
 def prompt_ctx(attn, q, k, v, attention_mask, kwargs) -> torch.Tensor | None:
     """config.adkv_prompt: the dense rows' attention ``[B, T, Hq, C]`` by the framework's own kernel, without weights; None where transformers' is to
-    run (``takes_prompts``; where a derivative is wanted).  With ``cu_seq_lens_q`` (transformers' name for the bounds of sequences packed into one row
-    axis) each sequence looks at itself only."""
+    run (``takes_prompts``; where a derivative is wanted).  It is causal whatever a mask of four axes shows.  With ``cu_seq_lens_q`` (transformers'
+    name for the bounds of sequences packed into one row axis) each sequence looks at itself only."""
     if not getattr(attn.config, "adkv_prompt", False):
         return None
     bounds = kwargs.get("cu_seq_lens_q")

@@ -7,10 +7,12 @@ from torch.autograd import forward_ad
 
 def takes_prompts(attn, dtype, device, kwargs) -> bool:
     """Whether ``prompt_ctx`` attends for ``attn`` itself, with rows of this type on this device and where no derivative is wanted; without
-    config.adkv_prompt, on the host, for other types and head sizes, where dropout or the weights are wanted, transformers' attention does."""
+    config.adkv_prompt, on the host, for other types and head sizes, where dropout or the weights are wanted, where later tokens are looked at
+    or scores have a bias of their own, transformers' attention does."""
     return bool(getattr(attn.config, "adkv_prompt", False) and device.type == "cuda" and dtype in (torch.float16, torch.bfloat16)
                 and attn.head_dim % 8 == 0 and attn.head_dim <= 256 and not (attn.training and attn.attention_dropout > 0)
-                and not kwargs.get("output_attentions") and not getattr(attn.config, "output_attentions", False))
+                and not kwargs.get("output_attentions") and not getattr(attn.config, "output_attentions", False)
+                and attn.is_causal and getattr(attn.config, "is_causal", True) and kwargs.get("is_causal") in (None, True) and kwargs.get("position_bias") is None)
 
 
 def refuse_cache(attn, cached: bool, kwargs) -> None:
@@ -50,7 +52,7 @@ def packed_mask(model, tokens: torch.Tensor, attention_mask, kwargs):
     how = model.config._attn_implementation
     if packs(model, kwargs):
         return torch.empty(1, 1, 0, 0, dtype=torch.bool, device=tokens.device)
-    if how not in ("sdpa", "eager"):
+    if how not in ("sdpa", "eager") or not getattr(model.config, "is_causal", True):
         return None                    # transformers' others know the bounds, or make masks from the positions
     at = torch.arange(tokens.shape[1], device=tokens.device)
     of = torch.searchsorted(bounds.to(at), at, right=True)

@@ -72,6 +72,10 @@ def test_what_the_kernel_takes():
     assert not takes_prompts(attn, torch.float32, dev, {}) and not takes_prompts(attn, torch.float16, torch.device("cpu"), {})
     assert not takes_prompts(attn, torch.float16, dev, dict(output_attentions=True)) and not takes_prompts(at(head_dim=36), torch.float16, dev, {})
     assert not takes_prompts(at(head_dim=264), torch.float16, dev, {}) and not takes_prompts(at(output_attentions=True, attn_implementation="eager"), torch.float16, dev, {})
+    assert takes_prompts(attn, torch.float16, dev, dict(is_causal=True, position_bias=None)) and not takes_prompts(attn, torch.float16, dev, dict(is_causal=False))
+    assert not takes_prompts(attn, torch.float16, dev, dict(position_bias=torch.zeros(1))) and not takes_prompts(at(is_causal=False), torch.float16, dev, {})
+    attn.is_causal = False
+    assert not takes_prompts(attn, torch.float16, dev, {})
     attn = at(attention_dropout=0.1)
     assert takes_prompts(attn, torch.float16, dev, {}) and not takes_prompts(attn.train(), torch.float16, dev, {})
 
