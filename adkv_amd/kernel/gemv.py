@@ -822,6 +822,9 @@ def take_sequences(tensors, index: torch.Tensor, *, used=None, into=None) -> Non
     if not index.is_cuda:
         _chk(all(0 <= r < B for r in index.tolist()), "index must be of the sequences")
     dev = _need_device(*tensors, *(into or ()))
+    if B == 0:                   # no row is one of none
+        for to in into or ():
+            to.zero_()
     if R == 0 or B == 0 or not rows:
         return
     index = index.to(device=dev, dtype=torch.int64).contiguous()

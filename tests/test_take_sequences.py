@@ -135,6 +135,17 @@ def test_nothing_to_do(gpu):
     check(tensors_of(2, 2, [("codes", 0)], gpu), torch.tensor([1, 0, 1], device=gpu), None, [torch.full((3, 2, 5, 32, 4, 4), 7, dtype=torch.uint8, device=gpu)])
 
 
+@pytest.mark.gpu
+def test_no_sequences(gpu):
+    """No index is one of theirs: new buffers are zeros, as for every such row."""
+    into = [torch.full((3, 2, n, 32, 4, 4), 7, dtype=torch.uint8, device=gpu) for n in (5, 6)]
+    index = torch.tensor([0, -1, 2], device=gpu)
+    gemv.take_sequences([torch.zeros(0, 2, 5, 32, 4, 4, dtype=torch.uint8, device=gpu)] * 2, index, used=[5, 0], into=into)
+    assert not any(t.any() for t in into)
+    with pytest.raises(RuntimeError, match="of the sequences"):
+        gemv.take_sequences([torch.zeros(0, 2, 5, 16, dtype=torch.uint8, device=gpu)], index.cpu(), into=[torch.zeros(3, 2, 5, 16, dtype=torch.uint8, device=gpu)])
+
+
 def test_refusals():
     t = torch.zeros(3, 2, 5, 32, 4, 4, dtype=torch.uint8)
     i = torch.tensor([0, 1])
