@@ -1056,7 +1056,9 @@ static int checked(int B, int Hq, int H, int Tq, int Tk, int D, int n_seq)
     if (D <= 0 || D > 256 || D % 8)
         return ADKV_E_DIM;
     const int64_t g = Hq / H;
-    // rows are counted in 31 bits and divided by g in 32; a grid is 2^32 threads at most
+    // rows are counted in 31 bits and divided by g in 32; a grid is 2^32 threads at most.  The first line keeps the products below 2^63.
+    if (g > 46340 || (int64_t)B * H >= 1 << 24 || (int64_t)B * Tq > INT32_MAX)
+        return ADKV_E_SHAPE;
     if (Tq * g * g > INT32_MAX || Tk > INT32_MAX - 256 || (Tq * g / ROWS + n_seq + 3) * B * H > (1 << 24) - 1 || (int64_t)B * Tq * Hq > INT32_MAX)
         return ADKV_E_SHAPE;
     return ADKV_OK;

@@ -183,6 +183,9 @@ extern "C" int adkv_take_sequences(const adkv_rows *tensors, int n, const int64_
         if (t.segments < 0 || t.used < 0 || t.pitch < t.used || (into && t.into_pitch < t.used) || (!into && rows > batch) || t.pitch > INT32_MAX - BLOCK ||
             t.into_pitch > INT32_MAX - BLOCK)
             return ADKV_E_SHAPE;
+        // no memory is that large, and products of what is taken stay below 2^63
+        if (t.segments > INT32_MAX || t.segments * std::max(t.pitch, into ? t.into_pitch : 0) > INT64_MAX / std::max(batch, MOST))
+            return ADKV_E_SHAPE;
         if (((uint64_t)t.data | (uint64_t)t.into | (uint64_t)t.pitch | (uint64_t)(into ? t.into_pitch : 0) | (uint64_t)t.used) & 15)
             return ADKV_E_ALIGN;
     }

@@ -462,3 +462,10 @@ def test_the_library_refuses_what_it_cannot_take():
         assert L.adkv_prompt_attention(*a.values()) == code, change
     assert L.adkv_prompt_attention_workspace_bytes(1, 3, 2, 8, 8, 64, 0) == -3
     assert L.adkv_prompt_attention_workspace_bytes(1, 4, 2, 8, 8, 63, 0) == -2
+
+
+def test_sizes_that_no_memory_has():
+    from adkv_amd import _lib
+    L, m = _lib.lib(), 2 ** 31 - 1
+    for B, Hq, H, Tq, n_seq in [(m, m, m, 4, 0), (m, m, m, 1, 0), (1, m, 1, m, 0), (1, m, m, 4, m), (m, 1, 1, m, 0), (1 << 24, 1, 1, 1, 0), (1, 46341, 1, 1, 0)]:
+        assert L.adkv_prompt_attention_workspace_bytes(B, Hq, H, Tq, min(Tq, 2 ** 30), 64, n_seq) == -3

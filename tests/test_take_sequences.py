@@ -183,6 +183,15 @@ def test_the_library_refuses_what_it_cannot_take():
     assert L.adkv_take_sequences(None, 0, 4096, 1, 1, None) == 0 and L.adkv_take_sequences(both, 2, None, 0, 1, None) == -6
 
 
+def test_sizes_that_no_memory_has():
+    """Their products pass 64 bits: refused, not taken for nothing to do."""
+    from adkv_amd import _lib
+    L = _lib.lib()
+    for batch, rows, segments, pitch, into_pitch, used in [(2, 2, 2 ** 60, 16, 0, 16), (2, 2, 2 ** 31, 64, 0, 32), (2 ** 31 - 1, 2, 2 ** 31 - 1, 2 ** 30, 0, 16), (1, 1024, 2 ** 31 - 1, 2 ** 30, 2 ** 30, 0)]:
+        t = (_lib.Rows * 1)(_lib.Rows(4096, 8192 if into_pitch else None, segments, pitch, into_pitch, used))
+        assert L.adkv_take_sequences(t, 1, 4096, rows, batch, None) == -3
+
+
 @pytest.mark.gpu
 def test_tensors_that_share_memory(gpu):
     """Refused where one of them is written; several of them may be copied from one."""
