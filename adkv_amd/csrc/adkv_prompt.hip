@@ -82,7 +82,6 @@ struct Args {
 
 template <int TYPE> struct Half;
 template <> struct Half<F16> {
-    typedef h8v v8;
     static constexpr float BIAS = 7.0f;
     static __device__ __forceinline__ f16v mfma(u4v a, u4v b, f16v c)
     {
@@ -99,7 +98,6 @@ template <> struct Half<F16> {
     static __device__ __forceinline__ float number(uint16_t w) { return (float)__builtin_bit_cast(_Float16, w); }
 };
 template <> struct Half<BF16> {
-    typedef b8v v8;
     static constexpr float BIAS = 0.0f;
     static __device__ __forceinline__ f16v mfma(u4v a, u4v b, f16v c)
     {
