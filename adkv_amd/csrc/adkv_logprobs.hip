@@ -5,8 +5,9 @@
 // The largest is left out of the sums, so that log(1 + S) keeps its digits where one token is nearly certain, and T is a sum of numbers of one sign.
 // A lane holds back the largest it has seen, adds the smaller of it and the next one, and sums relative to a reference r of its own, the largest of its
 // first logits (replaced where a logit is more than 2^FAR larger), all in powers of two: x log2(e) - r is one multiply-add, and r log2(e) - M log2(e) another
-// at the end, so that neither r nor log2(e) need be exact.  Logits below FLOOR, minus infinity among them, weigh nothing; rows whose largest is beyond
-// +-FLOOR are gone through again.  NaN is looked for beside it: v_med3 and v_max drop it.
+// at the end, so that neither r nor log2(e) need be exact.  References are within +-FLOOR, where r is off by 2^-4 at most (one of 10^10 would be off by 2^9, and
+// 2^d infinite).  Logits below FLOOR, minus infinity and what else stands for hidden tokens among them, weigh nothing; rows whose
+// largest is not within half of +-FLOOR are gone through again.  NaN is looked for beside it: v_med3 and v_max drop it.
 //
 // The likeliest: a key is the logit's bits in the order of numbers with the index, backwards, behind them, so that all keys differ and equal logits
 // come lowest index first.  The lanes' maxima of the first step, 64 groups of them, give a bound that at least `top` keys reach; what reaches it goes to a
@@ -39,7 +40,7 @@ constexpr int F32 = ADKV_DT_F32, F16 = ADKV_DT_F16, BF16 = ADKV_DT_BF16;
 constexpr int CAP = 1024, REFINE = 128; // keys of a list; above which it is looked through
 constexpr int TOP = 32;
 constexpr float L2E = 1.44269504088896340736f;
-constexpr float FLOOR = -0x1p126f; // times log2(e) it is exact, and its difference from itself zero
+constexpr float FLOOR = -0x1p20f; // times log2(e) it is exact, and its difference from itself zero
 constexpr float FAR = 60.0f;
 
 struct Args {
@@ -66,7 +67,7 @@ __device__ __forceinline__ void add(Sums &a, float x)
 __device__ __forceinline__ void refer(Sums &a, float r)
 {
     const float shift = a.r - r, e = __builtin_amdgcn_exp2f(shift);
-    a.t = e == 0.0f ? 0.0f : e * __builtin_fmaf(shift, a.s, a.t); // relative to FLOOR the product may be infinite
+    a.t = e == 0.0f ? 0.0f : e * __builtin_fmaf(shift, a.s, a.t);
     a.s *= e;
     a.r = r;
 }
@@ -355,14 +356,14 @@ __global__ __launch_bounds__(NT, WITH_TOP ? 6 : 8) void logprobs_kernel(const Ar
     sums = lane < NW ? left[lane] : (Sums){FLOOR, 0.0f, 0.0f, FLOOR * L2E};
     together(sums, lane);
     float M = sums.big;
-    const bool again = !(fabsf(M) < -FLOOR);
+    const bool again = !(fabsf(M) < -0.5f * FLOOR); // else e^FLOOR is nothing beside e^M
     if (wave != 0 && !slow && !again)
         return; // the rest is the first wave's
     const float shift = __builtin_fmaf(-M, L2E, sums.r), scale = __builtin_amdgcn_exp2f(shift);
     // T is the small difference of two large ones where the reference is not the largest
     float S = scale * sums.s, T = (float)(0.69314718055994530942 * ((double)scale * ((double)shift * sums.s + sums.t)));
     if (again) {
-        // logits of the type's lowest value only, or of minus or plus infinity: the definition, in two passes more
+        // logits beyond half a million, of the type's lowest value only, or of minus or plus infinity: the definition, in two passes more
         M = -INFINITY;
         for (int i = tid; i < a.V; i += NT)
             M = fmaxf(M, P::one(row, i));
@@ -373,18 +374,24 @@ __global__ __launch_bounds__(NT, WITH_TOP ? 6 : 8) void logprobs_kernel(const Ar
         __syncthreads();
         M = largest(left[lane % NW].big);
         S = T = 0.0f;
+        float equal = 0.0f; // of the largest, one of which is left out
         for (int i = tid; i < a.V; i += NT) {
             const double d = (double)P::one(row, i) - M;
             const float e = d > -200.0 ? expf((float)d) : 0.0f;
-            S += e;
-            T += e > 0.0f ? e * (float)d : 0.0f;
+            if (d == 0.0) {
+                equal += 1.0f;
+            } else if (e > 0.0f) {
+                S += e;
+                T += e * (float)d;
+            }
         }
         S = sum(S);
         T = sum(T);
+        equal = sum(equal);
         if (lane == 0)
-            left[wave].s = S, left[wave].t = T;
+            left[wave].s = S, left[wave].t = T, left[wave].r = equal;
         __syncthreads();
-        S = sum(lane < NW ? left[lane].s : 0.0f) - 1.0f;
+        S = sum(lane < NW ? left[lane].s : 0.0f) + (sum(lane < NW ? left[lane].r : 0.0f) - 1.0f);
         T = sum(lane < NW ? left[lane].t : 0.0f);
     }
     const float log1 = odd || fabsf(M) == INFINITY ? NAN : log1pf(S);

@@ -121,6 +121,44 @@ def test_infinities_and_what_is_no_number(gpu, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("where", ["front", "behind", "every other", "all", "all but one"])
+@pytest.mark.parametrize("value", [-1e4, -5e5, -1e6, -1e9, -1e10, -1e12, -1e20, -1e30, -8e37, -2e38, 4e5, 6e5, 1e6, 1e12, 1e38])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_logits_far_from_the_others(gpu, dtype, value, where):
+    """Hidden tokens, in front of the others too; rows of nothing else; large ones.  They are next to others or far beyond what e^x tells from nothing."""
+    for N, V, top in ((3, 100, 3), (3, 32000, 0), (2, 32000, 20), (1100, 3001, 0)):
+        x, tokens = logits_of(N, V, dtype, gpu, 4)
+        at = torch.arange(V, device=gpu)
+        x[:, {"front": at < V * 2 // 3, "behind": at > V // 3, "every other": at % 2 == 0, "all": at >= 0, "all but one": at != V // 2}[where]] = value
+        tokens[0] = V // 2
+        got = check(x, tokens, top)
+        assert torch.isfinite(got.logprobs).all()
+        # beside check(), which allows for references far from the largest: those that are hidden are none, so that they are within 2^60 of it
+        ent, (log, S, T) = got.entropy.cpu().double(), sums_of(x)
+        eps, share = (V / 256 + 18) * 2.0 ** -24 + 2.0 ** -22 + 300 * 2.0 ** -24, S / (1 + S)
+        want = log - T / (1 + S)
+        assert ((ent - want).abs() <= 2 * eps * (62 * share + (T / (1 + S)).abs()) + 2.0 ** -24 * want.abs() + 2.0 ** -97).all()
+
+
+def sums_of(x):
+    """log(1 + S), S and T of the formula, without the first of the largest."""
+    x = x.cpu().double()
+    d = x - x.amax(-1, keepdim=True)
+    e = torch.exp(d).scatter_(1, x.argmax(-1, keepdim=True), 0.0)
+    return torch.log1p(e.sum(-1)), e.sum(-1), torch.where(e > 0, e * d, 0.0).sum(-1)
+
+
+@pytest.mark.gpu
+def test_nearly_certain_tokens_keep_their_digits_far_from_zero(gpu):
+    """Logits around a million, in steps of 2^-4."""
+    x = torch.full((8, 5000), 1e6 - 20.0, device=gpu)
+    x[:, 77] = 1e6 - 4 + torch.arange(8, device=gpu) * 2.0
+    got = check(x, torch.full((8,), 77, device=gpu), 2)
+    want = -torch.log1p(4999 * torch.exp(-20 - (x[:, 77].double() - 1e6)))
+    assert ((got.logprobs.double() - want).abs() <= 1e-5 * want.abs()).all()
+
+
+@pytest.mark.gpu
 def test_nearly_certain_tokens_keep_their_digits(gpu):
     x = torch.full((40, 5000), -20.0, device=gpu)
     x[:, 77] = torch.linspace(-10, 60, 40, device=gpu)
