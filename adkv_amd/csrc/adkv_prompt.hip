@@ -539,16 +539,18 @@ struct Wave {
         outputs<1>(values, w);
     }
 
-    // whether a product's result, or the sum, is infinite or no number
+    // whether a product's result, or the sum, is infinite or no number, or nothing is left of a row that looks at something: references of 2^30 and more are
+    // rounded by what leaves no weight of the largest score
     __device__ __forceinline__ bool strange() const
     {
+        const bool lost = other_half(l, false) == 0.0f && m > -INFINITY;
         float nothing[4] = {l * 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int cb = 0; cb < CB; cb++)
 #pragma unroll
             for (int e = 0; e < 16; e++)
                 nothing[e & 3] = __builtin_fmaf(o[cb][e], 0.0f, nothing[e & 3]);
-        return __any((nothing[0] + nothing[1]) + (nothing[2] + nothing[3]) != 0.0f);
+        return __any(lost || (nothing[0] + nothing[1]) + (nothing[2] + nothing[3]) != 0.0f);
     }
 
     // To the output, 16 bytes at a time: two lanes have four channels each of the same eight of a row; an exchange leaves one of them with these and

@@ -168,6 +168,28 @@ def test_scores_that_grow_along_the_row_and_large_ones(gpu, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["none", "bool_keys", "some"])
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("size", [(20, 16, 1, 129, 129, 128), (2, 8, 1, 1101, 1101, 96), (1, 4, 2, 300, 301, 64), (1, 2, 1, 260, 300, 256), (1, 1, 4, 3, 1500, 128)], ids=str)
+def test_scores_of_ten_digits(gpu, size, dtype, kind):
+    """A step of such a score in 32 bits is more than e^x has room for.  Scores are at least 2^-8 of themselves apart, 250 and more, and off by 2^-16, so that a row's output is
+    the value of its largest one, which the products of 11 bits leave as it is."""
+    B, H, g, Tq, Tk, D = size
+    r = torch.Generator().manual_seed(7)
+    order = torch.randperm(Tk, generator=r)
+    k = (0x4780 - Tk + order).to(torch.int16).view(BF16).to(dtype).to(gpu)[None, None, :, None].expand(B, H, Tk, D)       # bfloat16's numbers up to 65280
+    v = rows(B, H, Tk, D, dtype, gpu, 2)
+    at = order.cummax(0)[1][Tk - Tq:].to(gpu)
+    m = {"none": None, "bool_keys": torch.ones(B, 1, 1, Tk, dtype=torch.bool, device=gpu), "some": torch.zeros(1, 1, Tq, Tk, dtype=dtype, device=gpu)}[kind]
+    if kind == "some":
+        m[..., ::2] = -1.0
+    for amount in (1e3, 3e4):
+        q = (torch.rand(B, H * g, Tq, 1, generator=r) + 1).mul(amount).to(dtype).to(gpu).expand(B, H * g, Tq, D)
+        got = gemv.prompt_attention(q, k, v, 1.0, m)
+        assert torch.equal(got, v[:, :, at].repeat_interleave(g, 1).transpose(1, 2)), amount
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F16, BF16], ids=["fp16", "bf16"])
 @pytest.mark.parametrize("H,g,ends", [(1, 1, [0, 1]), (2, 3, [0, 5, 5, 70, 133]), (1, 1, [0, 0, 0, 64]), (2, 1, [3, 40, 40, 99]), (1, 4, [0]),
                                       (16, 1, [0, 300, 301, 303, 700]), (8, 4, [0, 31, 63, 64, 65, 400, 500, 500]), (1, 1, [0, *range(1, 150)]), (40, 1, [*range(0, 9000, 60)])],
