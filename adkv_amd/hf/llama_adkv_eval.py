@@ -182,7 +182,7 @@ class KVCache_ADKV(list):
 
     def reorder_cache(self, beam_idx: torch.Tensor) -> None:
         """Sequence ``i`` goes on from what sequence ``beam_idx[i]`` holds (beam search), in place, all layers in a launch or two."""
-        layers = [layer for layer in self if layer._key_buf is not None]
+        layers = [layer for layer in self if layer._recent_len > 0]
         if beam_idx.dim() != 1 or any(beam_idx.shape[0] != layer._key_buf.shape[0] for layer in layers):
             raise ValueError("reorder_cache needs an index for every sequence")
         tensors, used = [], []

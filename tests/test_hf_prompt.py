@@ -235,6 +235,28 @@ def test_views_of_what_moved(monkeypatch):
         view.share(2)
 
 
+def test_moving_sequences_of_the_evaluation_cache(monkeypatch):
+    """In place, states and all; a layer whose first prompt was refused has buffers and nothing in them."""
+    from adkv_amd.hf import llama_adkv_eval as module
+    monkeypatch.setattr(module, "take_sequences", as_indexing)
+    c = module.KVCache_ADKV(3)
+    g = torch.Generator().manual_seed(0)
+    for layer in c[:2]:
+        layer._init_buffers(3, 8, torch.device("cpu"), torch.float32)
+    with pytest.raises(Exception):
+        c[1].update(torch.zeros(3, 2, 8), torch.zeros(3, 2, 8), *[None] * 10)
+    for t in (c[0]._key_buf, c[0]._value_buf):
+        t[:, :5] = torch.randn(3, 5, 8, generator=g)
+    c[0].key_dc, c[0].key_scale, c[0].value_dc, c[0].value_scale = (torch.randn(3, 8, generator=g) for _ in range(4))
+    c[0]._recent_len = 5
+    of = lambda: [t.clone() for t in (c[0].key_states, c[0].value_states, c[0].key_dc, c[0].key_scale, c[0].value_dc, c[0].value_scale)]
+    was, index = of(), torch.tensor([2, 0, 0])
+    c.reorder_cache(index)
+    assert all(torch.equal(a, b[index]) for a, b in zip(of(), was))
+    with pytest.raises(ValueError, match="every sequence"):
+        c.reorder_cache(torch.tensor([0, 1]))
+
+
 def test_slices_that_are_further_than_their_batch(monkeypatch):
     """What a slice has been prefilled or stepped with does not move before the batch knows of it: the states would move without the codes."""
     monkeypatch.setattr(cache_module, "take_sequences", as_indexing)
