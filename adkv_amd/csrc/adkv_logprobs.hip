@@ -15,8 +15,8 @@
 // the end each key of the list counts the larger ones.  Rows whose keys overrun the list (ascending logits) or that have a NaN are searched a key at a time instead.
 //
 // A workgroup per row; the launcher says how large.  MI355X: 4096 rows of 32000 bf16 logits 55 us, 4.7 TB/s, 1000 rows of 128001 fp32 ones 94, 5.4 TB/s: memory (a
-// copy runs at 5.15, reads alone faster).  With alternatives some 4 us more per round of rows, for the bound in front and the ranks behind: 1000 rows of 128001 fp16
-// ones with 20 of them 68 us where they are 50 without; four rows of 32000 10.6 where they are 6.2.
+// copy runs at 5.15, reads alone faster).  Alternatives cost the bound in front and the ranks behind, some 4 us of few rows and more of many that are in step: four rows
+// of 32000 10.6 us where they are 6.2 without; 1000 rows of 128001 fp16 ones with 20 of them, all resident at once, 69 where they are 50.
 #include <math.h>
 
 #include <algorithm>

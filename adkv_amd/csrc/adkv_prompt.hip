@@ -20,7 +20,7 @@
 //
 // What bounds it, MI355X: long prompts the clock that the matrix cores' power allows (16384 tokens, 32 heads on 8, bf16: 1.98 ms, 1.11 PFLOP/s, matrix cores
 // busy for 61 % of the time at 1.67 GHz; a library's product of 8192^3 runs at 1.40).  Batches of short ones memory and the way in and out of a workgroup
-// (128 of 512 tokens, 32 heads: 554 us, 3.9 TB/s, the matrix cores 33 % busy; of 128 tokens 112 us, 4.8 TB/s; a copy runs at 5.15), and few blocks the
+// (128 of 512 tokens, 32 heads: 539 us, 4.0 TB/s, the matrix cores 33 % busy; of 128 tokens 112 us, 4.8 TB/s; a copy runs at 5.15), and few blocks the
 // chain of a single one.  A row over many keys: memory (8 x 8 heads of four, 4097 tokens: 31 us, 4.4 TB/s).
 #include <math.h>
 
@@ -1019,23 +1019,23 @@ static Plan plan(int B, int Hq, int H, int Tq, int Tk, int D, int n_seq)
     // Where 128 rows at a time leave CUs without work, or with the longest rows alone at the end, more waves share a row's keys.  Workgroups of the forms
     // for that have a CU to themselves, or share it with one more (64 channels), and two rounds of them still pay where a unit has long rows beside short
     // ones.  us of many, some, few, bf16, channels: units x tokens
-    //    64: 16 x 512  10.4, 7.9, 7.0     32 x 512  10.6, 8.3, 7.9     32 x 1024  18, 14, 18     16 x 4096  59, 55, 75     64 x 1024  19, 23, 32
-    //   128: 16 x 512  13.7, 11.5, 9.8    32 x 512  13.8, 11.9, 15.7   16 x 1024  23, 17, 20     16 x 2048  41, 34, 53     64 x 512   16, 20, 30
-    //   256: 16 x 512  27, 25, 16         32 x 512  28, 26, 26         16 x 1024  46, 42, 34     64 x 256   19, 19, 22     32 x 1024  50, 53, 66
+    //    64: 16 x 512  10.5, 8.1, 7.3     32 x 512  10.7, 8.4, 8.1     32 x 1024  18, 14, 18     16 x 4096  60, 57, 76     64 x 1024  20, 24, 32
+    //   128: 16 x 512  13.5, 11.8, 10.2    32 x 512  14.0, 12.4, 16.2   16 x 1024  22, 17, 20     16 x 2048  40, 34, 53     64 x 512   16, 20, 30
+    //   256 (some do not fit): 16 x 512  27, 17      32 x 512  28, 27      16 x 1024  46, 35     64 x 256  18, 22     32 x 1024  48, 66
     const int64_t slots = D > 64 ? cus : 2ll * cus;
     const auto fits = [&](int each, int length) { // once, or twice with so many blocks of a sequence
         const int64_t all = (int64_t)p.units * blocks(each);
         return all <= slots || (all <= 2 * slots && blocks(each) >= (int64_t)length * std::max(1, n_seq));
     };
-    // A tile of keys leaves nothing to share: 64 tokens of 128 channels 5.6, 7.9, 6.4 us.
+    // A tile of keys leaves nothing to share: 64 tokens of 128 channels 5.8, 8.0, 6.6 us.
     p.rows = Tk <= 64 && D <= 128 ? MANY_ROWS : fits(FEW_ROWS, D > 128 ? 16 : INT32_MAX) ? FEW_ROWS : D <= 128 && fits(SOME_ROWS, 32) ? SOME_ROWS : MANY_ROWS;
     p.blocks = blocks(p.rows);
     p.pieces = 1;
     p.together = p.units;
     if (p.rows == MANY_ROWS) {
         // Many blocks: as many units at a time as fill the device once, so that their blocks find their keys in the XCDs' caches (us with that many, twice
-        // and four times as many, bf16: 128 sequences of 512 tokens, 32 heads 607, 585, 633; 64 of 300, eight heads of four queries 122, 129, 124; 101 of 278,
-        // 16 heads 124, 131, 138).  Else all of them, the longest first everywhere.
+        // and four times as many, bf16: 128 sequences of 512 tokens, 32 heads 555, 590, 635; 64 of 300, eight heads of four queries 122, 128, 126; 101 of 278,
+        // 16 heads 120, 131, 141).  Else all of them, the longest first everywhere.
         if ((int64_t)p.units * p.blocks > 8ll * cus)
             p.together = (int)std::min<int64_t>(p.units, (cus / p.blocks + 8) / 8 * 8);
     } else if (p.rows == FEW_ROWS) {

@@ -512,7 +512,7 @@ int adkv_fp16_decode(const void *q, const void *K, const void *V, void *out, voi
  *   dtype: of q, k, v, out, plus the mask's << 8.
  *   workspace: adkv_prompt_attention_workspace_bytes() (0: none is needed), 16-byte aligned.
  * Tq * (Hq / H)^2 and B * Tq * Hq are less than 2^31, workgroups of 32 rows fewer than 2^24 (ADKV_E_SHAPE).
- * Scores, maxima, sums and outputs are fp32; weights are rounded to the tensors' type.
+ * Scores, maxima, sums and outputs are fp32; weights are rounded to the tensors' type.  Values whose sum over the keys passes 3.4e38 leave infinities.
  */
 int64_t adkv_prompt_attention_workspace_bytes(int B, int Hq, int H, int Tq, int Tk, int D, int n_seq);
 int adkv_prompt_attention(const void *q, const int64_t *q_strides, const void *k, const int64_t *k_strides, const void *v,
