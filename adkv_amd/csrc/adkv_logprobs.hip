@@ -66,9 +66,10 @@ __device__ __forceinline__ void add(Sums &a, float x)
 
 __device__ __forceinline__ void refer(Sums &a, float r)
 {
-    const float shift = a.r - r, e = __builtin_amdgcn_exp2f(shift);
-    a.t = e == 0.0f ? 0.0f : e * __builtin_fmaf(shift, a.s, a.t);
-    a.s *= e;
+    // in two steps: what is up to 2^FAR above its reference is not lost before it is 2^-126 of the new one
+    const float shift = a.r - r, e = __builtin_amdgcn_exp2f(0.5f * shift);
+    a.t = __builtin_fmaf(shift, a.s, a.t) * e * e;
+    a.s = a.s * e * e;
     a.r = r;
 }
 

@@ -149,6 +149,22 @@ def sums_of(x):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("N", [400, 1600])
+@pytest.mark.parametrize("dtype", TYPES.values(), ids=TYPES.keys())
+def test_unlikely_tokens_beside_less_likely_ones(gpu, dtype, N):
+    """What a lane begins with is e^-36 of others that it sees, which are e^-64 of the row's largest: they are all that the largest's log probability is made of."""
+    for V, top in ((45, 0), (45, 3), (40001, 0)):
+        g = torch.Generator().manual_seed(V)
+        x = torch.full((N, V), -100.0)
+        x[torch.rand(N, V, generator=g) < 0.3] = -64.0
+        tokens = torch.randint(0, V, (N,), generator=g)
+        x[torch.arange(N), tokens] = 0.0
+        got = check(x.to(dtype).to(gpu), tokens.to(gpu), top)
+        want = -(x == -64).sum(-1) * math.exp(-64) - (x == -100).sum(-1) * math.exp(-100)
+        assert ((got.logprobs.cpu().double() - want).abs() <= 2e-5 * want.abs()).all()
+
+
+@pytest.mark.gpu
 def test_nearly_certain_tokens_keep_their_digits_far_from_zero(gpu):
     """Logits around a million, in steps of 2^-4."""
     x = torch.full((8, 5000), 1e6 - 20.0, device=gpu)
