@@ -80,7 +80,7 @@ class KVCacheLayer_ADKV:
         # whether a sequence's is that behind its last token, a byte per sequence, and the sequences that are this object's: a batch_view()
         # has its parent's bytes, which is how the parent knows that a slice was stepped
         self._valid, self._span = bytearray(), slice(0, 0)
-        self._reached: list = []  # tokens that a slice had of each sequence when it was last stepped, shared in the same way
+        self._reached: dict = {}  # tokens that a slice had when it was last stepped, by its first sequence and the one behind it; shared in the same way
         self._quant_len = 0
         self._cap_len = 0
         self._B = self._H = self._C = 0
@@ -110,7 +110,7 @@ class KVCacheLayer_ADKV:
         self._quant_len += tokens
         self._state_valid = state_valid
         if self._shares_storage:
-            self._reached[self._span] = [self._quant_len] * self._B
+            self._reached[self._span.start, self._span.stop] = self._quant_len
 
     # ------------------------------------------------------------------ HF cache protocol
     def get_seq_length(self) -> int:
@@ -173,7 +173,7 @@ class KVCacheLayer_ADKV:
          self._key_ckpt, self._value_ckpt) = self._new_buffers(tokens, alloc)
         mk = lambda: alloc((B, H, C, 2), dtype=torch.float16, device=device)
         self._key_state, self._value_state = mk(), mk()
-        self._valid, self._span, self._reached = bytearray(b"\1" * B), slice(0, B), [0] * B
+        self._valid, self._span, self._reached = bytearray(b"\1" * B), slice(0, B), {}
 
     def _cap_buffers(self, T: int):
         """Make room for ``T`` tokens.  New slots are zero, as the append kernels expect."""
@@ -464,7 +464,7 @@ class KVCacheLayer_ADKV:
             self._valid[self._span] = new
         else:
             self._valid.clear()
-            self._valid, self._span, self._reached = bytearray(new), slice(0, rows), [0] * rows
+            self._valid, self._span, self._reached = bytearray(new), slice(0, rows), {}
         self._B = rows
 
     # ------------------------------------------------------------------ save / restore
@@ -585,7 +585,8 @@ class KVCache_ADKV(list):
             raise ValueError("the layers hold different numbers of sequences")
         if any(layer._shares_storage for layer in layers) and (fresh or rows != B):
             raise ValueError("a batch view has as many sequences as it was made with")
-        if any(n > layer._quant_len for layer in layers for n in layer._reached[layer._span]):
+        if any(n > layer._quant_len and first < layer._span.stop and behind > layer._span.start for layer in layers if layer._reached
+               for (first, behind), n in layer._reached.items()):
             raise ValueError("slices of the batch hold more tokens than it knows of: commit() them first")
         where = None
         if not index.is_cuda:
