@@ -23,8 +23,12 @@ def refuse_cache(attn, cached: bool, kwargs) -> None:
 
 def derivatives_wanted(*tensors) -> bool:
     """Of what is computed from them: backward, forward, or a transform's."""
-    return any((t.requires_grad and torch.is_grad_enabled()) or torch._C._functorch.is_functorch_wrapped_tensor(t) or forward_ad.unpack_dual(t).tangent is not None
-               for t in tensors if isinstance(t, torch.Tensor))
+    backward, dual = torch.is_grad_enabled(), getattr(forward_ad, "_current_level", 0) >= 0      # without a level no tensor has a tangent
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and ((backward and t.requires_grad) or torch._C._functorch.is_functorch_wrapped_tensor(t)
+                                            or (dual and forward_ad.unpack_dual(t).tangent is not None)):
+            return True
+    return False
 
 
 def packs(model, kwargs) -> bool:
